@@ -3,7 +3,9 @@
 #include "iw_common.hpp"
 #include "iw_gemm.hpp"
 #include "iw_kernels.hpp"
+#include "iw_tree.hpp"
 
+#include <cmath>
 #include <string>
 
 namespace iw {
@@ -887,6 +889,211 @@ int iw_argmax_rows(const int8_t *x, int64_t rows, int64_t cols, int64_t ld, int6
   if (rows == 0) return IW_OK;
   IW_REQUIRE(x && out, "null tensor pointer");
   return launch_argmax_rows(x, rows, cols, ld, out, as_stream(stream));
+}
+
+// ---- trees of drafted tokens, token scores ----
+
+namespace {
+
+// [first, first + bytes) of two buffers share no byte
+bool apart(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x + (uintptr_t)a_bytes <= y || y + (uintptr_t)b_bytes <= x;
+}
+
+int check_tree_cache(int64_t heads, int64_t head_dim, int64_t cache_positions, int64_t v_sd, int64_t v_sq) {
+  IW_REQUIRE(heads > 0 && heads <= 4096 && head_dim > 0 && head_dim <= 128 && head_dim % 16 == 0,
+             "tree attention supports head_dim % 16 == 0, head_dim <= 128");
+  IW_REQUIRE(cache_positions > 0 && cache_positions < (1 << 24), "invalid number of cache positions");
+  if (v_sq != 4)
+    IW_REQUIRE(v_sd == 4 && v_sq >= 4 * head_dim,
+               "V in key quads needs v_sd == 4 and v_sq >= 4 * head_dim");
+  else
+    IW_REQUIRE(v_sd >= (cache_positions + 15) / 16 * 16, "transposed V rows must cover round_up(cache_positions, 16)");
+  return IW_OK;
+}
+
+}  // namespace
+
+int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *counts, const int32_t *lengths,
+                 int64_t batch, int64_t nodes, int32_t max_positions, int64_t *visible, int32_t *positions,
+                 iw_stream_t stream) {
+  IW_REQUIRE(batch >= 0 && batch <= (1 << 20) && nodes > 0 && nodes <= kTreeMaxNodes && parents_ld >= nodes,
+             "invalid tree shape (at most 64 nodes)");
+  IW_REQUIRE(max_positions > 0, "max_positions must be positive");
+  if (batch == 0) return IW_OK;
+  IW_REQUIRE(parents && visible, "null tensor pointer");
+  return launch_tree_plan(parents, parents_ld, counts, lengths, batch, (int)nodes, max_positions,
+                          reinterpret_cast<uint64_t *>(visible), positions, as_stream(stream));
+}
+
+int iw_attention_tree(const int8_t *q, int64_t q_sb, int64_t q_st, const int8_t *k_new, int64_t kn_sb,
+                      int64_t kn_st, const int8_t *v_new, int64_t vn_sb, int64_t vn_st, const int8_t *k,
+                      int64_t k_sb, int64_t k_sh, int64_t k_st, const int8_t *vt, int64_t v_sb, int64_t v_sh,
+                      int64_t v_sd, int64_t v_sq, const int32_t *lengths, const int64_t *visible,
+                      int64_t visible_sb, const int32_t *counts, int8_t *out, int64_t o_sb, int64_t o_st,
+                      int64_t batch, int64_t heads, int64_t nodes, int64_t head_dim, int64_t cache_positions,
+                      uint8_t qk_multiplier, int8_t qk_shift, int32_t frac_bits, uint8_t av_multiplier,
+                      int8_t av_shift, uint32_t rsqrt_offset, iw_stream_t stream) {
+  IW_REQUIRE(frac_bits > 0 && frac_bits < 14, "frac_bits must be in [1, 14)");
+  IW_REQUIRE(rsqrt_offset <= 29, "rsqrt_offset must be in [0,29]");
+  IW_REQUIRE(nodes > 0 && nodes <= kTreeMaxNodes, "a tree has 1 to 64 nodes");
+  const int rc = check_tree_cache(heads, head_dim, cache_positions, v_sd, v_sq);
+  if (rc) return rc;
+  IW_REQUIRE(batch >= 0 && batch * heads <= (1 << 22) && visible_sb >= 0, "invalid attention shape");
+  if (batch == 0) return IW_OK;
+  IW_REQUIRE(q && k_new && v_new && k && vt && lengths && visible && out, "null tensor pointer");
+  const uintptr_t align =
+      reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new) |
+      reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(vt) | reinterpret_cast<uintptr_t>(out) |
+      (uintptr_t)(q_sb | q_st | kn_sb | kn_st | vn_sb | vn_st | k_sb | k_sh | k_st | v_sb | v_sh | o_sb | o_st) |
+      (uintptr_t)(v_sq != 4 ? v_sq : v_sd);
+  IW_REQUIRE((align & 15) == 0, "tree attention operands must be 16-byte aligned");
+  TreeArgs t;
+  AttnArgs &a = t.a;
+  a.q = q;
+  a.q_sb = q_sb;
+  a.q_st = q_st;
+  a.k = k;
+  a.k_sb = k_sb;
+  a.k_sh = k_sh;
+  a.k_st = k_st;
+  a.vt = vt;
+  a.v_sb = v_sb;
+  a.v_sh = v_sh;
+  a.v_sd = v_sd;
+  a.v_sq = v_sq;
+  a.out = out;
+  a.o_sb = o_sb;
+  a.o_st = o_st;
+  a.B = (int32_t)batch;
+  a.H = (int32_t)heads;
+  a.Tq = (int32_t)nodes;
+  a.Tk = (int32_t)cache_positions;
+  a.D = (int32_t)head_dim;
+  a.qk_m = qk_multiplier;
+  a.qk_s = (uint32_t)(qk_shift > 0 ? qk_shift : 0);
+  a.frac_bits = frac_bits;
+  a.av_m = av_multiplier;
+  a.av_s = (uint32_t)(av_shift < 0 ? 0 : (av_shift > 32 ? 32 : av_shift));
+  a.rsqrt_off = rsqrt_offset;
+  t.kn = k_new;
+  t.kn_sb = kn_sb;
+  t.kn_st = kn_st;
+  t.vn = v_new;
+  t.vn_sb = vn_sb;
+  t.vn_st = vn_st;
+  t.lengths = lengths;
+  t.visible = reinterpret_cast<const uint64_t *>(visible);
+  t.vis_sb = visible_sb;
+  t.counts = counts;
+  return launch_attn_tree(t, as_stream(stream));
+}
+
+int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t *choice, const int32_t *counts,
+                   const int32_t *lengths, int64_t batch, int64_t nodes, int64_t eot, int32_t *path,
+                   int32_t *accepted, int64_t *next, int32_t *lengths_out, int64_t layers,
+                   const int8_t *const *k_new, const int8_t *const *v_new, int64_t kn_sb, int64_t kn_st,
+                   int64_t vn_sb, int64_t vn_st, int8_t *const *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                   int8_t *const *v, int64_t v_sb, int64_t v_sh, int64_t v_sd, int64_t v_sq, int64_t heads,
+                   int64_t head_dim, int64_t cache_positions, iw_stream_t stream) {
+  IW_REQUIRE(batch >= 0 && batch <= (1 << 20) && nodes > 0 && nodes <= kTreeMaxNodes,
+             "invalid tree shape (at most 64 nodes)");
+  IW_REQUIRE(layers >= 0 && layers <= 4096, "invalid number of layers");
+  const int rc = check_tree_cache(heads, head_dim, cache_positions, v_sd, v_sq);
+  if (rc) return rc;
+  if (batch == 0) return IW_OK;
+  IW_REQUIRE(tokens && parents && choice && lengths && path && accepted && next && lengths_out, "null tensor pointer");
+  // the blocks of a row's layers read its length while one of them writes the new one
+  IW_REQUIRE(apart(lengths, 4 * batch, lengths_out, 4 * batch), "lengths_out must not be part of lengths");
+  IW_REQUIRE(layers == 0 || (k_new && v_new && k && v), "null array of layer pointers");
+  uintptr_t align = (uintptr_t)(kn_sb | kn_st | vn_sb | vn_st | k_sb | k_sh | k_st);
+  for (int64_t i = 0; i < layers; ++i) {
+    IW_REQUIRE(k_new[i] && v_new[i] && k[i] && v[i], "null tensor pointer");
+    align |= reinterpret_cast<uintptr_t>(k_new[i]) | reinterpret_cast<uintptr_t>(v_new[i]) |
+             reinterpret_cast<uintptr_t>(k[i]);
+  }
+  IW_REQUIRE((align & 3) == 0, "the nodes' K and V and the K caches must be 4-byte aligned");
+  TreeAcceptArgs t;
+  t.tokens = tokens;
+  t.choice = choice;
+  t.parents = parents;
+  t.counts = counts;
+  t.lengths = lengths;
+  t.tok_ld = t.ch_ld = t.p_ld = nodes;
+  t.eot = eot;
+  t.path = path;
+  t.accepted = accepted;
+  t.next = next;
+  t.lengths_out = lengths_out;
+  t.nodes = (int)nodes;
+  t.cap = (int)cache_positions;
+  t.heads = (int)heads;
+  t.D = (int)head_dim;
+  t.kn_sb = kn_sb;
+  t.kn_st = kn_st;
+  t.vn_sb = vn_sb;
+  t.vn_st = vn_st;
+  t.k_sb = k_sb;
+  t.k_sh = k_sh;
+  t.k_st = k_st;
+  t.v_sb = v_sb;
+  t.v_sh = v_sh;
+  t.v_sd = v_sd;
+  t.v_sq = v_sq;
+  int64_t first = 0;
+  do {
+    const int n = (int)(layers - first < kTreeMaxLayers ? layers - first : kTreeMaxLayers);
+    TreeLayers l = {};
+    for (int i = 0; i < n; ++i) {
+      l.kn[i] = k_new[first + i];
+      l.vn[i] = v_new[first + i];
+      l.k[i] = k[first + i];
+      l.v[i] = v[first + i];
+    }
+    const int r = launch_tree_accept(t, l, n, batch, first == 0, as_stream(stream));
+    if (r) return r;
+    first += n;
+  } while (first < layers);
+  return IW_OK;
+}
+
+int64_t iw_token_logprobs_workspace(int64_t rows, int64_t cols, int64_t top) {
+  if (rows < 0 || cols < 0 || top < 0) return -1;
+  return score_workspace(rows, cols, top);
+}
+
+int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t cols, int64_t ld, float scale,
+                      const uint32_t *suppress, const int64_t *targets, float *logprob, float *entropy,
+                      int64_t top, int64_t *top_ids, float *top_logprobs, void *workspace, iw_stream_t stream) {
+  IW_REQUIRE(type >= LOGIT_I8 && type <= LOGIT_F16, "logits must be int8, float32, bfloat16 or float16");
+  IW_REQUIRE(rows >= 0 && rows <= (1 << 22) && cols > 0 && cols < (1 << 23) && ld >= cols,
+             "invalid logits shape (at most 2^22 rows of 2^23 - 1 columns)");
+  IW_REQUIRE(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
+  IW_REQUIRE(top >= 0 && top <= kScoreMaxTop && top <= cols, "top must be at most 32 and at most cols");
+  if (rows == 0) return IW_OK;
+  IW_REQUIRE(logits && (targets != nullptr) == (logprob != nullptr) && (top == 0 || (top_ids && top_logprobs)),
+             "null tensor pointer");
+  const uintptr_t item = type == LOGIT_I8 ? 1 : type == LOGIT_F32 ? 4 : 2;
+  IW_REQUIRE(reinterpret_cast<uintptr_t>(logits) % item == 0, "logits must be aligned to their type");
+  IW_REQUIRE(score_workspace(rows, cols, top) == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+             "iw_token_logprobs_workspace bytes of 16-byte aligned workspace are needed");
+  ScoreArgs a;
+  a.x = logits;
+  a.type = type;
+  a.rows = rows;
+  a.ld = ld;
+  a.cols = (int)cols;
+  a.scale = scale;
+  a.suppress = suppress;
+  a.targets = targets;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.top = (int)top;
+  a.top_ids = top_ids;
+  a.top_lp = top_logprobs;
+  a.workspace = workspace;
+  return launch_token_scores(a, as_stream(stream));
 }
 
 // ---- fragment-major decode operands ----

@@ -1,0 +1,388 @@
+"""Drafted tokens: several of them per row verified in one decoder pass, and tokens scored.
+
+The reference decodes one token per row and step (decoding.py:684-712). Here a
+row may bring a tree of up to 64 drafted tokens (of a smaller model, of an
+earlier window, of a beam); one pass through the decoder gives the model's
+choice after each of them, and the longest path of drafts that the model
+would have chosen itself is accepted. Greedy decoding over integer kernels is
+reproducible bit for bit, so the tokens are those of ``greedy_decode``.
+
+* ``tree_plan``       which node sees which, and each node's position
+* ``tree_attention``  the nodes' attention over the int8 KV caches and the tree
+* ``TreeCaches``      accepts a path: K and V of its nodes enter every layer's cache
+* ``token_logprobs``  log-probabilities of given tokens, entropy, best alternatives
+* ``TreeDecoder``     the pass itself, over a DecoderRunner's model and caches
+
+Node 0 of a row's tree is its last chosen token, whose keys and values are not
+in the caches yet; node i hangs on node ``parents[b, i] < i``. Work is queued
+on the current stream of the tensors' device and reads nothing back, so every
+call can be captured into a graph. Wrong dtypes, shapes and layouts raise
+RuntimeError.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _lib
+from .runtime import DecoderRunner, _ln, _lin8, _lin32_res, _mlp_gelu
+
+Tensor = torch.Tensor
+
+MAX_NODES = 64
+MAX_TOP = 32
+_LOGIT_TYPES = {torch.int8: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+
+
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Call an entry point on the current stream of ``dev``, the tensors' device."""
+    if dev.index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, _lib.stream())
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _lib.stream())
+
+
+def _check(t: Tensor, dtype: torch.dtype, shape: Sequence[int], name: str, dev: Optional[torch.device] = None,
+           contiguous: bool = True) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a GPU tensor, got device {t.device}")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {str(dtype).replace('torch.', '')}, got {t.dtype}")
+    if t.shape != shape:
+        raise RuntimeError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+    if dev is not None and t.device != dev:
+        raise RuntimeError(f"{name} is on {t.device}, the other tensors on {dev}")
+    if contiguous and not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _rows_strides(t: Tensor, shape, name: str, dev: torch.device):
+    """(batch, node) strides of an int8 [B, N, H * D] operand with contiguous rows."""
+    _check(t, torch.int8, shape, name, dev, contiguous=False)
+    sb, st, sc = t.stride()
+    if sc != 1:
+        raise RuntimeError(f"the rows of {name} must be contiguous")
+    return (sb if shape[0] > 1 else 0), (st if shape[1] > 1 else 0)
+
+
+def _cache_strides(k: Tensor, v: Tensor, B: int, H: int, D: int, dev: torch.device):
+    """Positions and strides (k_sb, k_sh, k_st), (v_sb, v_sh, v_sd, v_sq) of a layer's caches: K
+    [B, H, T, D], V in key quads [B, H, ceil(T / 4), D, 4] or transposed [B, H, D, round_up(T, 16)]."""
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise RuntimeError("k_cache must be [batch, heads, positions, head_dim]")
+    T = k.shape[2]
+    _check(k, torch.int8, (B, H, T, D), "k_cache", dev, contiguous=False)
+    if not isinstance(v, torch.Tensor) or v.dim() not in (4, 5):
+        raise RuntimeError("v_cache must be key quads [batch, heads, quads, head_dim, 4] or transposed "
+                           "[batch, heads, head_dim, positions]")
+    ks, vs = k.stride(), v.stride()
+    if v.dim() == 5:
+        quads = v.shape[2]
+        _check(v, torch.int8, (B, H, quads, D, 4), "v_cache", dev, contiguous=False)
+        if 4 * quads < T or vs[4] != 1 or vs[3] != 4:
+            raise RuntimeError("v_cache: packed key quads that cover every position of k_cache are needed")
+        v_sd, v_sq = 4, (vs[2] if quads > 1 else 4 * D)
+    else:
+        _check(v, torch.int8, (B, H, D, v.shape[3]), "v_cache", dev, contiguous=False)
+        if v.shape[3] < (T + 15) // 16 * 16 or vs[3] != 1:
+            raise RuntimeError("v_cache: transposed rows must cover the positions of k_cache rounded up to 16")
+        v_sd, v_sq = vs[2], 4
+    if ks[3] != 1:
+        raise RuntimeError("the rows of k_cache must be contiguous")
+    return (T, (ks[0] if B > 1 else 0, ks[1] if H > 1 else 0, ks[2] if T > 1 else 0),
+            (vs[0] if B > 1 else 0, vs[1] if H > 1 else 0, v_sd, v_sq))
+
+
+def _tree_shape(t: Tensor, name: str):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or not 1 <= t.shape[1] <= MAX_NODES:
+        raise RuntimeError(f"{name} must be [batch, nodes] with 1 to {MAX_NODES} nodes")
+    return t.shape
+
+
+class TreePlan(NamedTuple):
+    visible: Tensor    # int64 [B, N]: bit j of a node's word = it sees node j
+    positions: Tensor  # int32 [B, N]: the row's length plus the node's depth
+
+
+def tree_plan(parents: Tensor, counts: Optional[Tensor] = None, *, lengths: Optional[Tensor] = None,
+              max_positions: int = 2 ** 31 - 1) -> TreePlan:
+    """Which nodes a node sees (itself and its ancestors) and its position.
+
+    ``parents`` int32 [B, N] (a parent outside [0, i) makes node i a root);
+    ``counts`` int32 [B]: nodes in use, the others see nothing and sit at the
+    row's length; ``lengths`` int32 [B]: cached tokens. Positions stay below
+    ``max_positions``."""
+    B, N = _tree_shape(parents, "parents")
+    _check(parents, torch.int32, (B, N), "parents")
+    dev = parents.device
+    for t, name in ((counts, "counts"), (lengths, "lengths")):
+        if t is not None:
+            _check(t, torch.int32, (B,), name, dev)
+    visible = torch.empty((B, N), dtype=torch.int64, device=dev)
+    positions = torch.empty((B, N), dtype=torch.int32, device=dev)
+    _launch(dev, "iw_tree_plan", parents.data_ptr(), N, _ptr(counts), _ptr(lengths), B, N, max_positions,
+            visible.data_ptr(), positions.data_ptr())
+    return TreePlan(visible, positions)
+
+
+def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor,
+                   visible: Tensor, counts: Optional[Tensor] = None, *, heads: int, qk_multiplier: int,
+                   qk_shift: int, frac_bits: int, av_multiplier: int, av_shift: int, rsqrt_offset: int = 16,
+                   out: Optional[Tensor] = None) -> Tensor:
+    """Integer attention (model_int.py:774-1040) of each row's nodes over its first ``lengths[b]``
+    cached keys and the nodes of ``visible`` (``tree_plan``; [B, N], or [N] for one tree of all rows).
+
+    ``q``, ``k_new``, ``v_new`` int8 [B, N, heads * D], also as columns of one fused projection;
+    ``k_cache`` int8 [B, heads, T, D]; ``v_cache`` in key quads [B, heads, ceil(T / 4), D, 4] or transposed
+    [B, heads, D, round_up(T, 16)]. D is a multiple of 16 up to 128, strides are multiples of 16.
+    Lengths and counts are clamped to T and N on the device. Returns int8 [B, N, heads * D] (``out`` where
+    given); nodes past ``counts[b]`` and nodes that see no key give zeros. With one node a row it is a
+    decode step over rows of different lengths."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or not 1 <= q.shape[1] <= MAX_NODES:
+        raise RuntimeError(f"q must be [batch, nodes, heads * head_dim] with 1 to {MAX_NODES} nodes")
+    shape, dev = q.shape, q.device
+    B, N, C = shape
+    if heads <= 0 or C % heads:
+        raise RuntimeError("q.size(2) must be a multiple of heads")
+    D = C // heads
+    q_s = _rows_strides(q, shape, "q", dev)
+    kn_s = _rows_strides(k_new, shape, "k_new", dev)
+    vn_s = _rows_strides(v_new, shape, "v_new", dev)
+    T, k_s, v_s = _cache_strides(k_cache, v_cache, B, heads, D, dev)
+    _check(lengths, torch.int32, (B,), "lengths", dev)
+    shared = isinstance(visible, torch.Tensor) and visible.dim() == 1
+    _check(visible, torch.int64, (N,) if shared else (B, N), "visible", dev)
+    if counts is not None:
+        _check(counts, torch.int32, (B,), "counts", dev)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int8, device=dev)
+        o_s = (N * C, C)
+    else:
+        o_s = _rows_strides(out, shape, "out", dev)
+        if (B > 1 and o_s[0] < C) or (N > 1 and o_s[1] < C):
+            raise RuntimeError("the rows of out must not overlap")
+    _launch(dev, "iw_attention_tree", q.data_ptr(), *q_s, k_new.data_ptr(), *kn_s, v_new.data_ptr(), *vn_s,
+            k_cache.data_ptr(), *k_s, v_cache.data_ptr(), *v_s, lengths.data_ptr(), visible.data_ptr(),
+            0 if shared else N, _ptr(counts), out.data_ptr(), *o_s, B, heads, N, D, T, qk_multiplier, qk_shift,
+            frac_bits, av_multiplier, av_shift, rsqrt_offset)
+    return out
+
+
+class TreeAccept(NamedTuple):
+    path: Tensor        # int32 [B, N]: the accepted nodes, then -1
+    accepted: Tensor    # int32 [B]: their number (0 for a row without nodes or room)
+    next_token: Tensor  # int64 [B]: the model's choice after the last of them, -1 for none
+    lengths: Tensor     # int32 [B]: the rows' lengths with the path cached
+
+
+class TreeCaches:
+    """The layers' caches and the nodes' K and V that a decoder pass leaves for them.
+
+    Lists of one tensor per layer, all with the same shapes and strides:
+    ``k_new`` / ``v_new`` int8 [B, N, heads * D] (columns of the projection
+    that the pass writes) and the caches as ``tree_attention`` takes them."""
+
+    def __init__(self, k_new: Sequence[Tensor], v_new: Sequence[Tensor], k_cache: Sequence[Tensor],
+                 v_cache: Sequence[Tensor], *, heads: int):
+        self.tensors = [list(x) for x in (k_new, v_new, k_cache, v_cache)]
+        L = len(self.tensors[0])
+        if L == 0 or any(len(x) != L for x in self.tensors):
+            raise RuntimeError("one k_new, v_new, k_cache and v_cache of each layer are needed")
+        kn, vn, k, v = (x[0] for x in self.tensors)
+        if not isinstance(kn, torch.Tensor) or kn.dim() != 3 or not 1 <= kn.shape[1] <= MAX_NODES:
+            raise RuntimeError(f"k_new must be [batch, nodes, heads * head_dim] with 1 to {MAX_NODES} nodes")
+        self.batch, self.nodes, C = shape = kn.shape
+        if heads <= 0 or C % heads:
+            raise RuntimeError("k_new.size(2) must be a multiple of heads")
+        self.device = dev = kn.device
+        B, D = self.batch, C // heads
+        self._new = (*_rows_strides(kn, shape, "k_new", dev), *_rows_strides(vn, shape, "v_new", dev))
+        self.positions, k_s, v_s = _cache_strides(k, v, B, heads, D, dev)
+        for kn_l, vn_l, k_l, v_l in zip(*self.tensors):
+            same = (_rows_strides(kn_l, shape, "k_new", dev) + _rows_strides(vn_l, shape, "v_new", dev) == self._new
+                    and _cache_strides(k_l, v_l, B, heads, D, dev) == (self.positions, k_s, v_s))
+            if not same:
+                raise RuntimeError("the layers' tensors must have the same strides")
+        caches = self.tensors[2] + self.tensors[3]
+        if len({t.data_ptr() for t in caches}) != len(caches) or any(
+                0 in [s for s, n in zip(t.stride(), t.shape) if n > 1] for t in caches):
+            raise RuntimeError("the caches are written: each must be memory of its own")
+        arrays = [(ctypes.c_void_p * L)(*[t.data_ptr() for t in x]) for x in self.tensors]
+        self._layers = (L, arrays[0], arrays[1], *self._new, arrays[2], *k_s, arrays[3], *v_s, heads, D, self.positions)
+
+    def accept(self, tokens: Tensor, parents: Tensor, choice: Tensor, lengths: Tensor,
+               counts: Optional[Tensor] = None, *, eot: int = -1) -> TreeAccept:
+        """Greedy acceptance: from node 0 on, the first node that hangs on the current one and
+        holds the model's choice after it, until there is none, the choice is ``eot`` or the cache is
+        full. K and V of the path enter every layer's cache at ``lengths[b]`` and up.
+
+        ``tokens`` int64, ``parents`` int32, ``choice`` int64 (the model's token after each node,
+        ``token_logprobs(..., top=1).top_ids``) [B, N]; ``lengths`` and ``counts`` int32 [B]."""
+        dev, B, N = self.device, self.batch, self.nodes
+        shape = (B, N)
+        _check(tokens, torch.int64, shape, "tokens", dev)
+        _check(parents, torch.int32, shape, "parents", dev)
+        _check(choice, torch.int64, shape, "choice", dev)
+        _check(lengths, torch.int32, (B,), "lengths", dev)
+        if counts is not None:
+            _check(counts, torch.int32, (B,), "counts", dev)
+        path = torch.empty(shape, dtype=torch.int32, device=dev)
+        accepted, after = torch.empty((2, B), dtype=torch.int32, device=dev)
+        next_token = torch.empty(B, dtype=torch.int64, device=dev)
+        _launch(dev, "iw_tree_accept", tokens.data_ptr(), parents.data_ptr(), choice.data_ptr(), _ptr(counts),
+                lengths.data_ptr(), B, N, eot, path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(),
+                after.data_ptr(), *self._layers)
+        return TreeAccept(path, accepted, next_token, after)
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: Optional[Tensor]       # float32 [...]: of the targets; None without them
+    entropy: Tensor                 # float32 [...]
+    top_ids: Optional[Tensor]       # int64 [..., top]; None for top 0
+    top_logprobs: Optional[Tensor]  # float32 [..., top]
+
+
+def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, top: int = 0, scale: float = 1.0,
+                   suppress: Optional[Tensor] = None) -> TokenLogprobs:
+    """Scores of rows of logits [..., vocab] (int8, float32, bfloat16 or float16), in float32.
+
+    The real logits are ``logits * scale`` (for a decoder's int8 logits
+    1 / act_logits_alpha); ``suppress`` is a bit mask of tokens that count as
+    -inf (int32 or uint32 words, bit i % 32 of word i // 32, as the runners' filters hold it).
+    ``targets`` int64 [...]: tokens whose log-probability is asked for, NaN for one outside
+    the vocabulary. ``top`` (at most 32): the most probable tokens in order,
+    ties to the lowest index. A row with a NaN or +inf, or without a finite logit, has NaN scores."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() < 1:
+        raise RuntimeError("logits must be a GPU tensor [..., vocab]")
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    if kind is None:
+        raise RuntimeError(f"logits must be int8, float32, bfloat16 or float16, got {logits.dtype}")
+    dev, lead, V = logits.device, logits.shape[:-1], logits.shape[-1]
+    if logits.dim() != 2:
+        logits = logits.reshape(-1, V)
+    rows = logits.shape[0]
+    ld = logits.stride(0) if rows > 1 else V
+    if logits.stride(1) != 1 and V > 1 or ld < V:
+        logits = logits.contiguous()
+        ld = V
+    if not 0 <= top <= min(MAX_TOP, V):
+        raise RuntimeError(f"top must be in [0, {min(MAX_TOP, V)}]")
+    logprob = ids = lps = None
+    if targets is not None:
+        _check(targets, torch.int64, lead, "targets", dev, contiguous=False)
+        targets = targets.contiguous()
+        logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+    if suppress is not None:
+        if not isinstance(suppress, torch.Tensor) or suppress.dtype not in (torch.int32, torch.uint32):
+            raise RuntimeError("suppress must be int32 or uint32 words")
+        _check(suppress, suppress.dtype, ((V + 31) // 32,), "suppress", dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    if top:
+        ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+        lps = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+    need = _lib.value("iw_token_logprobs_workspace", rows, V, top)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _launch(dev, "iw_token_logprobs", logits.data_ptr(), kind, rows, V, ld, scale, _ptr(suppress), _ptr(targets),
+            _ptr(logprob), entropy.data_ptr(), top, _ptr(ids), _ptr(lps), _ptr(work))
+    return TokenLogprobs(logprob, entropy, ids, lps)
+
+
+class TreeStep(NamedTuple):
+    accept: TreeAccept
+    scores: TokenLogprobs  # of every node's logits [B, N]: top_ids[..., 0] is the model's choice
+    logits: Tensor         # int8 [B, N, vocab]
+
+
+class TreeDecoder:
+    """Decoder passes over trees of drafted tokens, with a DecoderRunner's model and caches.
+
+    Call ``runner.set_audio``, then ``start`` with the prompt, then ``step`` with each
+    round of trees. The rows advance by different numbers of tokens (``lengths``), so the
+    runner's own one-token steps are not mixed in before its next ``run``. The runner has
+    no logit filters: the choices are the plain first-index argmax."""
+
+    def __init__(self, runner: DecoderRunner, nodes: int):
+        if runner.filters is not None:
+            raise ValueError("tree decoding takes a runner built without logit filters")
+        if not 1 <= nodes <= MAX_NODES:
+            raise ValueError(f"a tree has 1 to {MAX_NODES} nodes")
+        self.runner, self.nodes = runner, nodes
+        r, dec = runner, runner.dec
+        B, C, H, D = r.B, r.C, r.H, r.D
+        self.M = M = B * nodes
+        dev = dec.positional_embedding.device
+        i8 = dict(dtype=torch.int8, device=dev)
+        # every layer's projection is kept until a path of it is accepted
+        self.qkv = [torch.empty((B, nodes, 3 * C), **i8) for _ in dec.blocks]
+        v_shape = (B, H, r.tcap16 // 4, D, 4) if r.v_quads else (B, H, D, r.tcap16)
+        self.v_cache = [v.view(v_shape) for v in r.v_self]
+        self.caches = TreeCaches([t[..., C:2 * C] for t in self.qkv], [t[..., 2 * C:] for t in self.qkv], r.k_self,
+                                 self.v_cache, heads=H)
+        self.x16 = torch.empty((M, C), dtype=torch.int16, device=dev)
+        self.h8 = torch.empty((M, C), **i8)
+        self.wv = torch.empty((B, nodes, C), **i8)
+        self.qc = torch.empty((M, C), **i8)
+        self.f8 = torch.empty((M, 4 * C), **i8)
+        self.lengths = torch.zeros(B, dtype=torch.int32, device=dev)
+
+    def start(self, prompt: Tensor) -> Tensor:
+        """The prompt step: returns each row's first token [B] (node 0 of its first tree)."""
+        r = self.runner
+        r.run(prompt, 1)
+        self.lengths = torch.full((r.B,), prompt.shape[1], dtype=torch.int32, device=prompt.device)
+        return r.tokens.clone()
+
+    def verify(self, tokens: Tensor, parents: Tensor, counts: Optional[Tensor] = None) -> Tensor:
+        """int8 logits [B, N, vocab] after every node; the caches stay as they are."""
+        r, dec, N, M = self.runner, self.runner.dec, self.nodes, self.M
+        B, C, H = r.B, r.C, r.H
+        dev = self.lengths.device
+        _check(tokens, torch.int64, (B, N), "tokens", dev)
+        _check(parents, torch.int32, (B, N), "parents", dev)
+        plan = tree_plan(parents, counts, lengths=self.lengths, max_positions=dec.n_ctx)
+        # unused nodes may hold any value
+        emb = dec.token_embedding.weight[tokens.clamp(0, dec.n_vocab - 1)]
+        pe = dec.positional_embedding[plan.positions]
+        sc0 = dec.scalars()
+        x16, h8, wv = self.x16, self.h8, self.wv
+        _launch(dev, "iw_add_requant15", emb.data_ptr(), pe.data_ptr(), sc0["m16"].data_ptr(), sc0["s"].data_ptr(),
+                x16.data_ptr(), 1, M, C, 1, 1)
+        for l, blk in enumerate(dec.blocks):
+            sc, s = blk._scalars(), blk.attn._scalars()
+            _ln(blk.attn_ln, x16, M, h8)
+            qkv = r.self_qkv[l].linear8(h8, M, self.qkv[l])
+            tree_attention(qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:], r.k_self[l], self.v_cache[l],
+                           self.lengths, plan.visible, counts, heads=H, qk_multiplier=s["qm"], qk_shift=s["qs"],
+                           frac_bits=s["f"], av_multiplier=s["am"], av_shift=s["as_"],
+                           rsqrt_offset=blk.attn.rsqrt_offset, out=wv)
+            _lin32_res(blk.attn.out, wv.data_ptr(), M, x16, sc["a"])
+            _ln(blk.cross_attn_ln, x16, M, h8)
+            _lin8(blk.cross_attn.query, h8.data_ptr(), M, self.qc)
+            r._cross_attend(blk.cross_attn, l, self.qc.data_ptr(), N * C, C, N, wv, r.cross_tables[l])
+            _lin32_res(blk.cross_attn.out, wv.data_ptr(), M, x16, sc["c"])
+            _ln(blk.mlp_ln, x16, M, h8)
+            _mlp_gelu(blk, h8.data_ptr(), M, self.f8)
+            _lin32_res(blk.mlp[2], self.f8.data_ptr(), M, x16, sc["m"])
+        _ln(dec.ln, x16, M, h8)
+        return dec.classify(h8.view(B, N, C))
+
+    def step(self, tokens: Tensor, parents: Tensor, counts: Optional[Tensor] = None, *, top: int = 1,
+             eot: int = -1) -> TreeStep:
+        """One round: ``verify``, the choices and their ``top`` alternatives, and the accepted paths."""
+        if top < 1:
+            raise ValueError("top must be at least 1")
+        logits = self.verify(tokens, parents, counts)
+        scores = token_logprobs(logits, top=top, scale=self.runner.logit_scale)
+        choice = scores.top_ids[..., 0].contiguous()
+        got = self.caches.accept(tokens, parents, choice, self.lengths, counts, eot=eot)
+        self.lengths = got.lengths
+        return TreeStep(got, scores, logits)

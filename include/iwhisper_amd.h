@@ -597,6 +597,86 @@ int iw_dtw(const float *x, int64_t rows, int64_t cols, int64_t ld, int8_t *trace
 int iw_median_filter(const float *x, int64_t rows, int64_t cols, int64_t ld, int32_t width, float *y,
                      int64_t y_ld, iw_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Trees of drafted tokens over the KV caches, and token scores. No
+ * counterpart in the reference, whose decoder takes one token per row and
+ * step (decoding.py:684-712): these verify up to 64 drafted tokens of each row
+ * in one decoder pass. Node 0 of a row's tree is its last chosen token, whose
+ * K and V are not in the caches yet; node i hangs on node parents[i] < i.
+ * Every row has its own number of cached keys (lengths) and of nodes in use
+ * (counts, NULL = all); both are read on the device and clamped to the sizes
+ * given here.
+ * ------------------------------------------------------------------------- */
+
+/* The plan of a tree: visible[b][i] (contiguous [batch][nodes]) has bit j set
+ * for node i itself and its ancestors, 0 for nodes past the count;
+ * positions[b][i] (or NULL) = min(lengths[b] + depth of i, max_positions - 1),
+ * depth 0 for nodes past the count. parents [batch][nodes] with row stride
+ * parents_ld; a parent outside [0, i) makes node i a root. lengths NULL = 0.
+ * nodes <= 64. */
+int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *counts, const int32_t *lengths,
+                 int64_t batch, int64_t nodes, int32_t max_positions, int64_t *visible, int32_t *positions,
+                 iw_stream_t stream);
+
+/* Attention of a tree's nodes: node i of row b attends to the cached keys
+ * 0 .. lengths[b] - 1 and to the nodes j of visible[b * visible_sb + i] that are
+ * in use (visible_sb 0 = one tree for every row). q, k_new and v_new: element
+ * (b, i, h, d) at base + b*sb + i*st + h*head_dim + d (columns of one fused
+ * projection); caches and scalars as iw_attention_decode_cache takes them, V
+ * transposed (v_sq == 4, v_sd >= round_up(cache_positions, 16)) or in key
+ * quads (v_sd == 4); out (b, i) at out + b*o_sb + i*o_st. Rows of nodes past
+ * the count, and of nodes that see no key, are zeros. nodes <= 64,
+ * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24; operands and
+ * strides are multiples of 16 bytes. The caches are read only: the nodes' K and V
+ * enter them with iw_tree_accept. */
+int iw_attention_tree(const int8_t *q, int64_t q_sb, int64_t q_st, const int8_t *k_new, int64_t kn_sb,
+                      int64_t kn_st, const int8_t *v_new, int64_t vn_sb, int64_t vn_st, const int8_t *k,
+                      int64_t k_sb, int64_t k_sh, int64_t k_st, const int8_t *vt, int64_t v_sb, int64_t v_sh,
+                      int64_t v_sd, int64_t v_sq, const int32_t *lengths, const int64_t *visible,
+                      int64_t visible_sb, const int32_t *counts, int8_t *out, int64_t o_sb, int64_t o_st,
+                      int64_t batch, int64_t heads, int64_t nodes, int64_t head_dim, int64_t cache_positions,
+                      uint8_t qk_multiplier, int8_t qk_shift, int32_t frac_bits, uint8_t av_multiplier,
+                      int8_t av_shift, uint32_t rsqrt_offset, iw_stream_t stream);
+
+/* Greedy acceptance: from node 0, the path goes on to the first node in use
+ * whose parent is the current node and whose token is choice[current] (the
+ * model's token after it), until there is none, the choice is eot (eot >= 0)
+ * or the cache is full. tokens, parents, choice: [batch][nodes] contiguous.
+ * path [batch][nodes]: its nodes, then -1; accepted [batch]: their number (0
+ * for a row without nodes or room); next [batch]: the choice after the last of
+ * them (-1 for 0); lengths_out = lengths + accepted (no part of lengths). The
+ * path's K and V of every layer are written to cache positions lengths[b] ..:
+ * k_new / v_new / k / v are host arrays of `layers` device pointers with one
+ * set of strides (layouts as iw_attention_tree, multiples of 4 bytes; read
+ * during the call). layers may be 0. */
+int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t *choice, const int32_t *counts,
+                   const int32_t *lengths, int64_t batch, int64_t nodes, int64_t eot, int32_t *path,
+                   int32_t *accepted, int64_t *next, int32_t *lengths_out, int64_t layers,
+                   const int8_t *const *k_new, const int8_t *const *v_new, int64_t kn_sb, int64_t kn_st,
+                   int64_t vn_sb, int64_t vn_st, int8_t *const *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                   int8_t *const *v, int64_t v_sb, int64_t v_sh, int64_t v_sd, int64_t v_sq, int64_t heads,
+                   int64_t head_dim, int64_t cache_positions, iw_stream_t stream);
+
+/* Scores of rows of logits (row stride ld) of a type below, real logit = value *
+ * scale (> 0), tokens of the bitmask suppress (as iw_greedy_advance_filtered;
+ * or NULL) -inf:
+ *   logprob[r]   log-softmax at targets[r] (both or neither NULL); NaN for a
+ *                target outside the vocabulary
+ *   entropy[r]   -sum p log p (or NULL)
+ *   top_ids, top_logprobs [rows][top], top <= 32: the most probable tokens in
+ *                order, ties to the lowest index; a NaN counts as the largest
+ * A row with a NaN or +inf, or without any finite logit, has NaN scores.
+ * Accumulated in float32. workspace: iw_token_logprobs_workspace bytes,
+ * 16-byte aligned, used during the call's work only (NULL where that is 0). */
+#define IW_LOGITS_INT8 0
+#define IW_LOGITS_FLOAT32 1
+#define IW_LOGITS_BFLOAT16 2
+#define IW_LOGITS_FLOAT16 3
+int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t cols, int64_t ld, float scale,
+                      const uint32_t *suppress, const int64_t *targets, float *logprob, float *entropy,
+                      int64_t top, int64_t *top_ids, float *top_logprobs, void *workspace, iw_stream_t stream);
+int64_t iw_token_logprobs_workspace(int64_t rows, int64_t cols, int64_t top);
+
 /* Per-head gather into a [b][h][t][d] cache (the cross-attention K of
  * model_int.py:722-730, computed once per utterance):
  * dst[b*dst_sb + h*dst_sh + (t_offset+t)*dst_st + d] = src[b*src_sb + t*src_st + h*D + d]. */
