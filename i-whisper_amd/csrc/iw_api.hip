@@ -1058,9 +1058,9 @@ int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t 
   return IW_OK;
 }
 
-int64_t iw_token_logprobs_workspace(int64_t rows, int64_t cols, int64_t top) {
-  if (rows < 0 || cols < 0 || top < 0) return -1;
-  return score_workspace(rows, cols, top);
+int64_t iw_token_logprobs_workspace(int32_t type, int64_t rows, int64_t cols, int64_t top) {
+  if (type < LOGIT_I8 || type > LOGIT_F16 || rows < 0 || cols < 0 || cols >= (1 << 23) || top < 0) return -1;
+  return cols == 0 ? 0 : score_workspace(type, rows, cols, top);
 }
 
 int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t cols, int64_t ld, float scale,
@@ -1076,7 +1076,7 @@ int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t co
              "null tensor pointer");
   const uintptr_t item = type == LOGIT_I8 ? 1 : type == LOGIT_F32 ? 4 : 2;
   IW_REQUIRE(reinterpret_cast<uintptr_t>(logits) % item == 0, "logits must be aligned to their type");
-  IW_REQUIRE(score_workspace(rows, cols, top) == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+  IW_REQUIRE(score_workspace(type, rows, cols, top) == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
              "iw_token_logprobs_workspace bytes of 16-byte aligned workspace are needed");
   ScoreArgs a;
   a.x = logits;

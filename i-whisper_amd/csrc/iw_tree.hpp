@@ -63,7 +63,7 @@ struct ScoreArgs {
   void *workspace = nullptr;
 };
 // bytes of the workspace for rows of cols logits
-int64_t score_workspace(int64_t rows, int64_t cols, int64_t top);
+int64_t score_workspace(int type, int64_t rows, int64_t cols, int64_t top);
 int launch_token_scores(const ScoreArgs &a, hipStream_t s);
 
 }  // namespace iw

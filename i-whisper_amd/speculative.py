@@ -289,7 +289,7 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, top: int
     if top:
         ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
         lps = torch.empty((*lead, top), dtype=torch.float32, device=dev)
-    need = _lib.value("iw_token_logprobs_workspace", rows, V, top)
+    need = _lib.value("iw_token_logprobs_workspace", kind, rows, V, top)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _launch(dev, "iw_token_logprobs", logits.data_ptr(), kind, rows, V, ld, scale, _ptr(suppress), _ptr(targets),
             _ptr(logprob), entropy.data_ptr(), top, _ptr(ids), _ptr(lps), _ptr(work))

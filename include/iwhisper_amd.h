@@ -675,7 +675,7 @@ int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t 
 int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t cols, int64_t ld, float scale,
                       const uint32_t *suppress, const int64_t *targets, float *logprob, float *entropy,
                       int64_t top, int64_t *top_ids, float *top_logprobs, void *workspace, iw_stream_t stream);
-int64_t iw_token_logprobs_workspace(int64_t rows, int64_t cols, int64_t top);
+int64_t iw_token_logprobs_workspace(int32_t type, int64_t rows, int64_t cols, int64_t top);
 
 /* Per-head gather into a [b][h][t][d] cache (the cross-attention K of
  * model_int.py:722-730, computed once per utterance):

@@ -92,9 +92,11 @@ def test_empty_batches_do_nothing(iw):
 
 def test_workspace_size(iw):
     v = iw._lib.value
-    assert v("iw_token_logprobs_workspace", 8, 51865, 32) >= 0
-    assert v("iw_token_logprobs_workspace", 8, 200000, 4) > 0
-    assert v("iw_token_logprobs_workspace", -1, 5, 0) == -1 and v("iw_token_logprobs_workspace", 1, -5, 0) == -1
+    for kind in range(4):
+        assert v("iw_token_logprobs_workspace", kind, 8, 51865, 32) >= 0
+        assert v("iw_token_logprobs_workspace", kind, 8, 200000, 4) > 0
+    for bad in ((0, -1, 5, 0), (0, 1, -5, 0), (0, 1, 5, -1), (4, 1, 5, 0), (-1, 1, 5, 0)):
+        assert v("iw_token_logprobs_workspace", *bad) == -1
 
 
 def i8(*shape):
