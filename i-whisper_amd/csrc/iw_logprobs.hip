@@ -7,15 +7,19 @@
 // both terms are positive and keep their digits where one token holds nearly
 // all of the probability. Alternatives are ordered by value, then by index.
 //
-// A block of 1024 threads holds its part of a row in registers: the logits
-// are read once. The maxima of 64 groups of its threads meet in LDS, which
-// gives every wave m and a bound that at least `top` logits reach; the sums
-// and the few logits that reach the bound follow, and each of those finds
-// its place by counting the larger ones.
+// A block holds its part of a row in registers: the logits are read once. The
+// largest of 64 groups of its threads meet in LDS, which gives every wave m
+// and a bound that at least `top` logits reach; the sums and the few logits
+// that reach the bound follow, and each of those finds its place by counting
+// the larger ones. int8 logits are counted instead, one LDS add each: m, the
+// sums and the exact bound come from the 256 counts, without an exp per logit
+// and in any order the same.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "iw_common.hpp"
 #include "iw_tree.hpp"
@@ -24,10 +28,11 @@ namespace iw {
 
 namespace {
 
-constexpr int NT = 1024, NW = NT / 64;
-constexpr int kPieces = 4096;  // 16-byte pieces of a block's part
-constexpr int kCand = 1024;    // candidates that the bound may leave
+constexpr int kCand = 1024;      // candidates that the bound may leave
+constexpr int kCopies = 4;       // of the int8 counts, for neighbouring lanes
 constexpr int kMaxParts = 1024;  // parts of a row
+constexpr int kPartBytes = 65536;  // of a block, in its registers
+constexpr int kFewBlocks = 256;  // up to here: 1024 threads a block
 
 // One block's part of a row: its largest logit, Z' and U' (in units of s)
 struct Part {
@@ -57,16 +62,25 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t wave_max_u32_dpp(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+  return max(max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+             max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
 // Sum over the wave, in every lane (DPP moves within 16 lanes, then their four sums)
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum_f32(float v) {
-  auto dpp = [](float x, auto ctrl) {
-    return __uint_as_float(
-        (uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, true));
-  };
-  v += dpp(v, std::integral_constant<int, 0xB1>{});
-  v += dpp(v, std::integral_constant<int, 0x4E>{});
-  v += dpp(v, std::integral_constant<int, 0x141>{});
-  v += dpp(v, std::integral_constant<int, 0x140>{});
+  v += dpp_f32<0xB1>(v);
+  v += dpp_f32<0x4E>(v);
+  v += dpp_f32<0x141>(v);
+  v += dpp_f32<0x140>(v);
   const int b = (int)__float_as_uint(v);
   auto at = [&](int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane(b, l)); };
   return (at(0) + at(16)) + (at(32) + at(48));
@@ -77,8 +91,7 @@ __device__ __forceinline__ bool suppressed(const uint32_t *words, int col) {
 }
 
 // The types. A piece is 16 bytes of logits; `off` has the bits of its
-// suppressed ones. Threshold values are 32-bit numbers in the order of the
-// logits, of which `rank_bits` from the top are looked at.
+// suppressed ones.
 template <typename T>
 struct Logit;
 
@@ -90,9 +103,35 @@ struct Logit<int8_t> {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
     return (float)(int8_t)(v[i >> 2] >> (8 * (i & 3)));
   }
+  // the largest in the upper bytes of two 16-bit halves: the odd bytes lead
+  // theirs, the even ones once shifted up
+  typedef int16_t v2s __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ v2s halves(const uint4 &w) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    v2s t{-32768, -32768};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const v2s b = __builtin_bit_cast(v2s, v[q]);
+      t = __builtin_elementwise_max(t, __builtin_elementwise_max(b, (v2s)(b << (int16_t)8)));
+    }
+    return t;
+  }
+  static __device__ __forceinline__ float max(const uint4 &w) {
+    const v2s t = halves(w);
+    return (float)::max(t.x >> 8, t.y >> 8);
+  }
+};
+template <typename D, int N>
+struct FloatMax {
+  static __device__ __forceinline__ float max(const uint4 &w) {
+    float t = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; ++e) t = fmaxf(t, D::get(w, e));
+    return t;
+  }
 };
 template <>
-struct Logit<float> {
+struct Logit<float> : FloatMax<Logit<float>, 4> {
   static constexpr int E = 4;
   static __device__ __forceinline__ float one(const float *p) { return *p; }
   static __device__ __forceinline__ float get(const uint4 &w, int i) {
@@ -117,7 +156,7 @@ struct Half {
   }
 };
 template <>
-struct Logit<__hip_bfloat16> : Half<0xff80u> {
+struct Logit<__hip_bfloat16> : Half<0xff80u>, FloatMax<Logit<__hip_bfloat16>, 8> {
   static __device__ __forceinline__ float one(const __hip_bfloat16 *p) {
     return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(p) << 16);
   }
@@ -127,7 +166,7 @@ struct Logit<__hip_bfloat16> : Half<0xff80u> {
   }
 };
 template <>
-struct Logit<__half> : Half<0xfc00u> {
+struct Logit<__half> : Half<0xfc00u>, FloatMax<Logit<__half>, 8> {
   static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
   static __device__ __forceinline__ float get(const uint4 &w, int i) {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -148,12 +187,13 @@ __device__ __forceinline__ uint32_t kth_largest(uint32_t v, int k) {
   return p;
 }
 
+template <int NT>
 struct Shared {
   uint32_t group[64];
-  float z[NW], u[NW], n[NW];
-  float e[256];  // int8: exp(-y s) of the distances y from m
+  float z[NT / 64], u[NT / 64], n[NT / 64];
+  uint32_t count[256 * kCopies];  // int8: logits of each value
   int cands;
-  uint64_t best[NW];
+  uint64_t best[NT / 64];
   uint64_t cand[kCand];
   uint64_t top[kScoreMaxTop];
 };
@@ -161,8 +201,9 @@ struct Shared {
 // The top alternatives of a block's part one after the other, each the largest
 // key below the last: for rows whose bound leaves too many candidates (whole
 // rows of ties) or too few (suppressed tokens among the alternatives, NaN).
-template <typename T>
-__device__ __noinline__ void top_by_rounds(const T *x, int c0, int n, const uint32_t *suppress, int top, Shared &s) {
+template <typename T, int NT>
+__device__ __noinline__ void top_by_rounds(const T *x, int c0, int n, const uint32_t *suppress, int top,
+                                           Shared<NT> &s) {
   uint64_t prev = ~0ull;
   for (int i = 0; i < top; ++i) {
     uint64_t k = 0;
@@ -175,7 +216,7 @@ __device__ __noinline__ void top_by_rounds(const T *x, int c0, int n, const uint
     if ((threadIdx.x & 63) == 0) s.best[threadIdx.x >> 6] = k;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) k = max64(k, s.best[w]);
+    for (int w = 0; w < NT / 64; ++w) k = max64(k, s.best[w]);
     if (threadIdx.x == 0) s.top[i] = k;  // 0: the part has no more logits
     prev = k;
   }
@@ -200,185 +241,206 @@ __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, float
 // log1p(Z'), NaN where the row has no finite maximum (all suppressed, an infinity, a NaN)
 __device__ __forceinline__ float row_log(float m, float z) { return log1pf(z) + (m - m); }
 
+// What a block works on at a time: the columns c0 .. c0 + n - 1 of a row, as
+// whole 16-byte pieces and up to 2 (E - 1) single logits before and behind them.
 template <typename T>
-__global__ __launch_bounds__(NT) void token_scores_kernel(ScoreArgs a, int chunks, int span) {
+struct Item {
+  const T *x;
+  int64_t row;
+  int c0, n, head, pieces;
+  __device__ __forceinline__ Item(const ScoreArgs &a, int chunks, int span, int64_t i) {
+    row = (uint32_t)i / (uint32_t)chunks;
+    c0 = (int)((uint32_t)i % (uint32_t)chunks) * span;
+    n = min(a.cols - c0, span);
+    x = reinterpret_cast<const T *>(a.x) + row * a.ld + c0;
+    head = min((int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)), n);
+    pieces = (n - head) / Logit<T>::E;
+  }
+};
+
+// P: 16-byte pieces of a thread
+template <typename T, int NT, int P>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ? 8 : 4))) void token_scores_kernel(
+    ScoreArgs a, int chunks, int span) {
   using L = Logit<T>;
   constexpr bool I8 = std::is_same<T, int8_t>::value;
-  constexpr int E = L::E, P = kPieces / NT;
-  __shared__ Shared s;
+  constexpr int E = L::E, NW = NT / 64;
+  __shared__ Shared<NT> s;
+  __shared__ uint32_t sWords[I8 ? 1 : NT * P * E / 32 + 2];  // the part's bits of the suppressed tokens
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x / chunks;
-  const int chunk = blockIdx.x % chunks;
-  const int c0 = chunk * span, n = min(a.cols - c0, span);  // this block's columns
-  const T *x = reinterpret_cast<const T *>(a.x) + row * a.ld + c0;
-  // whole 16-byte pieces, and up to 2 (E - 1) logits before and behind them
-  const int head = min((int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)), n);
-  const int pieces = (n - head) / E, tail0 = head + pieces * E;
-  const uint4 *xa = reinterpret_cast<const uint4 *>(x + head);
+  const int64_t item = blockIdx.x;
+  const Item<T> it(a, chunks, span, item);
+  if (!I8 && a.suppress)  // span is a multiple of 32
+    for (int i = tid; i < (it.n + 31) / 32; i += NT) sWords[i] = a.suppress[it.c0 / 32 + i];
   uint4 w[P];
-#pragma unroll
-  for (int p = 0; p < P; ++p)
-    if (p * NT + tid < pieces) w[p] = xa[p * NT + tid];
-  const int extra = tid < head ? tid : tail0 + tid - head;  // this thread's single logit
-  bool has_extra = extra < n;
-  float xe = has_extra ? L::one(x + extra) : -INFINITY;
-  if (has_extra && suppressed(a.suppress, c0 + extra)) {
-    xe = -INFINITY;
-    if (I8) has_extra = false;
-  }
-  uint32_t off[I8 ? P : 1];  // int8 has no -inf: its suppressed logits stay bits
-#pragma unroll
-  for (int p = 0; p < (I8 ? P : 1); ++p) off[p] = 0;
-  if (a.suppress) {
-    const int last = (a.cols - 1) >> 5;
+  T xr{};
+  {
+    const uint4 *xa = reinterpret_cast<const uint4 *>(it.x + it.head);
 #pragma unroll
     for (int p = 0; p < P; ++p)
-      if (p * NT + tid < pieces) {
-        const int col0 = c0 + head + (p * NT + tid) * E;
-        const uint64_t two = (uint64_t)a.suppress[min((col0 >> 5) + 1, last)] << 32 | a.suppress[col0 >> 5];
-        const uint32_t bits = (uint32_t)(two >> (col0 & 31)) & ((1u << E) - 1u);
-        if constexpr (I8)
-          off[p] = bits;
-        else
-          L::mask(w[p], bits);
-      }
+      if (p * NT + tid < it.pieces) w[p] = xa[p * NT + tid];
+    const int i = tid < it.head ? tid : it.head + it.pieces * E + tid - it.head;
+    if (i < it.n) xr = it.x[i];
   }
+  if (tid == 0) s.cands = 0;
+  if constexpr (I8)
+    for (int i = tid; i < 256 * kCopies; i += NT) s.count[i] = 0;
+  lds_barrier();
 
-  // ---- the thread's largest logit (int8: -129 for none) ----
-  float tmax = -INFINITY;
+  const int c0 = it.c0, n = it.n;
+  auto held = [&](int p) { return p * NT + tid < it.pieces; };
+  auto column = [&](int p) { return c0 + it.head + (p * NT + tid) * E; };
+  // the bits of a piece's suppressed logits (a piece may reach into the next word)
+  auto hidden = [&](int p) -> uint32_t {
+    const int at = column(p) - c0, i = at >> 5;
+    const uint32_t *words = I8 ? a.suppress + c0 / 32 : sWords;
+    const uint64_t two = (uint64_t)words[I8 ? min(i + 1, (n - 1) >> 5) : i + 1] << 32 | words[i];
+    return (uint32_t)(two >> (at & 31)) & ((1u << E) - 1u);
+  };
+  const int extra = tid < it.head ? tid : it.head + it.pieces * E + tid - it.head;  // this thread's single logit
+  bool has_extra = extra < n;
+  float xe = has_extra ? L::one(&xr) : -INFINITY;
+  if (!I8 && a.suppress && has_extra && ((sWords[extra >> 5] >> (extra & 31)) & 1u)) xe = -INFINITY;
+
+  float m, reach, tmax = INFINITY, z = 0.f, u = 0.f, eq = 0.f;
   if constexpr (I8) {
-    typedef int16_t v2s __attribute__((ext_vector_type(2)));
-    v2s hi{-32768, -32768}, lo{-32768, -32768};
-    bool any = has_extra;
+    uint32_t *const mine = s.count + (lane & (kCopies - 1));
+    // value v at 128 + v, that is the byte with its sign bit turned
 #pragma unroll
     for (int p = 0; p < P; ++p)
-      if (p * NT + tid < pieces) {
-        uint32_t v[4] = {w[p].x, w[p].y, w[p].z, w[p].w};
-        any = any || off[p] != 0xffffu;
-        if (off[p]) {
+      if (held(p)) {
+        const uint32_t v[4] = {w[p].x ^ 0x80808080u, w[p].y ^ 0x80808080u, w[p].z ^ 0x80808080u,
+                               w[p].w ^ 0x80808080u};
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if ((off[p] >> i) & 1u) v[i >> 2] = (v[i >> 2] & ~(0xffu << (8 * (i & 3)))) | 0x80u << (8 * (i & 3));
-        }
-        // the odd bytes lead their 16-bit halves, the even ones once shifted up
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          hi = __builtin_elementwise_max(hi, __builtin_bit_cast(v2s, v[q]));
-          lo = __builtin_elementwise_max(lo, __builtin_bit_cast(v2s, v[q]) << (int16_t)8);
-        }
+        for (int i = 0; i < 16; ++i) atomicAdd(mine + kCopies * ((v[i >> 2] >> (8 * (i & 3))) & 0xffu), 1u);
       }
-    int32_t t = max(max(hi.x >> 8, hi.y >> 8), max(lo.x >> 8, lo.y >> 8));
-    if (has_extra) t = max(t, (int32_t)xe);
-    tmax = any ? (float)t : -129.f;
+    if (has_extra) atomicAdd(mine + kCopies * ((int)xe + 128), 1u);
+    // the suppressed ones are few: looked up and taken off
+    if (a.suppress)
+      for (int i = tid; i < (n + 31) / 32; i += NT) {
+        uint32_t o = a.suppress[c0 / 32 + i];
+        if (n - 32 * i < 32) o &= (1u << (n - 32 * i)) - 1u;
+        for (; o; o &= o - 1) atomicSub(mine + kCopies * ((int)it.x[32 * i + __ffs((int)o) - 1] + 128), 1u);
+      }
+    lds_barrier();
+    // every wave: lane l has the values 4 l .. 4 l + 3 (above -128)
+    uint32_t c[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = 0;
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j) c[i] += s.count[(4 * lane + i) * kCopies + j];
+      sum += c[i];
+    }
+    const uint64_t any = __ballot(sum != 0);
+    const int high = c[3] ? 3 : c[2] ? 2 : c[1] ? 1 : 0;
+    const int hl = any ? 63 - __clzll((long long)any) : 0;
+    const int mi = 4 * hl + __shfl(high, hl) - 128;
+    m = any ? (float)mi : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = mi + 128 - (4 * lane + i);
+      if (d > 0 && c[i]) {
+        const float e = (float)c[i] * expf(-(float)d * a.scale);
+        z += e;
+        u += e * (float)d;
+      }
+      if (d == 0) eq = (float)c[i];
+    }
+    z = wave_sum_f32(z);
+    u = wave_sum_f32(u);
+    eq = wave_sum_f32(eq);
+    reach = -129.f;
+    if (a.top > 0) {
+      // the largest value that `top` logits reach: lanes from the top, then values
+      uint32_t above = sum;  // logits of this lane's values and the larger ones
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_down(above, o);
+        if (lane + o < 64) above += t;
+      }
+      const uint64_t full = __ballot(above >= (uint32_t)a.top);
+      if (full) {
+        const int at = 63 - __clzll((long long)full);
+        uint32_t have = __shfl(above - sum, at);
+        int i = 3;
+#pragma unroll
+        for (int j = 3; j > 0; --j) {
+          have += __shfl(c[j], at);
+          if (i == j && have < (uint32_t)a.top) i = j - 1;
+        }
+        reach = (float)(4 * at + i - 128);
+      }
+    }
   } else {
+    if (a.suppress) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (held(p)) {
+          const uint32_t o = hidden(p);
+          if (o) L::mask(w[p], o);
+        }
+    }
     tmax = xe;
 #pragma unroll
     for (int p = 0; p < P; ++p)
-      if (p * NT + tid < pieces) {
+      if (held(p)) {
 #pragma unroll
         for (int e = 0; e < E; ++e) tmax = fmaxf(tmax, L::get(w[p], e));
       }
-  }
-  // numbers in the logits' order, the largest of each 16 threads
-  uint32_t g = I8 ? (uint32_t)(int32_t)(tmax + 129.f) << 23 : ordered(tmax);
-  g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, 0xB1, 0xf, 0xf, true));
-  g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, 0x4E, 0xf, 0xf, true));
-  g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, 0x141, 0xf, 0xf, true));
-  g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, 0x140, 0xf, 0xf, true));
-  if ((lane & 15) == 0) s.group[tid >> 4] = g;
-  if (tid == 0) s.cands = 0;
-  __syncthreads();
-  g = s.group[lane];
-  const uint32_t bound = a.top > 0 ? kth_largest<I8 ? 9 : 16>(g, a.top) : 0u;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) g = max(g, (uint32_t)__shfl_xor((int)g, o));
-  const float m = I8 ? (g == 0 ? -INFINITY : (float)((int)(g >> 23) - 129)) : key_value((uint64_t)g << 32);
-  const float ms = m == -INFINITY ? 0.f : m;  // a part without finite logits sums to 0
-
-  // ---- Z', U' / s and the number of logits that equal m ----
-  float z = 0.f, u = 0.f, eq = 0.f;
-  const bool mine = tmax == m;  // few threads hold it and look for it
-  if constexpr (I8) {
-    // exp by a table over the distances y = m - x; 255 stands for a suppressed
-    // logit (below m = 127 no other has it)
-    if (tid < 256) s.e[tid] = tid == 0 || (tid == 255 && m < 127.f) ? 0.f : expf(-(float)tid * a.scale);
-    __syncthreads();
-    const uint32_t m4 = (uint32_t)((int)ms + 128) * 0x01010101u;
-    const bool clash = a.suppress && m == 127.f;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (p * NT + tid < pieces) {
-        const uint32_t v[4] = {w[p].x, w[p].y, w[p].z, w[p].w};
-        if (!clash) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t y = m4 - (v[q] ^ 0x80808080u);
-            if (off[p]) {
-              const uint32_t o4 = ((((off[p] >> (4 * q)) & 15u) * 0x00204081u) & 0x01010101u) * 0xffu;
-              // bytes of suppressed logits may lie above m: without borrows
-              y = (m4 - ((v[q] ^ 0x80808080u) & ~o4)) | o4;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t d = (y >> (8 * i)) & 0xffu;
-              const float e = s.e[d];
-              z += e;
-              u += e * (float)d;
-              if (mine && d == 0) eq += 1.f;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!((off[p] >> i) & 1u)) {
-              const int d = 127 - (int)(int8_t)(v[i >> 2] >> (8 * (i & 3)));
-              const float e = s.e[d];
-              z += e;
-              u += e * (float)d;
-              if (d == 0) eq += 1.f;
-            }
-        }
-      }
-    if (has_extra) {
-      const int d = (int)ms - (int)xe;
-      const float e = s.e[d];
-      z += e;
-      u += e * (float)d;
-      if (d == 0) eq += 1.f;
-    }
-  } else {
-    // d * log2(e) s in two parts, as the product's rounding would be the same for all
-    const double cd = (double)a.scale * 1.4426950408889634;
-    const float ch = (float)cd, cl = (float)(cd - (double)ch);
+    // the largest of each of 64 groups of threads
+    float g = tmax;
+    g = fmaxf(g, dpp_f32<0xB1>(g));
+    g = fmaxf(g, dpp_f32<0x4E>(g));
+    if (NT >= 512) g = fmaxf(g, dpp_f32<0x141>(g));
+    if (NT >= 1024) g = fmaxf(g, dpp_f32<0x140>(g));
+    if (tid % NW == 0) s.group[tid / NW] = ordered(g);
+    lds_barrier();
+    const uint32_t go = s.group[lane];
+    reach = a.top > 0 ? key_value((uint64_t)kth_largest<16>(go, a.top) << 32) : 0.f;
+    if (reach != reach) reach = -INFINITY;  // below every number: all logits
+    m = key_value((uint64_t)wave_max_u32_dpp(go) << 32);
+    const float ms = m == -INFINITY ? 0.f : m;  // a part without finite logits sums to 0
     auto add = [&](float v, bool all) {
       const float d = v - ms;
-      const float e = __builtin_amdgcn_exp2f(fmaf(d, ch, d * cl));
+      const float e = __builtin_amdgcn_exp2f(fmaf(d, a.log2_hi, d * a.log2_lo));
       if (all || d != 0.f) {
         z += e;
-        u -= e > 0.f ? d * e : 0.f;
+        u -= fmaxf(d, -3e38f) * e;  // -inf times its exp of 0 is 0
       } else {
         eq += 1.f;
       }
     };
     if (has_extra) add(xe, false);
-    if (mine) {
+    if (tmax == m) {  // few threads hold it and look for it
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        if (p * NT + tid < pieces)
+        if (held(p)) {
 #pragma unroll
           for (int e = 0; e < E; ++e) add(L::get(w[p], e), false);
+        }
     } else {
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        if (p * NT + tid < pieces)
+        if (held(p)) {
 #pragma unroll
           for (int e = 0; e < E; ++e) add(L::get(w[p], e), true);
+        }
     }
+    z = wave_sum_f32(z);
+    u = wave_sum_f32(u);
+    eq = wave_sum_f32(eq);
+    if (lane == 0) s.z[wave] = z, s.u[wave] = u, s.n[wave] = eq;
   }
 
   // ---- the logits that reach the bound ----
-  float reach = I8 ? (float)((int)(bound >> 23) - 129) : key_value((uint64_t)bound << 32);
-  if (reach != reach) reach = -INFINITY;  // below every number: all logits
+  if (I8 && a.top > 0) {
+    typename Logit<int8_t>::v2s t{-32768, -32768};
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (held(p)) t = __builtin_elementwise_max(t, Logit<int8_t>::halves(w[p]));
+    tmax = fmaxf((float)max(t.x >> 8, t.y >> 8), xe);
+  }
   if (a.top > 0 && tmax >= reach) {
     auto put = [&](float v, int col) {
       if (v >= reach) {
@@ -386,31 +448,31 @@ __global__ __launch_bounds__(NT) void token_scores_kernel(ScoreArgs a, int chunk
         if (at < kCand) s.cand[at] = key_of(v, col);
       }
     };
-    if (has_extra) put(xe, c0 + extra);
+    if (has_extra && !(I8 && suppressed(a.suppress, c0 + extra))) put(xe, c0 + extra);
 #pragma unroll
     for (int p = 0; p < P; ++p)
-      if (p * NT + tid < pieces)
-#pragma unroll
+      if (held(p) && L::max(w[p]) >= reach) {
+        const uint32_t o = I8 && a.suppress ? hidden(p) : 0u;
         for (int e = 0; e < E; ++e)
-          if (!I8 || !((off[I8 ? p : 0] >> e) & 1u)) put(L::get(w[p], e), c0 + head + (p * NT + tid) * E + e);
+          if (!((o >> e) & 1u)) put(L::get(w[p], e), column(p) + e);
+      }
   }
-  z = wave_sum_f32(z);
-  u = wave_sum_f32(u);
-  eq = wave_sum_f32(eq);
-  if (lane == 0) s.z[wave] = z, s.u[wave] = u, s.n[wave] = eq;
-  __syncthreads();
-  z = u = eq = 0.f;
+  lds_barrier();
+  if constexpr (!I8) {
+    z = u = eq = 0.f;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) z += s.z[i], u += s.u[i], eq += s.n[i];
+    for (int i = 0; i < NW; ++i) z += s.z[i], u += s.u[i], eq += s.n[i];
+  }
   if (eq > 0.f) z += eq - 1.f;
   const float l = row_log(m, z);
 
+  const int64_t row = it.row;
   const int cands = s.cands;
   const bool rounds = a.top > 0 && (cands > kCand || cands < min(a.top, n) || z != z || m - m != 0.f);
-  if (rounds) top_by_rounds<T>(x, c0, n, a.suppress, a.top, s);
+  if (rounds) top_by_rounds<T, NT>(it.x, c0, n, a.suppress, a.top, s);
   uint64_t *tops = nullptr;
   if (chunks > 1)
-    tops = reinterpret_cast<uint64_t *>(reinterpret_cast<Part *>(a.workspace) + a.rows * chunks) + (int64_t)blockIdx.x * a.top;
+    tops = reinterpret_cast<uint64_t *>(reinterpret_cast<Part *>(a.workspace) + a.rows * chunks) + item * a.top;
   auto place = [&](int at, uint64_t k) {
     if (tops) {
       tops[at] = k;
@@ -421,31 +483,38 @@ __global__ __launch_bounds__(NT) void token_scores_kernel(ScoreArgs a, int chunk
   };
   if (rounds) {
     if (tid < a.top) place(tid, s.top[tid]);
-  } else if (tid < cands) {
-    const uint64_t k = s.cand[tid];
-    int larger = 0;
-    for (int i = 0; i < cands; ++i) larger += s.cand[i] > k;
-    if (larger < a.top) place(larger, k);
-  } else if (tops && tid >= NT - 64 && cands + tid - (NT - 64) < a.top) {
-    tops[cands + tid - (NT - 64)] = 0;  // a part of fewer logits than alternatives
+  } else {
+    for (int j = tid; j < cands; j += NT) {
+      const uint64_t k = s.cand[j];
+      int larger = 0;
+      for (int i = 0; i < cands; ++i) larger += s.cand[i] > k;
+      if (larger < a.top) place(larger, k);
+    }
+    // a part of fewer logits than alternatives
+    if (tops && cands + tid < a.top) tops[cands + tid] = 0;
   }
-  if (tid != 0) return;
-  if (tops)
-    reinterpret_cast<Part *>(a.workspace)[blockIdx.x] = Part{m, z, u, 0.f};
-  else
-    write_row<T>(a, row, m, l, z, u);
+  if (tid == 0) {
+    if (tops)
+      reinterpret_cast<Part *>(a.workspace)[item] = Part{m, z, u, 0.f};
+    else
+      write_row<T>(a, row, m, l, z, u);
+  }
 }
 
-// Joins a row's parts, one wave per row.
+// Joins a row's parts, one block per row.
+constexpr int JT = 256, kJoinKeys = 2048;
 template <typename T>
-__global__ __launch_bounds__(64) void token_scores_join_kernel(ScoreArgs a, int chunks) {
+__global__ __launch_bounds__(JT) void token_scores_join_kernel(ScoreArgs a, int chunks) {
+  __shared__ uint64_t sKey[kJoinKeys];
+  __shared__ uint16_t sHead[kMaxParts];
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const Part *parts = reinterpret_cast<const Part *>(a.workspace) + row * chunks;
+  const int keys = chunks * a.top;
   const uint64_t *tops =
-      reinterpret_cast<const uint64_t *>(reinterpret_cast<const Part *>(a.workspace) + a.rows * chunks) +
-      row * chunks * a.top;
-  // the first part that holds the largest logit keeps it out of Z'
+      reinterpret_cast<const uint64_t *>(reinterpret_cast<const Part *>(a.workspace) + a.rows * chunks) + row * keys;
+  for (int i = tid; i < min(keys, kJoinKeys); i += JT) sKey[i] = tops[i];
+  // every wave sums the parts: the first that holds the largest logit keeps it out of Z'
   uint64_t best = 0;
   for (int c = lane; c < chunks; c += 64) best = max64(best, key_of(parts[c].m, c));
   best = wave_max64(best);
@@ -462,50 +531,87 @@ __global__ __launch_bounds__(64) void token_scores_join_kernel(ScoreArgs a, int 
   z = wave_sum_f32(z);
   u = wave_sum_f32(u);
   const float l = row_log(m, z);
-  if (a.top > 0) {
-    // the parts' lists are in order: the largest of their heads, one after the other
-    __shared__ uint8_t head[kMaxParts];
-    for (int c = lane; c < chunks; c += 64) head[c] = 0;
+  auto place = [&](int at, uint64_t k) {
+    a.top_ids[row * a.top + at] = key_col(k);
+    a.top_lp[row * a.top + at] = (key_value(k) - m) * a.scale - l;
+  };
+  __syncthreads();
+  if (keys <= kJoinKeys) {
+    for (int i = tid; i < keys; i += JT) {  // a key's place is the number of larger ones
+      const uint64_t k = sKey[i];
+      int larger = 0;
+      for (int j = 0; j < keys; ++j) larger += sKey[j] > k;
+      if (larger < a.top && k != 0) place(larger, k);
+    }
+  } else if (tid < 64) {  // the largest of the parts' heads, one after the other
+    for (int c = lane; c < chunks; c += 64) sHead[c] = 0;
     for (int i = 0; i < a.top; ++i) {
       uint64_t k = 0;
       for (int c = lane; c < chunks; c += 64)
-        if (head[c] < a.top) k = max64(k, tops[(int64_t)c * a.top + head[c]]);
+        if (sHead[c] < a.top) k = max64(k, tops[(int64_t)c * a.top + sHead[c]]);
       const uint64_t b = wave_max64(k);
       for (int c = lane; c < chunks; c += 64)
-        if (head[c] < a.top && tops[(int64_t)c * a.top + head[c]] == b) ++head[c];
-      if (lane == 0) {
-        a.top_ids[row * a.top + i] = key_col(b);
-        a.top_lp[row * a.top + i] = (key_value(b) - m) * a.scale - l;
-      }
+        if (sHead[c] < a.top && tops[(int64_t)c * a.top + sHead[c]] == b) ++sHead[c];
+      if (lane == 0) place(i, b);
     }
   }
-  if (lane == 0) write_row<T>(a, row, m, l, z, u);
+  if (tid == 0) write_row<T>(a, row, m, l, z, u);
 }
 
-// Parts of a row and their columns: at most what a block holds.
-void split(int item, int64_t rows, int64_t cols, int *chunks, int *span) {
-  const int64_t most = (int64_t)(kPieces - 1) * 16 / item;
-  *chunks = (int)((cols + most - 1) / most);
-  *span = (int)((cols + *chunks - 1) / *chunks + 63) / 64 * 64;
-  *chunks = (int)((cols + *span - 1) / *span);
+// Parts of a row and their columns, and the kernel's form. us of 256 threads of 16
+// pieces, 512 of 8 and 1024 of 4 (all a part of 64 KB):
+//   2048 rows of 51865 int8 logits 36.0 / 38.5 / 45.1, 512 rows of float32 33.7 / 33.3 / 33.9,
+//   512 rows of float16 33.2 / 28.3 / 29.3: fewer threads do less beside the logits, and int8
+//   has next to nothing to do for one;
+//   one row of int8 12 / 11 / 10.1, 91 of float32 15.0 / 12.8 / 12.8: few blocks wait for
+//   themselves, and more threads are a shorter chain.
+// Parts of 16 KB were slower for all (int8 50, float32 34.9, float16 32.7), and so were blocks that
+// stay and request their next part early (int8 48, float32 44): their registers cost more waves
+// than the reads gained. What is left above a read of the bytes (106 MB 19 us): int8 is bound by LDS adds
+// (8.6 cycles per 64 of them), the others by issuing ~9 instructions a logit at 2 GHz, and each
+// block's reading and computing do not overlap but with those of the blocks beside it.
+struct Split {
+  int chunks, span;
+  bool few;
+};
+Split split(int type, int64_t rows, int64_t cols) {
+  const int item = type == LOGIT_I8 ? 1 : type == LOGIT_F32 ? 4 : 2;
+  const int64_t most = kPartBytes / item - 16;
+  Split s;
+  s.chunks = (int)((cols + most - 1) / most);
+  s.few = rows * s.chunks <= kFewBlocks;
+  s.span = (int)((cols + s.chunks - 1) / s.chunks + 63) / 64 * 64;
+  s.chunks = (int)((cols + s.span - 1) / s.span);
+  return s;
+}
+
+template <typename T, int NT, int P>
+int launch_scores_p(const ScoreArgs &a, const Split &sp, hipStream_t s) {
+  hipLaunchKernelGGL((token_scores_kernel<T, NT, P>), dim3((unsigned)(a.rows * sp.chunks)), dim3(NT), 0, s, a,
+                     sp.chunks, sp.span);
+  if (sp.chunks > 1)
+    hipLaunchKernelGGL((token_scores_join_kernel<T>), dim3((unsigned)a.rows), dim3(JT), 0, s, a, sp.chunks);
+  return check_launch("token_scores_kernel");
 }
 
 template <typename T>
-int launch_scores(const ScoreArgs &a, hipStream_t s) {
-  int chunks, span;
-  split((int)sizeof(T), a.rows, a.cols, &chunks, &span);
-  if (chunks > kMaxParts || a.rows * chunks > (1LL << 32) / NT - 1) return fail("too many logits for one call");
-  hipLaunchKernelGGL((token_scores_kernel<T>), dim3((unsigned)(a.rows * chunks)), dim3(NT), 0, s, a, chunks, span);
-  if (chunks > 1)
-    hipLaunchKernelGGL((token_scores_join_kernel<T>), dim3((unsigned)a.rows), dim3(64), 0, s, a, chunks);
-  return check_launch("token_scores_kernel");
+int launch_scores(ScoreArgs a, hipStream_t s) {
+  const Split sp = split(a.type, a.rows, a.cols);
+  if (sp.chunks > kMaxParts || a.rows * sp.chunks > (1LL << 32) / 1024 - 1) return fail("too many logits for one call");
+  // log2(e) * scale in two parts, as the rounding of one would be the same for
+  // every logit; neither is negative, so that -inf times them stays -inf
+  const double c = (double)a.scale * 1.4426950408889634;
+  a.log2_hi = (float)c;
+  if ((double)a.log2_hi > c) a.log2_hi = std::nextafter(a.log2_hi, 0.f);
+  a.log2_lo = std::max((float)(c - (double)a.log2_hi), 1e-30f);
+  if (sp.few) return launch_scores_p<T, 1024, 4>(a, sp, s);
+  return launch_scores_p<T, sizeof(T) == 1 ? 256 : 512, sizeof(T) == 1 ? 16 : 8>(a, sp, s);
 }
 
 }  // namespace
 
 int64_t score_workspace(int type, int64_t rows, int64_t cols, int64_t top) {
-  int chunks, span;
-  split(type == LOGIT_I8 ? 1 : type == LOGIT_F32 ? 4 : 2, rows, cols, &chunks, &span);
+  const int chunks = split(type, rows, cols).chunks;
   return chunks > 1 ? rows * chunks * ((int64_t)sizeof(Part) + 8 * top) : 0;
 }
 
