@@ -949,6 +949,11 @@ int iw_attention_tree(const int8_t *q, int64_t q_sb, int64_t q_st, const int8_t 
       (uintptr_t)(q_sb | q_st | kn_sb | kn_st | vn_sb | vn_st | k_sb | k_sh | k_st | v_sb | v_sh | o_sb | o_st) |
       (uintptr_t)(v_sq != 4 ? v_sq : v_sd);
   IW_REQUIRE((align & 15) == 0, "tree attention operands must be 16-byte aligned");
+  // offsets within 64 keys or nodes and within a head's transposed rows are 32-bit numbers
+  const int64_t far = 1 << 25;
+  IW_REQUIRE(kn_st >= 0 && kn_st < far && vn_st >= 0 && vn_st < far && k_st >= 0 && k_st < far && v_sq >= 0 &&
+                 v_sq < far && v_sd >= 0 && v_sd < far,
+             "strides of nodes, keys, key quads and transposed rows must be below 2^25");
   TreeArgs t;
   AttnArgs &a = t.a;
   a.q = q;

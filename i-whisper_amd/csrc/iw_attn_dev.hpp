@@ -21,7 +21,7 @@ __device__ __forceinline__ int32_t med3i(int32_t x, int32_t lo, int32_t hi) {
 }
 
 // Table index of a raw score for a row maximum: min((rowmax + 1 - h16) mod
-// 2^16, L) with L the last table entry.
+// 2^16, L) with L the last table entry (one whose value is 0).
 //
 // Where every key of a chunk counts in the row maximum and that is below
 // 32767, rowmax + 1 - h16 lies in [1, 65535] and the index is
@@ -40,7 +40,9 @@ struct ScoreIndex {
   // short form
   uint32_t fsh, fw;
   int32_t fnm, fK, flo, fhi;
-  __device__ __forceinline__ ScoreIndex(const AttnArgs &a, int32_t rowmax) {
+  uint32_t last;  // L
+  __device__ __forceinline__ ScoreIndex(const AttnArgs &a, int32_t rowmax, int32_t last_ = IW_SEXP_LUT - 1) {
+    last = (uint32_t)last_;
     m24 = a.qk_s >= 32 ? 0 : (int32_t)a.qk_m;
     sh = a.qk_s >= 32 ? 0u : a.qk_s;
     half = sh ? 1u << (sh - 1) : 0u;
@@ -51,7 +53,7 @@ struct ScoreIndex {
     fw = min(fsh, 1u);
     const int32_t R = rowmax + 1;
     fK = (int32_t)(((uint32_t)R << fsh) + ((1u << fsh) - 1u) - (fsh ? 1u << (fsh - 1) : 0u));
-    flo = min(R - 32767, IW_SEXP_LUT - 1), fhi = min(R + 32768, IW_SEXP_LUT - 1);
+    flo = min(R - 32767, last_), fhi = min(R + 32768, last_);
   }
   // every key counts, row maximum below 32767
   __device__ __forceinline__ uint32_t full(int32_t s) const {
@@ -64,7 +66,7 @@ struct ScoreIndex {
     const int32_t v = __mul24(s, m24);
     const uint32_t tr = (uint32_t)v + half + (uint32_t)__builtin_amdgcn_sbfe(v, 31, w);
     const int32_t h16 = clampi((int32_t)tr >> sh, -32768, 32767);
-    return min((rmp1 - (uint32_t)h16) & 0xffffu, (uint32_t)(IW_SEXP_LUT - 1));
+    return min((rmp1 - (uint32_t)h16) & 0xffffu, last);
   }
 };
 

@@ -6,13 +6,18 @@
 // first, then P = E(S - rowmax - 1), sum P and P.V, exact modulo 2^32 in any
 // order, so the keys can be split over waves.
 //
-// One block per (batch, head); up to 64 nodes are four 16-query MFMA tiles. The
+// One block per (batch, head) and up to 32 nodes (two 16-query MFMA tiles). The
 // block's waves take 64-key chunks in turn, the tree itself is one more chunk.
 // In a chunk's four 16x16x64 score products, row 4g + r of product t is key
 // 16g + 4t + r: lane group g then holds the scores of the 16 consecutive keys
 // that its bytes of the P.V operand stand for, and no lane exchange is needed.
 // V's columns go to the products as d = 4n + c (lane n, product c): a lane
 // reads whole words, and its four sums are one word of the output.
+//
+// The shift exponential is 0 from a distance of about 4.9 * 2^frac_bits on. Up to
+// frac_bits 10 the distances below that are read from a table that the block
+// copies to LDS while its K and V are on the way (1249 bytes at 8, 4988 at 10);
+// beyond, each score computes its own.
 #include "iw_attn_dev.hpp"
 #include "iw_common.hpp"
 #include "iw_tree.hpp"
@@ -21,22 +26,45 @@ namespace iw {
 
 namespace {
 
+constexpr int kTableBits = 10, kTableBytes = 4992;
+
+// First distance from which every value is 0: 2^-(t / 2^f) in f (at most 7)
+// fractional bits is 0 once t > min(f, 7) 2^f, and t >= 23/16 n - 1.
+__host__ __device__ constexpr int shift_exp_zero(int f) { return (((f < 7 ? f : 7) << f) + 2) * 16 / 23 + 1; }
+// The tables lie one after the other, each in whole 16 bytes.
+__host__ __device__ constexpr int table_at(int f) {
+  int at = 0;
+  for (int i = 1; i < f; ++i) at += (shift_exp_zero(i) + 16) / 16 * 16;
+  return at;
+}
+static_assert(table_at(kTableBits + 1) - table_at(kTableBits) == kTableBytes, "the largest table fills the block's copy");
+
 // The shift exponential of -n (n the score's distance from the row maximum
 // plus one, 0 .. 32767): with t = n + ceil(n/2) - ceil(n/16) (n log2 e in
 // 16-bit steps), 2^-(t / 2^f) as a linear fraction and a shift. Distances
 // whose t passes 2^15 wrap there and give 0.
-struct ShiftExp {
-  int32_t f, down;
-  __device__ __forceinline__ explicit ShiftExp(int32_t frac) : f(frac), down(max(frac - 7, 0)) {}
-  __device__ __forceinline__ uint32_t operator()(int32_t n) const {
-    const int32_t t = n + ((n + 1) >> 1) - ((n + 15) >> 4);
-    const int32_t m = (1 << f) - 1;
-    const int32_t sh = (t + m) >> f;
-    const int32_t num = (1 << f) | ((-t & m) >> 1);
-    const uint32_t p = (uint32_t)num >> min(sh + down, 31);
-    return t > 32768 ? 0u : p;
+__host__ __device__ constexpr uint32_t shift_exp(int32_t n, int32_t f) {
+  const int32_t t = n + ((n + 1) >> 1) - ((n + 15) >> 4);
+  const int32_t m = (1 << f) - 1;
+  const int32_t sh = ((t + m) >> f) + (f > 7 ? f - 7 : 0);
+  const uint32_t num = (1u << f) | ((uint32_t)(-t & m) >> 1);
+  return t > 32768 ? 0u : num >> (sh < 31 ? sh : 31);
+}
+
+struct ShiftExpTables {
+  uint8_t v[table_at(kTableBits + 1)];
+  constexpr ShiftExpTables() : v() {
+    for (int f = 1; f <= kTableBits; ++f)
+      for (int i = 0; i < table_at(f + 1) - table_at(f); ++i) v[table_at(f) + i] = (uint8_t)shift_exp(i, f);
   }
 };
+__device__ __attribute__((aligned(16))) constexpr ShiftExpTables kTables{};
+
+// 0xff in the bytes of a 4-bit mask's set bits
+__device__ __forceinline__ uint32_t byte_mask(uint32_t four) {
+  const uint32_t ones = __umul24(four, 0x00204081u) & 0x01010101u;
+  return (ones << 8) - ones;
+}
 
 // four words of four bytes to their transpose
 __device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
@@ -50,21 +78,29 @@ __device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&o
   out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-// KS: 64-column parts of the head; QUADS: V in key quads; QT: 16-query tiles.
-template <int KS, bool QUADS, int QT, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
-  constexpr int QR = 16 * QT, OLD = 64 * KS + 4;
+// KS: 64-column parts of the head; QUADS: V in key quads; QT: 16-query tiles of
+// the block; NW waves; NC > 0: a wave has at most NC chunks, whose K and V
+// are all requested at the start and kept.
+template <int KS, bool QUADS, int QT, int NW, int NC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2 && KS == 1 ? (QT == 1 ? 4 : 3) : NC == 1 && KS * QT <= 2 ? 4 : NW == 16 ? 4 : 2))) void attn_tree_kernel(TreeArgs t, int qblocks, int blocks, int per_xcd,
+                                                       int per_word, int table_off) {
+  constexpr int QR = 16 * QT, OLD = 64 * KS + 4, HC = NC > 0 ? NC : 1;
+  __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
   __shared__ int32_t sMax[NW][QR];
   __shared__ uint32_t sSum[QR];
   __shared__ int32_t sInv[QR];
   __shared__ __attribute__((aligned(16))) uint32_t sO[QR * OLD];
 
+  // the blocks of a (batch, head) are neighbours on one XCD (blockIdx % 8) and share its L2
+  const int block = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (block >= blocks) return;
   const AttnArgs &a = t.a;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const int h = blockIdx.x % a.H;
-  const int64_t b = blockIdx.x / a.H;
+  const int q0 = block % qblocks * QR, bh = block / qblocks;
+  const int h = bh % a.H;
+  const int64_t b = bh / a.H;
   const int D = a.D, N = a.Tq;
   const int len = clampi(t.lengths[b], 0, a.Tk);
   const int cnt = t.counts ? clampi(t.counts[b], 0, N) : N;
@@ -73,19 +109,97 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
   const int8_t *const vbase = a.vt + b * a.v_sb + (int64_t)h * a.v_sh;
   const int8_t *const knew = t.kn + b * t.kn_sb + (int64_t)h * D;
   const int8_t *const vnew = t.vn + b * t.vn_sb + (int64_t)h * D;
+  int8_t *const obase = a.out + b * a.o_sb + (int64_t)h * D;
+  const int words = D / 4, rows = min(N - q0, QR);
+  // i / words for the i < 2^11 of the output
+  const auto by_words = [&](int i) { return (int)__umul24(i, per_word) >> 16; };
 
-  if (cnt == 0) {  // no node of this row is in use
-    for (int i = tid; i < N * (D / 4); i += 64 * NW)
-      *reinterpret_cast<uint32_t *>(a.out + b * a.o_sb + (int64_t)(i / (D / 4)) * a.o_st + (int64_t)h * D +
-                                    4 * (i % (D / 4))) = 0u;
+  if (q0 >= cnt) {  // no node of these is in use
+    for (int i = tid; i < rows * words; i += 64 * NW) {
+      const int q = by_words(i);
+      *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + q) * a.o_st + 4 * (i - q * words)) = 0u;
+    }
     return;
   }
 
+  const int nfk = len / 64;  // chunks in which every key counts
+
+  // The K operands of chunk c: keys past the last repeat it, head dims past D the
+  // last ones (the query is zero there). A chunk's base is uniform, its lanes'
+  // offsets fit 32 bits.
+  const int kcol = 16 * g, key0 = 16 * (n >> 2) + (n & 3);
+  auto load_k = [&](int c, v4i (&f)[4][KS]) {
+    const bool tree = c == nkc;
+    const uint32_t st = (uint32_t)(tree ? t.kn_st : a.k_st);
+    const int8_t *base = tree ? knew : kbase + (int64_t)(64 * c) * a.k_st;
+    const int last = (tree ? cnt : len - 64 * c) - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        f[i][ks] = *reinterpret_cast<const v4i *>(base + ((uint32_t)min(key0 + 4 * i, last) * st +
+                                                          (uint32_t)min(64 * ks + kcol, D - 16)));
+  };
+  // What the V operands are made of: quads and transposed rows hold words of four
+  // keys of one column, the tree's rows (word j of f[ks][i] from node 16 g + 4 j + i) four
+  // columns. Columns past D repeat the last ones; their sums are not stored.
+  auto load_v = [&](int c, v4i (&f)[KS][4]) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
+      if (c == nkc) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            f[ks][i][j] = *reinterpret_cast<const int32_t *>(
+                vnew + ((uint32_t)min(16 * g + 4 * j + i, cnt - 1) * (uint32_t)t.vn_st + d0));
+      } else if (QUADS) {
+        const int8_t *base = vbase + (int64_t)(16 * c) * a.v_sq;
+        const int last = ((len - 1) >> 2) - 16 * c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          f[ks][j] = *reinterpret_cast<const v4i *>(base + ((uint32_t)min(4 * g + j, last) * (uint32_t)a.v_sq + 4 * d0));
+      } else {
+        const int8_t *base = vbase + 64 * c;
+        const uint32_t at = (uint32_t)min(16 * g, (len - 1 - 64 * c) & ~15);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          f[ks][i] = *reinterpret_cast<const v4i *>(base + ((d0 + i) * (uint32_t)a.v_sd + at));
+      }
+    }
+  };
+  // the operand of product i: column 64 ks + 4 n + i of the lane group's 16 keys
+  auto v_operands = [&](int c, const v4i (&f)[4], v4i (&o)[4]) {
+    if (c == nkc) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t in[4] = {(uint32_t)f[0][j], (uint32_t)f[1][j], (uint32_t)f[2][j], (uint32_t)f[3][j]};
+        uint32_t x[4];
+        transpose4(in, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i][j] = (int)x[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = QUADS ? f[j][i] : f[i][j];
+    }
+  };
+
+  // ---- everything that the start can ask for ----
+  v4i kf[HC][4][KS], vf[HC][KS][4];
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i <= nkc) load_k(wave + NW * i, kf[i]);
+  }
   v4i qf[QT][KS];
   uint64_t vis[QT];
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
-    const int q = min(16 * u + n, cnt - 1);  // queries past the count repeat the last one
+    const int q = min(q0 + 16 * u + n, cnt - 1);  // queries past the count repeat the last one
     vis[u] = t.visible[b * t.vis_sb + q];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -94,59 +208,20 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
       if (d0 < D) qf[u][ks] = *reinterpret_cast<const v4i *>(a.q + b * a.q_sb + (int64_t)q * a.q_st + (int64_t)h * D + d0);
     }
   }
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i <= nkc) load_v(wave + NW * i, vf[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const bool table = table_off >= 0;
+  const int zero = table ? shift_exp_zero(a.frac_bits) : IW_SEXP_LUT - 1;
+  if (table)
+    for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
+      *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
+  for (int i = tid; i < QR; i += 64 * NW) sSum[i] = 0u;
+  for (int i = tid; i < QR * OLD; i += 64 * NW) sO[i] = 0u;
 
-  // the K operands of chunk c (keys past the last repeat it, head dims past D are zero)
-  auto load_k = [&](int c, v4i (&f)[4][KS]) {
-    const bool tree = c == nkc;
-    const int8_t *base = tree ? knew : kbase;
-    const int64_t st = tree ? t.kn_st : a.k_st;
-    const int last = (tree ? cnt : len) - 1, k0 = tree ? 0 : 64 * c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = min(k0 + 16 * (n >> 2) + 4 * i + (n & 3), last);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int d0 = 64 * ks + 16 * g;
-        f[i][ks] = v4i{0, 0, 0, 0};
-        if (d0 < D) f[i][ks] = *reinterpret_cast<const v4i *>(base + key * st + d0);
-      }
-    }
-  };
-  // the V operands: f[ks][c] holds column 64 ks + 4 n + c of the lane group's 16 keys
-  auto load_v = [&](int c, v4i (&f)[KS][4]) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d0 = 64 * ks + 4 * n;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[ks][i] = v4i{0, 0, 0, 0};
-      if (d0 >= D) continue;
-      if (c == nkc) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t w[4], o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = *reinterpret_cast<const uint32_t *>(vnew + (int64_t)min(16 * g + 4 * j + i, cnt - 1) * t.vn_st + d0);
-          transpose4(w, o);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[ks][i][j] = (int)o[i];
-        }
-      } else if (QUADS) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int quad = min(16 * c + 4 * g + j, (len - 1) >> 2);
-          const v4i w = *reinterpret_cast<const v4i *>(vbase + quad * a.v_sq + 4 * d0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[ks][i][j] = w[i];
-        }
-      } else {
-        const int key0 = min(64 * c + 16 * g, (len - 1) & ~15);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[ks][i] = *reinterpret_cast<const v4i *>(vbase + (int64_t)(d0 + i) * a.v_sd + key0);
-      }
-    }
-  };
   auto scores = [&](const v4i (&f)[KS], int u) {
     v4i s{0, 0, 0, 0};
 #pragma unroll
@@ -159,24 +234,41 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
     if (c == nkc) return (uint32_t)((vis[u] & in_use) >> (16 * g)) & 0xffffu;
     return (1u << clampi(len - 64 * c - 16 * g, 0, 16)) - 1u;
   };
-
   // ---- pass 1: row maximum of the raw scores ----
   int32_t mx[QT];
 #pragma unroll
   for (int u = 0; u < QT; ++u) mx[u] = INT32_MIN;
-  v4i kf[4][KS];
-  for (int c = wave; c <= nkc; c += NW) {
-    load_k(c, kf);
+  auto chunk_max = [&](int c, const v4i (&f)[4][KS]) {
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-      const uint32_t ok = counted(c, u);
+      if (c < nfk) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v4i s = scores(kf[i], u);
+        for (int i = 0; i < 4; ++i) {
+          const v4i s = scores(f[i], u);
+          mx[u] = max(max(mx[u], s[0]), s[1]);
+          mx[u] = max(max(mx[u], s[2]), s[3]);
+        }
+      } else {
+        const uint32_t ok = counted(c, u);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if ((ok >> (4 * i + r)) & 1u) mx[u] = max(mx[u], s[r]);
+        for (int i = 0; i < 4; ++i) {
+          const v4i s = scores(f[i], u);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((ok >> (4 * i + r)) & 1u) mx[u] = max(mx[u], s[r]);
+        }
       }
+    }
+  };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i <= nkc) chunk_max(wave + NW * i, kf[i]);
+  } else {
+#pragma unroll 1
+    for (int c = wave; c <= nkc; c += NW) {
+      load_k(c, kf[0]);
+      chunk_max(c, kf[0]);
     }
   }
 #pragma unroll
@@ -185,20 +277,22 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
     mx[u] = max(mx[u], __shfl_xor(mx[u], 32));
     if (lane < 16) sMax[wave][16 * u + lane] = mx[u];
   }
-  for (int i = tid; i < QR; i += 64 * NW) sSum[i] = 0u;
-  for (int i = tid; i < QR * OLD; i += 64 * NW) sO[i] = 0u;
-  __syncthreads();
+  lds_barrier();
   int32_t rowmax[QT];
+  bool sat = false;
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
 #pragma unroll
     for (int w = 0; w < NW; ++w) mx[u] = max(mx[u], sMax[w][16 * u + n]);
     // requantization keeps the order, so the maximum's is the maximum
     rowmax[u] = mx[u] == INT32_MIN ? -32768 : qk_requant16(mx[u], a.qk_m, a.qk_s);
+    sat = sat || rowmax[u] >= 32767;
   }
+  // the short index where no row maximum wraps: the keys that count lie at a
+  // distance of 1 at least, the others are taken for such
+  const bool brief = table && !__any(sat);
 
   // ---- pass 2: P and P.V over this wave's keys ----
-  const ShiftExp sexp(a.frac_bits);
   v4i o[QT][KS][4];
   uint32_t psum[QT];
 #pragma unroll
@@ -209,43 +303,76 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[u][ks][i] = v4i{0, 0, 0, 0};
   }
-  v4i vf[KS][4];
-  for (int c = wave; c <= nkc; c += NW) {
-    load_k(c, kf);
-    load_v(c, vf);
+  auto chunk_pv = [&](int c, const v4i (&f)[4][KS], const v4i (&vr)[KS][4]) {
+    v4i v[KS][4];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) v_operands(c, vr[ks], v[ks]);
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-      const ScoreIndex ix(a, rowmax[u]);
-      const uint32_t ok = counted(c, u);
-      v4i p;
+      ScoreIndex ix(a, rowmax[u], zero);
+      ix.flo = max(ix.flo, 1);
+      auto pv = [&](const v4i &p) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v4i s = scores(kf[i], u);
-        uint32_t w = 0;
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t e = (ok >> (4 * i + r)) & 1u ? sexp((int32_t)ix.any(s[r])) : 0u;
-          w |= (e & 0xffu) << (8 * r);
-        }
-        p[i] = (int)w;
-        psum[u] = __builtin_amdgcn_udot4(w, 0x01010101u, psum[u], false);
-      }
-      // P is unsigned and the product signed: a P of 128 (a row maximum of
-      // 32767 wraps) goes in as 0 and twice 64
-      v4i lo, hi;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lo[i] = p[i] & 0x7f7f7f7f, hi[i] = (int)(((uint32_t)p[i] >> 1) & 0x40404040u);
-      const bool any_hi = __any((hi[0] | hi[1] | hi[2] | hi[3]) != 0);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+          for (int i = 0; i < 4; ++i)
+            o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p, v[ks][i], o[u][ks][i], 0, 0, 0);
+      };
+      if (brief) {
+        v4i p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, vf[ks][i], o[u][ks][i], 0, 0, 0);
-          if (any_hi) {
-            o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, vf[ks][i], o[u][ks][i], 0, 0, 0);
-            o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, vf[ks][i], o[u][ks][i], 0, 0, 0);
-          }
+          const v4i s = scores(f[i], u);
+          p[i] = (int)((uint32_t)sTable[ix.full(s[0])] | (uint32_t)sTable[ix.full(s[1])] << 8 |
+                       (uint32_t)sTable[ix.full(s[2])] << 16 | (uint32_t)sTable[ix.full(s[3])] << 24);
         }
+        if (c >= nfk) {
+          const uint32_t ok = counted(c, u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] &= (int)byte_mask((ok >> (4 * i)) & 15u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) psum[u] = __builtin_amdgcn_udot4((uint32_t)p[i], 0x01010101u, psum[u], false);
+        pv(p);
+      } else {
+        const uint32_t ok = counted(c, u);
+        v4i p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4i s = scores(f[i], u);
+          uint32_t w = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t d = ix.any(s[r]);
+            const uint32_t e = table ? (uint32_t)sTable[d] : shift_exp((int32_t)d, a.frac_bits);
+            w |= ((ok >> (4 * i + r)) & 1u ? e & 0xffu : 0u) << (8 * r);
+          }
+          p[i] = (int)w;
+          psum[u] = __builtin_amdgcn_udot4(w, 0x01010101u, psum[u], false);
+        }
+        // P is unsigned and the product signed: a P of 128 (a row maximum of
+        // 32767 wraps) goes in as 0 and twice 64
+        v4i lo, hi;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lo[i] = p[i] & 0x7f7f7f7f, hi[i] = (int)(((uint32_t)p[i] >> 1) & 0x40404040u);
+        pv(lo);
+        if (__any((hi[0] | hi[1] | hi[2] | hi[3]) != 0)) {
+          pv(hi);
+          pv(hi);
+        }
+      }
+    }
+  };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i <= nkc) chunk_pv(wave + NW * i, kf[i], vf[i]);
+  } else {
+#pragma unroll 1
+    for (int c = wave; c <= nkc; c += NW) {
+      load_k(c, kf[0]);
+      load_v(c, vf[0]);
+      chunk_pv(c, kf[0], vf[0]);
     }
   }
 
@@ -263,14 +390,13 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
         for (int r = 0; r < 4; ++r)
           atomicAdd(&sO[(16 * u + 4 * g + r) * OLD + 64 * ks + 4 * n + i], (uint32_t)o[u][ks][i][r]);
   }
-  __syncthreads();
+  lds_barrier();
   if (tid < QR) sInv[tid] = fisr((int32_t)sSum[tid], a.rsqrt_off);
-  __syncthreads();
-  const int words = D / 4;
-  for (int i = tid; i < N * words; i += 64 * NW) {
-    const int q = i / words, d = 4 * (i % words);
+  lds_barrier();
+  for (int i = tid; i < rows * words; i += 64 * NW) {
+    const int q = by_words(i), d = 4 * (i - q * words);
     uint32_t w = 0;
-    if (q < cnt) {
+    if (q0 + q < cnt) {
       const int32_t inv = sInv[q];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -280,33 +406,48 @@ __global__ __launch_bounds__(64 * NW) void attn_tree_kernel(TreeArgs t) {
         w |= ((uint32_t)clampi(y, -127, 127) & 0xffu) << (8 * c);
       }
     }
-    *reinterpret_cast<uint32_t *>(a.out + b * a.o_sb + (int64_t)q * a.o_st + (int64_t)h * D + d) = w;
+    *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + q) * a.o_st + d) = w;
   }
 }
 
-template <int KS, bool QUADS, int QT>
+constexpr int kCus = 256;
+#ifndef FEW16
+#define FEW16 512
+#endif
+
+template <int KS, bool QUADS, int QT, int NW, int NC>
 int launch_tree(const TreeArgs &t, hipStream_t s) {
-  constexpr int NW = 4;
-  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW>), dim3((unsigned)(t.a.B * t.a.H)), dim3(64 * NW), 0, s, t);
+  const int qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT), blocks = qblocks * t.a.B * t.a.H, per_xcd = (blocks + 7) / 8;
+  const int words = t.a.D / 4, per_word = (65536 + words - 1) / words;
+  const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
+  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t,
+                     qblocks, blocks, per_xcd, per_word, table);
   return check_launch("attn_tree_kernel");
 }
 
-template <int KS, bool QUADS>
+template <int KS, bool QUADS, int QT>
 int launch_tree_q(const TreeArgs &t, hipStream_t s) {
-  switch ((t.a.Tq + 15) / 16) {
-    case 1: return launch_tree<KS, QUADS, 1>(t, s);
-    case 2: return launch_tree<KS, QUADS, 2>(t, s);
-    case 3: return launch_tree<KS, QUADS, 3>(t, s);
-    default: return launch_tree<KS, QUADS, 4>(t, s);
-  }
+  const int chunks = (t.a.Tk + 63) / 64 + 1;
+  const int64_t blocks = (int64_t)t.a.B * t.a.H * ((t.a.Tq + 16 * QT - 1) / (16 * QT));
+  if (chunks <= 8 && (blocks <= 2 * kCus || chunks <= 4)) return launch_tree<KS, QUADS, QT, 8, 1>(t, s);
+  if (chunks <= 8) return launch_tree<KS, QUADS, QT, 4, 2>(t, s);
+  if (QT == 1 && blocks <= FEW16) return launch_tree<KS, QUADS, 1, 16, 0>(t, s);
+  return launch_tree<KS, QUADS, QT, 8, 0>(t, s);
+}
+
+template <int KS, bool QUADS>
+int launch_tree_k(const TreeArgs &t, hipStream_t s) {
+  const int64_t heads = (int64_t)t.a.B * t.a.H;
+  if (t.a.Tq <= 16 || heads * ((t.a.Tq + 15) / 16) <= 2 * kCus) return launch_tree_q<KS, QUADS, 1>(t, s);
+  return launch_tree_q<KS, QUADS, 2>(t, s);
 }
 
 }  // namespace
 
 int launch_attn_tree(const TreeArgs &t, hipStream_t s) {
   const bool quads = t.a.v_sq != 4;
-  if (t.a.D <= 64) return quads ? launch_tree_q<1, true>(t, s) : launch_tree_q<1, false>(t, s);
-  return quads ? launch_tree_q<2, true>(t, s) : launch_tree_q<2, false>(t, s);
+  if (t.a.D <= 64) return quads ? launch_tree_k<1, true>(t, s) : launch_tree_k<1, false>(t, s);
+  return quads ? launch_tree_k<2, true>(t, s) : launch_tree_k<2, false>(t, s);
 }
 
 }  // namespace iw
