@@ -78,11 +78,24 @@ __device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&o
   out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
+// Four columns of a row's output from their sums and the row's inverse square root.
+__device__ __forceinline__ uint32_t output_word(const AttnArgs &a, const uint32_t *sums, int32_t inv) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    int32_t y = rshift((int32_t)(sums[c] * (uint32_t)inv), a.rsqrt_off);
+    y = rshift((int32_t)((uint32_t)y * (uint32_t)inv), a.rsqrt_off);
+    y = rshift((int32_t)((uint32_t)y * a.av_m), a.av_s);
+    w |= ((uint32_t)clampi(y, -127, 127) & 0xffu) << (8 * c);
+  }
+  return w;
+}
+
 // KS: 64-column parts of the head; QUADS: V in key quads; QT: 16-query tiles of
 // the block; NW waves; NC > 0: a wave has at most NC chunks, whose K and V
 // are all requested at the start and kept.
 template <int KS, bool QUADS, int QT, int NW, int NC>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2 && KS == 1 ? (QT == 1 ? 4 : 3) : NC == 1 && KS * QT <= 2 ? 4 : NW == 16 ? 4 : 2))) void attn_tree_kernel(TreeArgs t, int qblocks, int blocks, int per_xcd,
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2 && KS == 1 ? (QT == 1 ? 4 : 3) : NC == 1 && KS * QT <= 2 ? 4 : NC == 0 && QT * KS == 1 ? 4 : 2))) void attn_tree_kernel(TreeArgs t, int qblocks, int blocks, int per_xcd,
                                                        int per_word, int table_off) {
   constexpr int QR = 16 * QT, OLD = 64 * KS + 4, HC = NC > 0 ? NC : 1;
   __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
@@ -128,8 +141,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
   // last ones (the query is zero there). A chunk's base is uniform, its lanes'
   // offsets fit 32 bits.
   const int kcol = 16 * g, key0 = 16 * (n >> 2) + (n & 3);
-  auto load_k = [&](int c, v4i (&f)[4][KS]) {
-    const bool tree = c == nkc;
+  auto load_k = [&](int c, bool tree, v4i (&f)[4][KS]) {
     const uint32_t st = (uint32_t)(tree ? t.kn_st : a.k_st);
     const int8_t *base = tree ? knew : kbase + (int64_t)(64 * c) * a.k_st;
     const int last = (tree ? cnt : len - 64 * c) - 1;
@@ -141,37 +153,34 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
                                                           (uint32_t)min(64 * ks + kcol, D - 16)));
   };
   // What the V operands are made of: quads and transposed rows hold words of four
-  // keys of one column, the tree's rows (word j of f[ks][i] from node 16 g + 4 j + i) four
+  // keys of one column, the tree's rows (word j of f[i] from node 16 g + 4 j + i) four
   // columns. Columns past D repeat the last ones; their sums are not stored.
-  auto load_v = [&](int c, v4i (&f)[KS][4]) {
+  auto load_v = [&](int c, bool tree, int ks, v4i (&f)[4]) {
+    const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
+    if (tree) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
-      if (c == nkc) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            f[ks][i][j] = *reinterpret_cast<const int32_t *>(
-                vnew + ((uint32_t)min(16 * g + 4 * j + i, cnt - 1) * (uint32_t)t.vn_st + d0));
-      } else if (QUADS) {
-        const int8_t *base = vbase + (int64_t)(16 * c) * a.v_sq;
-        const int last = ((len - 1) >> 2) - 16 * c;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          f[ks][j] = *reinterpret_cast<const v4i *>(base + ((uint32_t)min(4 * g + j, last) * (uint32_t)a.v_sq + 4 * d0));
-      } else {
-        const int8_t *base = vbase + 64 * c;
-        const uint32_t at = (uint32_t)min(16 * g, (len - 1 - 64 * c) & ~15);
+          f[i][j] = *reinterpret_cast<const int32_t *>(
+              vnew + ((uint32_t)min(16 * g + 4 * j + i, cnt - 1) * (uint32_t)t.vn_st + d0));
+    } else if (QUADS) {
+      const int8_t *base = vbase + (int64_t)(16 * c) * a.v_sq;
+      const int last = ((len - 1) >> 2) - 16 * c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[ks][i] = *reinterpret_cast<const v4i *>(base + ((d0 + i) * (uint32_t)a.v_sd + at));
-      }
+      for (int j = 0; j < 4; ++j)
+        f[j] = *reinterpret_cast<const v4i *>(base + ((uint32_t)min(4 * g + j, last) * (uint32_t)a.v_sq + 4 * d0));
+    } else {
+      const int8_t *base = vbase + 64 * c;
+      const uint32_t at = (uint32_t)min(16 * g, (len - 1 - 64 * c) & ~15);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        f[i] = *reinterpret_cast<const v4i *>(base + ((d0 + i) * (uint32_t)a.v_sd + at));
     }
   };
   // the operand of product i: column 64 ks + 4 n + i of the lane group's 16 keys
-  auto v_operands = [&](int c, const v4i (&f)[4], v4i (&o)[4]) {
-    if (c == nkc) {
+  auto v_operands = [&](bool tree, const v4i (&f)[4], v4i (&o)[4]) {
+    if (tree) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t in[4] = {(uint32_t)f[0][j], (uint32_t)f[1][j], (uint32_t)f[2][j], (uint32_t)f[3][j]};
@@ -192,8 +201,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
   v4i kf[HC][4][KS], vf[HC][KS][4];
   if constexpr (NC > 0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (wave + NW * i <= nkc) load_k(wave + NW * i, kf[i]);
+    for (int i = 0; i < NC; ++i) {
+      const int c = wave + NW * i;
+      if (c <= nkc) load_k(c, c == nkc, kf[i]);
+    }
   }
   v4i qf[QT][KS];
   uint64_t vis[QT];
@@ -210,8 +221,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
   }
   if constexpr (NC > 0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (wave + NW * i <= nkc) load_v(wave + NW * i, vf[i]);
+    for (int i = 0; i < NC; ++i) {
+      const int c = wave + NW * i;
+      if (c <= nkc) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) load_v(c, c == nkc, ks, vf[i][ks]);
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);
   }
   const bool table = table_off >= 0;
@@ -230,15 +246,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
   };
   // which of the lane group's 16 keys of chunk c count for this lane's query of tile u
   const uint64_t in_use = cnt == 64 ? ~0ull : (1ull << cnt) - 1;
-  auto counted = [&](int c, int u) -> uint32_t {
-    if (c == nkc) return (uint32_t)((vis[u] & in_use) >> (16 * g)) & 0xffffu;
+  auto counted = [&](int c, bool tree, int u) -> uint32_t {
+    if (tree) return (uint32_t)((vis[u] & in_use) >> (16 * g)) & 0xffffu;
     return (1u << clampi(len - 64 * c - 16 * g, 0, 16)) - 1u;
   };
   // ---- pass 1: row maximum of the raw scores ----
   int32_t mx[QT];
 #pragma unroll
   for (int u = 0; u < QT; ++u) mx[u] = INT32_MIN;
-  auto chunk_max = [&](int c, const v4i (&f)[4][KS]) {
+  auto chunk_max = [&](int c, bool tree, const v4i (&f)[4][KS]) {
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
       if (c < nfk) {
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
           mx[u] = max(max(mx[u], s[2]), s[3]);
         }
       } else {
-        const uint32_t ok = counted(c, u);
+        const uint32_t ok = counted(c, tree, u);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const v4i s = scores(f[i], u);
@@ -262,13 +278,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
   };
   if constexpr (NC > 0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (wave + NW * i <= nkc) chunk_max(wave + NW * i, kf[i]);
+    for (int i = 0; i < NC; ++i) {
+      const int c = wave + NW * i;
+      if (c <= nkc) chunk_max(c, c == nkc, kf[i]);
+    }
   } else {
+    v4i kn[4][KS];
 #pragma unroll 1
-    for (int c = wave; c <= nkc; c += NW) {
-      load_k(c, kf[0]);
-      chunk_max(c, kf[0]);
+    for (int c = wave; c < nkc; c += 2 * NW) {
+      load_k(c, false, kf[0]);
+      if (c + NW < nkc) load_k(c + NW, false, kn);
+      chunk_max(c, false, kf[0]);
+      if (c + NW < nkc) chunk_max(c + NW, false, kn);
+    }
+    if (nkc % NW == wave) {
+      load_k(nkc, true, kf[0]);
+      chunk_max(nkc, true, kf[0]);
     }
   }
 #pragma unroll
@@ -303,40 +328,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[u][ks][i] = v4i{0, 0, 0, 0};
   }
-  auto chunk_pv = [&](int c, const v4i (&f)[4][KS], const v4i (&vr)[KS][4]) {
-    v4i v[KS][4];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) v_operands(c, vr[ks], v[ks]);
+  // P of chunk c as the operands of its products; hi where a P of 128 (a row maximum
+  // of 32767 wraps) is left out, as the product is signed: it goes in as twice 64
+  auto chunk_p = [&](int c, bool tree, const v4i (&f)[4][KS], v4i (&p)[QT], v4i (&hi)[QT]) {
+    bool any_hi = false;
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
       ScoreIndex ix(a, rowmax[u], zero);
       ix.flo = max(ix.flo, 1);
-      auto pv = [&](const v4i &p) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p, v[ks][i], o[u][ks][i], 0, 0, 0);
-      };
       if (brief) {
-        v4i p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const v4i s = scores(f[i], u);
-          p[i] = (int)((uint32_t)sTable[ix.full(s[0])] | (uint32_t)sTable[ix.full(s[1])] << 8 |
-                       (uint32_t)sTable[ix.full(s[2])] << 16 | (uint32_t)sTable[ix.full(s[3])] << 24);
+          p[u][i] = (int)((uint32_t)sTable[ix.full(s[0])] | (uint32_t)sTable[ix.full(s[1])] << 8 |
+                          (uint32_t)sTable[ix.full(s[2])] << 16 | (uint32_t)sTable[ix.full(s[3])] << 24);
         }
         if (c >= nfk) {
-          const uint32_t ok = counted(c, u);
+          const uint32_t ok = counted(c, tree, u);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] &= (int)byte_mask((ok >> (4 * i)) & 15u);
+          for (int i = 0; i < 4; ++i) p[u][i] &= (int)byte_mask((ok >> (4 * i)) & 15u);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) psum[u] = __builtin_amdgcn_udot4((uint32_t)p[i], 0x01010101u, psum[u], false);
-        pv(p);
+        for (int i = 0; i < 4; ++i) psum[u] = __builtin_amdgcn_udot4((uint32_t)p[u][i], 0x01010101u, psum[u], false);
       } else {
-        const uint32_t ok = counted(c, u);
-        v4i p;
+        const uint32_t ok = counted(c, tree, u);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const v4i s = scores(f[i], u);
@@ -347,33 +362,56 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
             const uint32_t e = table ? (uint32_t)sTable[d] : shift_exp((int32_t)d, a.frac_bits);
             w |= ((ok >> (4 * i + r)) & 1u ? e & 0xffu : 0u) << (8 * r);
           }
-          p[i] = (int)w;
           psum[u] = __builtin_amdgcn_udot4(w, 0x01010101u, psum[u], false);
+          p[u][i] = (int)(w & 0x7f7f7f7fu), hi[u][i] = (int)((w >> 1) & 0x40404040u);
         }
-        // P is unsigned and the product signed: a P of 128 (a row maximum of
-        // 32767 wraps) goes in as 0 and twice 64
-        v4i lo, hi;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lo[i] = p[i] & 0x7f7f7f7f, hi[i] = (int)(((uint32_t)p[i] >> 1) & 0x40404040u);
-        pv(lo);
-        if (__any((hi[0] | hi[1] | hi[2] | hi[3]) != 0)) {
-          pv(hi);
-          pv(hi);
-        }
+        any_hi = any_hi || (hi[u][0] | hi[u][1] | hi[u][2] | hi[u][3]) != 0;
       }
     }
+    return __any(any_hi) != 0;
   };
+  auto chunk_pv = [&](bool tree, int ks, const v4i (&vr)[4], const v4i (&p)[QT], const v4i (&hi)[QT], bool any_hi) {
+    v4i v[4];
+    v_operands(tree, vr, v);
+    auto pv = [&](const v4i (&x)[QT]) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u], v[i], o[u][ks][i], 0, 0, 0);
+    };
+    pv(p);
+    if (any_hi) {
+      pv(hi);
+      pv(hi);
+    }
+  };
+  v4i p[QT], hi[QT];
   if constexpr (NC > 0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (wave + NW * i <= nkc) chunk_pv(wave + NW * i, kf[i], vf[i]);
-  } else {
-#pragma unroll 1
-    for (int c = wave; c <= nkc; c += NW) {
-      load_k(c, kf[0]);
-      load_v(c, vf[0]);
-      chunk_pv(c, kf[0], vf[0]);
+    for (int i = 0; i < NC; ++i) {
+      const int c = wave + NW * i;
+      if (c <= nkc) {
+        const bool any_hi = chunk_p(c, c == nkc, kf[i], p, hi);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) chunk_pv(c == nkc, ks, vf[i][ks], p, hi, any_hi);
+      }
     }
+  } else {
+    auto chunk = [&](int c, bool tree) {
+      load_k(c, tree, kf[0]);
+      load_v(c, tree, 0, vf[0][0]);
+      const bool any_hi = chunk_p(c, tree, kf[0], p, hi);
+      // the second half of a wide head's V follows where K was
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks > 0) load_v(c, tree, ks, vf[0][0]);
+        chunk_pv(tree, ks, vf[0][0], p, hi, any_hi);
+      }
+    };
+#pragma unroll 1
+    for (int c = wave; c < nkc; c += NW) chunk(c, false);
+    if (nkc % NW == wave) chunk(nkc, true);
   }
 
   // ---- the waves' sums meet in LDS ----
@@ -396,32 +434,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2
   for (int i = tid; i < rows * words; i += 64 * NW) {
     const int q = by_words(i), d = 4 * (i - q * words);
     uint32_t w = 0;
-    if (q0 + q < cnt) {
-      const int32_t inv = sInv[q];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        int32_t y = rshift((int32_t)(sO[q * OLD + d + c] * (uint32_t)inv), a.rsqrt_off);
-        y = rshift((int32_t)((uint32_t)y * (uint32_t)inv), a.rsqrt_off);
-        y = rshift((int32_t)((uint32_t)y * a.av_m), a.av_s);
-        w |= ((uint32_t)clampi(y, -127, 127) & 0xffu) << (8 * c);
-      }
-    }
+    if (q0 + q < cnt) w = output_word(a, &sO[q * OLD + d], sInv[q]);
     *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + q) * a.o_st + d) = w;
   }
 }
 
 constexpr int kCus = 256;
-#ifndef FEW16
-#define FEW16 512
-#endif
 
 template <int KS, bool QUADS, int QT, int NW, int NC>
 int launch_tree(const TreeArgs &t, hipStream_t s) {
   const int qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT), blocks = qblocks * t.a.B * t.a.H, per_xcd = (blocks + 7) / 8;
   const int words = t.a.D / 4, per_word = (65536 + words - 1) / words;
   const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
-  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t,
-                     qblocks, blocks, per_xcd, per_word, table);
+  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t, qblocks, blocks, per_xcd, per_word, table);
   return check_launch("attn_tree_kernel");
 }
 
@@ -431,7 +456,6 @@ int launch_tree_q(const TreeArgs &t, hipStream_t s) {
   const int64_t blocks = (int64_t)t.a.B * t.a.H * ((t.a.Tq + 16 * QT - 1) / (16 * QT));
   if (chunks <= 8 && (blocks <= 2 * kCus || chunks <= 4)) return launch_tree<KS, QUADS, QT, 8, 1>(t, s);
   if (chunks <= 8) return launch_tree<KS, QUADS, QT, 4, 2>(t, s);
-  if (QT == 1 && blocks <= FEW16) return launch_tree<KS, QUADS, 1, 16, 0>(t, s);
   return launch_tree<KS, QUADS, QT, 8, 0>(t, s);
 }
 

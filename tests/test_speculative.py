@@ -146,12 +146,20 @@ def test_tree_attention_caches(iw, oracle, gpu, cap, D, N, layout):
     assert np.array_equal(host(c.run(iw)), c.expected(oracle))
 
 
-@pytest.mark.parametrize("B,H", [(1, 20), (40, 20), (129, 3)])
-def test_tree_attention_grids(iw, oracle, gpu, B, H):
-    print("case: tree attention grid", B, H, flush=True)
+@pytest.mark.parametrize("layout", ["vt", "quads"])
+@pytest.mark.parametrize("B,H,D,cap,N", [(1, 20, 64, 100, 7), (40, 20, 64, 100, 7), (129, 3, 64, 100, 7),
+                                         (65, 9, 64, 448, 33), (90, 6, 96, 448, 20), (300, 1, 64, 460, 3),
+                                         (60, 9, 64, 500, 18), (60, 9, 128, 500, 18), (1, 1, 64, 100000, 2)])
+def test_tree_attention_grids(iw, oracle, gpu, B, H, D, cap, N, layout):
+    """Few and many blocks, one and two tiles of nodes a block, caches above 448 positions with
+    their keys in one block and shared by several."""
+    print("case: tree attention grid", B, H, D, cap, N, layout, flush=True)
     r = gen.rng(B)
-    c = Case(B + H, B, H, 64, 100, 7, r.integers(0, 101, B), r.integers(0, 8, B), "quads")
-    assert np.array_equal(host(c.run(iw)), c.expected(oracle))
+    c = Case(B + H, B, H, D, cap, N, r.integers(0, cap + 1, B), r.integers(0, N + 1, B), layout)
+    c.lengths[0], c.counts[0] = cap, N
+    c.visible = words(c.parents, c.counts)
+    rows = sorted({0, B - 1, *r.integers(0, B, 12).tolist()})
+    assert np.array_equal(host(c.run(iw))[rows], c.expected(oracle, rows)[rows])
 
 
 @pytest.mark.parametrize("f", range(1, 14))
