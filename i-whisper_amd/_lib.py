@@ -104,11 +104,8 @@ SIGNATURES = {
                                        _p, _i64, _i64, _p],
     "iw_classifier_frag": [_p, _p, _u32, _i8, _p, _i64, _i64, _i64, _p],
     "iw_tree_plan": [_p, _i64, _p, _p, _i64, _i64, _i32, _p, _p, _p],
-    "iw_attention_tree": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
-                          _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _u8, _i8, _i32, _u8,
-                          _i8, _u32, _p],
-    "iw_tree_accept": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p,
-                       _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p],
+    "iw_attention_tree": [_p, _p],
+    "iw_tree_accept": [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _p],
     "iw_token_logprobs": [_p, _i32, _i64, _i64, _i64, _f, _p, _p, _p, _p, _i64, _p, _p, _p, _p],
 }
 

@@ -927,96 +927,95 @@ int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *coun
                           reinterpret_cast<uint64_t *>(visible), positions, as_stream(stream));
 }
 
-int iw_attention_tree(const int8_t *q, int64_t q_sb, int64_t q_st, const int8_t *k_new, int64_t kn_sb,
-                      int64_t kn_st, const int8_t *v_new, int64_t vn_sb, int64_t vn_st, const int8_t *k,
-                      int64_t k_sb, int64_t k_sh, int64_t k_st, const int8_t *vt, int64_t v_sb, int64_t v_sh,
-                      int64_t v_sd, int64_t v_sq, const int32_t *lengths, const int64_t *visible,
-                      int64_t visible_sb, const int32_t *counts, int8_t *out, int64_t o_sb, int64_t o_st,
-                      int64_t batch, int64_t heads, int64_t nodes, int64_t head_dim, int64_t cache_positions,
-                      uint8_t qk_multiplier, int8_t qk_shift, int32_t frac_bits, uint8_t av_multiplier,
-                      int8_t av_shift, uint32_t rsqrt_offset, iw_stream_t stream) {
-  IW_REQUIRE(frac_bits > 0 && frac_bits < 14, "frac_bits must be in [1, 14)");
-  IW_REQUIRE(rsqrt_offset <= 29, "rsqrt_offset must be in [0,29]");
-  IW_REQUIRE(nodes > 0 && nodes <= kTreeMaxNodes, "a tree has 1 to 64 nodes");
-  const int rc = check_tree_cache(heads, head_dim, cache_positions, v_sd, v_sq);
+int iw_attention_tree(const iw_attention_tree_args *args, iw_stream_t stream) {
+  IW_REQUIRE(args, "null arguments");
+  const iw_attention_tree_args &p = *args;
+  IW_REQUIRE(p.frac_bits > 0 && p.frac_bits < 14, "frac_bits must be in [1, 14)");
+  IW_REQUIRE(p.rsqrt_offset >= 0 && p.rsqrt_offset <= 29, "rsqrt_offset must be in [0,29]");
+  IW_REQUIRE(p.qk_multiplier >= 0 && p.qk_multiplier <= 255 && p.av_multiplier >= 0 && p.av_multiplier <= 255,
+             "multipliers must be uint8");
+  IW_REQUIRE(p.qk_shift >= -128 && p.qk_shift <= 127 && p.av_shift >= -128 && p.av_shift <= 127,
+             "shifts must be int8");
+  IW_REQUIRE(p.nodes > 0 && p.nodes <= kTreeMaxNodes, "a tree has 1 to 64 nodes");
+  const int rc = check_tree_cache(p.heads, p.head_dim, p.cache_positions, p.v_sd, p.v_sq);
   if (rc) return rc;
-  IW_REQUIRE(batch >= 0 && batch * heads <= (1 << 22) && visible_sb >= 0, "invalid attention shape");
-  if (batch == 0) return IW_OK;
-  IW_REQUIRE(q && k_new && v_new && k && vt && lengths && visible && out, "null tensor pointer");
+  IW_REQUIRE(p.batch >= 0 && p.batch <= (1 << 22) && p.batch * p.heads <= (1 << 22) && p.visible_sb >= 0,
+             "invalid attention shape");
+  if (p.batch == 0) return IW_OK;
+  IW_REQUIRE(p.q && p.k_new && p.v_new && p.k && p.vt && p.lengths && p.visible && p.out, "null tensor pointer");
   const uintptr_t align =
-      reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new) |
-      reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(vt) | reinterpret_cast<uintptr_t>(out) |
-      (uintptr_t)(q_sb | q_st | kn_sb | kn_st | vn_sb | vn_st | k_sb | k_sh | k_st | v_sb | v_sh | o_sb | o_st) |
-      (uintptr_t)(v_sq != 4 ? v_sq : v_sd);
+      reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k_new) | reinterpret_cast<uintptr_t>(p.v_new) |
+      reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.vt) | reinterpret_cast<uintptr_t>(p.out) |
+      (uintptr_t)(p.q_sb | p.q_st | p.kn_sb | p.kn_st | p.vn_sb | p.vn_st | p.k_sb | p.k_sh | p.k_st | p.v_sb | p.v_sh |
+                  p.o_sb | p.o_st) |
+      (uintptr_t)(p.v_sq != 4 ? p.v_sq : p.v_sd);
   IW_REQUIRE((align & 15) == 0, "tree attention operands must be 16-byte aligned");
   // offsets within 64 keys or nodes and within a head's transposed rows are 32-bit numbers
   const int64_t far = 1 << 25;
-  IW_REQUIRE(kn_st >= 0 && kn_st < far && vn_st >= 0 && vn_st < far && k_st >= 0 && k_st < far && v_sq >= 0 &&
-                 v_sq < far && v_sd >= 0 && v_sd < far,
+  IW_REQUIRE(p.kn_st >= 0 && p.kn_st < far && p.vn_st >= 0 && p.vn_st < far && p.k_st >= 0 && p.k_st < far &&
+                 p.v_sq >= 0 && p.v_sq < far && p.v_sd >= 0 && p.v_sd < far,
              "strides of nodes, keys, key quads and transposed rows must be below 2^25");
   TreeArgs t;
   AttnArgs &a = t.a;
-  a.q = q;
-  a.q_sb = q_sb;
-  a.q_st = q_st;
-  a.k = k;
-  a.k_sb = k_sb;
-  a.k_sh = k_sh;
-  a.k_st = k_st;
-  a.vt = vt;
-  a.v_sb = v_sb;
-  a.v_sh = v_sh;
-  a.v_sd = v_sd;
-  a.v_sq = v_sq;
-  a.out = out;
-  a.o_sb = o_sb;
-  a.o_st = o_st;
-  a.B = (int32_t)batch;
-  a.H = (int32_t)heads;
-  a.Tq = (int32_t)nodes;
-  a.Tk = (int32_t)cache_positions;
-  a.D = (int32_t)head_dim;
-  a.qk_m = qk_multiplier;
-  a.qk_s = (uint32_t)(qk_shift > 0 ? qk_shift : 0);
-  a.frac_bits = frac_bits;
-  a.av_m = av_multiplier;
-  a.av_s = (uint32_t)(av_shift < 0 ? 0 : (av_shift > 32 ? 32 : av_shift));
-  a.rsqrt_off = rsqrt_offset;
-  t.kn = k_new;
-  t.kn_sb = kn_sb;
-  t.kn_st = kn_st;
-  t.vn = v_new;
-  t.vn_sb = vn_sb;
-  t.vn_st = vn_st;
-  t.lengths = lengths;
-  t.visible = reinterpret_cast<const uint64_t *>(visible);
-  t.vis_sb = visible_sb;
-  t.counts = counts;
+  a.q = p.q;
+  a.q_sb = p.q_sb;
+  a.q_st = p.q_st;
+  a.k = p.k;
+  a.k_sb = p.k_sb;
+  a.k_sh = p.k_sh;
+  a.k_st = p.k_st;
+  a.vt = p.vt;
+  a.v_sb = p.v_sb;
+  a.v_sh = p.v_sh;
+  a.v_sd = p.v_sd;
+  a.v_sq = p.v_sq;
+  a.out = p.out;
+  a.o_sb = p.o_sb;
+  a.o_st = p.o_st;
+  a.B = (int32_t)p.batch;
+  a.H = (int32_t)p.heads;
+  a.Tq = (int32_t)p.nodes;
+  a.Tk = (int32_t)p.cache_positions;
+  a.D = (int32_t)p.head_dim;
+  a.qk_m = (uint32_t)p.qk_multiplier;
+  a.qk_s = (uint32_t)(p.qk_shift > 0 ? p.qk_shift : 0);
+  a.frac_bits = (int32_t)p.frac_bits;
+  a.av_m = (uint32_t)p.av_multiplier;
+  a.av_s = (uint32_t)(p.av_shift < 0 ? 0 : (p.av_shift > 32 ? 32 : p.av_shift));
+  a.rsqrt_off = (uint32_t)p.rsqrt_offset;
+  t.kn = p.k_new;
+  t.kn_sb = p.kn_sb;
+  t.kn_st = p.kn_st;
+  t.vn = p.v_new;
+  t.vn_sb = p.vn_sb;
+  t.vn_st = p.vn_st;
+  t.lengths = p.lengths;
+  t.visible = reinterpret_cast<const uint64_t *>(p.visible);
+  t.vis_sb = p.visible_sb;
+  t.counts = p.counts;
   return launch_attn_tree(t, as_stream(stream));
 }
 
-int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t *choice, const int32_t *counts,
-                   const int32_t *lengths, int64_t batch, int64_t nodes, int64_t eot, int32_t *path,
-                   int32_t *accepted, int64_t *next, int32_t *lengths_out, int64_t layers,
-                   const int8_t *const *k_new, const int8_t *const *v_new, int64_t kn_sb, int64_t kn_st,
-                   int64_t vn_sb, int64_t vn_st, int8_t *const *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
-                   int8_t *const *v, int64_t v_sb, int64_t v_sh, int64_t v_sd, int64_t v_sq, int64_t heads,
-                   int64_t head_dim, int64_t cache_positions, iw_stream_t stream) {
-  IW_REQUIRE(batch >= 0 && batch <= (1 << 20) && nodes > 0 && nodes <= kTreeMaxNodes,
+int iw_tree_accept(const iw_tree_caches *caches, const int64_t *tokens, const int32_t *parents,
+                   const int64_t *choice, const int32_t *counts, const int32_t *lengths, int64_t eot,
+                   int32_t *path, int32_t *accepted, int64_t *next, int32_t *lengths_out, iw_stream_t stream) {
+  IW_REQUIRE(caches, "null arguments");
+  const iw_tree_caches &c = *caches;
+  IW_REQUIRE(c.batch >= 0 && c.batch <= (1 << 20) && c.nodes > 0 && c.nodes <= kTreeMaxNodes,
              "invalid tree shape (at most 64 nodes)");
-  IW_REQUIRE(layers >= 0 && layers <= 4096, "invalid number of layers");
-  const int rc = check_tree_cache(heads, head_dim, cache_positions, v_sd, v_sq);
+  IW_REQUIRE(c.layers >= 0 && c.layers <= 4096, "invalid number of layers");
+  const int rc = check_tree_cache(c.heads, c.head_dim, c.cache_positions, c.v_sd, c.v_sq);
   if (rc) return rc;
-  if (batch == 0) return IW_OK;
+  if (c.batch == 0) return IW_OK;
   IW_REQUIRE(tokens && parents && choice && lengths && path && accepted && next && lengths_out, "null tensor pointer");
   // the blocks of a row's layers read its length while one of them writes the new one
-  IW_REQUIRE(apart(lengths, 4 * batch, lengths_out, 4 * batch), "lengths_out must not be part of lengths");
-  IW_REQUIRE(layers == 0 || (k_new && v_new && k && v), "null array of layer pointers");
-  uintptr_t align = (uintptr_t)(kn_sb | kn_st | vn_sb | vn_st | k_sb | k_sh | k_st);
-  for (int64_t i = 0; i < layers; ++i) {
-    IW_REQUIRE(k_new[i] && v_new[i] && k[i] && v[i], "null tensor pointer");
-    align |= reinterpret_cast<uintptr_t>(k_new[i]) | reinterpret_cast<uintptr_t>(v_new[i]) |
-             reinterpret_cast<uintptr_t>(k[i]);
+  IW_REQUIRE(apart(lengths, 4 * c.batch, lengths_out, 4 * c.batch), "lengths_out must not be part of lengths");
+  IW_REQUIRE(c.layers == 0 || (c.k_new && c.v_new && c.k && c.v), "null array of layer pointers");
+  uintptr_t align = (uintptr_t)(c.kn_sb | c.kn_st | c.vn_sb | c.vn_st | c.k_sb | c.k_sh | c.k_st);
+  for (int64_t i = 0; i < c.layers; ++i) {
+    IW_REQUIRE(c.k_new[i] && c.v_new[i] && c.k[i] && c.v[i], "null tensor pointer");
+    align |= reinterpret_cast<uintptr_t>(c.k_new[i]) | reinterpret_cast<uintptr_t>(c.v_new[i]) |
+             reinterpret_cast<uintptr_t>(c.k[i]);
   }
   IW_REQUIRE((align & 3) == 0, "the nodes' K and V and the K caches must be 4-byte aligned");
   TreeAcceptArgs t;
@@ -1025,41 +1024,41 @@ int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t 
   t.parents = parents;
   t.counts = counts;
   t.lengths = lengths;
-  t.tok_ld = t.ch_ld = t.p_ld = nodes;
+  t.tok_ld = t.ch_ld = t.p_ld = c.nodes;
   t.eot = eot;
   t.path = path;
   t.accepted = accepted;
   t.next = next;
   t.lengths_out = lengths_out;
-  t.nodes = (int)nodes;
-  t.cap = (int)cache_positions;
-  t.heads = (int)heads;
-  t.D = (int)head_dim;
-  t.kn_sb = kn_sb;
-  t.kn_st = kn_st;
-  t.vn_sb = vn_sb;
-  t.vn_st = vn_st;
-  t.k_sb = k_sb;
-  t.k_sh = k_sh;
-  t.k_st = k_st;
-  t.v_sb = v_sb;
-  t.v_sh = v_sh;
-  t.v_sd = v_sd;
-  t.v_sq = v_sq;
+  t.nodes = (int)c.nodes;
+  t.cap = (int)c.cache_positions;
+  t.heads = (int)c.heads;
+  t.D = (int)c.head_dim;
+  t.kn_sb = c.kn_sb;
+  t.kn_st = c.kn_st;
+  t.vn_sb = c.vn_sb;
+  t.vn_st = c.vn_st;
+  t.k_sb = c.k_sb;
+  t.k_sh = c.k_sh;
+  t.k_st = c.k_st;
+  t.v_sb = c.v_sb;
+  t.v_sh = c.v_sh;
+  t.v_sd = c.v_sd;
+  t.v_sq = c.v_sq;
   int64_t first = 0;
   do {
-    const int n = (int)(layers - first < kTreeMaxLayers ? layers - first : kTreeMaxLayers);
+    const int n = (int)(c.layers - first < kTreeMaxLayers ? c.layers - first : kTreeMaxLayers);
     TreeLayers l = {};
     for (int i = 0; i < n; ++i) {
-      l.kn[i] = k_new[first + i];
-      l.vn[i] = v_new[first + i];
-      l.k[i] = k[first + i];
-      l.v[i] = v[first + i];
+      l.kn[i] = c.k_new[first + i];
+      l.vn[i] = c.v_new[first + i];
+      l.k[i] = c.k[first + i];
+      l.v[i] = c.v[first + i];
     }
-    const int r = launch_tree_accept(t, l, n, batch, first == 0, as_stream(stream));
+    const int r = launch_tree_accept(t, l, n, c.batch, first == 0, as_stream(stream));
     if (r) return r;
     first += n;
-  } while (first < layers);
+  } while (first < c.layers);
   return IW_OK;
 }
 

@@ -22,6 +22,7 @@ RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -34,18 +35,24 @@ Tensor = torch.Tensor
 MAX_NODES = 64
 MAX_TOP = 32
 _LOGIT_TYPES = {torch.int8: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+_I8, _I32, _I64 = torch.int8, torch.int32, torch.int64
+_ATTENTION_ARGS = struct.Struct("36q")  # iw_attention_tree_args
+_CACHES = struct.Struct("21q")          # iw_tree_caches
 
 
-def _launch(dev: torch.device, name: str, *args) -> None:
-    """Call an entry point on the current stream of ``dev``, the tensors' device."""
-    if dev.index == torch._C._cuda_getDevice():
-        _lib.call(name, *args, _lib.stream())
+def _launch(dev: int, name: str, *args) -> None:
+    """Call an entry point on the current stream of device ``dev``, the tensors'."""
+    if dev == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
             _lib.call(name, *args, _lib.stream())
 
 
-def _check(t: Tensor, dtype: torch.dtype, shape: Sequence[int], name: str, dev: Optional[torch.device] = None,
+# A call's tensors are looked over in one expression; only where that fails are
+# they taken one by one, for the message.
+
+def _check(t: Tensor, dtype: torch.dtype, shape: Sequence[int], name: str, dev: Optional[int] = None,
            contiguous: bool = True) -> None:
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor")
@@ -53,51 +60,69 @@ def _check(t: Tensor, dtype: torch.dtype, shape: Sequence[int], name: str, dev: 
         raise RuntimeError(f"{name} must be a GPU tensor, got device {t.device}")
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {str(dtype).replace('torch.', '')}, got {t.dtype}")
-    if t.shape != shape:
+    if t.shape != tuple(shape):
         raise RuntimeError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
-    if dev is not None and t.device != dev:
-        raise RuntimeError(f"{name} is on {t.device}, the other tensors on {dev}")
+    if dev is not None and t.get_device() != dev:
+        raise RuntimeError(f"{name} is on {t.device}, the other tensors on device {dev}")
     if contiguous and not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
+
+
+def _is(t: Optional[Tensor], dtype: torch.dtype, shape: Sequence[int], dev: int) -> bool:
+    """Whether ``_check`` has nothing to say."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev
+            and t.is_contiguous())
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _rows_strides(t: Tensor, shape, name: str, dev: torch.device):
+def _pack(layout: struct.Struct, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except struct.error as e:
+        raise RuntimeError(f"sizes and scalars must be whole numbers of 64 bits: {e}") from None
+
+
+def _rows_strides(t: Tensor, shape, name: str, dev: int):
     """(batch, node) strides of an int8 [B, N, H * D] operand with contiguous rows."""
-    _check(t, torch.int8, shape, name, dev, contiguous=False)
+    if not (isinstance(t, torch.Tensor) and t.dtype is _I8 and t.shape == shape and t.get_device() == dev):
+        _check(t, _I8, shape, name, dev, contiguous=False)
     sb, st, sc = t.stride()
     if sc != 1:
         raise RuntimeError(f"the rows of {name} must be contiguous")
     return (sb if shape[0] > 1 else 0), (st if shape[1] > 1 else 0)
 
 
-def _cache_strides(k: Tensor, v: Tensor, B: int, H: int, D: int, dev: torch.device):
+def _cache_strides(k: Tensor, v: Tensor, B: int, H: int, D: int, dev: int):
     """Positions and strides (k_sb, k_sh, k_st), (v_sb, v_sh, v_sd, v_sq) of a layer's caches: K
     [B, H, T, D], V in key quads [B, H, ceil(T / 4), D, 4] or transposed [B, H, D, round_up(T, 16)]."""
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise RuntimeError("k_cache must be [batch, heads, positions, head_dim]")
     T = k.shape[2]
-    _check(k, torch.int8, (B, H, T, D), "k_cache", dev, contiguous=False)
+    if not (k.dtype is _I8 and k.shape == (B, H, T, D) and k.get_device() == dev):
+        _check(k, _I8, (B, H, T, D), "k_cache", dev, contiguous=False)
     if not isinstance(v, torch.Tensor) or v.dim() not in (4, 5):
         raise RuntimeError("v_cache must be key quads [batch, heads, quads, head_dim, 4] or transposed "
                            "[batch, heads, head_dim, positions]")
-    ks, vs = k.stride(), v.stride()
-    if v.dim() == 5:
-        quads = v.shape[2]
-        _check(v, torch.int8, (B, H, quads, D, 4), "v_cache", dev, contiguous=False)
-        if 4 * quads < T or vs[4] != 1 or vs[3] != 4:
+    vs, last = v.stride(), v.shape[2 if v.dim() == 5 else 3]
+    want = (B, H, last, D, 4) if len(vs) == 5 else (B, H, D, last)
+    if not (v.dtype is _I8 and v.shape == want and v.get_device() == dev):
+        _check(v, _I8, want, "v_cache", dev, contiguous=False)
+    if len(vs) == 5:
+        if 4 * last < T or vs[4] != 1 or vs[3] != 4:
             raise RuntimeError("v_cache: packed key quads that cover every position of k_cache are needed")
-        v_sd, v_sq = 4, (vs[2] if quads > 1 else 4 * D)
+        v_sd, v_sq = 4, (vs[2] if last > 1 else 4 * D)
     else:
-        _check(v, torch.int8, (B, H, D, v.shape[3]), "v_cache", dev, contiguous=False)
-        if v.shape[3] < (T + 15) // 16 * 16 or vs[3] != 1:
+        if last < (T + 15) // 16 * 16 or vs[3] != 1:
             raise RuntimeError("v_cache: transposed rows must cover the positions of k_cache rounded up to 16")
         v_sd, v_sq = vs[2], 4
+    ks = k.stride()
     if ks[3] != 1:
         raise RuntimeError("the rows of k_cache must be contiguous")
+    if B > 1 and H > 1 and T > 1:
+        return T, ks[:3], (vs[0], vs[1], v_sd, v_sq)
     return (T, (ks[0] if B > 1 else 0, ks[1] if H > 1 else 0, ks[2] if T > 1 else 0),
             (vs[0] if B > 1 else 0, vs[1] if H > 1 else 0, v_sd, v_sq))
 
@@ -105,6 +130,14 @@ def _cache_strides(k: Tensor, v: Tensor, B: int, H: int, D: int, dev: torch.devi
 def _tree_shape(t: Tensor, name: str):
     if not isinstance(t, torch.Tensor) or t.dim() != 2 or not 1 <= t.shape[1] <= MAX_NODES:
         raise RuntimeError(f"{name} must be [batch, nodes] with 1 to {MAX_NODES} nodes")
+    return t.shape
+
+
+def _node_shape(t: Tensor, heads: int, name: str):
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or not 1 <= t.shape[1] <= MAX_NODES:
+        raise RuntimeError(f"{name} must be [batch, nodes, heads * head_dim] with 1 to {MAX_NODES} nodes")
+    if heads <= 0 or t.shape[2] % heads:
+        raise RuntimeError(f"{name}.size(2) must be a multiple of heads")
     return t.shape
 
 
@@ -122,13 +155,15 @@ def tree_plan(parents: Tensor, counts: Optional[Tensor] = None, *, lengths: Opti
     row's length; ``lengths`` int32 [B]: cached tokens. Positions stay below
     ``max_positions``."""
     B, N = _tree_shape(parents, "parents")
-    _check(parents, torch.int32, (B, N), "parents")
-    dev = parents.device
-    for t, name in ((counts, "counts"), (lengths, "lengths")):
-        if t is not None:
-            _check(t, torch.int32, (B,), name, dev)
-    visible = torch.empty((B, N), dtype=torch.int64, device=dev)
-    positions = torch.empty((B, N), dtype=torch.int32, device=dev)
+    dev = parents.get_device()
+    if not (dev >= 0 and _is(parents, _I32, (B, N), dev) and (counts is None or _is(counts, _I32, (B,), dev))
+            and (lengths is None or _is(lengths, _I32, (B,), dev))):
+        _check(parents, _I32, (B, N), "parents")
+        for t, name in ((counts, "counts"), (lengths, "lengths")):
+            if t is not None:
+                _check(t, _I32, (B,), name, dev)
+    positions = torch.empty_like(parents)
+    visible = torch.empty_like(parents, dtype=_I64)
     _launch(dev, "iw_tree_plan", parents.data_ptr(), N, _ptr(counts), _ptr(lengths), B, N, max_positions,
             visible.data_ptr(), positions.data_ptr())
     return TreePlan(visible, positions)
@@ -147,33 +182,34 @@ def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_c
     Lengths and counts are clamped to T and N on the device. Returns int8 [B, N, heads * D] (``out`` where
     given); nodes past ``counts[b]`` and nodes that see no key give zeros. With one node a row it is a
     decode step over rows of different lengths."""
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or not 1 <= q.shape[1] <= MAX_NODES:
-        raise RuntimeError(f"q must be [batch, nodes, heads * head_dim] with 1 to {MAX_NODES} nodes")
-    shape, dev = q.shape, q.device
+    shape = _node_shape(q, heads, "q")
+    dev = q.get_device()
     B, N, C = shape
-    if heads <= 0 or C % heads:
-        raise RuntimeError("q.size(2) must be a multiple of heads")
     D = C // heads
     q_s = _rows_strides(q, shape, "q", dev)
     kn_s = _rows_strides(k_new, shape, "k_new", dev)
     vn_s = _rows_strides(v_new, shape, "v_new", dev)
     T, k_s, v_s = _cache_strides(k_cache, v_cache, B, heads, D, dev)
-    _check(lengths, torch.int32, (B,), "lengths", dev)
     shared = isinstance(visible, torch.Tensor) and visible.dim() == 1
-    _check(visible, torch.int64, (N,) if shared else (B, N), "visible", dev)
-    if counts is not None:
-        _check(counts, torch.int32, (B,), "counts", dev)
+    if not (dev >= 0 and _is(lengths, _I32, (B,), dev) and _is(visible, _I64, (N,) if shared else (B, N), dev)
+            and (counts is None or _is(counts, _I32, (B,), dev))):
+        _check(q, _I8, shape, "q", contiguous=False)
+        _check(lengths, _I32, (B,), "lengths", dev)
+        _check(visible, _I64, (N,) if shared else (B, N), "visible", dev)
+        if counts is not None:
+            _check(counts, _I32, (B,), "counts", dev)
     if out is None:
-        out = torch.empty(shape, dtype=torch.int8, device=dev)
+        out = q.new_empty(shape)
         o_s = (N * C, C)
     else:
         o_s = _rows_strides(out, shape, "out", dev)
         if (B > 1 and o_s[0] < C) or (N > 1 and o_s[1] < C):
             raise RuntimeError("the rows of out must not overlap")
-    _launch(dev, "iw_attention_tree", q.data_ptr(), *q_s, k_new.data_ptr(), *kn_s, v_new.data_ptr(), *vn_s,
-            k_cache.data_ptr(), *k_s, v_cache.data_ptr(), *v_s, lengths.data_ptr(), visible.data_ptr(),
-            0 if shared else N, _ptr(counts), out.data_ptr(), *o_s, B, heads, N, D, T, qk_multiplier, qk_shift,
-            frac_bits, av_multiplier, av_shift, rsqrt_offset)
+    args = _pack(_ATTENTION_ARGS, q.data_ptr(), *q_s, k_new.data_ptr(), *kn_s, v_new.data_ptr(), *vn_s,
+                 k_cache.data_ptr(), *k_s, v_cache.data_ptr(), *v_s, lengths.data_ptr(), visible.data_ptr(),
+                 0 if shared else N, 0 if counts is None else counts.data_ptr(), out.data_ptr(), *o_s, B, heads, N, D, T,
+                 qk_multiplier, qk_shift, frac_bits, av_multiplier, av_shift, rsqrt_offset)
+    _launch(dev, "iw_attention_tree", args)
     return out
 
 
@@ -198,17 +234,15 @@ class TreeCaches:
         if L == 0 or any(len(x) != L for x in self.tensors):
             raise RuntimeError("one k_new, v_new, k_cache and v_cache of each layer are needed")
         kn, vn, k, v = (x[0] for x in self.tensors)
-        if not isinstance(kn, torch.Tensor) or kn.dim() != 3 or not 1 <= kn.shape[1] <= MAX_NODES:
-            raise RuntimeError(f"k_new must be [batch, nodes, heads * head_dim] with 1 to {MAX_NODES} nodes")
-        self.batch, self.nodes, C = shape = kn.shape
-        if heads <= 0 or C % heads:
-            raise RuntimeError("k_new.size(2) must be a multiple of heads")
-        self.device = dev = kn.device
+        self.batch, self.nodes, C = shape = _node_shape(kn, heads, "k_new")
+        self.device = dev = kn.get_device()
+        if dev < 0:
+            _check(kn, _I8, shape, "k_new", contiguous=False)
         B, D = self.batch, C // heads
-        self._new = (*_rows_strides(kn, shape, "k_new", dev), *_rows_strides(vn, shape, "v_new", dev))
+        new = (*_rows_strides(kn, shape, "k_new", dev), *_rows_strides(vn, shape, "v_new", dev))
         self.positions, k_s, v_s = _cache_strides(k, v, B, heads, D, dev)
         for kn_l, vn_l, k_l, v_l in zip(*self.tensors):
-            same = (_rows_strides(kn_l, shape, "k_new", dev) + _rows_strides(vn_l, shape, "v_new", dev) == self._new
+            same = (_rows_strides(kn_l, shape, "k_new", dev) + _rows_strides(vn_l, shape, "v_new", dev) == new
                     and _cache_strides(k_l, v_l, B, heads, D, dev) == (self.positions, k_s, v_s))
             if not same:
                 raise RuntimeError("the layers' tensors must have the same strides")
@@ -216,8 +250,10 @@ class TreeCaches:
         if len({t.data_ptr() for t in caches}) != len(caches) or any(
                 0 in [s for s, n in zip(t.stride(), t.shape) if n > 1] for t in caches):
             raise RuntimeError("the caches are written: each must be memory of its own")
-        arrays = [(ctypes.c_void_p * L)(*[t.data_ptr() for t in x]) for x in self.tensors]
-        self._layers = (L, arrays[0], arrays[1], *self._new, arrays[2], *k_s, arrays[3], *v_s, heads, D, self.positions)
+        self._arrays = [(ctypes.c_void_p * L)(*[t.data_ptr() for t in x]) for x in self.tensors]
+        kn_a, vn_a, k_a, v_a = map(ctypes.addressof, self._arrays)
+        self._image = _pack(_CACHES, L, B, self.nodes, heads, D, self.positions, kn_a, *new[:2], vn_a, *new[2:], k_a,
+                            *k_s, v_a, *v_s)
 
     def accept(self, tokens: Tensor, parents: Tensor, choice: Tensor, lengths: Tensor,
                counts: Optional[Tensor] = None, *, eot: int = -1) -> TreeAccept:
@@ -227,20 +263,23 @@ class TreeCaches:
 
         ``tokens`` int64, ``parents`` int32, ``choice`` int64 (the model's token after each node,
         ``token_logprobs(..., top=1).top_ids``) [B, N]; ``lengths`` and ``counts`` int32 [B]."""
-        dev, B, N = self.device, self.batch, self.nodes
-        shape = (B, N)
-        _check(tokens, torch.int64, shape, "tokens", dev)
-        _check(parents, torch.int32, shape, "parents", dev)
-        _check(choice, torch.int64, shape, "choice", dev)
-        _check(lengths, torch.int32, (B,), "lengths", dev)
-        if counts is not None:
-            _check(counts, torch.int32, (B,), "counts", dev)
-        path = torch.empty(shape, dtype=torch.int32, device=dev)
-        accepted, after = torch.empty((2, B), dtype=torch.int32, device=dev)
-        next_token = torch.empty(B, dtype=torch.int64, device=dev)
-        _launch(dev, "iw_tree_accept", tokens.data_ptr(), parents.data_ptr(), choice.data_ptr(), _ptr(counts),
-                lengths.data_ptr(), B, N, eot, path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(),
-                after.data_ptr(), *self._layers)
+        dev, rows = self.device, (self.batch,)
+        shape = (self.batch, self.nodes)
+        if not (_is(tokens, _I64, shape, dev) and _is(parents, _I32, shape, dev) and _is(choice, _I64, shape, dev)
+                and _is(lengths, _I32, rows, dev) and (counts is None or _is(counts, _I32, rows, dev))):
+            _check(tokens, _I64, shape, "tokens", dev)
+            _check(parents, _I32, shape, "parents", dev)
+            _check(choice, _I64, shape, "choice", dev)
+            _check(lengths, _I32, rows, "lengths", dev)
+            if counts is not None:
+                _check(counts, _I32, rows, "counts", dev)
+        path = torch.empty_like(parents)
+        accepted = torch.empty_like(lengths)
+        after = torch.empty_like(lengths)
+        next_token = torch.empty_like(lengths, dtype=_I64)
+        _launch(dev, "iw_tree_accept", self._image, tokens.data_ptr(), parents.data_ptr(), choice.data_ptr(),
+                _ptr(counts), lengths.data_ptr(), eot, path.data_ptr(), accepted.data_ptr(), next_token.data_ptr(),
+                after.data_ptr())
         return TreeAccept(path, accepted, next_token, after)
 
 
@@ -266,7 +305,7 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, top: int
     kind = _LOGIT_TYPES.get(logits.dtype)
     if kind is None:
         raise RuntimeError(f"logits must be int8, float32, bfloat16 or float16, got {logits.dtype}")
-    dev, lead, V = logits.device, logits.shape[:-1], logits.shape[-1]
+    dev, lead, V = logits.get_device(), logits.shape[:-1], logits.shape[-1]
     if logits.dim() != 2:
         logits = logits.reshape(-1, V)
     rows = logits.shape[0]
@@ -277,20 +316,21 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, top: int
     if not 0 <= top <= min(MAX_TOP, V):
         raise RuntimeError(f"top must be in [0, {min(MAX_TOP, V)}]")
     logprob = ids = lps = None
+    entropy = logits.new_empty(lead, dtype=torch.float32)
     if targets is not None:
-        _check(targets, torch.int64, lead, "targets", dev, contiguous=False)
-        targets = targets.contiguous()
-        logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+        if not _is(targets, _I64, lead, dev):
+            _check(targets, _I64, lead, "targets", dev, contiguous=False)
+            targets = targets.contiguous()
+        logprob = torch.empty_like(entropy)
     if suppress is not None:
-        if not isinstance(suppress, torch.Tensor) or suppress.dtype not in (torch.int32, torch.uint32):
+        if not isinstance(suppress, torch.Tensor) or suppress.dtype not in (_I32, torch.uint32):
             raise RuntimeError("suppress must be int32 or uint32 words")
         _check(suppress, suppress.dtype, ((V + 31) // 32,), "suppress", dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     if top:
-        ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-        lps = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        ids = logits.new_empty((*lead, top), dtype=_I64)
+        lps = logits.new_empty((*lead, top), dtype=torch.float32)
     need = _lib.value("iw_token_logprobs_workspace", kind, rows, V, top)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    work = logits.new_empty(need, dtype=torch.uint8) if need > 0 else None
     _launch(dev, "iw_token_logprobs", logits.data_ptr(), kind, rows, V, ld, scale, _ptr(suppress), _ptr(targets),
             _ptr(logprob), entropy.data_ptr(), top, _ptr(ids), _ptr(lps), _ptr(work))
     return TokenLogprobs(logprob, entropy, ids, lps)
@@ -345,9 +385,9 @@ class TreeDecoder:
         """int8 logits [B, N, vocab] after every node; the caches stay as they are."""
         r, dec, N, M = self.runner, self.runner.dec, self.nodes, self.M
         B, C, H = r.B, r.C, r.H
-        dev = self.lengths.device
-        _check(tokens, torch.int64, (B, N), "tokens", dev)
-        _check(parents, torch.int32, (B, N), "parents", dev)
+        dev = self.lengths.get_device()
+        _check(tokens, _I64, (B, N), "tokens", dev)
+        _check(parents, _I32, (B, N), "parents", dev)
         plan = tree_plan(parents, counts, lengths=self.lengths, max_positions=dec.n_ctx)
         # unused nodes may hold any value
         emb = dec.token_embedding.weight[tokens.clamp(0, dec.n_vocab - 1)]

@@ -627,16 +627,30 @@ int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *coun
  * quads (v_sd == 4); out (b, i) at out + b*o_sb + i*o_st. Rows of nodes past
  * the count, and of nodes that see no key, are zeros. nodes <= 64,
  * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24; operands and
- * strides are multiples of 16 bytes. The caches are read only: the nodes' K and V
- * enter them with iw_tree_accept. */
-int iw_attention_tree(const int8_t *q, int64_t q_sb, int64_t q_st, const int8_t *k_new, int64_t kn_sb,
-                      int64_t kn_st, const int8_t *v_new, int64_t vn_sb, int64_t vn_st, const int8_t *k,
-                      int64_t k_sb, int64_t k_sh, int64_t k_st, const int8_t *vt, int64_t v_sb, int64_t v_sh,
-                      int64_t v_sd, int64_t v_sq, const int32_t *lengths, const int64_t *visible,
-                      int64_t visible_sb, const int32_t *counts, int8_t *out, int64_t o_sb, int64_t o_st,
-                      int64_t batch, int64_t heads, int64_t nodes, int64_t head_dim, int64_t cache_positions,
-                      uint8_t qk_multiplier, int8_t qk_shift, int32_t frac_bits, uint8_t av_multiplier,
-                      int8_t av_shift, uint32_t rsqrt_offset, iw_stream_t stream);
+ * strides are multiples of 16 bytes; kn_st, vn_st, k_st, v_sd, v_sq < 2^25. The
+ * caches are read only: the nodes' K and V enter them with iw_tree_accept. The
+ * struct is read during the call. */
+typedef struct iw_attention_tree_args {
+  const int8_t *q;
+  int64_t q_sb, q_st;
+  const int8_t *k_new;
+  int64_t kn_sb, kn_st;
+  const int8_t *v_new;
+  int64_t vn_sb, vn_st;
+  const int8_t *k;
+  int64_t k_sb, k_sh, k_st;
+  const int8_t *vt;
+  int64_t v_sb, v_sh, v_sd, v_sq;
+  const int32_t *lengths;
+  const int64_t *visible;
+  int64_t visible_sb;
+  const int32_t *counts;
+  int8_t *out;
+  int64_t o_sb, o_st;
+  int64_t batch, heads, nodes, head_dim, cache_positions;
+  int64_t qk_multiplier, qk_shift, frac_bits, av_multiplier, av_shift, rsqrt_offset;
+} iw_attention_tree_args;
+int iw_attention_tree(const iw_attention_tree_args *args, iw_stream_t stream);
 
 /* Greedy acceptance: from node 0, the path goes on to the first node in use
  * whose parent is the current node and whose token is choice[current] (the
@@ -645,17 +659,25 @@ int iw_attention_tree(const int8_t *q, int64_t q_sb, int64_t q_st, const int8_t 
  * path [batch][nodes]: its nodes, then -1; accepted [batch]: their number (0
  * for a row without nodes or room); next [batch]: the choice after the last of
  * them (-1 for 0); lengths_out = lengths + accepted (no part of lengths). The
- * path's K and V of every layer are written to cache positions lengths[b] ..:
- * k_new / v_new / k / v are host arrays of `layers` device pointers with one
- * set of strides (layouts as iw_attention_tree, multiples of 4 bytes; read
- * during the call). layers may be 0. */
-int iw_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t *choice, const int32_t *counts,
-                   const int32_t *lengths, int64_t batch, int64_t nodes, int64_t eot, int32_t *path,
-                   int32_t *accepted, int64_t *next, int32_t *lengths_out, int64_t layers,
-                   const int8_t *const *k_new, const int8_t *const *v_new, int64_t kn_sb, int64_t kn_st,
-                   int64_t vn_sb, int64_t vn_st, int8_t *const *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
-                   int8_t *const *v, int64_t v_sb, int64_t v_sh, int64_t v_sd, int64_t v_sq, int64_t heads,
-                   int64_t head_dim, int64_t cache_positions, iw_stream_t stream);
+ * path's K and V of every layer are written to cache positions lengths[b] .. (layouts
+ * as iw_attention_tree, operands and strides multiples of 4 bytes). */
+
+/* The layers' caches: host arrays of `layers` device pointers with one set of
+ * strides. layers may be 0. Read during the call. */
+typedef struct iw_tree_caches {
+  int64_t layers, batch, nodes, heads, head_dim, cache_positions;
+  const int8_t *const *k_new;
+  int64_t kn_sb, kn_st;
+  const int8_t *const *v_new;
+  int64_t vn_sb, vn_st;
+  int8_t *const *k;
+  int64_t k_sb, k_sh, k_st;
+  int8_t *const *v;
+  int64_t v_sb, v_sh, v_sd, v_sq;
+} iw_tree_caches;
+int iw_tree_accept(const iw_tree_caches *caches, const int64_t *tokens, const int32_t *parents,
+                   const int64_t *choice, const int32_t *counts, const int32_t *lengths, int64_t eot,
+                   int32_t *path, int32_t *accepted, int64_t *next, int32_t *lengths_out, iw_stream_t stream);
 
 /* Scores of rows of logits (row stride ld) of a type below, real logit = value *
  * scale (> 0), tokens of the bitmask suppress (as iw_greedy_advance_filtered;

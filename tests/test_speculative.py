@@ -266,7 +266,9 @@ def test_tree_attention_refuses_layouts(iw, gpu):
                       ((q, kn, vn, k, v, ln.long(), vis), "int32"), ((q, kn, vn, k, v, ln[:1], vis), "shape"),
                       ((q, kn, vn, k, v, ln, vis.int()), "int64"), ((q, kn, vn, k, v, ln, vis[:, :3]), "shape"),
                       ((q, kn, vn, k, T(np.zeros((2, 2, 8, 64, 4), np.int8)), ln, vis), "every position"),
-                      ((q.cpu(), kn, vn, k, v, ln, vis), "GPU")]:
+                      ((q.cpu(), kn, vn, k, v, ln, vis), "GPU|device"),
+                      ((q, kn, vn, k, v, ln.cpu(), vis), "GPU"), ((q, kn, vn, k.cpu(), v, ln, vis), "GPU"),
+                      ((q, kn, vn, k, v, None, vis), "tensor"), ((q, kn, vn, k, v, ln, None), "tensor")]:
         with pytest.raises(RuntimeError, match=what):
             f(*bad, **sc)
     with pytest.raises(RuntimeError, match="16-byte"):

@@ -2,6 +2,8 @@
 points with sizes, alignments and overlaps they do not take, and the Python
 layer with tensors that are not what it needs. No GPU."""
 import ctypes
+import struct
+from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
@@ -30,13 +32,32 @@ SCORE = dict(x=P, type=0, rows=2, cols=100, ld=100, scale=1.0, suppress=None, ta
              ids=P, lps=P, work=None, stream=None)
 
 
+CACHE_FIELDS = ("layers", "batch", "nodes", "heads", "D", "cap", "kn", "kn_sb", "kn_st", "vn", "vn_sb", "vn_st", "k", "k_sb",
+                "k_sh", "k_st", "v", "v_sb", "v_sh", "v_sd", "v_sq")
+ACCEPT_ARGS = ("tokens", "parents", "choice", "counts", "lengths", "eot", "path", "accepted", "next", "lengths_out", "stream")
+
+
+def arguments(name, a):
+    """The entry point's arguments; those of the structs as their fields' 64-bit images."""
+    def image(values):
+        return struct.pack(f"{len(values)}q", *[0 if v is None else v for v in values])
+    if name == "iw_attention_tree":
+        return image([v for k, v in a.items() if k != "stream"]), None
+    if name == "iw_tree_accept":
+        arrays = [(ctypes.c_void_p * 1)(P if a[k] == "a" else None) for k in ("kn", "vn", "k", "v")]
+        a = dict(a)
+        for k, x in zip(("kn", "vn", "k", "v"), arrays):
+            a[k] = None if a[k] is None else ctypes.addressof(x)
+        KEPT[:] = arrays
+        return (image([a[k] for k in CACHE_FIELDS]), *[a[k] for k in ACCEPT_ARGS])
+    return tuple(a.values())
+
+
+KEPT = []  # the arrays that the last image names
+
+
 def refused(iw, name, args, change, what):
-    a = dict(args)
-    a.update(change)
-    for k, v in a.items():
-        if v in ("a", "null"):
-            a[k] = (ctypes.c_void_p * 1)(P if v == "a" else None)
-    rc, msg = entry(iw, name, a.values())
+    rc, msg = entry(iw, name, arguments(name, {**args, **change}))
     assert rc == -1 and what in msg, msg
 
 
@@ -57,7 +78,9 @@ def test_plan_refusals(iw, change, what):
     (dict(out=P + 8), "16-byte"), (dict(kn_st=130), "16-byte"), (dict(v_sq=4, v_sd=40), "16-byte"),
     (dict(k_st=72), "16-byte"), (dict(q=None), "null"), (dict(lengths=None), "null"), (dict(visible=None), "null"),
     (dict(out=None), "null"), (dict(batch=-1), "attention shape"), (dict(batch=1 << 22), "attention shape"),
-    (dict(vis_sb=-1), "attention shape")])
+    (dict(vis_sb=-1), "attention shape"), (dict(k_st=1 << 25), "2^25"), (dict(kn_st=1 << 25), "2^25"),
+    (dict(v_sq=1 << 25), "2^25"), (dict(qm=256), "uint8"), (dict(am=-1), "uint8"), (dict(qs=128), "int8"),
+    (dict(as_=-129), "int8"), (dict(off=-1), "rsqrt_offset")])
 def test_attention_refusals(iw, change, what):
     refused(iw, "iw_attention_tree", ATTN, change, what)
 
@@ -87,7 +110,23 @@ def test_score_refusals(iw, change, what):
 def test_empty_batches_do_nothing(iw):
     for name, args in (("iw_tree_plan", dict(PLAN, batch=0)), ("iw_attention_tree", dict(ATTN, batch=0)),
                        ("iw_token_logprobs", dict(SCORE, rows=0))):
-        assert entry(iw, name, args.values())[0] == 0
+        assert entry(iw, name, arguments(name, args))[0] == 0
+
+
+def test_null_structs(iw):
+    assert entry(iw, "iw_attention_tree", (None, None)) == (-1, "null arguments")
+    args = dict(ACCEPT)
+    assert entry(iw, "iw_tree_accept", (None, *[args[k] for k in ACCEPT_ARGS])) == (-1, "null arguments")
+
+
+def test_struct_images(iw):
+    """The packed images have the fields of the header's structs, 8 bytes each."""
+    text = (Path(__file__).resolve().parents[1] / "include" / "iwhisper_amd.h").read_text()
+    for name, image in (("iw_attention_tree_args", iw.speculative._ATTENTION_ARGS), ("iw_tree_caches", iw.speculative._CACHES)):
+        body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
+        fields = sum(line.count(",") + 1 for line in body.splitlines()[1:] if line.strip().endswith(";"))
+        assert image.size == 8 * fields
+        assert all(f in ("int64_t", "const") or "*" in line for line in body.splitlines()[1:] for f in line.split()[:1])
 
 
 def test_workspace_size(iw):
@@ -117,6 +156,15 @@ def test_python_layer_refuses(iw):
     q, k, v = i8(1, 4, 32), i8(1, 2, 8, 16), i8(1, 2, 2, 16, 4)
     with pytest.raises(RuntimeError, match="GPU"):
         sp.tree_attention(q, q, q, k, v, i32(1), i64(1, 4), heads=2, **sc)
+    for bad in (None, 3, [1]):
+        with pytest.raises(RuntimeError):
+            sp.tree_attention(q, bad, q, k, v, i32(1), i64(1, 4), heads=2, **sc)
+        with pytest.raises(RuntimeError):
+            sp.tree_attention(q, q, q, k, v, bad, i64(1, 4), heads=2, **sc)
+    with pytest.raises(RuntimeError, match="whole numbers"):
+        sp._pack(sp._CACHES, *[1.5] * 21)
+    with pytest.raises(RuntimeError, match="whole numbers"):
+        sp._pack(sp._CACHES, *[2 ** 64] * 21)
     with pytest.raises(RuntimeError, match="multiple of heads"):
         sp.tree_attention(q, q, q, k, v, i32(1), i64(1, 4), heads=3, **sc)
     with pytest.raises(RuntimeError, match="1 to 64 nodes"):
