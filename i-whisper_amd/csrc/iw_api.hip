@@ -1073,7 +1073,8 @@ int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t co
   IW_REQUIRE(type >= LOGIT_I8 && type <= LOGIT_F16, "logits must be int8, float32, bfloat16 or float16");
   IW_REQUIRE(rows >= 0 && rows <= (1 << 22) && cols > 0 && cols < (1 << 23) && ld >= cols,
              "invalid logits shape (at most 2^22 rows of 2^23 - 1 columns)");
-  IW_REQUIRE(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
+  // below, logits further apart than float32 reaches could still have probabilities
+  IW_REQUIRE(scale >= 0x1p-100f && std::isfinite(scale), "scale must be finite and at least 2^-100");
   IW_REQUIRE(top >= 0 && top <= kScoreMaxTop && top <= cols, "top must be at most 32 and at most cols");
   if (rows == 0) return IW_OK;
   IW_REQUIRE(logits && (targets != nullptr) == (logprob != nullptr) && (top == 0 || (top_ids && top_logprobs)),

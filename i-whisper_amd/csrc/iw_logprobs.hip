@@ -402,11 +402,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
     m = key_value((uint64_t)wave_max_u32_dpp(go) << 32);
     const float ms = m == -INFINITY ? 0.f : m;  // a part without finite logits sums to 0
     auto add = [&](float v, bool all) {
-      const float d = v - ms;
-      const float e = __builtin_amdgcn_exp2f(fmaf(d, a.log2_hi, d * a.log2_lo));
+      const float d = v - ms, finite = fmaxf(d, -3e38f);
+      // log2(e) * scale in two parts, as the rounding of one would be the same for every logit
+      const float e = __builtin_amdgcn_exp2f(fmaf(d, a.log2_hi, finite * a.log2_lo));
       if (all || d != 0.f) {
         z += e;
-        u -= fmaxf(d, -3e38f) * e;  // -inf times its exp of 0 is 0
+        u -= finite * e;  // -inf times its exp of 0 is 0
       } else {
         eq += 1.f;
       }
@@ -598,12 +599,9 @@ template <typename T>
 int launch_scores(ScoreArgs a, hipStream_t s) {
   const Split sp = split(a.type, a.rows, a.cols);
   if (sp.chunks > kMaxParts || a.rows * sp.chunks > (1LL << 32) / 1024 - 1) return fail("too many logits for one call");
-  // log2(e) * scale in two parts, as the rounding of one would be the same for
-  // every logit; neither is negative, so that -inf times them stays -inf
   const double c = (double)a.scale * 1.4426950408889634;
-  a.log2_hi = (float)c;
-  if ((double)a.log2_hi > c) a.log2_hi = std::nextafter(a.log2_hi, 0.f);
-  a.log2_lo = std::max((float)(c - (double)a.log2_hi), 1e-30f);
+  a.log2_hi = (float)std::min(c, 3.4e38);
+  a.log2_lo = (float)(c - (double)a.log2_hi);
   if (sp.few) return launch_scores_p<T, 1024, 4>(a, sp, s);
   return launch_scores_p<T, sizeof(T) == 1 ? 256 : 512, sizeof(T) == 1 ? 16 : 8>(a, sp, s);
 }

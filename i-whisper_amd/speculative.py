@@ -155,6 +155,8 @@ def tree_plan(parents: Tensor, counts: Optional[Tensor] = None, *, lengths: Opti
     row's length; ``lengths`` int32 [B]: cached tokens. Positions stay below
     ``max_positions``."""
     B, N = _tree_shape(parents, "parents")
+    if not 1 <= max_positions < 2 ** 31:
+        raise RuntimeError("max_positions must be in [1, 2^31)")
     dev = parents.get_device()
     if not (dev >= 0 and _is(parents, _I32, (B, N), dev) and (counts is None or _is(counts, _I32, (B,), dev))
             and (lengths is None or _is(lengths, _I32, (B,), dev))):
@@ -180,7 +182,7 @@ def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_c
     ``k_cache`` int8 [B, heads, T, D]; ``v_cache`` in key quads [B, heads, ceil(T / 4), D, 4] or transposed
     [B, heads, D, round_up(T, 16)]. D is a multiple of 16 up to 128, strides are multiples of 16.
     Lengths and counts are clamped to T and N on the device. Returns int8 [B, N, heads * D] (``out`` where
-    given); nodes past ``counts[b]`` and nodes that see no key give zeros. With one node a row it is a
+    given, which shares no memory with K, V or the caches); nodes past ``counts[b]`` and nodes that see no key give zeros. With one node a row it is a
     decode step over rows of different lengths."""
     shape = _node_shape(q, heads, "q")
     dev = q.get_device()
@@ -203,7 +205,9 @@ def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_c
         o_s = (N * C, C)
     else:
         o_s = _rows_strides(out, shape, "out", dev)
-        if (B > 1 and o_s[0] < C) or (N > 1 and o_s[1] < C):
+        sb, st = o_s
+        if (B > 1 and sb < C) or (N > 1 and st < C) or (
+                B > 1 and N > 1 and sb < (N - 1) * st + C and st < (B - 1) * sb + C):
             raise RuntimeError("the rows of out must not overlap")
     args = _pack(_ATTENTION_ARGS, q.data_ptr(), *q_s, k_new.data_ptr(), *kn_s, v_new.data_ptr(), *vn_s,
                  k_cache.data_ptr(), *k_s, v_cache.data_ptr(), *v_s, lengths.data_ptr(), visible.data_ptr(),
@@ -294,7 +298,7 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, top: int
                    suppress: Optional[Tensor] = None) -> TokenLogprobs:
     """Scores of rows of logits [..., vocab] (int8, float32, bfloat16 or float16), in float32.
 
-    The real logits are ``logits * scale`` (for a decoder's int8 logits
+    The real logits are ``logits * scale`` (2^-100 or more; for a decoder's int8 logits
     1 / act_logits_alpha); ``suppress`` is a bit mask of tokens that count as
     -inf (int32 or uint32 words, bit i % 32 of word i // 32, as the runners' filters hold it).
     ``targets`` int64 [...]: tokens whose log-probability is asked for, NaN for one outside

@@ -628,8 +628,8 @@ int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *coun
  * the count, and of nodes that see no key, are zeros. nodes <= 64,
  * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24; operands and
  * strides are multiples of 16 bytes; kn_st, vn_st, k_st, v_sd, v_sq < 2^25. The
- * caches are read only: the nodes' K and V enter them with iw_tree_accept. The
- * struct is read during the call. */
+ * caches are read only: the nodes' K and V enter them with iw_tree_accept. out shares
+ * no memory with k_new, v_new or the caches. The struct is read during the call. */
 typedef struct iw_attention_tree_args {
   const int8_t *q;
   int64_t q_sb, q_st;
@@ -680,7 +680,7 @@ int iw_tree_accept(const iw_tree_caches *caches, const int64_t *tokens, const in
                    int32_t *path, int32_t *accepted, int64_t *next, int32_t *lengths_out, iw_stream_t stream);
 
 /* Scores of rows of logits (row stride ld) of a type below, real logit = value *
- * scale (> 0), tokens of the bitmask suppress (as iw_greedy_advance_filtered;
+ * scale (2^-100 or more), tokens of the bitmask suppress (as iw_greedy_advance_filtered;
  * or NULL) -inf:
  *   logprob[r]   log-softmax at targets[r] (both or neither NULL); NaN for a
  *                target outside the vocabulary

@@ -274,6 +274,8 @@ def test_tree_attention_refuses_layouts(iw, gpu):
     with pytest.raises(RuntimeError, match="16-byte"):
         f(qkv[..., 1:C + 1], kn, vn, k, v, ln, vis, **sc)
     with pytest.raises(RuntimeError, match="overlap"):
+        f(q, kn, vn, k, v, ln, vis, out=torch.empty(8 * C, dtype=torch.int8, device="cuda").as_strided((2, 4, C), (C, C, 1)), **sc)
+    with pytest.raises(RuntimeError, match="overlap"):
         f(q, kn, vn, k, v, ln, vis, out=torch.empty(C, dtype=torch.int8, device="cuda").expand(2, 4, C), **sc)
 
 
@@ -512,6 +514,33 @@ def test_token_logprobs_special_values(iw, gpu, V, dtype):
     assert host(got.top_ids[3]).tolist() == [0, 1, 2, 3, 4]
     assert int(got.top_ids[4, 0]) == V // 3 and int(got.top_ids[5, 0]) == V // 3
     assert host(got.top_ids[6]).tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("scale", [0.1, 0.3, 0.7, 1.1, 1.3, 2.0, 3.7])
+def test_token_logprobs_scales_of_masked_rows(iw, gpu, scale, dtype):
+    """-inf stays without probability under every scale, whatever the sign of its rounding."""
+    r = gen.rng(int(10 * scale))
+    x = logits_of(r, 4, 5000, dtype, 1.0)
+    x[:, ::3] = -math.inf
+    got = iw.speculative.token_logprobs(x.cuda(), T(np.array([1, 2, 0, 5])), top=4, scale=scale)
+    check_scores(got, x, np.array([1, 2, 0, 5]), 4, float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("scale,size", [(2.0 ** -100, 2.0 ** 101), (2.0 ** -100, 3e38),
+                                        (2.0 ** 120, 2.0 ** -118), (2e38, 1.0)])
+def test_token_logprobs_extreme_scales(iw, gpu, scale, size):
+    """Scales and logits near the ends of float32 (smaller scales are refused)."""
+    r = gen.rng(7)
+    x = torch.from_numpy(r.uniform(-1, 1, (3, 2000)) * size).float()
+    got = iw.speculative.token_logprobs(x.cuda(), T(np.array([1, 2, 3])), top=2, scale=scale)
+    with np.errstate(over="ignore"):
+        lp = (x.double() * float(np.float32(scale))).log_softmax(1)
+    want = lp[torch.arange(3), torch.tensor([1, 2, 3])]
+    a = got.logprob.double().cpu()
+    assert bool(((a - want).abs() <= 600 * 2.0 ** -24 + want.abs() * 2.0 ** -22).logical_or(
+        (a == -math.inf) & (want < -3e38)).all())
+    assert torch.equal(got.top_ids.cpu(), x.topk(2, 1).indices)
 
 
 def test_token_logprobs_targets_outside(iw, gpu):

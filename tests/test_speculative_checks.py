@@ -2,7 +2,10 @@
 points with sizes, alignments and overlaps they do not take, and the Python
 layer with tensors that are not what it needs. No GPU."""
 import ctypes
+import re
+import shutil
 import struct
+import subprocess
 from pathlib import Path
 from types import SimpleNamespace
 
@@ -99,7 +102,8 @@ def test_accept_refusals(iw, change, what):
     (dict(type=4), "int8, float32"), (dict(type=-1), "int8, float32"), (dict(rows=-1), "logits shape"),
     (dict(cols=0), "logits shape"), (dict(cols=1 << 23, ld=1 << 23), "logits shape"), (dict(ld=99), "logits shape"),
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"),
-    (dict(scale=float("nan")), "scale"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(cols=3, top=4), "top"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=1e-40), "scale"),
+    (dict(scale=2.0 ** -120), "scale"), (dict(scale=1.2e-38), "scale"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(cols=3, top=4), "top"),
     (dict(x=None), "null"), (dict(targets=None), "null"), (dict(logprob=None), "null"), (dict(ids=None), "null"),
     (dict(type=1, x=P + 2), "aligned"), (dict(type=2, x=P + 1), "aligned"),
     (dict(cols=100000, ld=100000), "workspace")])
@@ -175,6 +179,9 @@ def test_python_layer_refuses(iw):
         sp.tree_plan(i32(1, 65))
     with pytest.raises(RuntimeError, match="GPU"):
         sp.tree_plan(i32(1, 8))
+    for bad in (0, -1, 2 ** 31, 2 ** 40):
+        with pytest.raises(RuntimeError, match="max_positions"):
+            sp.tree_plan(i32(1, 8), max_positions=bad)
     with pytest.raises(RuntimeError, match="GPU"):
         sp.token_logprobs(torch.zeros(2, 5))
     with pytest.raises(RuntimeError, match="of each layer"):
@@ -193,3 +200,20 @@ def test_tree_decoder_refuses(iw):
             iw.speculative.TreeDecoder(SimpleNamespace(filters=None), nodes)
     with pytest.raises(ValueError, match="top"):
         iw.speculative.TreeDecoder.step(SimpleNamespace(), i64(1, 4), i32(1, 4), top=0)
+
+
+def test_kernels_keep_their_values_in_registers(iw, tmp_path):
+    """The tree attention's instances spill neither vector nor scalar registers (an early form with
+    scalar spills gave wrong probabilities in one lane)."""
+    llvm = Path("/opt/rocm/llvm/bin")
+    if not (llvm / "llvm-objdump").exists():
+        pytest.skip("no llvm-objdump")
+    shutil.copy(iw._lib.LIB_PATH, tmp_path / "lib.so")
+    subprocess.run([llvm / "llvm-objdump", "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
+    spills = {}
+    for code in sorted(tmp_path.glob("*gfx950*")):
+        out = subprocess.run([llvm / "llvm-readelf", "--notes", code], check=True, capture_output=True, text=True).stdout
+        for m in re.finditer(r"\.name: +(\S*attn_tree_kernel\S*).*?\.sgpr_spill_count: (\d+).*?\.vgpr_spill_count: (\d+)",
+                             out, re.S):
+            spills[m[1]] = (int(m[2]), int(m[3]))
+    assert len(spills) >= 24 and not any(map(any, spills.values())), spills
