@@ -93,10 +93,16 @@ __device__ __forceinline__ uint32_t output_word(const AttnArgs &a, const uint32_
 
 // KS: 64-column parts of the head; QUADS: V in key quads; QT: 16-query tiles of
 // the block; NW waves; NC > 0: a wave has at most NC chunks, whose K and V
-// are all requested at the start and kept.
+// are all requested at the start and kept. Waves per SIMD are asked for where the
+// registers allow them: held chunks of 64-wide heads in 128 registers, which the compiler
+// exceeds on its own (206, two waves: 16 nodes of 2560 heads 38 us, with four 28).
+constexpr int tree_waves(int ks, int qt, int nc) {
+  if (nc == 2) return ks == 1 ? (qt == 1 ? 4 : 3) : 2;
+  return nc == 1 || ks * qt == 1 ? 4 : 2;
+}
 template <int KS, bool QUADS, int QT, int NW, int NC>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NC == 2 && KS == 1 ? (QT == 1 ? 4 : 3) : NC == 1 && KS * QT <= 2 ? 4 : NC == 0 && QT * KS == 1 ? 4 : 2))) void attn_tree_kernel(TreeArgs t, int qblocks, int blocks, int per_xcd,
-                                                       int per_word, int table_off) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_waves(KS, QT, NC)))) void attn_tree_kernel(
+    TreeArgs t, int qblocks, int blocks, int per_xcd, int per_word, int table_off) {
   constexpr int QR = 16 * QT, OLD = 64 * KS + 4, HC = NC > 0 ? NC : 1;
   __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
   __shared__ int32_t sMax[NW][QR];
@@ -446,24 +452,39 @@ int launch_tree(const TreeArgs &t, hipStream_t s) {
   const int qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT), blocks = qblocks * t.a.B * t.a.H, per_xcd = (blocks + 7) / 8;
   const int words = t.a.D / 4, per_word = (65536 + words - 1) / words;
   const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
-  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t, qblocks, blocks, per_xcd, per_word, table);
+  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t,
+                     qblocks, blocks, per_xcd, per_word, table);
   return check_launch("attn_tree_kernel");
 }
 
+// Caches of up to 448 positions are eight chunks with the tree's: a wave each while a block has
+// a CU to itself (26 nodes of 20 heads, us with eight waves of one chunk, four of two and eight in a loop over
+// both passes: 4.9 / 5.5 / 5.2), else four waves of two, which leave more blocks to a CU (16
+// nodes of 2560 heads over 224 keys on average 25.7 / 24.2 / 33.3, one node over 447 31.3 / 30.3 / 38.6).
+// Longer ones loop; a CU draws about 25 bytes a ns from beyond L2, twice over for K, and that
+// bounds few heads over many keys (40 heads of 128 over 2500 keys 39 us of which 26 from warm caches).
+// Parts of the keys on several CUs, with launches for the maxima and the joining, took 42 to 47 us there
+// and 15.6 / 15.6 for 20 heads of 64 over 4096 keys, 7.3 / 11.8 over 1500.
 template <int KS, bool QUADS, int QT>
 int launch_tree_q(const TreeArgs &t, hipStream_t s) {
   const int chunks = (t.a.Tk + 63) / 64 + 1;
   const int64_t blocks = (int64_t)t.a.B * t.a.H * ((t.a.Tq + 16 * QT - 1) / (16 * QT));
-  if (chunks <= 8 && (blocks <= 2 * kCus || chunks <= 4)) return launch_tree<KS, QUADS, QT, 8, 1>(t, s);
-  if (chunks <= 8) return launch_tree<KS, QUADS, QT, 4, 2>(t, s);
-  return launch_tree<KS, QUADS, QT, 8, 0>(t, s);
+  if (chunks > 8) return launch_tree<KS, QUADS, QT, 8, 0>(t, s);
+  if constexpr (QT == 1)
+    if (blocks <= kCus) return launch_tree<KS, QUADS, QT, 8, 1>(t, s);
+  return launch_tree<KS, QUADS, QT, 4, 2>(t, s);
 }
 
+// 16 nodes a block, or 32 over one set of K and V fragments. us of either: 32 nodes of 20, 320
+// and 1280 heads 4.9 / 6.8, 9.7 / 11.4 and 23.7 / 25.9, 64 nodes of 640 heads 20.8 / 21.2: fewer
+// registers are more waves, and neighbouring blocks find K and V in L2. 64 nodes of 1536
+// heads (V transposed) 45.6 / 40.4, of 96 wide ones 102 / 72, of 768 heads over 2300 keys 112 / 100.
+constexpr int64_t kPairTiles = 10 * kCus;
 template <int KS, bool QUADS>
 int launch_tree_k(const TreeArgs &t, hipStream_t s) {
-  const int64_t heads = (int64_t)t.a.B * t.a.H;
-  if (t.a.Tq <= 16 || heads * ((t.a.Tq + 15) / 16) <= 2 * kCus) return launch_tree_q<KS, QUADS, 1>(t, s);
-  return launch_tree_q<KS, QUADS, 2>(t, s);
+  const int64_t tiles = (int64_t)t.a.B * t.a.H * ((t.a.Tq + 15) / 16);
+  if (t.a.Tq > 32 && tiles > kPairTiles) return launch_tree_q<KS, QUADS, 2>(t, s);
+  return launch_tree_q<KS, QUADS, 1>(t, s);
 }
 
 }  // namespace

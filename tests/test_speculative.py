@@ -149,7 +149,9 @@ def test_tree_attention_caches(iw, oracle, gpu, cap, D, N, layout):
 @pytest.mark.parametrize("layout", ["vt", "quads"])
 @pytest.mark.parametrize("B,H,D,cap,N", [(1, 20, 64, 100, 7), (40, 20, 64, 100, 7), (129, 3, 64, 100, 7),
                                          (65, 9, 64, 448, 33), (90, 6, 96, 448, 20), (300, 1, 64, 460, 3),
-                                         (60, 9, 64, 500, 18), (60, 9, 128, 500, 18), (1, 1, 64, 100000, 2)])
+                                         (60, 9, 64, 500, 18), (60, 9, 128, 500, 18), (1, 1, 64, 100000, 2),
+                                         (70, 10, 64, 130, 64), (70, 10, 96, 130, 61), (100, 10, 64, 500, 33),
+                                         (100, 10, 128, 500, 40)])
 def test_tree_attention_grids(iw, oracle, gpu, B, H, D, cap, N, layout):
     """Few and many blocks, one and two tiles of nodes a block, caches above 448 positions with
     their keys in one block and shared by several."""

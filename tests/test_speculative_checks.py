@@ -216,4 +216,4 @@ def test_kernels_keep_their_values_in_registers(iw, tmp_path):
         for m in re.finditer(r"\.name: +(\S*attn_tree_kernel\S*).*?\.sgpr_spill_count: (\d+).*?\.vgpr_spill_count: (\d+)",
                              out, re.S):
             spills[m[1]] = (int(m[2]), int(m[3]))
-    assert len(spills) >= 24 and not any(map(any, spills.values())), spills
+    assert len(spills) >= 20 and not any(map(any, spills.values())), spills
