@@ -267,6 +267,8 @@ class TreeCaches:
 
         ``tokens`` int64, ``parents`` int32, ``choice`` int64 (the model's token after each node,
         ``token_logprobs(..., top=1).top_ids``) [B, N]; ``lengths`` and ``counts`` int32 [B]."""
+        if not -1 << 63 <= eot < 1 << 63:
+            raise RuntimeError("eot must be a token id, or negative for none")
         dev, rows = self.device, (self.batch,)
         shape = (self.batch, self.nodes)
         if not (_is(tokens, _I64, shape, dev) and _is(parents, _I32, shape, dev) and _is(choice, _I64, shape, dev)
@@ -296,7 +298,8 @@ class TokenLogprobs(NamedTuple):
 
 def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, top: int = 0, scale: float = 1.0,
                    suppress: Optional[Tensor] = None) -> TokenLogprobs:
-    """Scores of rows of logits [..., vocab] (int8, float32, bfloat16 or float16), in float32.
+    """Scores of rows of logits [..., vocab] (int8, float32, bfloat16 or float16), in float32,
+    without gradients.
 
     The real logits are ``logits * scale`` (2^-100 or more; for a decoder's int8 logits
     1 / act_logits_alpha); ``suppress`` is a bit mask of tokens that count as
@@ -350,7 +353,8 @@ class TreeDecoder:
     """Decoder passes over trees of drafted tokens, with a DecoderRunner's model and caches.
 
     Call ``runner.set_audio``, then ``start`` with the prompt, then ``step`` with each
-    round of trees. The rows advance by different numbers of tokens (``lengths``), so the
+    round of trees. The rows advance by different numbers of tokens (``lengths``, updated in
+    place: a captured ``step`` replays on new trees in the same tensors), so the
     runner's own one-token steps are not mixed in before its next ``run``. The runner has
     no logit filters: the choices are the plain first-index argmax."""
 
@@ -382,7 +386,7 @@ class TreeDecoder:
         """The prompt step: returns each row's first token [B] (node 0 of its first tree)."""
         r = self.runner
         r.run(prompt, 1)
-        self.lengths = torch.full((r.B,), prompt.shape[1], dtype=torch.int32, device=prompt.device)
+        self.lengths.fill_(prompt.shape[1])
         return r.tokens.clone()
 
     def verify(self, tokens: Tensor, parents: Tensor, counts: Optional[Tensor] = None) -> Tensor:
@@ -428,5 +432,5 @@ class TreeDecoder:
         scores = token_logprobs(logits, top=top, scale=self.runner.logit_scale)
         choice = scores.top_ids[..., 0].contiguous()
         got = self.caches.accept(tokens, parents, choice, self.lengths, counts, eot=eot)
-        self.lengths = got.lengths
+        self.lengths.add_(got.accepted)
         return TreeStep(got, scores, logits)

@@ -376,6 +376,9 @@ def test_tree_caches_refuse(iw, gpu):
         c.accept(t[:, :3], p, t, ln)
     with pytest.raises(RuntimeError, match="shape"):
         c.accept(t, p, t, ln[:1])
+    for eot in (1 << 63, 1 << 64, -(1 << 70)):
+        with pytest.raises(RuntimeError, match="eot"):
+            c.accept(t, p, t, ln, eot=eot)
 
 
 # ---------------------------------------------------------------------------
@@ -719,3 +722,44 @@ def test_tree_decoder_is_greedy_decoding(iw, gpu, heads, nodes):
             else:
                 a, b = a[..., :n], b[..., :n]
             assert torch.equal(a, b)
+
+
+def test_tree_decoder_step_replays(iw, gpu):
+    """A captured step: its replays on new trees advance the rows as eager steps do."""
+    dims, model = small_model(iw)
+    B, N, rounds = 2, 5, 6
+    mel = iw.synth.synthetic_mel(B, dims.n_mels, 2 * dims.n_audio_ctx, seed=22)
+    prompt = T(np.array([[1, 2, 3], [4, 5, 6]], np.int64))
+    tokens = torch.zeros((B, N), dtype=torch.int64, device="cuda")
+    parents = torch.zeros((B, N), dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        feats = model.embed_audio(T(mel))
+        runs = []
+        for captured in (False, True):
+            runner = iw.DecoderRunner(model.decoder, B, dims.n_audio_ctx)
+            runner.set_audio(feats)
+            tree = iw.speculative.TreeDecoder(runner, N)
+            if captured:
+                tree.start(prompt)
+                tree.step(tokens, parents)
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    res = tree.step(tokens, parents)
+            r = gen.rng(9)
+            last = tree.start(prompt)
+            kept = []
+            for _ in range(rounds):
+                tokens.copy_(T(r.integers(0, dims.n_vocab, (B, N))))
+                tokens[:, 0] = last
+                parents.copy_(T(random_tree(r, B, N)))
+                if captured:
+                    g.replay()
+                else:
+                    res = tree.step(tokens, parents)
+                last = res.accept.next_token.clone()
+                kept += [t.clone() for t in (*res.accept, res.logits, tree.lengths)]
+                torch.cuda.synchronize()
+            assert (tree.lengths >= 3 + rounds).all()
+            runs.append(kept)
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
