@@ -112,6 +112,7 @@ SIGNATURES = {
 # entry points that return a value rather than a status
 VALUE_FUNCS = {"iw_frag_bytes": ([_i64, _i64], C.c_int64),
                "iw_log_mel_scratch_floats": ([_i64, _i64], C.c_int64),
+               "iw_attention_tree_workspace": ([_i64, _i64, _i64, _i64, _i64], C.c_int64),
                "iw_token_logprobs_workspace": ([_i32, _i64, _i64, _i64], C.c_int64)}
 
 _lock = threading.Lock()

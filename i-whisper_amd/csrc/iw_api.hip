@@ -955,6 +955,9 @@ int iw_attention_tree(const iw_attention_tree_args *args, iw_stream_t stream) {
   IW_REQUIRE(p.kn_st >= 0 && p.kn_st < far && p.vn_st >= 0 && p.vn_st < far && p.k_st >= 0 && p.k_st < far &&
                  p.v_sq >= 0 && p.v_sq < far && p.v_sd >= 0 && p.v_sd < far,
              "strides of nodes, keys, key quads and transposed rows must be below 2^25");
+  IW_REQUIRE(attn_tree_workspace(p.batch * p.heads, p.nodes, p.head_dim, p.cache_positions) == 0 ||
+                 (p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 15) == 0),
+             "iw_attention_tree_workspace bytes of 16-byte aligned workspace are needed");
   TreeArgs t;
   AttnArgs &a = t.a;
   a.q = p.q;
@@ -993,7 +996,16 @@ int iw_attention_tree(const iw_attention_tree_args *args, iw_stream_t stream) {
   t.visible = reinterpret_cast<const uint64_t *>(p.visible);
   t.vis_sb = p.visible_sb;
   t.counts = p.counts;
+  t.workspace = static_cast<uint32_t *>(p.workspace);
   return launch_attn_tree(t, as_stream(stream));
+}
+
+int64_t iw_attention_tree_workspace(int64_t batch, int64_t heads, int64_t nodes, int64_t head_dim,
+                                    int64_t cache_positions) {
+  if (batch < 0 || batch > (1 << 22) || heads <= 0 || heads > 4096 || nodes <= 0 || nodes > kTreeMaxNodes || head_dim <= 0 ||
+      head_dim > 128 || cache_positions <= 0 || cache_positions >= (1 << 24))
+    return -1;
+  return batch == 0 ? 0 : attn_tree_workspace(batch * heads, nodes, head_dim, cache_positions);
 }
 
 int iw_tree_accept(const iw_tree_caches *caches, const int64_t *tokens, const int32_t *parents,

@@ -6,7 +6,7 @@
 // first, then P = E(S - rowmax - 1), sum P and P.V, exact modulo 2^32 in any
 // order, so the keys can be split over waves.
 //
-// One block per (batch, head) and up to 32 nodes (two 16-query MFMA tiles). The
+// One block per (batch, head) and 16 or 32 nodes (one or two 16-query MFMA tiles). The
 // block's waves take 64-key chunks in turn, the tree itself is one more chunk.
 // In a chunk's four 16x16x64 score products, row 4g + r of product t is key
 // 16g + 4t + r: lane group g then holds the scores of the 16 consecutive keys
@@ -18,6 +18,12 @@
 // frac_bits 10 the distances below that are read from a table that the block
 // copies to LDS while its K and V are on the way (1249 bytes at 8, 4988 at 10);
 // beyond, each score computes its own.
+//
+// Where a long cache meets few heads, several blocks share the keys of a block's
+// nodes: a first launch leaves each part's row maxima in the workspace, a second
+// each part's sums, a third adds them.
+#include <algorithm>
+
 #include "iw_attn_dev.hpp"
 #include "iw_common.hpp"
 #include "iw_tree.hpp"
@@ -91,19 +97,33 @@ __device__ __forceinline__ uint32_t output_word(const AttnArgs &a, const uint32_
   return w;
 }
 
+// A part in the workspace: the sums of P.V of its rows, those of P, the row maxima
+constexpr int64_t part_words(int ks, int qt) { return 16 * qt * (64 * ks + 2); }
+template <int KS, int QT>
+__device__ __forceinline__ uint32_t *part_of(const TreeArgs &t, int block, int part, int parts) {
+  return t.workspace + ((int64_t)block * parts + part) * part_words(KS, QT);
+}
+// chunks of a part, of the nkc cached ones and the tree's
+__device__ __forceinline__ int part_share(int nkc, int parts) { return (nkc + parts) / parts; }
+
+// Of all keys, or of blockIdx.y's part of them: the row maxima, or with every part's maxima the sums
+enum { ALL, PART_MAX, PART_SUM };
+
 // KS: 64-column parts of the head; QUADS: V in key quads; QT: 16-query tiles of
 // the block; NW waves; NC > 0: a wave has at most NC chunks, whose K and V
 // are all requested at the start and kept. Waves per SIMD are asked for where the
 // registers allow them: held chunks of 64-wide heads in 128 registers, which the compiler
 // exceeds on its own (206, two waves: 16 nodes of 2560 heads 38 us, with four 28).
-constexpr int tree_waves(int ks, int qt, int nc) {
+constexpr int tree_waves(int ks, int qt, int nc, int mode) {
+  if (mode == PART_MAX) return 4;
   if (nc == 2) return ks == 1 ? (qt == 1 ? 4 : 3) : 2;
   return nc == 1 || ks * qt == 1 ? 4 : 2;
 }
-template <int KS, bool QUADS, int QT, int NW, int NC>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_waves(KS, QT, NC)))) void attn_tree_kernel(
+template <int KS, bool QUADS, int QT, int NW, int NC, int MODE>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_waves(KS, QT, NC, MODE)))) void attn_tree_kernel(
     TreeArgs t, int qblocks, int blocks, int per_xcd, int per_word, int table_off) {
   constexpr int QR = 16 * QT, OLD = 64 * KS + 4, HC = NC > 0 ? NC : 1;
+  static_assert(MODE == ALL || NC == 0, "parts loop over their chunks");
   __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
   __shared__ int32_t sMax[NW][QR];
   __shared__ uint32_t sSum[QR];
@@ -124,6 +144,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   const int len = clampi(t.lengths[b], 0, a.Tk);
   const int cnt = t.counts ? clampi(t.counts[b], 0, N) : N;
   const int nkc = (len + 63) / 64;  // cached chunks; chunk nkc is the tree
+  const int parts = MODE == ALL ? 1 : (int)gridDim.y, part = MODE == ALL ? 0 : (int)blockIdx.y;
+  const int share = part_share(nkc, parts);
+  // this block's cached chunks, and whether the tree is its too
+  const int c_lo = part * share, c_hi = min(c_lo + share, nkc);
+  const bool has_tree = c_lo <= nkc && c_lo + share > nkc;
   const int8_t *const kbase = a.k + b * a.k_sb + (int64_t)h * a.k_sh;
   const int8_t *const vbase = a.vt + b * a.v_sb + (int64_t)h * a.v_sh;
   const int8_t *const knew = t.kn + b * t.kn_sb + (int64_t)h * D;
@@ -133,6 +158,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   // i / words for the i < 2^11 of the output
   const auto by_words = [&](int i) { return (int)__umul24(i, per_word) >> 16; };
 
+  if (MODE != ALL && (q0 >= cnt || c_lo > nkc)) return;
   if (q0 >= cnt) {  // no node of these is in use
     for (int i = tid; i < rows * words; i += 64 * NW) {
       const int q = by_words(i);
@@ -238,11 +264,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   }
   const bool table = table_off >= 0;
   const int zero = table ? shift_exp_zero(a.frac_bits) : IW_SEXP_LUT - 1;
-  if (table)
-    for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
-      *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
-  for (int i = tid; i < QR; i += 64 * NW) sSum[i] = 0u;
-  for (int i = tid; i < QR * OLD; i += 64 * NW) sO[i] = 0u;
+  if (MODE != PART_MAX) {
+    if (table)
+      for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
+        *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
+    for (int i = tid; i < QR; i += 64 * NW) sSum[i] = 0u;
+    for (int i = tid; i < QR * OLD; i += 64 * NW) sO[i] = 0u;
+  }
 
   auto scores = [&](const v4i (&f)[KS], int u) {
     v4i s{0, 0, 0, 0};
@@ -288,22 +316,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
       const int c = wave + NW * i;
       if (c <= nkc) chunk_max(c, c == nkc, kf[i]);
     }
-  } else {
+  } else if constexpr (MODE != PART_SUM) {
     v4i kn[4][KS];
 #pragma unroll 1
-    for (int c = wave; c < nkc; c += 2 * NW) {
+    for (int c = c_lo + wave; c < c_hi; c += 2 * NW) {
       load_k(c, false, kf[0]);
-      if (c + NW < nkc) load_k(c + NW, false, kn);
+      if (c + NW < c_hi) load_k(c + NW, false, kn);
       chunk_max(c, false, kf[0]);
-      if (c + NW < nkc) chunk_max(c + NW, false, kn);
+      if (c + NW < c_hi) chunk_max(c + NW, false, kn);
     }
-    if (nkc % NW == wave) {
+    if (has_tree && (nkc - c_lo) % NW == wave) {
       load_k(nkc, true, kf[0]);
       chunk_max(nkc, true, kf[0]);
     }
   }
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
+    if (MODE == PART_SUM)  // the maxima of the parts that have chunks, shared out to the waves' lane groups
+      for (int p = NW * g + wave; p * share <= nkc; p += 4 * NW)
+        mx[u] = max(mx[u], (int32_t)part_of<KS, QT>(t, block, p, parts)[QR * (64 * KS + 1) + 16 * u + n]);
     mx[u] = max(mx[u], __shfl_xor(mx[u], 16));
     mx[u] = max(mx[u], __shfl_xor(mx[u], 32));
     if (lane < 16) sMax[wave][16 * u + lane] = mx[u];
@@ -315,10 +346,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   for (int u = 0; u < QT; ++u) {
 #pragma unroll
     for (int w = 0; w < NW; ++w) mx[u] = max(mx[u], sMax[w][16 * u + n]);
+    if constexpr (MODE == PART_MAX) {
+      if (tid < 16) part_of<KS, QT>(t, block, part, parts)[QR * (64 * KS + 1) + 16 * u + tid] = (uint32_t)mx[u];
+      continue;
+    }
     // requantization keeps the order, so the maximum's is the maximum
     rowmax[u] = mx[u] == INT32_MIN ? -32768 : qk_requant16(mx[u], a.qk_m, a.qk_s);
     sat = sat || rowmax[u] >= 32767;
   }
+  if constexpr (MODE == PART_MAX) return;
   // the short index where no row maximum wraps: the keys that count lie at a
   // distance of 1 at least, the others are taken for such
   const bool brief = table && !__any(sat);
@@ -416,8 +452,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
       }
     };
 #pragma unroll 1
-    for (int c = wave; c < nkc; c += NW) chunk(c, false);
-    if (nkc % NW == wave) chunk(nkc, true);
+    for (int c = c_lo + wave; c < c_hi; c += NW) chunk(c, false);
+    if (has_tree && (nkc - c_lo) % NW == wave) chunk(nkc, true);
   }
 
   // ---- the waves' sums meet in LDS ----
@@ -435,6 +471,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
           atomicAdd(&sO[(16 * u + 4 * g + r) * OLD + 64 * ks + 4 * n + i], (uint32_t)o[u][ks][i][r]);
   }
   lds_barrier();
+  if constexpr (MODE == PART_SUM) {
+    uint32_t *mine = part_of<KS, QT>(t, block, part, parts);
+    for (int i = 4 * tid; i < QR * 64 * KS; i += 4 * 64 * NW)
+      *reinterpret_cast<v4i *>(mine + i) = *reinterpret_cast<const v4i *>(&sO[i / (64 * KS) * OLD + i % (64 * KS)]);
+    if (tid < QR) mine[QR * 64 * KS + tid] = sSum[tid];
+    return;
+  }
   if (tid < QR) sInv[tid] = fisr((int32_t)sSum[tid], a.rsqrt_off);
   lds_barrier();
   for (int i = tid; i < rows * words; i += 64 * NW) {
@@ -445,26 +488,92 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   }
 }
 
+// Adds the parts of a block's row and finishes it, a wave a row: lane l has word l % W of parts l / W,
+// l / W + 64 / W, ..., four of them on the way at once.
+template <int KS, int QT>
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs t, int qblocks, int parts) {
+  constexpr int QR = 16 * QT, W = 16 * KS, AT_ONCE = 64 / W;
+  const AttnArgs &a = t.a;
+  const int lane = threadIdx.x & 63, w = lane % W;
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), block = blockIdx.y;
+  const int q = block % qblocks * QR + row, bh = block / qblocks, h = bh % a.H;
+  const int64_t b = bh / a.H;
+  if (q >= a.Tq) return;
+  const int nkc = (clampi(t.lengths[b], 0, a.Tk) + 63) / 64;
+  const int cnt = t.counts ? clampi(t.counts[b], 0, a.Tq) : a.Tq;
+  const int used = nkc / part_share(nkc, parts) + 1;  // parts that have chunks
+  uint32_t sums[4] = {0u, 0u, 0u, 0u}, psum = 0u;
+  if (q < cnt) {
+    for (int p0 = lane / W; p0 < used; p0 += 4 * AT_ONCE) {
+      v4i x[4];
+      uint32_t y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t *from = part_of<KS, QT>(t, block, min(p0 + j * AT_ONCE, used - 1), parts);
+        x[j] = *reinterpret_cast<const v4i *>(from + row * 64 * KS + 4 * w);
+        y[j] = from[QR * 64 * KS + row];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (p0 + j * AT_ONCE < used) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sums[c] += (uint32_t)x[j][c];
+          psum += y[j];
+        }
+    }
+#pragma unroll
+    for (int m = W; m < 64; m *= 2) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sums[c] += (uint32_t)__shfl_xor((int)sums[c], m);
+      psum += (uint32_t)__shfl_xor((int)psum, m);
+    }
+  }
+  if (lane < a.D / 4)
+    *reinterpret_cast<uint32_t *>(a.out + b * a.o_sb + (int64_t)q * a.o_st + (int64_t)h * a.D + 4 * lane) =
+        q < cnt ? output_word(a, sums, fisr((int32_t)psum, a.rsqrt_off)) : 0u;
+}
+
 constexpr int kCus = 256;
 
-template <int KS, bool QUADS, int QT, int NW, int NC>
-int launch_tree(const TreeArgs &t, hipStream_t s) {
+template <int KS, bool QUADS, int QT, int NW, int NC, int MODE = ALL>
+int launch_tree(const TreeArgs &t, hipStream_t s, int parts = 1) {
   const int qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT), blocks = qblocks * t.a.B * t.a.H, per_xcd = (blocks + 7) / 8;
   const int words = t.a.D / 4, per_word = (65536 + words - 1) / words;
   const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
-  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t,
-                     qblocks, blocks, per_xcd, per_word, table);
+  hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC, MODE>), dim3((unsigned)(8 * per_xcd), (unsigned)parts),
+                     dim3(64 * NW), 0, s, t, qblocks, blocks, per_xcd, per_word, table);
   return check_launch("attn_tree_kernel");
 }
 
+template <int KS, bool QUADS, int QT>
+int launch_tree_parts(const TreeArgs &t, int parts, hipStream_t s) {
+  int rc = launch_tree<KS, true, QT, 8, 0, PART_MAX>(t, s, parts);  // reads K only
+  if (rc == 0) rc = launch_tree<KS, QUADS, QT, 8, 0, PART_SUM>(t, s, parts);
+  if (rc) return rc;
+  const int qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT);
+  hipLaunchKernelGGL((attn_tree_join_kernel<KS, QT>), dim3((unsigned)(4 * QT), (unsigned)(qblocks * t.a.B * t.a.H)),
+                     dim3(256), 0, s, t, qblocks, parts);
+  return check_launch("attn_tree_join_kernel");
+}
+
+// Blocks to the keys of one (batch, head) and its 16 nodes, or 32 where there are more: as many as the CUs hold at
+// one each. A CU draws 25 to 40 bytes a ns from beyond L2, which bounds a long cache's blocks where they are
+// few, but three launches are about 15 us. us split and not: 40 heads of 128 over up to 4096 keys, 61 nodes 27.1 / 39.6,
+// 16 nodes 18.7 / 39.2, over up to 1024 18.8 / 15.6 and 15.5 / 15.5, 120 heads over 1500 21.0 / 20.9, over 2048 24.1 / 27.9.
+// Narrow heads, 16 and 61 nodes of 40: over 4096 keys 14.5 / 14.3 and 18.4 / 14.4, 8192 17.0 / 23.1 and 23.1 / 22.7,
+// 16384 24.7 / 52.1 and 35.4 / 47.7. Two groups of waves with 32 nodes each on the same keys took 28.9 in the place of
+// 27.1, 64 nodes a wave 38.7 (spills), the next keys requested ahead 27.3.
+constexpr int kSplitNarrow = 8192, kSplitWide = 1536;  // positions
+int tree_parts(int64_t heads, int64_t nodes, int64_t head_dim, int64_t cap) {
+  if (cap < (head_dim <= 64 ? kSplitNarrow : kSplitWide)) return 1;
+  const int64_t blocks = heads * (nodes <= 16 ? 1 : (nodes + 31) / 32), chunks = (cap + 63) / 64 + 1;
+  return (int)std::max<int64_t>(1, std::min(kCus / blocks, (chunks + 7) / 8));
+}
 // Caches of up to 448 positions are eight chunks with the tree's: a wave each while a block has
 // a CU to itself (26 nodes of 20 heads, us with eight waves of one chunk, four of two and eight in a loop over
 // both passes: 4.9 / 5.5 / 5.2), else four waves of two, which leave more blocks to a CU (16
 // nodes of 2560 heads over 224 keys on average 25.7 / 24.2 / 33.3, one node over 447 31.3 / 30.3 / 38.6).
-// Longer ones loop; a CU draws about 25 bytes a ns from beyond L2, twice over for K, and that
-// bounds few heads over many keys (40 heads of 128 over 2500 keys 39 us of which 26 from warm caches).
-// Parts of the keys on several CUs, with launches for the maxima and the joining, took 42 to 47 us there
-// and 15.6 / 15.6 for 20 heads of 64 over 4096 keys, 7.3 / 11.8 over 1500.
+// Longer ones loop.
 template <int KS, bool QUADS, int QT>
 int launch_tree_q(const TreeArgs &t, hipStream_t s) {
   const int chunks = (t.a.Tk + 63) / 64 + 1;
@@ -482,12 +591,21 @@ int launch_tree_q(const TreeArgs &t, hipStream_t s) {
 constexpr int64_t kPairTiles = 10 * kCus;
 template <int KS, bool QUADS>
 int launch_tree_k(const TreeArgs &t, hipStream_t s) {
+  const int parts = tree_parts((int64_t)t.a.B * t.a.H, t.a.Tq, t.a.D, t.a.Tk);
+  if (parts > 1)
+    return t.a.Tq <= 16 ? launch_tree_parts<KS, QUADS, 1>(t, parts, s) : launch_tree_parts<KS, QUADS, 2>(t, parts, s);
   const int64_t tiles = (int64_t)t.a.B * t.a.H * ((t.a.Tq + 15) / 16);
   if (t.a.Tq > 32 && tiles > kPairTiles) return launch_tree_q<KS, QUADS, 2>(t, s);
   return launch_tree_q<KS, QUADS, 1>(t, s);
 }
 
 }  // namespace
+
+int64_t attn_tree_workspace(int64_t heads, int64_t nodes, int64_t head_dim, int64_t cap) {
+  const int64_t parts = tree_parts(heads, nodes, head_dim, cap), qt = nodes <= 16 ? 1 : 2;
+  if (parts == 1) return 0;
+  return 4 * heads * ((nodes + 16 * qt - 1) / (16 * qt)) * parts * part_words(head_dim <= 64 ? 1 : 2, (int)qt);
+}
 
 int launch_attn_tree(const TreeArgs &t, hipStream_t s) {
   const bool quads = t.a.v_sq != 4;

@@ -21,7 +21,9 @@ struct TreeArgs {
   const uint64_t *visible = nullptr;          // [b][node] bits of the nodes that a node sees
   int64_t vis_sb = 0;
   const int32_t *counts = nullptr;            // nodes in use of each row; null = a.Tq
+  uint32_t *workspace = nullptr;              // attn_tree_workspace bytes
 };
+int64_t attn_tree_workspace(int64_t heads, int64_t nodes, int64_t head_dim, int64_t cap);  // heads of all rows
 int launch_attn_tree(const TreeArgs &t, hipStream_t s);
 
 int launch_tree_plan(const int32_t *parents, int64_t p_ld, const int32_t *counts, const int32_t *lengths,

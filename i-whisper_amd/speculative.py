@@ -36,7 +36,7 @@ MAX_NODES = 64
 MAX_TOP = 32
 _LOGIT_TYPES = {torch.int8: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
 _I8, _I32, _I64 = torch.int8, torch.int32, torch.int64
-_ATTENTION_ARGS = struct.Struct("36q")  # iw_attention_tree_args
+_ATTENTION_ARGS = struct.Struct("37q")  # iw_attention_tree_args
 _CACHES = struct.Struct("21q")          # iw_tree_caches
 
 
@@ -209,10 +209,14 @@ def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_c
         if (B > 1 and sb < C) or (N > 1 and st < C) or (
                 B > 1 and N > 1 and sb < (N - 1) * st + C and st < (B - 1) * sb + C):
             raise RuntimeError("the rows of out must not overlap")
+    # shorter caches need none
+    need = _lib.value("iw_attention_tree_workspace", B, heads, N, D, T) if T >= 1536 else 0
+    work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     args = _pack(_ATTENTION_ARGS, q.data_ptr(), *q_s, k_new.data_ptr(), *kn_s, v_new.data_ptr(), *vn_s,
                  k_cache.data_ptr(), *k_s, v_cache.data_ptr(), *v_s, lengths.data_ptr(), visible.data_ptr(),
                  0 if shared else N, 0 if counts is None else counts.data_ptr(), out.data_ptr(), *o_s, B, heads, N, D, T,
-                 qk_multiplier, qk_shift, frac_bits, av_multiplier, av_shift, rsqrt_offset)
+                 qk_multiplier, qk_shift, frac_bits, av_multiplier, av_shift, rsqrt_offset,
+                 0 if work is None else work.data_ptr())
     _launch(dev, "iw_attention_tree", args)
     return out
 

@@ -629,7 +629,9 @@ int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *coun
  * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24; operands and
  * strides are multiples of 16 bytes; kn_st, vn_st, k_st, v_sd, v_sq < 2^25. The
  * caches are read only: the nodes' K and V enter them with iw_tree_accept. out shares
- * no memory with k_new, v_new or the caches. The struct is read during the call. */
+ * no memory with k_new, v_new or the caches. workspace: iw_attention_tree_workspace
+ * bytes, 16-byte aligned, used during the call's work only (NULL where that is 0: at
+ * least for all caches of fewer than 1536 positions). The struct is read during the call. */
 typedef struct iw_attention_tree_args {
   const int8_t *q;
   int64_t q_sb, q_st;
@@ -649,8 +651,11 @@ typedef struct iw_attention_tree_args {
   int64_t o_sb, o_st;
   int64_t batch, heads, nodes, head_dim, cache_positions;
   int64_t qk_multiplier, qk_shift, frac_bits, av_multiplier, av_shift, rsqrt_offset;
+  void *workspace;
 } iw_attention_tree_args;
 int iw_attention_tree(const iw_attention_tree_args *args, iw_stream_t stream);
+int64_t iw_attention_tree_workspace(int64_t batch, int64_t heads, int64_t nodes, int64_t head_dim,
+                                    int64_t cache_positions);
 
 /* Greedy acceptance: from node 0, the path goes on to the first node in use
  * whose parent is the current node and whose token is choice[current] (the

@@ -164,6 +164,34 @@ def test_tree_attention_grids(iw, oracle, gpu, B, H, D, cap, N, layout):
     assert np.array_equal(host(c.run(iw))[rows], c.expected(oracle, rows)[rows])
 
 
+@pytest.mark.parametrize("layout", ["vt", "quads"])
+@pytest.mark.parametrize("D,cap,N", [(128, 1536, 1), (128, 1600, 16), (80, 2100, 17), (128, 2049, 33), (112, 1999, 64),
+                                     (64, 8192, 5), (48, 8300, 50)])
+def test_tree_attention_shared_keys(iw, oracle, gpu, D, cap, N, layout):
+    """Caches whose keys several blocks share: parts without a chunk, with the tree alone, rows without
+    nodes or keys, and a workspace with other values in it."""
+    print("case: tree attention shared keys", D, cap, N, layout, flush=True)
+    B, H = 8, 1
+    assert iw._lib.value("iw_attention_tree_workspace", B, H, N, D, cap) > 0
+    c = Case(cap, B, H, D, cap, N, [0, 1, 64, cap - 1, cap, cap // 2, 0, cap // 3], [N, N, 1, N, N, (N + 1) // 2, N, 0], layout)
+    c.visible[6] = 0  # no key at all
+    c.visible[5, 0] = 0
+    torch.full((1 << 23,), 0x7f, dtype=torch.uint8, device="cuda")
+    want = c.expected(oracle)
+    assert not want[6:].any()
+    out = torch.full((B, N, H * D), 77, dtype=torch.int8, device="cuda")
+    assert np.array_equal(host(c.run(iw, out=out)), want)
+    assert np.array_equal(host(c.run(iw)), want)
+
+
+@pytest.mark.parametrize("f", [1, 8, 10, 11, 13])
+@pytest.mark.parametrize("qk", [(255, 0), (200, 4), (255, 40)])
+def test_tree_attention_shared_keys_scalars(iw, oracle, gpu, f, qk):
+    print("case: tree attention shared keys, scalars", f, qk, flush=True)
+    c = Case(f, 2, 1, 96, 1700, 18, [1700, 900], [18, 11], "quads", scalars=(*qk, f, 255, 7))
+    assert np.array_equal(host(c.run(iw)), c.expected(oracle))
+
+
 @pytest.mark.parametrize("f", range(1, 14))
 @pytest.mark.parametrize("qk", [(255, 0), (1, 0), (200, 4), (3, 9), (255, 31), (255, 40), (0, 3)])
 def test_tree_attention_scalars(iw, oracle, gpu, f, qk):
@@ -642,6 +670,41 @@ def test_captured_round_replays(iw, gpu):
         torch.cuda.synchronize()
         for a, b in zip([*outs, k, v], want):
             assert torch.equal(a, b) or torch.equal(a.isnan(), b.isnan())
+
+
+def test_captured_long_cache_replays(iw, gpu):
+    """Two graphs of a cache whose keys several blocks share, replayed on two streams at once."""
+    B, H, D, cap, N = 2, 2, 128, 2000, 9
+    cases = [Case(i, B, H, D, cap, N, [cap, 300 + i], [N, N - 2], "vt") for i in range(2)]
+    graphs, got = [], []
+    for c in cases:
+        c.args = T(c.qkv), T(c.k), T(c.vc), T(c.lengths), T(c.visible), T(c.counts)
+
+    def run(c):
+        qkv, k, v, ln, vis, cnt = c.args
+        C = H * D
+        return iw.speculative.tree_attention(qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:], k, v, ln, vis, cnt,
+                                             heads=H, qk_multiplier=90, qk_shift=9, frac_bits=8, av_multiplier=100,
+                                             av_shift=6)
+    for c in cases:
+        run(c)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(run(c))
+    streams = [torch.cuda.Stream() for _ in cases]
+    for i in range(4):
+        for c in cases:
+            r = gen.rng(10 * i + cases.index(c))
+            c.args[0].copy_(T(gen.i8(r, c.qkv.shape)))
+            c.args[3].copy_(T(r.integers(0, cap + 1, B).astype(np.int32)))
+        want = [run(c).clone() for c in cases]
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_two_streams_at_once(iw, gpu):

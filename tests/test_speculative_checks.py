@@ -26,7 +26,7 @@ PLAN = dict(parents=P, ld=8, counts=None, lengths=None, batch=2, nodes=8, maxp=4
 ATTN = dict(q=P, q_sb=1024, q_st=128, kn=P, kn_sb=1024, kn_st=128, vn=P, vn_sb=1024, vn_st=128, k=P, k_sb=4096,
             k_sh=2048, k_st=64, v=P, v_sb=4096, v_sh=2048, v_sd=4, v_sq=256, lengths=P, visible=P, vis_sb=8,
             counts=None, out=P, o_sb=1024, o_st=128, batch=1, heads=2, nodes=8, D=64, cap=32, qm=3, qs=4, f=8, am=3,
-            as_=4, off=16, stream=None)
+            as_=4, off=16, work=None, stream=None)
 ACCEPT = dict(tokens=P, parents=P, choice=P, counts=None, lengths=P, batch=2, nodes=8, eot=-1, path=P, accepted=P,
               next=P, lengths_out=P + 64, layers=1, kn="a", vn="a", kn_sb=1024, kn_st=128, vn_sb=1024, vn_st=128,
               k="a", k_sb=4096, k_sh=2048, k_st=64, v="a", v_sb=4096, v_sh=2048, v_sd=4, v_sq=256, heads=2, D=64,
@@ -83,7 +83,8 @@ def test_plan_refusals(iw, change, what):
     (dict(out=None), "null"), (dict(batch=-1), "attention shape"), (dict(batch=1 << 22), "attention shape"),
     (dict(vis_sb=-1), "attention shape"), (dict(k_st=1 << 25), "2^25"), (dict(kn_st=1 << 25), "2^25"),
     (dict(v_sq=1 << 25), "2^25"), (dict(qm=256), "uint8"), (dict(am=-1), "uint8"), (dict(qs=128), "int8"),
-    (dict(as_=-129), "int8"), (dict(off=-1), "rsqrt_offset")])
+    (dict(as_=-129), "int8"), (dict(off=-1), "rsqrt_offset"), (dict(cap=20000), "workspace"),
+    (dict(cap=20000, work=P + 8), "workspace")])
 def test_attention_refusals(iw, change, what):
     refused(iw, "iw_attention_tree", ATTN, change, what)
 
@@ -140,6 +141,13 @@ def test_workspace_size(iw):
         assert v("iw_token_logprobs_workspace", kind, 8, 200000, 4) > 0
     for bad in ((0, -1, 5, 0), (0, 1, -5, 0), (0, 1, 5, -1), (4, 1, 5, 0), (-1, 1, 5, 0)):
         assert v("iw_token_logprobs_workspace", *bad) == -1
+    for T in (1, 448, 1535):
+        assert all(v("iw_attention_tree_workspace", 1, h, 64, D, T) == 0 for h in (1, 40) for D in (64, 128))
+    assert 0 < v("iw_attention_tree_workspace", 5, 8, 61, 128, 4096) < 1 << 23
+    assert 0 < v("iw_attention_tree_workspace", 1, 1, 1, 16, (1 << 24) - 1) < 1 << 23
+    assert v("iw_attention_tree_workspace", 0, 8, 61, 128, 4096) == 0
+    for bad in ((-1, 8, 8, 64, 64), (1, 0, 8, 64, 64), (1, 8, 65, 64, 64), (1, 8, 8, 129, 64), (1, 8, 8, 64, 1 << 24)):
+        assert v("iw_attention_tree_workspace", *bad) == -1
 
 
 def i8(*shape):
