@@ -116,9 +116,18 @@ struct Logit<int8_t> {
     }
     return t;
   }
-  static __device__ __forceinline__ float max(const uint4 &w) {
-    const v2s t = halves(w);
-    return (float)::max(t.x >> 8, t.y >> 8);
+  // bit 8 i + q for each byte i of word q that is v or more (v from -128 on)
+  static __device__ __forceinline__ uint32_t reaching(const uint4 &w, int v) {
+    constexpr uint32_t H = 0x80808080u;
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w}, low = (uint32_t)(v & 0x7f) * 0x01010101u;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // the bytes' lower seven bits are those of v or more; a byte's own sign decides if v has the other
+      const uint32_t ge = (x[q] | H) - low;
+      bits |= ((v < 0 ? ~x[q] | ge : ~x[q] & ge) & H) >> (7 - q);
+    }
+    return bits;
   }
 };
 template <typename D, int N>
@@ -302,7 +311,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
   float xe = has_extra ? L::one(&xr) : -INFINITY;
   if (!I8 && a.suppress && has_extra && ((sWords[extra >> 5] >> (extra & 31)) & 1u)) xe = -INFINITY;
 
-  float m, reach, tmax = INFINITY, z = 0.f, u = 0.f, eq = 0.f;
+  float m, reach, tmax, z = 0.f, u = 0.f, eq = 0.f;
   if constexpr (I8) {
     uint32_t *const mine = s.count + (lane & (kCopies - 1));
     // value v at 128 + v, that is the byte with its sign bit turned
@@ -435,27 +444,38 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
   }
 
   // ---- the logits that reach the bound ----
-  if (I8 && a.top > 0) {
-    typename Logit<int8_t>::v2s t{-32768, -32768};
+  auto put = [&](float v, int col) {
+    if (v >= reach) {
+      const int at = atomicAdd(&s.cands, 1);
+      if (at < kCand) s.cand[at] = key_of(v, col);
+    }
+  };
+  if constexpr (I8) {
+    if (a.top > 0) {
+      const int least = max((int)reach, -128);
+      // a piece whose largest byte is below it has none
+      using v2s = typename L::v2s;
+      const int16_t under = (int16_t)(256 * least - (least > -128));
+      const v2s bound{under, under};
+      if (has_extra && !suppressed(a.suppress, c0 + extra)) put(xe, c0 + extra);
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (held(p)) t = __builtin_elementwise_max(t, Logit<int8_t>::halves(w[p]));
-    tmax = fmaxf((float)max(t.x >> 8, t.y >> 8), xe);
-  }
-  if (a.top > 0 && tmax >= reach) {
-    auto put = [&](float v, int col) {
-      if (v >= reach) {
-        const int at = atomicAdd(&s.cands, 1);
-        if (at < kCand) s.cand[at] = key_of(v, col);
-      }
-    };
-    if (has_extra && !(I8 && suppressed(a.suppress, c0 + extra))) put(xe, c0 + extra);
+      for (int p = 0; p < P; ++p)
+        if (held(p) && (least == -128 || __builtin_bit_cast(uint32_t, __builtin_elementwise_max(L::halves(w[p]), bound)) !=
+                                             __builtin_bit_cast(uint32_t, bound))) {
+          uint32_t bits = L::reaching(w[p], least);
+          const uint32_t o = a.suppress ? hidden(p) : 0u;
+          for (; bits; bits &= bits - 1) {
+            const int at = __ffs((int)bits) - 1, e = 4 * (at & 7) + (at >> 3);
+            if (!((o >> e) & 1u)) put(L::get(w[p], e), column(p) + e);
+          }
+        }
+    }
+  } else if (a.top > 0 && tmax >= reach) {
+    if (has_extra) put(xe, c0 + extra);
 #pragma unroll
     for (int p = 0; p < P; ++p)
       if (held(p) && L::max(w[p]) >= reach) {
-        const uint32_t o = I8 && a.suppress ? hidden(p) : 0u;
-        for (int e = 0; e < E; ++e)
-          if (!((o >> e) & 1u)) put(L::get(w[p], e), column(p) + e);
+        for (int e = 0; e < E; ++e) put(L::get(w[p], e), column(p) + e);
       }
   }
   lds_barrier();
