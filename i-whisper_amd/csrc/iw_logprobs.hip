@@ -267,6 +267,14 @@ struct Item {
   }
 };
 
+// In the place of pieces and words that there are none of; a choice between it and an argument is
+// known to be device memory only as a number
+__device__ __attribute__((aligned(16))) const uint32_t kNothing[4] = {};
+template <typename V>
+__device__ __forceinline__ const V __attribute__((address_space(1))) *in_global(const void *p) {
+  return reinterpret_cast<const V __attribute__((address_space(1))) *>(reinterpret_cast<uintptr_t>(p));
+}
+
 // P: 16-byte pieces of a thread
 template <typename T, int NT, int P>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ? 8 : 4))) void token_scores_kernel(
@@ -275,22 +283,34 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   constexpr int E = L::E, NW = NT / 64;
   __shared__ Shared<NT> s;
-  __shared__ uint32_t sWords[I8 ? 1 : NT * P * E / 32 + 2];  // the part's bits of the suppressed tokens
+  constexpr int S = I8 ? 0 : (P * E + 31) / 32;  // a thread's words of the part's suppressed tokens; span is a multiple of 32
+  __shared__ uint32_t sWords[S * NT + 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t item = blockIdx.x;
   const Item<T> it(a, chunks, span, item);
-  if (!I8 && a.suppress)  // span is a multiple of 32
-    for (int i = tid; i < (it.n + 31) / 32; i += NT) sWords[i] = a.suppress[it.c0 / 32 + i];
   uint4 w[P];
-  T xr{};
+  // no branch between the loads, so that the first pieces are used while the others are on the way
+  uint32_t sw[S + 1];
   {
-    const uint4 *xa = reinterpret_cast<const uint4 *>(it.x + it.head);
+    const auto *from = in_global<uint32_t>(a.suppress ? a.suppress + it.c0 / 32 : &kNothing[0]);
+    const int last = a.suppress ? (it.n - 1) / 32 : 0;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (p * NT + tid < it.pieces) w[p] = xa[p * NT + tid];
-    const int i = tid < it.head ? tid : it.head + it.pieces * E + tid - it.head;
-    if (i < it.n) xr = it.x[i];
+    for (int i = 0; i < S; ++i) sw[i] = from[min(i * NT + tid, last)];
   }
+  const int extra = tid < it.head ? tid : it.head + it.pieces * E + tid - it.head;
+  const bool has_extra = extra < it.n;
+  const T xr = it.x[min(extra, it.n - 1)];
+  {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    const auto *xa = in_global<v4u>(it.pieces > 0 ? static_cast<const void *>(it.x + it.head) : kNothing);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const v4u x = xa[min(p * NT + tid, max(it.pieces - 1, 0))];
+      w[p] = make_uint4(x.x, x.y, x.z, x.w);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S; ++i) sWords[i * NT + tid] = sw[i];
   if (tid == 0) s.cands = 0;
   if constexpr (I8)
     for (int i = tid; i < 256 * kCopies; i += NT) s.count[i] = 0;
@@ -306,8 +326,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
     const uint64_t two = (uint64_t)words[I8 ? min(i + 1, (n - 1) >> 5) : i + 1] << 32 | words[i];
     return (uint32_t)(two >> (at & 31)) & ((1u << E) - 1u);
   };
-  const int extra = tid < it.head ? tid : it.head + it.pieces * E + tid - it.head;  // this thread's single logit
-  bool has_extra = extra < n;
   float xe = has_extra ? L::one(&xr) : -INFINITY;
   if (!I8 && a.suppress && has_extra && ((sWords[extra >> 5] >> (extra & 31)) & 1u)) xe = -INFINITY;
 
@@ -588,9 +606,11 @@ __global__ __launch_bounds__(JT) void token_scores_join_kernel(ScoreArgs a, int 
 //   themselves, and more threads are a shorter chain.
 // Parts of 16 KB were slower for all (int8 50, float32 34.9, float16 32.7), and so were blocks that
 // stay and request their next part early (int8 48, float32 44): their registers cost more waves
-// than the reads gained. What is left above a read of the bytes (106 MB 19 us): int8 is bound by LDS adds
-// (8.6 cycles per 64 of them), the others by issuing ~9 instructions a logit at 2 GHz, and each
-// block's reading and computing do not overlap but with those of the blocks beside it.
+// than the reads gained. With pieces used as they arrive and alternatives found by words, 2048
+// rows of int8 take 34.0 us, 41.7 with four alternatives, targets and suppressed tokens (42.9 where a
+// block waited for all of its pieces), 512 of float32 32.6, 2048 of float32 77 (5.5 TB/s). What is
+// left above a read of the bytes (106 MB 19 us): int8 is bound by LDS adds (8.6 cycles per 64
+// of them), the others by issuing ~9 instructions a logit at 2 GHz.
 struct Split {
   int chunks, span;
   bool few;
