@@ -610,6 +610,42 @@ def test_token_logprobs_certain_rows(iw, gpu):
     assert np.allclose(host(got.entropy), np.log1p(z) + u / (1 + z), rtol=600 * 2.0 ** -24, atol=0)
 
 
+@pytest.mark.parametrize("dtype", ["int8", "bfloat16"])
+def test_token_logprobs_far_rows(iw, gpu, dtype):
+    """Rows and columns beyond 2^31 elements are those of a copy near the start."""
+    print("case: far rows", dtype, flush=True)
+    rows, V = 33000, 70001
+    x = torch.empty((rows, V), dtype=DTYPES[dtype], device="cuda")
+    near = T(gen.i8(gen.rng(4), (3, V))).to(x.dtype)
+    x[:3] = near
+    x[-3:] = near
+    t = T(np.array([0, V - 1, 9], np.int64))
+    want = iw.speculative.token_logprobs(near, t, top=5, scale=0.1)
+    targets = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    targets[:3], targets[-3:] = t, t
+    got = iw.speculative.token_logprobs(x, targets, top=5, scale=0.1)
+    for a, b in zip(got, want):
+        for part in (a[:3], a[-3:]):
+            if b.dtype == torch.int64:
+                assert torch.equal(part, b)
+            else:  # few and many blocks share the sums out differently: a few roundings of numbers up to 30
+                assert (part - b).abs().max() < 30 * 64 * 2.0 ** -24
+
+
+def test_empty_batches(iw, gpu):
+    sp = iw.speculative
+    e = lambda *shape, dtype=torch.int8: torch.empty(shape, dtype=dtype, device="cuda")
+    plan = sp.tree_plan(e(0, 8, dtype=torch.int32))
+    assert plan.visible.shape == plan.positions.shape == (0, 8)
+    q, k, v, ln = e(0, 8, 128), e(0, 2, 32, 64), e(0, 2, 8, 64, 4), e(0, dtype=torch.int32)
+    y = sp.tree_attention(q, q, q, k, v, ln, plan.visible, heads=2, qk_multiplier=90, qk_shift=9, frac_bits=8,
+                          av_multiplier=100, av_shift=6)
+    assert y.shape == (0, 8, 128)
+    for lead in ((0,), (0, 3), (3, 0)):
+        s = sp.token_logprobs(e(*lead, 100, dtype=torch.float32), e(*lead, dtype=torch.int64), top=2)
+        assert s.logprob.shape == s.entropy.shape == lead and s.top_ids.shape == s.top_logprobs.shape == (*lead, 2)
+
+
 def test_token_logprobs_refuses(iw, gpu):
     f = iw.speculative.token_logprobs
     x = torch.zeros((2, 40), device="cuda")
