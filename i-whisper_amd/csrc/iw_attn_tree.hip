@@ -7,7 +7,9 @@
 // order, so the keys can be split over waves.
 //
 // One block per (batch, head) and 16 or 32 nodes (one or two 16-query MFMA tiles). The
-// block's waves take 64-key chunks in turn, the tree itself is one more chunk.
+// block's waves take 64-key chunks in turn, the tree itself is one more chunk; their sums
+// meet in LDS as whole words, a copy each (added there one by one, 64 nodes of 2560
+// heads took 67 us in the place of 53).
 // In a chunk's four 16x16x64 score products, row 4g + r of product t is key
 // 16g + 4t + r: lane group g then holds the scores of the 16 consecutive keys
 // that its bytes of the P.V operand stand for, and no lane exchange is needed.
@@ -126,9 +128,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   static_assert(MODE == ALL || NC == 0, "parts loop over their chunks");
   __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
   __shared__ int32_t sMax[NW][QR];
-  __shared__ uint32_t sSum[QR];
+  __shared__ uint32_t sSum[NW][QR];
   __shared__ int32_t sInv[QR];
-  __shared__ __attribute__((aligned(16))) uint32_t sO[QR * OLD];
+  __shared__ __attribute__((aligned(16))) uint32_t sO[NW][QR * OLD];
 
   // the blocks of a (batch, head) are neighbours on one XCD (blockIdx % 8) and share its L2
   const int block = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
@@ -264,13 +266,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
   }
   const bool table = table_off >= 0;
   const int zero = table ? shift_exp_zero(a.frac_bits) : IW_SEXP_LUT - 1;
-  if (MODE != PART_MAX) {
-    if (table)
-      for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
-        *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
-    for (int i = tid; i < QR; i += 64 * NW) sSum[i] = 0u;
-    for (int i = tid; i < QR * OLD; i += 64 * NW) sO[i] = 0u;
-  }
+  if (MODE != PART_MAX && table)
+    for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
+      *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
 
   auto scores = [&](const v4i (&f)[KS], int u) {
     v4i s{0, 0, 0, 0};
@@ -456,34 +454,48 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(tree_wa
     if (has_tree && (nkc - c_lo) % NW == wave) chunk(nkc, true);
   }
 
-  // ---- the waves' sums meet in LDS ----
+  // ---- the waves' sums meet in LDS: a lane's four products are four columns of a row ----
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
     psum[u] += (uint32_t)__shfl_xor((int)psum[u], 16);
     psum[u] += (uint32_t)__shfl_xor((int)psum[u], 32);
-    if (lane < 16) atomicAdd(&sSum[16 * u + lane], psum[u]);
+    if (lane < 16) sSum[wave][16 * u + lane] = psum[u];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          atomicAdd(&sO[(16 * u + 4 * g + r) * OLD + 64 * ks + 4 * n + i], (uint32_t)o[u][ks][i][r]);
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<v4i *>(&sO[wave][(16 * u + 4 * g + r) * OLD + 64 * ks + 4 * n]) =
+            v4i{o[u][ks][0][r], o[u][ks][1][r], o[u][ks][2][r], o[u][ks][3][r]};
   }
   lds_barrier();
+  auto sum_of = [&](int at) {
+    v4i v = *reinterpret_cast<const v4i *>(&sO[0][at]);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const v4i *>(&sO[w][at]);
+    return v;
+  };
+  uint32_t sum = 0;
+  if (tid < QR) {
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += sSum[w][tid];
+  }
   if constexpr (MODE == PART_SUM) {
     uint32_t *mine = part_of<KS, QT>(t, block, part, parts);
     for (int i = 4 * tid; i < QR * 64 * KS; i += 4 * 64 * NW)
-      *reinterpret_cast<v4i *>(mine + i) = *reinterpret_cast<const v4i *>(&sO[i / (64 * KS) * OLD + i % (64 * KS)]);
-    if (tid < QR) mine[QR * 64 * KS + tid] = sSum[tid];
+      *reinterpret_cast<v4i *>(mine + i) = sum_of(i / (64 * KS) * OLD + i % (64 * KS));
+    if (tid < QR) mine[QR * 64 * KS + tid] = sum;
     return;
   }
-  if (tid < QR) sInv[tid] = fisr((int32_t)sSum[tid], a.rsqrt_off);
+  if (tid < QR) sInv[tid] = fisr((int32_t)sum, a.rsqrt_off);
   lds_barrier();
   for (int i = tid; i < rows * words; i += 64 * NW) {
     const int q = by_words(i), d = 4 * (i - q * words);
     uint32_t w = 0;
-    if (q0 + q < cnt) w = output_word(a, &sO[q * OLD + d], sInv[q]);
+    if (q0 + q < cnt) {
+      const v4i v = sum_of(q * OLD + d);
+      const uint32_t sums[4] = {(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
+      w = output_word(a, sums, sInv[q]);
+    }
     *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + q) * a.o_st + d) = w;
   }
 }
@@ -569,6 +581,7 @@ int tree_parts(int64_t heads, int64_t nodes, int64_t head_dim, int64_t cap) {
   const int64_t blocks = heads * (nodes <= 16 ? 1 : (nodes + 31) / 32), chunks = (cap + 63) / 64 + 1;
   return (int)std::max<int64_t>(1, std::min(kCus / blocks, (chunks + 7) / 8));
 }
+
 // Caches of up to 448 positions are eight chunks with the tree's: a wave each while a block has
 // a CU to itself (26 nodes of 20 heads, us with eight waves of one chunk, four of two and eight in a loop over
 // both passes: 4.9 / 5.5 / 5.2), else four waves of two, which leave more blocks to a CU (16
@@ -584,18 +597,19 @@ int launch_tree_q(const TreeArgs &t, hipStream_t s) {
   return launch_tree<KS, QUADS, QT, 4, 2>(t, s);
 }
 
-// 16 nodes a block, or 32 over one set of K and V fragments. us of either: 32 nodes of 20, 320
-// and 1280 heads 4.9 / 6.8, 9.7 / 11.4 and 23.7 / 25.9, 64 nodes of 640 heads 20.8 / 21.2: fewer
-// registers are more waves, and neighbouring blocks find K and V in L2. 64 nodes of 1536
-// heads (V transposed) 45.6 / 40.4, of 96 wide ones 102 / 72, of 768 heads over 2300 keys 112 / 100.
-constexpr int64_t kPairTiles = 10 * kCus;
+// 16 nodes a block, or 32 over one set of K and V fragments, where the blocks of either are many (wide heads
+// count twice). us of either: 32 nodes of 20, 320 and 640 heads 5.0 / 7.0, 9.5 / 11.4 and 13.4 / 14.3, of 1040
+// 19.7 / 20.0, 1280 23.6 / 22.8, 2560 37.8 / 35.0; 64 nodes of 320 heads 13.0 / 13.3, 480 17.0 / 15.6, 640 20.5 / 19.0, 2560
+// 64.3 / 52.9, of 240 96 wide ones 19.3 / 15.2, of 320 128 wide ones over 2300 keys 131 / 86; 48 nodes, whose last
+// block has 16, of 1280 heads 29.3 / 31.0.
+constexpr int64_t kPairTiles = 7 * kCus;
 template <int KS, bool QUADS>
 int launch_tree_k(const TreeArgs &t, hipStream_t s) {
   const int parts = tree_parts((int64_t)t.a.B * t.a.H, t.a.Tq, t.a.D, t.a.Tk);
   if (parts > 1)
     return t.a.Tq <= 16 ? launch_tree_parts<KS, QUADS, 1>(t, parts, s) : launch_tree_parts<KS, QUADS, 2>(t, parts, s);
   const int64_t tiles = (int64_t)t.a.B * t.a.H * ((t.a.Tq + 15) / 16);
-  if (t.a.Tq > 32 && tiles > kPairTiles) return launch_tree_q<KS, QUADS, 2>(t, s);
+  if (t.a.Tq > 16 && KS * tiles > kPairTiles) return launch_tree_q<KS, QUADS, 2>(t, s);
   return launch_tree_q<KS, QUADS, 1>(t, s);
 }
 
