@@ -429,12 +429,13 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
     m = key_value((uint64_t)wave_max_u32_dpp(go) << 32);
     const float ms = m == -INFINITY ? 0.f : m;  // a part without finite logits sums to 0
     auto add = [&](float v, bool all) {
-      const float d = v - ms, finite = fmaxf(d, -3e38f);
+      // beyond log2_far exp2 is 0, and near stays where its product with any log2_lo is small
+      const float d = v - ms, near = fmaxf(d, a.log2_far);
       // log2(e) * scale in two parts, as the rounding of one would be the same for every logit
-      const float e = __builtin_amdgcn_exp2f(fmaf(d, a.log2_hi, finite * a.log2_lo));
+      const float e = __builtin_amdgcn_exp2f(fmaf(d, a.log2_hi, near * a.log2_lo));
       if (all || d != 0.f) {
         z += e;
-        u -= finite * e;  // -inf times its exp of 0 is 0
+        u -= near * e;  // -inf times its exp of 0 is 0
       } else {
         eq += 1.f;
       }
@@ -642,6 +643,7 @@ int launch_scores(ScoreArgs a, hipStream_t s) {
   const double c = (double)a.scale * 1.4426950408889634;
   a.log2_hi = (float)std::min(c, 3.4e38);
   a.log2_lo = (float)(c - (double)a.log2_hi);
+  a.log2_far = (float)(-200.0 / (double)a.log2_hi);
   if (sp.few) return launch_scores_p<T, 1024, 4>(a, sp, s);
   return launch_scores_p<T, sizeof(T) == 1 ? 256 : 512, sizeof(T) == 1 ? 16 : 8>(a, sp, s);
 }

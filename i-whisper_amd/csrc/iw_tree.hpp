@@ -56,6 +56,7 @@ struct ScoreArgs {
   int64_t rows = 0, ld = 0;
   int cols = 0;
   float scale = 1.f, log2_hi = 0.f, log2_lo = 0.f;  // log2(e) * scale in two parts, set at launch
+  float log2_far = 0.f;                             // times log2_hi: -200
   const uint32_t *suppress = nullptr;
   const int64_t *targets = nullptr;
   float *logprob = nullptr, *entropy = nullptr;

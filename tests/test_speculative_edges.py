@@ -1,0 +1,65 @@
+"""Token scores at the ends of their ranges, against float64: scales and logits whose products or
+distances leave float32."""
+import numpy as np
+import pytest
+import torch
+
+from tests import gen
+from tests.test_speculative import T, bit_words, host, logits_of
+
+FLOATS = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+FLT_MAX = float(np.finfo(np.float32).max)
+
+
+def check(got, logits, targets, top, scale, suppress=()):
+    """Against float64, with the tolerances of test_speculative.check_scores: 600 * 2^-24 for what an
+    exp enters, three roundings of a log-probability itself. One that float32 does not reach is -inf."""
+    x = logits.double().numpy().copy()
+    x[:, list(suppress)] = -np.inf
+    scale = float(np.float32(scale))
+    with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+        d = (x - x.max(1, keepdims=True)) * scale
+        e = np.exp(d)
+        lp = d - np.log(e.sum(1, keepdims=True))
+        entropy = -np.where(e > 0, np.exp(lp) * lp, 0).sum(1)
+    lp[lp < -FLT_MAX] = -np.inf
+    r = 600 * 2.0 ** -24
+
+    def close(a, b, room):
+        a, fin = host(a).astype(np.float64), np.isfinite(b)
+        assert np.array_equal(np.isneginf(a), np.isneginf(b)) and not np.isnan(a).any(), (a, b)
+        assert (np.abs(a[fin] - b[fin]) <= room[fin]).all(), (a[fin], b[fin])
+
+    def room(b):
+        return r + np.where(np.isfinite(b), np.abs(b), 0) * 3 * 2.0 ** -24
+    close(got.entropy, entropy, r * (1 + np.abs(entropy)))
+    want = lp[np.arange(len(lp)), targets]
+    close(got.logprob, want, room(want))
+    ids = np.argsort(-x, axis=1, kind="stable")[:, :top]
+    assert np.array_equal(host(got.top_ids), ids)
+    want = np.take_along_axis(lp, ids, 1)
+    close(got.top_logprobs, want, room(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 5000, 70001])
+@pytest.mark.parametrize("dtype", list(FLOATS))
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -60, 1e-7, 2.4e7, 6e7, 1e8, 1.1e9, 1e10, 1e12, 1e20, 1e30, 2e38,
+                                   3.3e38])
+def test_masked_rows_under_any_scale(iw, gpu, scale, dtype, V):
+    """-inf, suppressed tokens and the type's lowest value have no probability under small and large
+    scales, beside logits that differ by about 1 / scale and by far more."""
+    print("case: masked rows", scale, dtype, V, flush=True)
+    r = gen.rng(V)
+    x = logits_of(r, 5, V, "float32", 1.0)
+    x[0] = torch.from_numpy(r.uniform(0, min(5 / scale, 3e38), V))
+    x[1] = torch.from_numpy(r.uniform(-1, 0, V) * min(30 / scale, 3e38))
+    x = x.clamp(torch.finfo(FLOATS[dtype]).min, torch.finfo(FLOATS[dtype]).max).to(FLOATS[dtype])
+    x[:3, ::3] = -np.inf
+    x[3, 1::2] = torch.finfo(x.dtype).min
+    tg = np.array([1, 2, 0, 5, 7])
+    got = iw.speculative.token_logprobs(x.cuda(), T(tg), top=4, scale=scale)
+    check(got, x, tg, 4, scale)
+    off = r.integers(0, V, 20)
+    got = iw.speculative.token_logprobs(x.cuda(), T(tg), top=4, scale=scale, suppress=T(bit_words(off, V)))
+    check(got, x, tg, 4, scale, off)
