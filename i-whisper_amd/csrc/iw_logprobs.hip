@@ -232,6 +232,12 @@ __device__ __noinline__ void top_by_rounds(const T *x, int c0, int n, const uint
   __syncthreads();
 }
 
+// (v - m) * scale. Where v - m passes float32 the product need not: half of it and twice the scale.
+__device__ __forceinline__ float scaled_distance(float v, float m, float scale) {
+  const float d = v - m;
+  return d == -INFINITY && v != -INFINITY ? (0.5f * v - 0.5f * m) * (2.f * scale) : d * scale;
+}
+
 template <typename T>
 __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, float m, float l, float z, float u) {
   if (a.logprob) {
@@ -240,7 +246,7 @@ __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, float
     if (at >= 0 && at < a.cols) {
       const float v = suppressed(a.suppress, (int)at) ? -INFINITY
                                                       : Logit<T>::one(reinterpret_cast<const T *>(a.x) + row * a.ld + at);
-      lp = (v - m) * a.scale - l;
+      lp = scaled_distance(v, m, a.scale) - l;
     }
     a.logprob[row] = lp;
   }
@@ -518,7 +524,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 1024 ?
       tops[at] = k;
     } else {
       a.top_ids[row * a.top + at] = key_col(k);
-      a.top_lp[row * a.top + at] = (key_value(k) - m) * a.scale - l;
+      a.top_lp[row * a.top + at] = scaled_distance(key_value(k), m, a.scale) - l;
     }
   };
   if (rounds) {
@@ -573,7 +579,7 @@ __global__ __launch_bounds__(JT) void token_scores_join_kernel(ScoreArgs a, int 
   const float l = row_log(m, z);
   auto place = [&](int at, uint64_t k) {
     a.top_ids[row * a.top + at] = key_col(k);
-    a.top_lp[row * a.top + at] = (key_value(k) - m) * a.scale - l;
+    a.top_lp[row * a.top + at] = scaled_distance(key_value(k), m, a.scale) - l;
   };
   __syncthreads();
   if (keys <= kJoinKeys) {

@@ -63,3 +63,26 @@ def test_masked_rows_under_any_scale(iw, gpu, scale, dtype, V):
     off = r.integers(0, V, 20)
     got = iw.speculative.token_logprobs(x.cuda(), T(tg), top=4, scale=scale, suppress=T(bit_words(off, V)))
     check(got, x, tg, 4, scale, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -70, 1e-10, 0.5, 0.99, 1.0, 3.0])
+def test_logits_further_apart_than_float32(iw, gpu, scale, dtype):
+    """v - m passes float32 where (v - m) * scale need not."""
+    print("case: far apart", scale, dtype, flush=True)
+    r = gen.rng(5)
+    x = torch.from_numpy(r.uniform(-3.3e38, 3.3e38, (6, 900))).to(FLOATS[dtype])
+    x[:, 3], x[:, 4], x[4, 5] = 3.3e38, -3.3e38, -np.inf
+    x[5] = torch.finfo(x.dtype).min
+    x[5, 8] = torch.finfo(x.dtype).max
+    tg = np.array([4, 4, 3, 700, 5, 8])
+    check(iw.speculative.token_logprobs(x.cuda(), T(tg), top=32, scale=scale), x, tg, 32, scale)
+    two = x[:, 3:5].contiguous()
+    tg = np.array([0, 1, 1, 0, 1, 1])
+    check(iw.speculative.token_logprobs(two.cuda(), T(tg), top=2, scale=scale), two, tg, 2, scale)
+    long = torch.zeros((6, 70001), dtype=x.dtype)  # rows in parts
+    long[:, -900:] = x
+    long[:, 0] = -3.3e38
+    tg = np.array([0, 69101 + 4, 69101 + 3, 5, 0, 69101])
+    check(iw.speculative.token_logprobs(long.cuda(), T(tg), top=32, scale=scale), long, tg, 32, scale)
