@@ -40,10 +40,11 @@ struct Part {
 };
 
 // A logit and its column as one whole number: larger logits first, then lower
-// columns; both zeros are one value and a NaN is the largest.
+// columns; both zeros are one value and a NaN is the largest. Every key is above 0 and
+// below ~0, also a NaN's in column 0.
 __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);
-  if (v != v) return 0xffffffffu;
+  if (v != v) return 0xfffffffeu;
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t key_of(float v, int col) {

@@ -1,5 +1,5 @@
 """Token scores at the ends of their ranges, against float64: scales and logits whose products or
-distances leave float32."""
+distances leave float32, rows with NaN."""
 import numpy as np
 import pytest
 import torch
@@ -86,3 +86,32 @@ def test_logits_further_apart_than_float32(iw, gpu, scale, dtype):
     long[:, 0] = -3.3e38
     tg = np.array([0, 69101 + 4, 69101 + 3, 5, 0, 69101])
     check(iw.speculative.token_logprobs(long.cuda(), T(tg), top=32, scale=scale), long, tg, 32, scale)
+
+
+def nan_order(row, top):
+    """Columns in the order of alternatives: NaN first, then by value, ties to the lowest index."""
+    v = row.double().tolist()
+    return sorted(range(len(v)), key=lambda i: (0, 0.0, i) if v[i] != v[i] else (1, -v[i], i))[:top]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(FLOATS))
+@pytest.mark.parametrize("V,top", [(1, 1), (2, 2), (5, 5), (32, 32), (40, 7), (3000, 32), (51865, 3), (70001, 32)])
+def test_alternatives_of_rows_with_nan(iw, gpu, V, top, dtype):
+    """A NaN is the largest wherever it stands, the first column and whole rows included; as many
+    alternatives as there are tokens are all of them."""
+    print("case: nan order", V, top, dtype, flush=True)
+    r = gen.rng(V)
+    x = logits_of(r, 7, V, dtype, 1.0)
+    x[0, 0] = np.nan
+    x[1] = np.nan
+    x[2, ::2] = np.nan
+    x[3, V - 1] = -torch.tensor(np.nan)
+    x[4], x[4, 0] = np.inf, np.nan
+    x[5], x[5, 0] = -np.inf, np.nan
+    x[6] = -np.inf
+    tg = np.zeros(7, np.int64)
+    got = iw.speculative.token_logprobs(x.cuda(), T(tg), top=top)
+    assert host(got.top_ids).tolist() == [nan_order(row, top) for row in x]
+    assert bool(got.logprob.isnan().all()) and bool(got.entropy.isnan().all())
+    assert bool(got.top_logprobs.isnan().all())
