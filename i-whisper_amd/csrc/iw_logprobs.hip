@@ -646,7 +646,8 @@ int launch_scores_p(const ScoreArgs &a, const Split &sp, hipStream_t s) {
 template <typename T>
 int launch_scores(ScoreArgs a, hipStream_t s) {
   const Split sp = split(a.type, a.rows, a.cols);
-  if (sp.chunks > kMaxParts || a.rows * sp.chunks > (1LL << 32) / 1024 - 1) return fail("too many logits for one call");
+  // blocks of 512 threads at most where they are many, fewer than 2^32 threads
+  if (sp.chunks > kMaxParts || a.rows * sp.chunks > (1LL << 32) / 512 - 1) return fail("too many logits for one call");
   const double c = (double)a.scale * 1.4426950408889634;
   a.log2_hi = (float)std::min(c, 3.4e38);
   a.log2_lo = (float)(c - (double)a.log2_hi);

@@ -115,3 +115,22 @@ def test_alternatives_of_rows_with_nan(iw, gpu, V, top, dtype):
     assert host(got.top_ids).tolist() == [nan_order(row, top) for row in x]
     assert bool(got.logprob.isnan().all()) and bool(got.entropy.isnan().all())
     assert bool(got.top_logprobs.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int8", "float32"])
+def test_as_many_rows_as_a_call_takes(iw, gpu, dtype):
+    """2^22 rows: the scores of a row are those of the same row among few; one row more is refused."""
+    print("case: 2^22 rows", dtype, flush=True)
+    V, n = 3, 1 << 22
+    few = T(gen.i8(gen.rng(1), (64, V), -40, 40)).to(getattr(torch, dtype))
+    tg = torch.arange(64, device="cuda") % V
+    want = iw.speculative.token_logprobs(few, tg, top=2, scale=0.1)
+    got = iw.speculative.token_logprobs(few.repeat(n // 64, 1), tg.repeat(n // 64), top=2, scale=0.1)
+    r = 600 * 2.0 ** -24
+    assert torch.equal(got.top_ids, want.top_ids.repeat(n // 64, 1))
+    for a, b in ((got.logprob, want.logprob.repeat(n // 64)), (got.entropy, want.entropy.repeat(n // 64)),
+                 (got.top_logprobs, want.top_logprobs.repeat(n // 64, 1))):
+        assert bool(((a - b).abs() <= r * (1 + b.abs())).all())
+    with pytest.raises(RuntimeError, match="2\\^22 rows"):
+        iw.speculative.token_logprobs(few[:1].repeat(n + 1, 1))
