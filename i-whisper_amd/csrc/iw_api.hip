@@ -3,6 +3,7 @@
 #include "iw_common.hpp"
 #include "iw_gemm.hpp"
 #include "iw_kernels.hpp"
+#include "iw_overlap.hpp"
 #include "iw_tree.hpp"
 
 #include <cmath>
@@ -895,12 +896,6 @@ int iw_argmax_rows(const int8_t *x, int64_t rows, int64_t cols, int64_t ld, int6
 
 namespace {
 
-// [first, first + bytes) of two buffers share no byte
-bool apart(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x + (uintptr_t)a_bytes <= y || y + (uintptr_t)b_bytes <= x;
-}
-
 int check_tree_cache(int64_t heads, int64_t head_dim, int64_t cache_positions, int64_t v_sd, int64_t v_sq) {
   IW_REQUIRE(heads > 0 && heads <= 4096 && head_dim > 0 && head_dim <= 128 && head_dim % 16 == 0,
              "tree attention supports head_dim % 16 == 0, head_dim <= 128");
@@ -958,6 +953,26 @@ int iw_attention_tree(const iw_attention_tree_args *args, iw_stream_t stream) {
   IW_REQUIRE(attn_tree_workspace(p.batch * p.heads, p.nodes, p.head_dim, p.cache_positions) == 0 ||
                  (p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 15) == 0),
              "iw_attention_tree_workspace bytes of 16-byte aligned workspace are needed");
+  // a block writes its rows while others still read theirs
+  const NodeRows out{p.out, p.o_sb, p.o_st, p.batch, p.nodes, p.heads * p.head_dim};
+  const auto beside = [&](const int8_t *x, int64_t sb, int64_t st) {
+    return apart(out, NodeRows{x, sb, st, out.batch, out.nodes, out.bytes});
+  };
+  const NodeRows q{p.q, p.q_sb, p.q_st, p.batch, p.nodes, out.bytes};
+  IW_REQUIRE(rows_apart(out), "the rows of out must not overlap");
+  IW_REQUIRE(out.same(q) || apart(out, q), "out must be q itself or must not overlap q");
+  IW_REQUIRE(beside(p.k_new, p.kn_sb, p.kn_st) && beside(p.v_new, p.vn_sb, p.vn_st), "out must not overlap k_new or v_new");
+  // a batch row's part of a cache: rows of its heads
+  const auto cached = [&](const int8_t *x, int64_t row, int64_t sh, int64_t sb) {
+    const Runs heads(x, row, sh, p.heads);
+    return Runs(heads.at, heads.reach(), sb, p.batch);
+  };
+  const int64_t quads = (p.cache_positions + 3) / 4, wide = (p.cache_positions + 15) / 16 * 16;
+  const int64_t k_row = p.k_st * (p.cache_positions - 1) + p.head_dim;
+  const int64_t v_row = p.v_sq != 4 ? p.v_sq * (quads - 1) + 4 * p.head_dim : p.v_sd * (p.head_dim - 1) + wide;
+  IW_REQUIRE(apart(out.of_batch(), cached(p.k, k_row, p.k_sh, p.k_sb)) &&
+                 apart(out.of_batch(), cached(p.vt, v_row, p.v_sh, p.v_sb)),
+             "out must not overlap the caches");
   TreeArgs t;
   AttnArgs &a = t.a;
   a.q = p.q;
@@ -1021,7 +1036,7 @@ int iw_tree_accept(const iw_tree_caches *caches, const int64_t *tokens, const in
   if (c.batch == 0) return IW_OK;
   IW_REQUIRE(tokens && parents && choice && lengths && path && accepted && next && lengths_out, "null tensor pointer");
   // the blocks of a row's layers read its length while one of them writes the new one
-  IW_REQUIRE(apart(lengths, 4 * c.batch, lengths_out, 4 * c.batch), "lengths_out must not be part of lengths");
+  IW_REQUIRE(apart(Runs(lengths, 4, 4, c.batch), Runs(lengths_out, 4, 4, c.batch)), "lengths_out must not be part of lengths");
   IW_REQUIRE(c.layers == 0 || (c.k_new && c.v_new && c.k && c.v), "null array of layer pointers");
   uintptr_t align = (uintptr_t)(c.kn_sb | c.kn_st | c.vn_sb | c.vn_st | c.k_sb | c.k_sh | c.k_st);
   for (int64_t i = 0; i < c.layers; ++i) {

@@ -182,8 +182,9 @@ def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_c
     ``k_cache`` int8 [B, heads, T, D]; ``v_cache`` in key quads [B, heads, ceil(T / 4), D, 4] or transposed
     [B, heads, D, round_up(T, 16)]. D is a multiple of 16 up to 128, strides are multiples of 16.
     Lengths and counts are clamped to T and N on the device. Returns int8 [B, N, heads * D] (``out`` where
-    given, which shares no memory with K, V or the caches); nodes past ``counts[b]`` and nodes that see no key give zeros. With one node a row it is a
-    decode step over rows of different lengths."""
+    given: ``q`` itself, or memory that K, V, the caches and ``q`` have no part in, other columns of the
+    same rows included); nodes past ``counts[b]`` and nodes that see no key give zeros. With one node
+    a row it is a decode step over rows of different lengths."""
     shape = _node_shape(q, heads, "q")
     dev = q.get_device()
     B, N, C = shape
@@ -205,10 +206,6 @@ def tree_attention(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_c
         o_s = (N * C, C)
     else:
         o_s = _rows_strides(out, shape, "out", dev)
-        sb, st = o_s
-        if (B > 1 and sb < C) or (N > 1 and st < C) or (
-                B > 1 and N > 1 and sb < (N - 1) * st + C and st < (B - 1) * sb + C):
-            raise RuntimeError("the rows of out must not overlap")
     # shorter caches need none
     need = _lib.value("iw_attention_tree_workspace", B, heads, N, D, T) if T >= 1536 else 0
     work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None

@@ -628,8 +628,10 @@ int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *coun
  * the count, and of nodes that see no key, are zeros. nodes <= 64,
  * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24; operands and
  * strides are multiples of 16 bytes; kn_st, vn_st, k_st, v_sd, v_sq < 2^25. The
- * caches are read only: the nodes' K and V enter them with iw_tree_accept. out shares
- * no memory with k_new, v_new or the caches. workspace: iw_attention_tree_workspace
+ * caches are read only: the nodes' K and V enter them with iw_tree_accept. out is q itself
+ * or shares no memory with q, and none with k_new, v_new or the caches; it may lie in other columns
+ * of their rows where the strides are the same, and is refused where it interleaves with
+ * them at other strides. workspace: iw_attention_tree_workspace
  * bytes, 16-byte aligned, used during the call's work only (NULL where that is 0: at
  * least for all caches of fewer than 1536 positions). The struct is read during the call. */
 typedef struct iw_attention_tree_args {
