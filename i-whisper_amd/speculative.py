@@ -225,12 +225,60 @@ class TreeAccept(NamedTuple):
     lengths: Tensor     # int32 [B]: the rows' lengths with the path cached
 
 
+def _runs(t: Tensor):
+    """The addresses of an int8 tensor's runs of bytes, and their length."""
+    dims = sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1)
+    length = 1
+    while dims and dims[0][0] == length:
+        length *= dims.pop(0)[1]
+    at = torch.tensor([t.data_ptr()], dtype=torch.int64)
+    for s, n in reversed(dims):
+        at = (at[:, None] + s * torch.arange(n)).flatten()
+    return at, length
+
+
+def _own_memory(written: Sequence[Tensor], read: Sequence[Tensor]) -> bool:
+    """Whether the int8 tensors ``written`` share no byte with one another, with themselves or with
+    ``read``. Exact: caches may be parts of one buffer in any order of its dims."""
+    spans = sorted(((t.data_ptr(), t.data_ptr() + 1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)), i)
+                    for i, t in enumerate([*written, *read]) if t.numel()), key=lambda x: x[:2])
+    group, end = [], 0
+    for lo, hi, i in [*spans, (1 << 62, 1 << 62, -1)]:
+        if lo >= end:  # none of the tensors before reaches here
+            if not _group_apart([written[j] for j in group if j < len(written)],
+                                [read[j - len(written)] for j in group if j >= len(written)]):
+                return False
+            group = []
+        group.append(i)
+        end = max(end, hi)
+    return True
+
+
+def _group_apart(written: Sequence[Tensor], read: Sequence[Tensor]) -> bool:
+    if not written:
+        return True
+    runs = [_runs(t) for t in written]
+    at = torch.cat([a for a, _ in runs])
+    to = torch.cat([a + n for a, n in runs])
+    at, order = at.sort()
+    to = to[order]
+    if bool((to[:-1] > at[1:]).any()):
+        return False
+    # the last run that starts before a read one ends must end before that one starts
+    for a, n in map(_runs, read):
+        before = torch.searchsorted(at, a + n) - 1
+        if bool(((before >= 0) & (to[before.clamp(min=0)] > a)).any()):
+            return False
+    return True
+
+
 class TreeCaches:
     """The layers' caches and the nodes' K and V that a decoder pass leaves for them.
 
     Lists of one tensor per layer, all with the same shapes and strides:
     ``k_new`` / ``v_new`` int8 [B, N, heads * D] (columns of the projection
-    that the pass writes) and the caches as ``tree_attention`` takes them."""
+    that the pass writes) and the caches as ``tree_attention`` takes them, which
+    share no memory with one another or with the nodes' K and V."""
 
     def __init__(self, k_new: Sequence[Tensor], v_new: Sequence[Tensor], k_cache: Sequence[Tensor],
                  v_cache: Sequence[Tensor], *, heads: int):
@@ -251,9 +299,7 @@ class TreeCaches:
                     and _cache_strides(k_l, v_l, B, heads, D, dev) == (self.positions, k_s, v_s))
             if not same:
                 raise RuntimeError("the layers' tensors must have the same strides")
-        caches = self.tensors[2] + self.tensors[3]
-        if len({t.data_ptr() for t in caches}) != len(caches) or any(
-                0 in [s for s, n in zip(t.stride(), t.shape) if n > 1] for t in caches):
+        if not _own_memory(self.tensors[2] + self.tensors[3], self.tensors[0] + self.tensors[1]):
             raise RuntimeError("the caches are written: each must be memory of its own")
         self._arrays = [(ctypes.c_void_p * L)(*[t.data_ptr() for t in x]) for x in self.tensors]
         kn_a, vn_a, k_a, v_a = map(ctypes.addressof, self._arrays)

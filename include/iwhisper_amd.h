@@ -670,7 +670,8 @@ int64_t iw_attention_tree_workspace(int64_t batch, int64_t heads, int64_t nodes,
  * as iw_attention_tree, operands and strides multiples of 4 bytes). */
 
 /* The layers' caches: host arrays of `layers` device pointers with one set of
- * strides. layers may be 0. Read during the call. */
+ * strides. layers may be 0. The caches share no memory with one another, nor with
+ * k_new and v_new. Read during the call. */
 typedef struct iw_tree_caches {
   int64_t layers, batch, nodes, heads, head_dim, cache_positions;
   const int8_t *const *k_new;

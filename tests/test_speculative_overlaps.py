@@ -161,3 +161,95 @@ def test_out_in_the_place_of_q_and_between_columns(iw, oracle, gpu, N, cap):
         with pytest.raises(RuntimeError, match="caches"):
             iw.speculative.tree_attention(y[..., :C], y[..., C:2 * C], y[..., 2 * C:3 * C], k, v, ln, vis, cnt,
                                           out=cache.flatten()[-3 * N * C:].view(3, N, C), **sc)
+
+
+def buf(*shape):
+    return torch.zeros(shape, dtype=torch.int8)
+
+
+def test_written_tensors_have_memory_of_their_own(iw):
+    """Parts of one buffer in any order of its dims are told apart from those that share a byte."""
+    own = iw.speculative._own_memory
+    x = buf(3, 4, 2, 5, 8)  # [batch, layers, K or V, positions, D]
+    parts = [x[:, l, i] for l in range(4) for i in range(2)]
+    assert own(parts, []) and own(parts[:4], parts[4:]) and own([], parts + parts) and own([], [])
+    assert own(parts[:3], [parts[3], parts[3]])
+    assert not own(parts + parts[:1], []) and not own(parts, parts[:1])
+    assert not own([x[:, 0], x[:, 0, 1]], []) and not own([x[:, 0, 0]], [x[2, 0, 0, 4, 7:]])
+    assert own([x[:, 0, 0]], [x[2, 0, 1, 0, :1]])
+    assert own([x[..., :4], x[..., 4:]], []) and not own([x[..., :5], x[..., 4:]], [])
+    assert own([x.transpose(0, 3)], []) and own([x[:, :, :, ::2], x[:, :, :, 1::2]], [])
+    assert not own([x[:1].expand(3, 4, 2, 5, 8)], [])
+    flat = buf(1000)
+    assert not own([flat.as_strided((4, 10), (9, 1))], []) and own([flat.as_strided((4, 10), (10, 1))], [])
+    assert not own([flat[:500], flat[499:]], []) and own([flat[:500], flat[500:]], [])
+    assert not own([flat[:500]], [flat[499:]]) and own([flat[:500]], [flat[500:]])
+    assert own([buf(0, 4), buf(0, 4), flat[:0]], [buf(0)])
+    assert own([flat[10:20], flat[30:40]], [flat[20:30], flat[:10], flat[40:]])
+    assert not own([flat[10:20], flat[30:40]], [flat[25:31]]) and not own([flat[10:20], flat[30:40]], [flat[19:22]])
+
+
+def test_written_tensors_against_sets_of_bytes(iw):
+    own = iw.speculative._own_memory
+    r = random.Random(3)
+    flat = buf(4000)
+    seen = [0, 0]
+    for _ in range(1500):
+        def view():
+            if r.random() < 0.5:  # a part of a padded block
+                s = (96, 24, 4)
+                shape = (r.randint(1, 3), r.randint(1, 4), r.randint(1, 4))
+            else:
+                s = tuple(r.choice((1, 2, 4, 12, 24, 96)) for _ in range(3))
+                shape = tuple(r.randint(0 if r.random() < 0.05 else 1, 4) for _ in range(3))
+            return flat.as_strided(shape, s, r.randint(0, 200))
+        written, read = [view() for _ in range(r.randint(0, 3))], [view() for _ in range(r.randint(0, 2))]
+
+        def bytes_of(t):
+            return touched(t.data_ptr(), 1, *zip(t.stride(), t.shape))
+        w = [b for t in written for b in bytes_of(t)]
+        want = len(set(w)) == len(w) and not set(w) & {b for t in read for b in bytes_of(t)}
+        assert own(written, read) == want, [(t.stride(), t.shape, t.storage_offset()) for t in written + read]
+        seen[want] += bool(w)
+    assert min(seen) > 200
+
+
+@pytest.mark.gpu
+def test_tree_caches_memory(iw, gpu):
+    """Caches that are parts of one buffer accept as separate ones do; ones that share memory are refused."""
+    sp = iw.speculative
+    L, B, H, T_, D, N = 3, 2, 2, 32, 64, 4
+    C = H * D
+    qkv = [torch.randint(-127, 128, (B, N, 3 * C), dtype=torch.int8, device="cuda") for _ in range(L)]
+    kn, vn = [x[..., C:2 * C] for x in qkv], [x[..., 2 * C:] for x in qkv]
+    one = torch.zeros((B, L, 2, H, T_ * D), dtype=torch.int8, device="cuda")
+    k = [one[:, l, 0].unflatten(2, (T_, D)) for l in range(L)]
+    v = [one[:, l, 1].unflatten(2, (T_ // 4, D, 4)) for l in range(L)]
+    k2, v2 = [x.contiguous() for x in k], [x.contiguous() for x in v]
+    tok = torch.zeros((B, N), dtype=torch.int64, device="cuda")
+    par = torch.arange(-1, N - 1, dtype=torch.int32, device="cuda").repeat(B, 1)
+    ln = torch.tensor([5, 31], dtype=torch.int32, device="cuda")
+    a = sp.TreeCaches(kn, vn, k, v, heads=H).accept(tok, par, tok, ln)
+    b = sp.TreeCaches(kn, vn, k2, v2, heads=H).accept(tok, par, tok, ln)
+    assert host(a.accepted).tolist() == host(b.accepted).tolist() == [4, 1]
+    assert all(torch.equal(x, y) for x, y in zip(k + v, k2 + v2)) and any(bool(x.any()) for x in k)
+    near = torch.zeros(2 * B * H * T_ * D, dtype=torch.int8, device="cuda")
+    k0 = near[:B * H * T_ * D].view(B, H, T_, D)
+    for bad in ((kn, vn, k, k), (kn, vn, [k2[0], k2[0], k2[1]], v2)):
+        with pytest.raises(RuntimeError, match="memory of its own|v_cache"):
+            sp.TreeCaches(*bad, heads=H)
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        sp.TreeCaches(kn[:1], vn[:1], [k0], [near[64:64 + k0.numel()].view(B, H, T_ // 4, D, 4)], heads=H)
+    with pytest.raises(RuntimeError, match="memory of its own"):
+        sp.TreeCaches([near[:3 * B * N * C].view(B, N, 3 * C)[..., :C]], vn[:1], [k0], v2[:1], heads=H)
+
+
+@pytest.mark.gpu
+def test_tree_caches_without_rows(iw, gpu):
+    sp = iw.speculative
+    e = lambda *shape, dtype=torch.int8: torch.empty(shape, dtype=dtype, device="cuda")
+    caches = sp.TreeCaches([e(0, 4, 128)] * 2, [e(0, 4, 128)] * 2, [e(0, 2, 32, 64) for _ in range(2)],
+                           [e(0, 2, 8, 64, 4) for _ in range(2)], heads=2)
+    got = caches.accept(e(0, 4, dtype=torch.int64), e(0, 4, dtype=torch.int32), e(0, 4, dtype=torch.int64),
+                        e(0, dtype=torch.int32))
+    assert got.path.shape == (0, 4) and got.accepted.shape == got.next_token.shape == got.lengths.shape == (0,)
