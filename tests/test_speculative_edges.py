@@ -1,11 +1,11 @@
 """Token scores at the ends of their ranges, against float64: scales and logits whose products or
-distances leave float32, rows with NaN."""
+distances leave float32, rows with NaN. Captured rounds and filled workspaces, compared to the byte."""
 import numpy as np
 import pytest
 import torch
 
 from tests import gen
-from tests.test_speculative import T, bit_words, host, logits_of
+from tests.test_speculative import Case, T, bit_words, host, logits_of, random_tree
 
 FLOATS = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 FLT_MAX = float(np.finfo(np.float32).max)
@@ -134,3 +134,72 @@ def test_as_many_rows_as_a_call_takes(iw, gpu, dtype):
         assert bool(((a - b).abs() <= r * (1 + b.abs())).all())
     with pytest.raises(RuntimeError, match="2\\^22 rows"):
         iw.speculative.token_logprobs(few[:1].repeat(n + 1, 1))
+
+
+def differing(names, got, want):
+    """Names of the outputs whose bytes are not the same."""
+    return [n for n, a, b in zip(names, got, want, strict=True)
+            if a.dtype != b.dtype or a.shape != b.shape
+            or not torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))]
+
+
+def test_differing_sees_one_byte():
+    a = [torch.tensor([1, 2, 3]), torch.tensor([0.0, 1.0]), torch.tensor([float("nan")]), torch.zeros(2, 0)]
+    names = "abcd"
+    assert differing(names, a, [t.clone() for t in a]) == []
+    for i, j, v in ((0, 2, 4), (1, 0, -0.0), (2, 0, 1.0)):
+        b = [t.clone() for t in a]
+        b[i][j] = v
+        assert differing(names, b, a) == [names[i]]
+    with pytest.raises(ValueError):
+        differing(names, a[:3], a)
+
+
+@pytest.mark.gpu
+def test_captured_round_replays_byte_for_byte(iw, gpu):
+    """Plan, attention, scores and acceptance captured as one graph: every replay on new inputs,
+    between eager rounds of the same, leaves the eager outputs and caches to the byte."""
+    sp = iw.speculative
+    B, H, D, cap, N, V = 3, 2, 64, 96, 7, 70000
+    C = H * D
+    c = Case(1, B, H, D, cap, N, [10, 50, 80], [7, 5, 7], "quads")
+    qkv, k, v = T(c.qkv), T(c.k), c.v_view(T(c.vc))
+    ln, cnt, par = T(c.lengths), T(c.counts), T(c.parents)
+    logits = T(gen.i8(gen.rng(3), (B, N, V)))
+    tok, eot = torch.zeros((B, N), dtype=torch.int64, device="cuda"), 2
+    caches = sp.TreeCaches([qkv[..., C:2 * C]], [qkv[..., 2 * C:]], [k], [v], heads=H)
+    names = ("visible", "positions", "attention", "logprob", "entropy", "top_ids", "top_logprobs", "path", "accepted", "next",
+             "lengths", "k", "v")
+
+    def round_():
+        plan = sp.tree_plan(par, cnt, lengths=ln, max_positions=cap)
+        y = sp.tree_attention(qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:], k, v, ln, plan.visible, cnt, heads=H,
+                              qk_multiplier=90, qk_shift=9, frac_bits=8, av_multiplier=100, av_shift=6)
+        s = sp.token_logprobs(logits, tok, top=3, scale=0.1)
+        a = caches.accept(tok, par, s.top_ids[..., 0].contiguous(), ln, cnt, eot=eot)
+        return [*plan, y, *s, *a]
+    round_()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = round_()
+    accepted = set()
+    for i in range(6):
+        r = gen.rng(100 + i)
+        qkv.copy_(T(gen.i8(r, c.qkv.shape)))
+        x = gen.i8(r, (B, N, V), -127, 100)
+        top = r.integers(0, 3, (B, N))
+        x[np.arange(B)[:, None], np.arange(N), top] = 127  # few choices, so that paths go on
+        logits.copy_(T(x))
+        par.copy_(T(random_tree(r, B, N)))
+        ln.copy_(T(r.integers(0, cap - N, B).astype(np.int32)))
+        cnt.copy_(T(r.integers(0, N + 1, B).astype(np.int32)))
+        tok.copy_(T(r.integers(0, 3, (B, N))))
+        saved = k.clone(), v.clone()
+        want = [t.clone() for t in round_()] + [k.clone(), v.clone()]
+        k.copy_(saved[0]), v.copy_(saved[1])
+        g.replay()
+        torch.cuda.synchronize()
+        assert differing(names, [*outs, k, v], want) == []
+        accepted |= set(host(outs[8]).tolist())
+    assert len(accepted) > 2  # paths of several lengths
