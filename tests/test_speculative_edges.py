@@ -203,3 +203,66 @@ def test_captured_round_replays_byte_for_byte(iw, gpu):
         assert differing(names, [*outs, k, v], want) == []
         accepted |= set(host(outs[8]).tolist())
     assert len(accepted) > 2  # paths of several lengths
+
+
+GUARD = 4096
+
+
+def workspace(iw, name, sizes, fill):
+    """A workspace of the size that the entry point names, filled, with a guard behind it."""
+    need = iw._lib.value(name, *sizes)
+    assert need > 0
+    w = torch.full((need + GUARD,), fill, dtype=torch.uint8, device="cuda")
+    return w, need
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [0x00, 0x7f, 0xff])
+@pytest.mark.parametrize("layout", ["vt", "quads"])
+@pytest.mark.parametrize("D,cap,N", [(128, 1536, 1), (96, 1600, 16), (80, 2100, 17), (128, 2049, 33), (112, 1999, 64),
+                                     (64, 8192, 5), (48, 8300, 50)])
+def test_tree_attention_any_workspace(iw, oracle, gpu, D, cap, N, layout, fill):
+    """Whatever the workspace holds before, the outputs are the same and nothing behind it is written:
+    parts without a chunk, with the tree alone, rows without nodes or keys."""
+    print("case: attention workspace", D, cap, N, layout, fill, flush=True)
+    B, H = 6, 1
+    c = Case(cap, B, H, D, cap, N, [0, 1, cap, cap // 2, 0, cap // 3], [N, 1, N, (N + 1) // 2, N, 0], layout)
+    c.visible[4] = 0
+    C = H * D
+    w, need = workspace(iw, "iw_attention_tree_workspace", (B, H, N, D, cap), fill)
+    qkv, k, vc, ln, vis, cnt = T(c.qkv), T(c.k), c.v_view(T(c.vc)), T(c.lengths), T(c.visible), T(c.counts)
+    out = torch.full((B, N, C), 77, dtype=torch.int8, device="cuda")
+    vs = vc.stride()
+    v_s = (vs[0], vs[1], 4, vs[2]) if layout == "quads" else (vs[0], vs[1], vs[2], 4)
+    qm, qs, f, am, as_ = c.sc
+    q = qkv.data_ptr()
+    args = iw.speculative._pack(iw.speculative._ATTENTION_ARGS, q, N * 3 * C, 3 * C, q + C, N * 3 * C, 3 * C, q + 2 * C,
+                                N * 3 * C, 3 * C, k.data_ptr(), *k.stride()[:3], vc.data_ptr(), *v_s, ln.data_ptr(),
+                                vis.data_ptr(), N, cnt.data_ptr(), out.data_ptr(), N * C, C, B, H, N, D, cap, qm, qs, f, am,
+                                as_, 16, w.data_ptr())
+    iw._lib.call("iw_attention_tree", args, iw._lib.stream())
+    assert np.array_equal(host(out), c.expected(oracle))
+    assert bool((w[need:] == fill).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [0x00, 0x7f, 0xff])
+@pytest.mark.parametrize("kind,dtype", enumerate(["int8", "float32", "bfloat16", "float16"]))
+@pytest.mark.parametrize("V,top", [(65537, 32), (70001, 0), (200003, 9)])
+def test_token_logprobs_any_workspace(iw, gpu, V, top, kind, dtype, fill):
+    print("case: scores workspace", V, top, dtype, fill, flush=True)
+    r = gen.rng(V)
+    scale = 0.125 if dtype == "int8" else 0.5
+    x, tg = logits_of(r, 5, V, dtype, scale), r.integers(0, V, 5)
+    x[1] = x[1].abs()
+    if dtype != "int8":
+        x[2, V // 2:] = -np.inf
+    xd, t = x.cuda(), T(tg)
+    w, need = workspace(iw, "iw_token_logprobs_workspace", (kind, 5, V, top), fill)
+    lp, ent, lps = (torch.full(s, 7.0, device="cuda") for s in ((5,), (5,), (5, max(top, 1))))
+    ids = torch.full((5, max(top, 1)), -7, dtype=torch.int64, device="cuda")
+    iw._lib.call("iw_token_logprobs", xd.data_ptr(), kind, 5, V, V, scale, None, t.data_ptr(), lp.data_ptr(), ent.data_ptr(),
+                 top, ids.data_ptr(), lps.data_ptr(), w.data_ptr(), iw._lib.stream())
+    assert bool((w[need:] == fill).all())
+    got = iw.speculative.TokenLogprobs(lp, ent, ids[:, :top], lps[:, :top])
+    check(got, x, tg, top, scale)
