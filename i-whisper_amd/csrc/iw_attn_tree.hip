@@ -552,6 +552,8 @@ int launch_tree(const TreeArgs &t, hipStream_t s, int parts = 1) {
   const int qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT), blocks = qblocks * t.a.B * t.a.H, per_xcd = (blocks + 7) / 8;
   const int words = t.a.D / 4, per_word = (65536 + words - 1) / words;
   const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
+  // a grid has fewer than 2^32 threads
+  if (8LL * per_xcd * 64 * NW >= 1LL << 32) return fail("too many heads and nodes for one call");
   hipLaunchKernelGGL((attn_tree_kernel<KS, QUADS, QT, NW, NC, MODE>), dim3((unsigned)(8 * per_xcd), (unsigned)parts),
                      dim3(64 * NW), 0, s, t, qblocks, blocks, per_xcd, per_word, table);
   return check_launch("attn_tree_kernel");

@@ -626,7 +626,8 @@ int iw_tree_plan(const int32_t *parents, int64_t parents_ld, const int32_t *coun
  * transposed (v_sq == 4, v_sd >= round_up(cache_positions, 16)) or in key
  * quads (v_sd == 4); out (b, i) at out + b*o_sb + i*o_st. Rows of nodes past
  * the count, and of nodes that see no key, are zeros. nodes <= 64,
- * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24; operands and
+ * head_dim % 16 == 0, head_dim <= 128, cache_positions < 2^24, batch * heads <= 2^22
+ * (2^22 - 4 where more than 32 nodes meet more than 448 positions); operands and
  * strides are multiples of 16 bytes; kn_st, vn_st, k_st, v_sd, v_sq < 2^25. The
  * caches are read only: the nodes' K and V enter them with iw_tree_accept. out is q itself
  * or shares no memory with q, and none with k_new, v_new or the caches; it may lie in other columns
@@ -696,6 +697,7 @@ int iw_tree_accept(const iw_tree_caches *caches, const int64_t *tokens, const in
  *   top_ids, top_logprobs [rows][top], top <= 32: the most probable tokens in
  *                order, ties to the lowest index; a NaN counts as the largest
  * A row with a NaN or +inf, or without any finite logit, has NaN scores.
+ * rows <= 2^22, cols < 2^23, fewer than 2^23 parts of a row (64 KB each) in all.
  * Accumulated in float32. workspace: iw_token_logprobs_workspace bytes,
  * 16-byte aligned, used during the call's work only (NULL where that is 0). */
 #define IW_LOGITS_INT8 0

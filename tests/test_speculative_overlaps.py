@@ -1,5 +1,5 @@
 """Operands of the drafted-token operators that share memory: told apart exactly, refused where a
-call would read what it writes. The refusals need no GPU."""
+call would read what it writes. Grids beyond the launch limit. The refusals need no GPU."""
 import random
 import shutil
 import subprocess
@@ -253,3 +253,14 @@ def test_tree_caches_without_rows(iw, gpu):
     got = caches.accept(e(0, 4, dtype=torch.int64), e(0, 4, dtype=torch.int32), e(0, 4, dtype=torch.int64),
                         e(0, dtype=torch.int32))
     assert got.path.shape == (0, 4) and got.accepted.shape == got.next_token.shape == got.lengths.shape == (0,)
+
+
+def test_grid_of_the_largest_batches(iw):
+    """2^22 heads of 33 to 64 nodes over long caches would be 2^32 threads: refused by name."""
+    far = 1 << 40
+    big = dict(ATTN, q=far, kn=2 * far, vn=3 * far, k=4 * far, v=5 * far, lengths=6 * far, visible=7 * far, out=8 * far,
+               batch=1 << 22, heads=1, nodes=64, D=16, cap=512, q_sb=1024, q_st=16, kn_sb=1024, kn_st=16, vn_sb=1024, vn_st=16,
+               k_sb=8192, k_sh=8192, k_st=16, v_sb=8192, v_sh=8192, v_sd=4, v_sq=64, o_sb=1024, o_st=16)
+    for nodes in (33, 64):
+        refused(iw, "iw_attention_tree", big, dict(nodes=nodes), "too many heads")
+    refused(iw, "iw_attention_tree", big, dict(batch=(1 << 22) - 3), "too many heads")
