@@ -240,16 +240,30 @@ def _runs(t: Tensor):
 def _own_memory(written: Sequence[Tensor], read: Sequence[Tensor]) -> bool:
     """Whether the int8 tensors ``written`` share no byte with one another, with themselves or with
     ``read``. Exact: caches may be parts of one buffer in any order of its dims."""
-    spans = sorted(((t.data_ptr(), t.data_ptr() + 1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)), i)
-                    for i, t in enumerate([*written, *read]) if t.numel()), key=lambda x: x[:2])
+    spans, layouts = [], {}  # first and last byte; (extent, whether each dim steps over the smaller ones)
+    for i, t in enumerate([*written, *read]):
+        shape, stride = t.shape, t.stride()
+        if (shape, stride) not in layouts:
+            end, nested = 1, True
+            for s, n in sorted(zip(stride, shape)):
+                if n > 1:
+                    nested = nested and s >= end
+                    end += s * (n - 1)
+            layouts[shape, stride] = (0 if 0 in shape else end), nested
+        end, nested = layouts[shape, stride]
+        if end:
+            at = t.data_ptr()
+            spans.append((at, at + end, i, nested))
+    spans.sort()
     group, end = [], 0
-    for lo, hi, i in [*spans, (1 << 62, 1 << 62, -1)]:
+    for lo, hi, i, nested in [*spans, (1 << 62, 1 << 62, -1, True)]:
         if lo >= end:  # none of the tensors before reaches here
-            if not _group_apart([written[j] for j in group if j < len(written)],
-                                [read[j - len(written)] for j in group if j >= len(written)]):
+            if (len(group) > 1 or group and not group[0][1]) and not _group_apart(
+                    [written[j] for j, _ in group if j < len(written)],
+                    [read[j - len(written)] for j, _ in group if j >= len(written)]):
                 return False
             group = []
-        group.append(i)
+        group.append((i, nested))
         end = max(end, hi)
     return True
 
