@@ -210,7 +210,11 @@ struct Shared {
 
 // The top alternatives of a block's part one after the other, each the largest
 // key below the last: for rows whose bound leaves too many candidates (whole
-// rows of ties) or too few (suppressed tokens among the alternatives, NaN).
+// rows of ties) or too few (suppressed tokens among the alternatives, NaN). Also for
+// short rows of floats that fill fewer of the 64 groups of threads than there are
+// alternatives (a group has up to 64 float32 or 128 16-bit columns) and have more
+// than kCand logits: 64 rows of float16 with 32 alternatives take 61.5 us at 3000 columns,
+// 9.8 at 4100, with 16 alternatives 6.4 and 6.2.
 template <typename T, int NT>
 __device__ __noinline__ void top_by_rounds(const T *x, int c0, int n, const uint32_t *suppress, int top,
                                            Shared<NT> &s) {
