@@ -446,17 +446,23 @@ class TreeDecoder:
     def start(self, prompt: Tensor) -> Tensor:
         """The prompt step: returns each row's first token [B] (node 0 of its first tree)."""
         r = self.runner
-        r.run(prompt, 1)
+        with torch.cuda.device(self.lengths.device):  # the runner launches on the current device
+            r.run(prompt, 1)
         self.lengths.fill_(prompt.shape[1])
         return r.tokens.clone()
 
     def verify(self, tokens: Tensor, parents: Tensor, counts: Optional[Tensor] = None) -> Tensor:
         """int8 logits [B, N, vocab] after every node; the caches stay as they are."""
+        dev, shape = self.lengths.get_device(), (self.runner.B, self.nodes)
+        _check(tokens, _I64, shape, "tokens", dev)
+        _check(parents, _I32, shape, "parents", dev)
+        with torch.cuda.device(dev):  # the runner's parts launch on the current device
+            return self._pass(tokens, parents, counts)
+
+    def _pass(self, tokens: Tensor, parents: Tensor, counts: Optional[Tensor]) -> Tensor:
         r, dec, N, M = self.runner, self.runner.dec, self.nodes, self.M
         B, C, H = r.B, r.C, r.H
         dev = self.lengths.get_device()
-        _check(tokens, _I64, (B, N), "tokens", dev)
-        _check(parents, _I32, (B, N), "parents", dev)
         plan = tree_plan(parents, counts, lengths=self.lengths, max_positions=dec.n_ctx)
         # unused nodes may hold any value
         emb = dec.token_embedding.weight[tokens.clamp(0, dec.n_vocab - 1)]

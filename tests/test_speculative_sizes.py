@@ -131,3 +131,48 @@ def test_suppressed_words_of_the_runners(iw, gpu, dtype):
     tg = np.array([1, off[0], 2])
     got = iw.speculative.token_logprobs(x.cuda(), T(tg), top=6, scale=0.5, suppress=torch.from_numpy(words).cuda())
     check_scores(got, x, tg, 6, 0.5, off)
+
+
+def test_tree_decoder_launches_on_its_device(iw, gpu, monkeypatch):
+    """Every launch of a decoder's start and step is made with the tensors' device as the current
+    one, whichever is current outside: of the calls into the library, those that name the stream of the
+    current device are made within torch.cuda.device of the tensors'."""
+    dims, model = small_model(iw)
+    mel = iw.synth.synthetic_mel(1, dims.n_mels, 2 * dims.n_audio_ctx, seed=24)
+    sp, entered, outside, streams = iw.speculative, [], [], []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            entered.pop()
+            return super().__exit__(*a)
+    with torch.no_grad():
+        runner = iw.DecoderRunner(model.decoder, 1, dims.n_audio_ctx)
+        runner.set_audio(model.embed_audio(T(mel)))
+        tree = sp.TreeDecoder(runner, 3)
+        call, launch = iw._lib.call, sp._launch
+        own = []  # within _launch, which turns to the tensors' device itself
+
+        def counted(name, *args):
+            streams.append(name)
+            if not own and entered[-1:] != [0]:
+                outside.append(name)
+            return call(name, *args)
+
+        def launching(*args):
+            own.append(1)
+            try:
+                return launch(*args)
+            finally:
+                own.pop()
+        monkeypatch.setattr(torch.cuda, "device", Device)
+        monkeypatch.setattr(iw._lib, "call", counted)
+        monkeypatch.setattr(sp, "_launch", launching)
+        last = tree.start(T(np.array([[1, 2, 3]], np.int64)))
+        tokens = torch.cat([last, last, last])[None].contiguous()
+        tree.step(tokens, torch.tensor([[-1, 0, 1]], dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+    assert len(streams) > 20 and outside == []
