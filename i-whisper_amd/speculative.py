@@ -231,9 +231,9 @@ def _runs(t: Tensor):
     length = 1
     while dims and dims[0][0] == length:
         length *= dims.pop(0)[1]
-    at = torch.tensor([t.data_ptr()], dtype=torch.int64)
+    at = torch.tensor([t.data_ptr()], dtype=torch.int64, device="cpu")
     for s, n in reversed(dims):
-        at = (at[:, None] + s * torch.arange(n)).flatten()
+        at = (at[:, None] + s * torch.arange(n, device="cpu")).flatten()
     return at, length
 
 

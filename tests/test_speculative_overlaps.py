@@ -264,3 +264,10 @@ def test_grid_of_the_largest_batches(iw):
     for nodes in (33, 64):
         refused(iw, "iw_attention_tree", big, dict(nodes=nodes), "too many heads")
     refused(iw, "iw_attention_tree", big, dict(batch=(1 << 22) - 3), "too many heads")
+
+
+def test_addresses_are_compared_on_the_host(iw):
+    """Whatever torch's default device is."""
+    x = buf(2, 2, 8)
+    with torch.device("meta"):
+        assert iw.speculative._own_memory([x[:, 0], x[:, 1]], []) and not iw.speculative._own_memory([x[:, 0], x[:, 0]], [])
