@@ -116,10 +116,10 @@ LAID = dict(ATTN, q=P, kn=P + 2048, vn=P + 4096, k=P + 8192, v=P + 16384, length
     (dict(out=P + 128), "overlap q"), (dict(out=P, o_st=256, o_sb=2048), "overlap q"), (dict(out=P, q_sb=2048), "overlap q"),
     (dict(out=P + 2048), "k_new"), (dict(out=P + 2048 - 16), "overlap q"), (dict(out=P + 4096 - 16), "k_new"),
     (dict(out=P + 6144 - 16), "k_new or v_new"), (dict(out=P + 4096), "k_new or v_new"),
-    (dict(q=P, q_sb=3072, q_st=384, kn=P + 128, kn_sb=3072, kn_st=384, vn=P + 256, vn_sb=3072, vn_st=384, out=P + 16, o_sb=3072,
-          o_st=384), "overlap q"),
-    (dict(q=P, q_sb=3072, q_st=384, kn=P + 128, kn_sb=3072, kn_st=384, vn=P + 256, vn_sb=3072, vn_st=384, out=P + 240, o_sb=3072,
-          o_st=384), "k_new"),
+    (dict(q=P, q_sb=4096, q_st=512, kn=P + 128, kn_sb=4096, kn_st=512, vn=P + 256, vn_sb=4096, vn_st=512, out=P + 16, o_sb=4096,
+          o_st=512), "overlap q"),
+    (dict(q=P, q_sb=4096, q_st=512, kn=P + 128, kn_sb=4096, kn_st=512, vn=P + 256, vn_sb=4096, vn_st=512, out=P + 240, o_sb=4096,
+          o_st=512), "k_new"),
     (dict(out=P + 8192), "caches"), (dict(out=P + 8192 - 2032, o_sb=1024), "caches"), (dict(out=P + 16384 - 16), "caches"),
     (dict(out=P + 16384 + 4096), "caches"), (dict(out=P + 24576 - 16), "caches"),
     (dict(v_sq=4, v_sd=32, out=P + 16384 + 2 * 4096 - 16), "caches")])
