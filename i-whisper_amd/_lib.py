@@ -106,6 +106,9 @@ SIGNATURES = {
     "iw_tree_plan": [_p, _i64, _p, _p, _i64, _i64, _i32, _p, _p, _p],
     "iw_attention_tree": [_p, _p],
     "iw_tree_accept": [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _p],
+    "iw_attention_window": [_p, _p],
+    "iw_sample_tokens": [_p, _p],
+    "iw_verify_drafts": [_p, _p],
     "iw_token_logprobs": [_p, _i32, _i64, _i64, _i64, _f, _p, _p, _p, _p, _i64, _p, _p, _p, _p],
 }
 
@@ -113,7 +116,10 @@ SIGNATURES = {
 VALUE_FUNCS = {"iw_frag_bytes": ([_i64, _i64], C.c_int64),
                "iw_log_mel_scratch_floats": ([_i64, _i64], C.c_int64),
                "iw_attention_tree_workspace": ([_i64, _i64, _i64, _i64, _i64], C.c_int64),
-               "iw_token_logprobs_workspace": ([_i32, _i64, _i64, _i64], C.c_int64)}
+               "iw_token_logprobs_workspace": ([_i32, _i64, _i64, _i64], C.c_int64),
+               "iw_attention_window_workspace": ([_i64] * 8, C.c_int64),
+               "iw_sample_tokens_workspace": ([_i32, _i64, _i64], C.c_int64),
+               "iw_verify_drafts_workspace": ([_i32, _i64, _i64, _i64, _b], C.c_int64)}
 
 _lock = threading.Lock()
 _lib = None

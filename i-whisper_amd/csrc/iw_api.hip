@@ -4,6 +4,7 @@
 #include "iw_gemm.hpp"
 #include "iw_kernels.hpp"
 #include "iw_overlap.hpp"
+#include "iw_drafts.hpp"
 #include "iw_tree.hpp"
 
 #include <cmath>
@@ -1126,6 +1127,212 @@ int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t co
   a.top_lp = top_logprobs;
   a.workspace = workspace;
   return launch_token_scores(a, as_stream(stream));
+}
+
+// ---- sampled decoding with drafts ----
+
+int64_t iw_attention_window_workspace(int64_t batch, int64_t heads, int64_t queries, int64_t head_dim,
+                                      int64_t cache_positions, int64_t before, int64_t after, int64_t sinks) {
+  if (batch < 0 || batch > (1 << 22) || heads <= 0 || heads > 4096 || queries < 0 || queries > (1 << 24) || head_dim <= 0 ||
+      head_dim > 128 || cache_positions <= 0 || cache_positions >= (1 << 24) || before < 0 || after < 0 || sinks < 0 ||
+      before > INT32_MAX || after > INT32_MAX || sinks > INT32_MAX)
+    return -1;
+  if (batch == 0 || queries == 0) return 0;
+  return attn_window_workspace(batch * heads, queries, head_dim, cache_positions, before, after, sinks);
+}
+
+int iw_attention_window(const iw_attention_window_args *args, iw_stream_t stream) {
+  IW_REQUIRE(args, "null arguments");
+  const iw_attention_window_args &p = *args;
+  IW_REQUIRE(p.frac_bits > 0 && p.frac_bits < 14, "frac_bits must be in [1, 14)");
+  IW_REQUIRE(p.rsqrt_offset >= 0 && p.rsqrt_offset <= 29, "rsqrt_offset must be in [0,29]");
+  IW_REQUIRE(p.qk_multiplier >= 0 && p.qk_multiplier <= 255 && p.av_multiplier >= 0 && p.av_multiplier <= 255,
+             "multipliers must be uint8");
+  IW_REQUIRE(p.qk_shift >= -128 && p.qk_shift <= 127 && p.av_shift >= -128 && p.av_shift <= 127,
+             "shifts must be int8");
+  IW_REQUIRE(p.heads > 0 && p.heads <= 4096 && p.head_dim > 0 && p.head_dim <= 128 && p.head_dim % 16 == 0,
+             "window attention supports head_dim % 16 == 0, head_dim <= 128");
+  const int rc = check_tree_cache(p.heads, p.head_dim, p.cache_positions, p.v_sd, p.v_sq);
+  if (rc) return rc;
+  IW_REQUIRE(p.queries >= 0 && p.queries <= (1 << 24), "at most 2^24 queries of a row");
+  IW_REQUIRE(p.batch >= 0 && p.batch <= (1 << 22) && p.batch * p.heads <= (1 << 22) && p.positions_sb >= 0 &&
+                 p.batch * p.heads * ((p.queries + 15) / 16) < (1 << 25),
+             "invalid attention shape");
+  IW_REQUIRE(p.before >= 0 && p.before <= INT32_MAX && p.after >= 0 && p.after <= INT32_MAX && p.sinks >= 0 &&
+                 p.sinks <= INT32_MAX,
+             "before, after and sinks must be in [0, 2^31)");
+  if (p.batch == 0 || p.queries == 0) return IW_OK;
+  IW_REQUIRE(p.q && p.k && p.vt && p.out, "null tensor pointer");
+  const uintptr_t align = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) |
+                          reinterpret_cast<uintptr_t>(p.vt) | reinterpret_cast<uintptr_t>(p.out) |
+                          (uintptr_t)(p.q_sb | p.q_st | p.k_sb | p.k_sh | p.k_st | p.v_sb | p.v_sh | p.o_sb | p.o_st) |
+                          (uintptr_t)(p.v_sq != 4 ? p.v_sq : p.v_sd);
+  IW_REQUIRE((align & 15) == 0, "window attention operands must be 16-byte aligned");
+  // offsets within 64 keys and within a head's transposed rows are 32-bit numbers
+  const int64_t far = 1 << 25;
+  IW_REQUIRE(p.k_st >= 0 && p.k_st < far && p.v_sq >= 0 && p.v_sq < far && p.v_sd >= 0 && p.v_sd < far,
+             "strides of keys, key quads and transposed rows must be below 2^25");
+  IW_REQUIRE(attn_window_workspace(p.batch * p.heads, p.queries, p.head_dim, p.cache_positions, p.before, p.after, p.sinks) == 0 ||
+                 (p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 15) == 0),
+             "iw_attention_window_workspace bytes of 16-byte aligned workspace are needed");
+  // a block writes its rows while others still read theirs
+  const int64_t C = p.heads * p.head_dim;
+  const NodeRows out{p.out, p.o_sb, p.o_st, p.batch, p.queries, C}, q{p.q, p.q_sb, p.q_st, p.batch, p.queries, C};
+  IW_REQUIRE(rows_apart(out), "the rows of out must not overlap");
+  IW_REQUIRE(out.same(q) || apart(out, q), "out must be q itself or must not overlap q");
+  const int64_t quads = (p.cache_positions + 3) / 4, wide = (p.cache_positions + 15) / 16 * 16;
+  const auto cached = [&](const int8_t *x, int64_t row, int64_t sh, int64_t sb) {
+    const Runs heads(x, row, sh, p.heads);
+    return Runs(heads.at, heads.reach(), sb, p.batch);
+  };
+  const int64_t k_row = p.k_st * (p.cache_positions - 1) + p.head_dim;
+  const int64_t v_row = p.v_sq != 4 ? p.v_sq * (quads - 1) + 4 * p.head_dim : p.v_sd * (p.head_dim - 1) + wide;
+  // keys whose heads lie side by side are rows, and out may be other columns of theirs
+  const bool k_apart = apart(out.of_batch(), cached(p.k, k_row, p.k_sh, p.k_sb)) ||
+                       ((p.heads == 1 || p.k_sh == p.head_dim) &&
+                        apart(out, NodeRows{p.k, p.k_sb, p.k_st, p.batch, p.cache_positions, C}));
+  IW_REQUIRE(k_apart && apart(out.of_batch(), cached(p.vt, v_row, p.v_sh, p.v_sb)), "out must not overlap the keys or values");
+  WindowArgs t;
+  AttnArgs &a = t.a;
+  a.q = p.q;
+  a.q_sb = p.q_sb;
+  a.q_st = p.q_st;
+  a.k = p.k;
+  a.k_sb = p.k_sb;
+  a.k_sh = p.k_sh;
+  a.k_st = p.k_st;
+  a.vt = p.vt;
+  a.v_sb = p.v_sb;
+  a.v_sh = p.v_sh;
+  a.v_sd = p.v_sd;
+  a.v_sq = p.v_sq;
+  a.out = p.out;
+  a.o_sb = p.o_sb;
+  a.o_st = p.o_st;
+  a.B = (int32_t)p.batch;
+  a.H = (int32_t)p.heads;
+  a.Tq = (int32_t)p.queries;
+  a.Tk = (int32_t)p.cache_positions;
+  a.D = (int32_t)p.head_dim;
+  a.qk_m = (uint32_t)p.qk_multiplier;
+  a.qk_s = (uint32_t)(p.qk_shift > 0 ? p.qk_shift : 0);
+  a.frac_bits = (int32_t)p.frac_bits;
+  a.av_m = (uint32_t)p.av_multiplier;
+  a.av_s = (uint32_t)(p.av_shift < 0 ? 0 : (p.av_shift > 32 ? 32 : p.av_shift));
+  a.rsqrt_off = (uint32_t)p.rsqrt_offset;
+  t.lengths = p.lengths;
+  t.positions = p.positions;
+  t.pos_sb = p.positions_sb;
+  t.counts = p.counts;
+  t.before = p.before;
+  t.after = p.after;
+  t.sinks = (int32_t)p.sinks;
+  t.workspace = static_cast<uint32_t *>(p.workspace);
+  return launch_attn_window(t, as_stream(stream));
+}
+
+namespace {
+
+int check_logit_rows(int64_t type, const void *logits, int64_t rows, int64_t cols) {
+  IW_REQUIRE(type >= LOGIT_I8 && type <= LOGIT_F16, "logits must be int8, float32, bfloat16 or float16");
+  IW_REQUIRE(rows >= 0 && cols > 0 && cols < (1 << 23), "invalid logits shape (at most 2^23 - 1 columns)");
+  const uintptr_t item = type == LOGIT_I8 ? 1 : type == LOGIT_F32 ? 4 : 2;
+  IW_REQUIRE(reinterpret_cast<uintptr_t>(logits) % item == 0, "logits must be aligned to their type");
+  return IW_OK;
+}
+
+int check_scale(double scale, double temperature, const float *temperatures) {
+  IW_REQUIRE(scale > 0 && scale <= 0x1p100, "scale must be above 0 and at most 2^100");
+  IW_REQUIRE(temperatures || (temperature >= 0 && temperature <= 0x1p100), "temperature must be in [0, 2^100]");
+  return IW_OK;
+}
+
+}  // namespace
+
+int64_t iw_sample_tokens_workspace(int32_t type, int64_t rows, int64_t cols) {
+  if (type < LOGIT_I8 || type > LOGIT_F16 || rows < 0 || rows > (1 << 22) || cols <= 0 || cols >= (1 << 23)) return -1;
+  return sample_workspace(type, rows, cols);
+}
+
+int iw_sample_tokens(const iw_sample_tokens_args *args, iw_stream_t stream) {
+  IW_REQUIRE(args, "null arguments");
+  const iw_sample_tokens_args &p = *args;
+  int rc = check_logit_rows(p.type, p.logits, p.rows, p.cols);
+  if (rc) return rc;
+  IW_REQUIRE(p.rows <= (1 << 22) && p.ld >= p.cols, "invalid logits shape (at most 2^22 rows)");
+  rc = check_scale(p.scale, p.temperature, p.temperatures);
+  if (rc) return rc;
+  if (p.rows == 0) return IW_OK;
+  IW_REQUIRE(p.logits && p.uniforms && p.tokens, "null tensor pointer");
+  IW_REQUIRE(p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 15) == 0,
+             "iw_sample_tokens_workspace bytes of 16-byte aligned workspace are needed");
+  SampleArgs a;
+  a.d.x = p.logits;
+  a.d.sb = p.ld;
+  a.d.scale = p.scale;
+  a.d.temperature = p.temperature;
+  a.d.temperatures = p.temperatures;
+  a.type = (int)p.type;
+  a.rows = p.rows;
+  a.cols = (int)p.cols;
+  a.suppress = p.suppress;
+  a.uniforms = p.uniforms;
+  a.tokens = p.tokens;
+  a.logprob = p.logprob;
+  a.workspace = p.workspace;
+  return launch_sample_tokens(a, as_stream(stream));
+}
+
+int64_t iw_verify_drafts_workspace(int32_t type, int64_t batch, int64_t nodes, int64_t cols, bool draft) {
+  if (type < LOGIT_I8 || type > LOGIT_F16 || batch < 0 || batch > (1 << 20) || nodes <= 0 || nodes > kVerifyMaxNodes ||
+      cols <= 0 || cols >= (1 << 23))
+    return -1;
+  return verify_workspace(type, batch, nodes, cols, draft);
+}
+
+int iw_verify_drafts(const iw_verify_drafts_args *args, iw_stream_t stream) {
+  IW_REQUIRE(args, "null arguments");
+  const iw_verify_drafts_args &p = *args;
+  int rc = check_logit_rows(p.type, p.logits, p.batch, p.cols);
+  if (rc == IW_OK) rc = check_logit_rows(p.type, p.draft_logits, p.batch, p.cols);
+  if (rc) return rc;
+  IW_REQUIRE(p.nodes > 0 && p.nodes <= kVerifyMaxNodes && p.batch <= (1 << 20), "a row has 1 to 64 nodes, a call at most 2^20 rows");
+  IW_REQUIRE(p.sb >= 0 && p.sn >= 0 && p.draft_sb >= 0 && p.draft_sn >= 0, "strides must not be negative");
+  rc = check_scale(p.scale, p.temperature, p.temperatures);
+  if (rc == IW_OK && p.draft_logits) rc = check_scale(p.draft_scale, p.draft_temperature, p.draft_temperatures);
+  if (rc) return rc;
+  if (p.batch == 0) return IW_OK;
+  IW_REQUIRE(p.logits && p.tokens && p.uniforms && p.choice && p.accepted && p.next, "null tensor pointer");
+  IW_REQUIRE(p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 15) == 0,
+             "iw_verify_drafts_workspace bytes of 16-byte aligned workspace are needed");
+  VerifyArgs a;
+  a.target.x = p.logits;
+  a.target.sb = p.sb;
+  a.target.st = p.sn;
+  a.target.inner = p.nodes;
+  a.target.scale = p.scale;
+  a.target.temperature = p.temperature;
+  a.target.temperatures = p.temperatures;
+  if (p.nodes > 1) a.draft.x = p.draft_logits;
+  a.draft.sb = p.draft_sb;
+  a.draft.st = p.draft_sn;
+  a.draft.inner = p.nodes > 1 ? p.nodes - 1 : 1;
+  a.draft.scale = p.draft_scale;
+  a.draft.temperature = p.draft_temperature;
+  a.draft.temperatures = p.draft_temperatures;
+  a.type = (int)p.type;
+  a.batch = p.batch;
+  a.nodes = (int)p.nodes;
+  a.cols = (int)p.cols;
+  a.suppress = p.suppress;
+  a.tokens = p.tokens;
+  a.counts = p.counts;
+  a.uniforms = p.uniforms;
+  a.choice = p.choice;
+  a.accepted = p.accepted;
+  a.next = p.next;
+  a.workspace = p.workspace;
+  return launch_verify_drafts(a, as_stream(stream));
 }
 
 // ---- fragment-major decode operands ----

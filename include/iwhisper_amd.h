@@ -709,6 +709,118 @@ int iw_token_logprobs(const void *logits, int32_t type, int64_t rows, int64_t co
                       int64_t top, int64_t *top_ids, float *top_logprobs, void *workspace, iw_stream_t stream);
 int64_t iw_token_logprobs_workspace(int32_t type, int64_t rows, int64_t cols, int64_t top);
 
+/* ---------------------------------------------------------------------------
+ * Sampled decoding with drafts: attention over a window of the keys, tokens
+ * drawn from logits by given random numbers, and drafted tokens verified
+ * against the model's probabilities. The reference draws its tokens with
+ * Categorical(logits / temperature).sample() (decoding.py:275-287), one per row
+ * and step, and always attends to every key.
+ * ------------------------------------------------------------------------- */
+
+/* Attention of each query over a window of the keys around its position and
+ * the first keys. Query i of row b at position p sees key j where
+ *   0 <= j < lengths[b] and j <= p + after and (j >= p - before or j < sinks);
+ * p = positions[b * positions_sb + i], or for positions NULL
+ * lengths[b] - counts[b] + i: the queries are the row's last ones. lengths NULL =
+ * cache_positions, counts NULL = queries; both are read on the device and clamped to
+ * [0, cache_positions] and [0, queries]. q and out: element (b, i, h, d) at
+ * base + b*sb + i*st + h*head_dim + d; K and V as iw_attention_tree takes them
+ * (K of projected rows has k_sh = head_dim), scalars as there. Rows of queries past the count, and
+ * of queries that see no key, are zeros. queries <= 2^24, head_dim % 16 == 0, head_dim
+ * <= 128, cache_positions < 2^24, batch * heads <= 2^22, fewer than 2^25 blocks of 16
+ * queries; before, after and sinks in [0, 2^31); operands and strides are multiples
+ * of 16 bytes; k_st, v_sd, v_sq < 2^25. out is q itself or shares no memory with q,
+ * K or V; it may lie in other columns of rows of K with its strides. workspace:
+ * iw_attention_window_workspace bytes, 16-byte aligned, used during the call's work
+ * only (NULL where that is 0). The struct is read during the call. */
+typedef struct iw_attention_window_args {
+  const int8_t *q;
+  int64_t q_sb, q_st;
+  const int8_t *k;
+  int64_t k_sb, k_sh, k_st;
+  const int8_t *vt;
+  int64_t v_sb, v_sh, v_sd, v_sq;
+  const int32_t *lengths;
+  const int32_t *positions;
+  int64_t positions_sb;
+  const int32_t *counts;
+  int8_t *out;
+  int64_t o_sb, o_st;
+  int64_t batch, heads, queries, head_dim, cache_positions;
+  int64_t before, after, sinks;
+  int64_t qk_multiplier, qk_shift, frac_bits, av_multiplier, av_shift, rsqrt_offset;
+  void *workspace;
+} iw_attention_window_args;
+int iw_attention_window(const iw_attention_window_args *args, iw_stream_t stream);
+/* of a call with these sizes, whether positions are given or not; -1 for invalid ones */
+int64_t iw_attention_window_workspace(int64_t batch, int64_t heads, int64_t queries, int64_t head_dim,
+                                      int64_t cache_positions, int64_t before, int64_t after, int64_t sinks);
+
+/* A token of each row of logits, drawn by a given number. Row r's weights are
+ * w_j = exp((x_j - max x) * scale / T), 0 for a token of the bitmask suppress (or NULL)
+ * and for -inf; tokens[r] is the least j with w_0 + .. + w_j > uniforms[r] * (sum of w),
+ * logprob[r] (or NULL) log(w_j / sum). T is temperatures[r] (float32), or for NULL the
+ * scalar temperature; where it is not above 0 the token is the first of the
+ * largest logits, with logprob 0. uniforms are clamped to [0, 1 - 2^-24], a NaN is 0. A
+ * row with a NaN or +inf, or without any finite logit, gives token -1 and logprob NaN.
+ * logits: type as iw_token_logprobs, row stride ld. Weights and sums are 64-bit. rows <=
+ * 2^22, cols < 2^23. workspace: iw_sample_tokens_workspace bytes, 16-byte aligned,
+ * used during the call's work only. The struct is read during the call. */
+typedef struct iw_sample_tokens_args {
+  const void *logits;
+  int64_t type, rows, cols, ld;
+  double scale, temperature;
+  const float *temperatures;
+  const uint32_t *suppress;
+  const float *uniforms;
+  int64_t *tokens;
+  float *logprob;
+  void *workspace;
+} iw_sample_tokens_args;
+int iw_sample_tokens(const iw_sample_tokens_args *args, iw_stream_t stream);
+int64_t iw_sample_tokens_workspace(int32_t type, int64_t rows, int64_t cols);
+
+/* Verification of drafted tokens. Node 0 of row b is its last chosen token, nodes 1 ..
+ * counts[b] - 1 (counts NULL = nodes; clamped to [0, nodes] on the device) are drafts,
+ * each drafted after the one before. With p_i the distribution (as iw_sample_tokens
+ * has it) of logits[b][i] at `scale` and the row's temperature, and q_i that of
+ * draft_logits[b][i] at draft_scale and draft_temperature, from which token i + 1 was
+ * drawn (draft_logits NULL: certain drafts, q_i is 1 at token i + 1):
+ *   from i = 0 on, token x = tokens[b][i + 1] is accepted where
+ *   uniforms[b][i] * q_i(x) < p_i(x), up to the first that is not;
+ *   with a accepted, next[b] is drawn by uniforms[b][nodes - 1] from
+ *   max(p_a - q_a, 0) where a draft was refused (from p_a where nothing is left of
+ *   it), else from p_a.
+ * So the tokens are distributed as p whatever q is. choice[b][i] = tokens[b][i + 1]
+ * for i < a, next[b] for i = a, then -1: what iw_tree_accept takes for a chain. A row
+ * without nodes has a = 0 and next -1, and so has one whose p_a has a NaN or +inf or no finite
+ * logit; a token outside the vocabulary has probability 0, a draft row without a
+ * distribution is refused and leaves p. tokens, uniforms (float32), choice [batch][nodes], accepted,
+ * next [batch] contiguous; logits and draft_logits at base + b*sb + i*sn (in logits),
+ * of one type; suppress counts for both. temperatures, draft_temperatures: float32
+ * [batch], or NULL for the scalars. nodes <= 64, batch <= 2^20, cols < 2^23. workspace:
+ * iw_verify_drafts_workspace bytes, 16-byte aligned, used during the call's work
+ * only. The struct is read during the call. */
+typedef struct iw_verify_drafts_args {
+  const void *logits;
+  int64_t sb, sn;
+  const void *draft_logits;
+  int64_t draft_sb, draft_sn;
+  int64_t type, batch, nodes, cols;
+  double scale, temperature, draft_scale, draft_temperature;
+  const float *temperatures, *draft_temperatures;
+  const uint32_t *suppress;
+  const int64_t *tokens;
+  const int32_t *counts;
+  const float *uniforms;
+  int64_t *choice;
+  int32_t *accepted;
+  int64_t *next;
+  void *workspace;
+} iw_verify_drafts_args;
+int iw_verify_drafts(const iw_verify_drafts_args *args, iw_stream_t stream);
+int64_t iw_verify_drafts_workspace(int32_t type, int64_t batch, int64_t nodes, int64_t cols, bool draft);
+
 /* Per-head gather into a [b][h][t][d] cache (the cross-attention K of
  * model_int.py:722-730, computed once per utterance):
  * dst[b*dst_sb + h*dst_sh + (t_offset+t)*dst_st + d] = src[b*src_sb + t*src_st + h*D + d]. */
