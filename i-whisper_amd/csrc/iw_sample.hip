@@ -12,10 +12,12 @@
 // 64-bit numbers (vector units add them as fast as 32-bit ones here). An int8 row has at most 256
 // distances from M, whose weights are a table in LDS.
 //
-// A row is cut into spans of 4 KB, a wave each: its maximum and its sum relative to that are all
-// that the first launch leaves (the one read of the logits). The row's block then adds up
-// the spans, finds the one where the running sum passes u Z, and looks into that again. For
-// drafts a launch between finds the first rejection, and another one the spans of max(p - q, 0).
+// A row is cut into spans of 256 pieces of 16 bytes, a wave each: its maximum and its sum relative to that are all
+// that the first launch leaves (the one read of the logits). The row's block then adds up the spans, finds the one
+// where the running sum passes u Z, and looks into that again. For drafts a launch between finds the first
+// rejection from the sums, and another one the sums of max(p - q, 0) over 64 pieces each. (All of that in one launch, a
+// block of 16 waves a row, took 26.4 us for 5 rows of int8 logits in the place of 3.7 + 6.9 + 6.6, and 36.3 for 24 times 6 of
+// float32 in the place of 5.4 + 4.8 + 6.0: 40 KB of instructions that every block fetches and runs once.)
 #include <algorithm>
 #include <type_traits>
 
@@ -28,7 +30,7 @@ namespace iw {
 
 namespace {
 
-constexpr int kSpanBytes = 4096, kSpanPieces = kSpanBytes / 16;  // one piece a thread of a row's block
+constexpr int kSpanPieces = 256;
 constexpr int kWaves = 4, NT = 64 * kWaves;
 constexpr double kLog2E = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
@@ -40,31 +42,27 @@ struct Span {
   double z;
 };
 
-// ln(2)^n / n!
-constexpr double exp2_term(int n) {
-  double t = 1.0;
-  for (int i = 1; i <= n; ++i) t = t * kLn2 / i;
-  return t;
+// 2^f for |f| <= 1/2: the polynomial of degree 8 with the smallest relative error, 7.8e-13 (found by exchange; a
+// degree more or less, 1.4e-14 or 4.0e-11). A vocabulary of 2^16 tokens has its borders right to 8e-13 of the whole then,
+// and 4e-8 of all numbers would draw another token than exact ones.
+__device__ __forceinline__ double exp2_part(double f) {
+  // the two constants of the first step: an instruction reads one from scalar registers
+  double second = 0x1.00dad2504eb63p-16;
+  asm("" : "+v"(second));
+  double p = fma(0x1.61afcebb0e8b4p-20, f, second);
+  p = fma(p, f, 0x1.430acca346a3ep-13);
+  p = fma(p, f, 0x1.5d874838559edp-10);
+  p = fma(p, f, 0x1.3b2ab5c52926cp-7);
+  p = fma(p, f, 0x1.c6b08dd46d391p-5);
+  p = fma(p, f, 0x1.ebfbdff9319e1p-3);
+  p = fma(p, f, 0x1.62e42fef8615ep-1);
+  return fma(p, f, 0x1.ffffffffff7a3p-1);
 }
-
-// 2^t, 0 far below: the nearest whole number is the exponent, of the rest (at most 1/2) the Taylor sum to its
-// 11th power, off by 6e-15. A NaN (a masked logit of a row that has no other) gives 0.
+// 2^t, 0 far below. A NaN (a masked logit of a row that has no other) gives 0.
 __device__ __forceinline__ double exp2_64(double t) {
   t = fmax(t, -1100.0);
-  const double k = rint(t), f = t - k;
-  double p = exp2_term(11);
-  p = fma(p, f, exp2_term(10));
-  p = fma(p, f, exp2_term(9));
-  p = fma(p, f, exp2_term(8));
-  p = fma(p, f, exp2_term(7));
-  p = fma(p, f, exp2_term(6));
-  p = fma(p, f, exp2_term(5));
-  p = fma(p, f, exp2_term(4));
-  p = fma(p, f, exp2_term(3));
-  p = fma(p, f, exp2_term(2));
-  p = fma(p, f, exp2_term(1));
-  p = fma(p, f, 1.0);
-  return ldexp(p, (int)k);
+  const double k = rint(t);
+  return ldexp(exp2_part(t - k), (int)k);
 }
 
 template <int CTRL>
@@ -88,14 +86,22 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   v += dpp_f64<0x140>(v);
   return (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
 }
-// Sum of this lane's and the lower lanes' values
-__device__ __forceinline__ double wave_scan_f64(double v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(v, o);
-    if (lane >= o) v += t;
-  }
-  return v;
+// Sum of this lane's and the lower lanes' values: shifts by 1, 2, 4 and 8 within rows of 16 lanes, then the last lane
+// of the row before for every other row, and lane 31 for the upper half
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double scan_step(double x) {
+  const uint64_t b = __double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+  return x + __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  v = scan_step<0x111, 0xf>(v);
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);
+  return scan_step<0x143, 0xc>(v);
 }
 
 __device__ __forceinline__ float clamp_uniform(float u) { return fminf(fmaxf(u, 0.f), 0x1.fffffep-1f); }
@@ -129,8 +135,8 @@ struct Row {
   }
 };
 template <typename T>
-__device__ __forceinline__ const T *row_of(const DistRows &d, int64_t row) {
-  return reinterpret_cast<const T *>(d.x) + row / d.inner * d.sb + row % d.inner * d.st;
+__device__ __forceinline__ const T *row_of(const DistRows &d, int64_t outer, int inner) {
+  return reinterpret_cast<const T *>(d.x) + outer * d.sb + inner * d.st;
 }
 
 // Weight of a logit relative to the largest, m; int8 rows have those of all distances in a table. The
@@ -150,13 +156,15 @@ __device__ __forceinline__ void fill_table(double *table, double c, int tid) {
   for (int d = tid; d < 256; d += NT) table[d] = exp2_64(-((double)d * c));
 }
 
+// A row's pieces, the last of them perhaps in part, and spans
 template <typename T>
 struct Cut {
   static constexpr int E = Logit<T>::E;
-  int cols, pieces, spans;
-  __host__ __device__ Cut(int cols_) : cols(cols_), pieces(cols_ / E) {
-    const int n = (pieces + kSpanPieces - 1) / kSpanPieces;
-    spans = n > 0 ? n : 1;
+  int cols, full, spans, parts;  // parts of 64 pieces
+  __host__ __device__ Cut(int cols_) : cols(cols_), full(cols_ / E) {
+    const int pieces = (cols_ + E - 1) / E;
+    spans = (pieces + kSpanPieces - 1) / kSpanPieces;
+    parts = (pieces + 63) / 64;
   }
 };
 
@@ -170,96 +178,176 @@ struct SpanArgs {
   Span *spans = nullptr;
 };
 
+// The larger of two, NaN where either is
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Sum of 2^((x - m) c) as 2^(x c - M) * 2^(M - m c), M = m c as a whole number: a constant's low word counts the exponents, and
+// the part beyond the whole number is exact, so a logit takes 14 instructions. `least` stands for -inf: its weight is 0.
+struct SumWeights {
+  double c, magic, rest, least;
+  bool fits;
+  __device__ __forceinline__ SumWeights(double c_, float m) : c(c_) {
+    const double mc = (double)m * c, whole = rint(mc);
+    magic = 0x1.8p52 - whole;
+    rest = fma((double)m, c, -whole);
+    least = (double)m - 1200.0 / c;
+    fits = fabs(mc) < 0x1p40 && c > 0x1p-60;
+  }
+  __device__ __forceinline__ double of(float x) const {
+    const double v = fmax((double)x, least), u = fma(v, c, magic), n = u - magic;
+    return ldexp(exp2_part(fma(v, c, -n)), (int)(uint32_t)__double_as_longlong(u));
+  }
+  __device__ __forceinline__ double scaled(double sum) const { return sum * exp2_64(-rest); }
+};
+
 template <typename T>
 __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
   using L = Logit<T>;
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   constexpr int E = L::E, P = kSpanPieces / 64;
+  constexpr uint32_t ALL = (1u << E) - 1u;
   __shared__ double sTable[I8 ? 256 : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = (uint32_t)blockIdx.x / (uint32_t)groups;
-  const int which = row >= a.first;
-  const DistRows &d = a.d[which];
-  const int64_t r = which ? row - a.first : row, outer = r / d.inner;
-  if (a.counts && (int)(r % d.inner) >= a.counts[outer] - which) return;
-  const Row dist(d, outer);
-  if (I8) {
-    fill_table(sTable, dist.c, tid);
-    lds_barrier();
-  }
+  const bool second = row >= a.first;
+  const int64_t r = second ? row - a.first : row;
+  const uint32_t inner = (uint32_t)(second ? a.d[1].inner : a.d[0].inner);
+  const uint32_t outer = (uint32_t)r / inner, at = (uint32_t)r % inner;
+  if (a.counts && (int)at >= a.counts[outer] - (second ? 1 : 0)) return;
   const Cut<T> cut(a.cols);
   const int s = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (s >= cut.spans) return;
-  const T *x = row_of<T>(d, r);
+  const T *x = reinterpret_cast<const T *>(second ? a.d[1].x : a.d[0].x) +
+               (int64_t)outer * (second ? a.d[1].sb : a.d[0].sb) + (int64_t)at * (second ? a.d[1].st : a.d[0].st);
+  // all that the wave reads is on the way before it waits for anything; pieces past the last read that again
   const int p0 = s * kSpanPieces + lane;
   uint4 w[P];
-  uint32_t off[P];
+  if (cut.full > 0) {
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int at = p0 + 64 * p;
-    w[p] = make_uint4(0u, 0u, 0u, 0u);
-    off[p] = (1u << E) - 1u;
-    if (at < cut.pieces) {
-      w[p] = load_piece(x + (int64_t)at * E);
-      off[p] = hidden_bits(a.suppress, at * E, E, a.cols);
-    }
+    for (int p = 0; p < P; ++p) w[p] = load_piece(x + (int64_t)min(p0 + 64 * p, cut.full - 1) * E);
   }
-  // what the last piece leaves, one logit a lane
-  const int extra = cut.pieces * E + lane;
+  const int extra = cut.full * E + lane;
   const bool has_extra = s == cut.spans - 1 && extra < a.cols && !suppressed(a.suppress, extra);
   const float xe = has_extra ? L::one(x + extra) : -INFINITY;
-
-  // NaN is the largest
-  uint32_t top = has_extra ? ordered(xe) : ordered(-INFINITY);
+  uint32_t off[P];  // not counted: past the last piece, or suppressed
 #pragma unroll
   for (int p = 0; p < P; ++p)
+    off[p] = p0 + 64 * p >= cut.full ? ALL : hidden_bits(a.suppress, (p0 + 64 * p) * E, E, a.cols);
+  const Row dist = second ? Row(a.d[1], outer) : Row(a.d[0], outer);
+  if (I8) {
+    if (!dist.greedy) fill_table(sTable, dist.c, tid);
+    lds_barrier();
+  }
+  if (s >= cut.spans) return;
+
+  // int8 logits that do not count are -128, of which `hidden` are taken off the sum again; others -inf
+  float m;
+  int hidden = 0;
+  if constexpr (I8) {
+    using v2s = typename L::v2s;
+    v2s most{-32768, -32768};
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (!((off[p] >> e) & 1u)) top = max(top, ordered(L::get(w[p], e)));
-  top = wave_max_u32_dpp(top);
-  const float m = key_value((uint64_t)top << 32);
+    for (int p = 0; p < P; ++p) {
+      if (off[p] != 0u) {
+        hidden += __popc(off[p]);
+        uint32_t *v = &w[p].x;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t bits = __umul24((off[p] >> (4 * q)) & 15u, 0x00204081u) & 0x01010101u;
+          const uint32_t no = __builtin_amdgcn_perm(0u, 0u, bits | 0x0c0c0c0cu);
+          v[q] = (v[q] & ~no) | (0x80808080u & no);
+        }
+      }
+      most = __builtin_elementwise_max(most, L::halves(w[p]));
+    }
+    // a half's value is its upper byte
+    const int top = wave_max_dpp(max(has_extra ? (int)xe : -128, max((int)most.x >> 8, (int)most.y >> 8)));
+    const bool any = __any(has_extra || hidden < P * E);
+    m = any ? (float)top : -INFINITY;
+  } else {
+    float top = xe;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (off[p] != 0u) L::mask(w[p], off[p]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max_nan(top, L::get(w[p], e));
+    }
+    m = key_value((uint64_t)wave_max_u32_dpp(ordered(top)) << 32);
+  }
 
   Span out{m, -1, 0.0};
   if (dist.greedy) {
-    uint32_t col = has_extra && ordered(xe) == top ? (uint32_t)extra : ~0u;
+    uint32_t col = has_extra && xe == m ? (uint32_t)extra : ~0u;
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (!((off[p] >> e) & 1u) && ordered(L::get(w[p], e)) == top) col = min(col, (uint32_t)((p0 + 64 * p) * E + e));
+        if (!((off[p] >> e) & 1u) && L::get(w[p], e) == m) col = min(col, (uint32_t)((p0 + 64 * p) * E + e));
     out.col = (int32_t)~wave_max_u32_dpp(~col);
-  } else {
-    const Weigh wt(dist.c, m, sTable);
+  } else if (m - m == 0.f) {
     double z = 0.0;
-    if (has_extra) z = wt.of<T>(xe);
+    if constexpr (I8) {
+      const uint32_t top = (uint32_t)((int)m + 128) * 0x01010101u;
+      const char *table = reinterpret_cast<const char *>(sTable);
+      if (has_extra) z = sTable[(int)m - (int)xe];
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+      for (int p = 0; p < P; ++p) {
+        // distances from m, byte by byte: none borrows
+        const uint32_t v[4] = {top - (w[p].x ^ 0x80808080u), top - (w[p].y ^ 0x80808080u), top - (w[p].z ^ 0x80808080u),
+                               top - (w[p].w ^ 0x80808080u)};
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const double v = wt.of<T>(L::get(w[p], e));
-        z += (off[p] >> e) & 1u ? 0.0 : v;
+        for (int q = 0; q < 4; ++q) {
+          const double a0 = *reinterpret_cast<const double *>(table + ((v[q] << 3) & 0x7f8u));
+          const double a1 = *reinterpret_cast<const double *>(table + ((v[q] >> 5) & 0x7f8u));
+          const double a2 = *reinterpret_cast<const double *>(table + ((v[q] >> 13) & 0x7f8u));
+          const double a3 = *reinterpret_cast<const double *>(table + ((v[q] >> 21) & 0x7f8u));
+          z += (a0 + a1) + (a2 + a3);
+        }
       }
+      // the rest of a sum that cancels is whole multiples of one weight, or far above its rounding
+      z -= (double)hidden * sTable[(int)m + 128];
+    } else {
+      const SumWeights sum(dist.c, m);
+      if (sum.fits) {
+        if (has_extra) z = sum.of(xe);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          if (__any(off[p] != ALL)) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) z += sum.of(L::get(w[p], e));
+          }
+        z = sum.scaled(z);
+      } else {
+        const Weigh wt(dist.c, m, nullptr);
+        if (has_extra) z = wt.of<T>(xe);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int e = 0; e < E; ++e) z += wt.of<T>(L::get(w[p], e));
+      }
+    }
     out.z = wave_sum_f64(z);
   }
   if (lane == 0) a.spans[row * cut.spans + s] = out;
 }
 
 // ---- a row's block: from the spans to a token ----
+template <int W>
 struct Block {
-  double wave[kWaves];
-  uint32_t max[kWaves];
+  double wave[W];
+  uint32_t max[W];
   int owner;
   int found;
   double base;
 };
 
 // The largest of every thread's values, in every thread
-__device__ __forceinline__ uint32_t block_max(uint32_t v, Block &s, int tid) {
+template <int W>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, Block<W> &s, int tid) {
   v = wave_max_u32_dpp(v);
   if ((tid & 63) == 0) s.max[tid >> 6] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) v = max(v, s.max[w]);
+  for (int w = 0; w < W; ++w) v = max(v, s.max[w]);
   __syncthreads();
   return v;
 }
@@ -267,26 +355,26 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, Block &s, int tid) {
 // Which thread holds the place where the running sum of the threads' sums passes a target (made from the whole),
 // and the sum below it. Only threads with a sum are asked, as rounding may lift the running sum over one without.
 // If none passes, the last thread with a sum; -1 if there is none.
-template <typename F>
-__device__ __forceinline__ int find_owner(double sum, F target_of, double *target, double *base, Block &s, int tid) {
+template <int W, typename F>
+__device__ __forceinline__ int find_owner(double sum, F target_of, double *target, double *base, Block<W> &s, int tid) {
   const int lane = tid & 63, wave = tid >> 6;
-  const double up = wave_scan_f64(sum, lane);
+  const double up = wave_scan_f64(sum);
   if (tid == 0) s.owner = -1;
   if (lane == 63) s.wave[wave] = up;
   __syncthreads();
   double below = 0.0, total = 0.0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w == wave) below = total;
     total += s.wave[w];
   }
   *target = target_of(total);
   const uint64_t some = __ballot(sum > 0.0), passed = __ballot(sum > 0.0 && below + up > *target);
-  if (lane == 0 && passed != 0) atomicMax(&s.owner, (1 << 20) + (NT - 1 - (64 * wave + __ffsll((long long)passed) - 1)));
+  if (lane == 0 && passed != 0) atomicMax(&s.owner, (1 << 20) + (64 * W - 1 - (64 * wave + __ffsll((long long)passed) - 1)));
   if (lane == 0 && some != 0) atomicMax(&s.owner, 64 * wave + 63 - __clzll((long long)some));
   __syncthreads();
   const int o = s.owner;
-  const int owner = o >= 1 << 20 ? NT - 1 - (o - (1 << 20)) : o;
+  const int owner = o >= 1 << 20 ? 64 * W - 1 - (o - (1 << 20)) : o;
   if (tid == owner) s.base = below + (up - sum);
   __syncthreads();
   *base = s.base;
@@ -294,10 +382,10 @@ __device__ __forceinline__ int find_owner(double sum, F target_of, double *targe
   return owner;
 }
 
-// The first of a thread's n numbers whose running sum from `base` passes target, else the last above 0, else `none`
+// The first of n numbers whose running sum from `base` passes target, else the last above 0, else 0; and the sum below it
 template <typename F>
-__device__ __forceinline__ int find_at(int n, double *base, double target, F value, int none) {
-  int got = none;
+__device__ __forceinline__ int find_at(int n, double *base, double target, F value) {
+  int got = 0;
   double run = *base;
   for (int i = 0; i < n; ++i) {
     const double v = value(i);
@@ -310,48 +398,78 @@ __device__ __forceinline__ int find_at(int n, double *base, double target, F val
   return got;
 }
 
-// The token of a row whose spans have the sums span_sum(s): the place of u times their sum, found again among
-// the weights(col, e) of that span's logits.
-template <typename T, typename F, typename G>
-__device__ __forceinline__ int draw(const Cut<T> &cut, double u, F span_sum, G weight, double *whole, Block &s, int tid) {
+// The token of a row whose `spans` spans of `pieces` pieces have the sums span_sum(s): the place of u times their sum,
+// found again among the weights of that span's logits, a piece a thread (weigh(piece, w): the weights of its columns, 0
+// past the last).
+template <typename T, int W, typename F, typename G>
+__device__ __forceinline__ int draw(int spans, int pieces, double u, F span_sum, G weigh, double *whole, Block<W> &s, int tid) {
   constexpr int E = Cut<T>::E;
-  const int each = (cut.spans + NT - 1) / NT, s0 = tid * each, n = clampi(cut.spans - s0, 0, each);
+  const int each = (spans + 64 * W - 1) / (64 * W), s0 = tid * each, n = clampi(spans - s0, 0, each);
   double sum = 0.0;
   for (int i = 0; i < n; ++i) sum += span_sum(s0 + i);
   double target, base;
   int owner = find_owner(sum, [&](double total) { *whole = total; return u * total; }, &target, &base, s, tid);
   if (owner < 0) return -1;  // no weight at all
   if (tid == owner) {
-    s.found = s0 + find_at(n, &base, target, [&](int i) { return span_sum(s0 + i); }, 0);
+    s.found = s0 + find_at(n, &base, target, [&](int i) { return span_sum(s0 + i); });
     s.base = base;
   }
   __syncthreads();
   const int span = s.found;
   const double below = s.base;
   __syncthreads();
-  // a piece a thread, the row's last logits with the last piece
-  const int first = span * kSpanPieces, here = min(cut.pieces - first, kSpanPieces);
-  const int col = (first + tid) * E;
-  int m = tid < here ? E : 0;
-  if (span == cut.spans - 1 && tid == max(here - 1, 0)) m = cut.cols - col;
+  double w[E];
   sum = 0.0;
-  for (int i = 0; i < m; ++i) sum += weight(col + i);
+  if (tid < pieces) {
+    weigh(span * pieces + tid, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+  }
   owner = find_owner(sum, [&](double) { return target - below; }, &target, &base, s, tid);
   if (owner < 0) return -1;
-  if (tid == owner) s.found = col + find_at(m, &base, target, [&](int i) { return weight(col + i); }, 0);
+  if (tid == owner) {
+    // the first whose running sum passes, else the last with a weight
+    int got = 0;
+    bool passed = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (!passed && w[e] > 0.0) {
+        got = e;
+        base += w[e];
+        passed = base > target;
+      }
+    }
+    s.found = (span * pieces + tid) * E + got;
+  }
   __syncthreads();
   return s.found;
 }
 
-// a row's largest logit; its first column for rows that take it
+// The logits of a piece, and the bits of those that count
 template <typename T>
-__device__ __forceinline__ float row_max(const Span *spans, const Cut<T> &cut, bool greedy, int *col, Block &s, int tid) {
+__device__ __forceinline__ uint32_t piece_of(const T *x, int piece, const Cut<T> &cut, const uint32_t *suppress, float (&v)[Cut<T>::E]) {
+  constexpr int E = Cut<T>::E;
+  if (piece < cut.full) {
+    const uint4 w = load_piece(x + (int64_t)piece * E);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = Logit<T>::get(w, e);
+    return ~hidden_bits(suppress, piece * E, E, cut.cols);
+  }
+  const int left = max(cut.cols - piece * E, 0);  // fewer than E
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = e < left ? Logit<T>::one(x + (int64_t)piece * E + e) : 0.f;
+  return left > 0 ? ~hidden_bits(suppress, piece * E, E, cut.cols) & ((1u << left) - 1u) : 0u;
+}
+
+// a row's largest logit; its first column for rows that take it
+template <typename T, int W>
+__device__ __forceinline__ float row_max(const Span *spans, const Cut<T> &cut, bool greedy, int *col, Block<W> &s, int tid) {
   uint32_t top = 0;
-  for (int i = tid; i < cut.spans; i += NT) top = max(top, ordered(spans[i].m));
+  for (int i = tid; i < cut.spans; i += 64 * W) top = max(top, ordered(spans[i].m));
   top = block_max(top, s, tid);
   if (greedy) {
     uint32_t c = 0;
-    for (int i = tid; i < cut.spans; i += NT)
+    for (int i = tid; i < cut.spans; i += 64 * W)
       if (ordered(spans[i].m) == top) c = max(c, ~(uint32_t)spans[i].col);
     *col = (int)~block_max(c, s, tid);
   }
@@ -370,13 +488,13 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
   using L = Logit<T>;
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   __shared__ double sTable[I8 ? 256 : 1];
-  __shared__ Block s;
+  __shared__ Block<kWaves> s;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const Cut<T> cut(a.cols);
-  const Row dist(a.d, row / a.d.inner);
+  const Row dist(a.d, row);
   const Span *spans = static_cast<const Span *>(a.workspace) + row * cut.spans;
-  const T *x = row_of<T>(a.d, row);
+  const T *x = row_of<T>(a.d, row, 0);
   if (I8) fill_table(sTable, dist.c, tid);
   int tok = -1;
   const float m = row_max(spans, cut, dist.greedy, &tok, s, tid);
@@ -387,9 +505,14 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
   } else if (!dist.greedy) {
     const Weigh wt(dist.c, m, sTable);
     double z = 0.0;
-    tok = draw(cut, (double)clamp_uniform(a.uniforms[row]),
-               [&](int i) { return span_sum(spans[i], wt); },
-               [&](int col) { return suppressed(a.suppress, col) ? 0.0 : wt.of<T>(L::one(x + col)); }, &z, s, tid);
+    tok = draw<T>(cut.spans, kSpanPieces, (double)clamp_uniform(a.uniforms[row]), [&](int i) { return span_sum(spans[i], wt); },
+               [&](int piece, double (&w)[L::E]) {
+                 float v[L::E];
+                 const uint32_t on = piece_of(x, piece, cut, a.suppress, v);
+#pragma unroll
+                 for (int e = 0; e < L::E; ++e) w[e] = (on >> e) & 1u ? wt.of<T>(v[e]) : 0.0;
+               },
+               &z, s, tid);
     if (tid == 0) lp = (float)(wt.log2_of(L::one(x + tok)) * kLn2 - log(z));
   }
   if (tid == 0) {
@@ -415,22 +538,24 @@ struct RowSum {
   double z;
 };
 __device__ __forceinline__ RowSum row_sum(const Span *spans, int n, const Row &dist, int lane) {
-  uint32_t top = 0;
-  for (int i = lane; i < n; i += 64) top = max(top, ordered(spans[i].m));
+  const Span none{-INFINITY, -1, 0.0};
+  Span mine = lane < n ? spans[lane] : none;  // all of a row of 64 spans, the others are read again
+  uint32_t top = ordered(mine.m);
+  for (int i = lane + 64; i < n; i += 64) top = max(top, ordered(spans[i].m));
   top = wave_max_u32_dpp(top);
   RowSum r;
   r.m = key_value((uint64_t)top << 32);
   r.col = -1;
   r.z = 1.0;
   if (dist.greedy) {
-    uint32_t c = 0;
-    for (int i = lane; i < n; i += 64)
+    uint32_t c = lane < n && ordered(mine.m) == top ? ~(uint32_t)mine.col : 0u;
+    for (int i = lane + 64; i < n; i += 64)
       if (ordered(spans[i].m) == top) c = max(c, ~(uint32_t)spans[i].col);
     r.col = (int32_t)~wave_max_u32_dpp(c);
   } else {
     const Weigh wt(dist.c, r.m, nullptr);
-    double z = 0.0;
-    for (int i = lane; i < n; i += 64) z += span_sum(spans[i], wt);
+    double z = span_sum(mine, wt);
+    for (int i = lane + 64; i < n; i += 64) z += span_sum(spans[i], wt);
     r.z = wave_sum_f64(z);
   }
   return r;
@@ -459,7 +584,7 @@ __device__ __forceinline__ double share_of(const T *x, int64_t col, int cols, co
 
 struct VerifyWork {
   Span *spans;      // of the target's rows, then of the draft's
-  double *rest;     // [batch][spans]
+  double *rest;     // [batch][parts]
   Verdict *verdict;
 };
 template <typename T>
@@ -471,42 +596,47 @@ __device__ __forceinline__ VerifyWork verify_work(const VerifyArgs &a, const Cut
   return w;
 }
 
-// One block per batch row, its waves take the nodes in turn.
-template <typename T>
-__global__ __launch_bounds__(NT) void verify_decide_kernel(VerifyArgs a) {
-  __shared__ RowSum sP[kVerifyMaxNodes], sQ[kVerifyMaxNodes];
-  __shared__ int sOk[kVerifyMaxNodes];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t b = blockIdx.x;
-  const Cut<T> cut(a.cols);
-  const VerifyWork w = verify_work(a, cut);
+// The first rejection of batch row b: the waves of its block take the target's and the draft's rows in turn.
+template <int W>
+struct Nodes {
+  RowSum p[kVerifyMaxNodes], q[kVerifyMaxNodes];
+  Verdict verdict;
+};
+template <typename T, int W>
+__device__ __forceinline__ void decide(const VerifyArgs &a, const VerifyWork &w, const Cut<T> &cut, int64_t b, Nodes<W> &s, int tid) {
+  const int lane = tid & 63;
   const int N = a.nodes, cnt = a.counts ? clampi(a.counts[b], 0, N) : N;
   const Row dp(a.target, b), dq(a.draft, b);
-  for (int i = tid >> 6; i < cnt; i += kWaves) {
-    const int64_t row = b * N + i, drow = b * (N - 1) + i;
-    const RowSum p = row_sum(w.spans + row * cut.spans, cut.spans, dp, lane);
-    RowSum q{0.f, -1, 1.0};
-    bool ok = false;
-    if (i + 1 < cnt) {
-      const int64_t x = a.tokens[row + 1];
-      const double px = share_of(row_of<T>(a.target, row), x, a.cols, a.suppress, dp, p);
-      double qx = 1.0;
-      if (a.draft.x) {
-        q = row_sum(w.spans + (a.batch * N + drow) * cut.spans, cut.spans, dq, lane);
-        qx = share_of(row_of<T>(a.draft, drow), x, a.cols, a.suppress, dq, q);
-        if (!(q.m - q.m == 0.f)) qx = __longlong_as_double(0x7ff8000000000000ll);  // a draft without a distribution
-      }
-      ok = p.m - p.m == 0.f && (double)clamp_uniform(a.uniforms[row]) * qx < px;
-    }
-    if (lane == 0) sP[i] = p, sQ[i] = q, sOk[i] = ok;
+  const int drafts = a.draft.x ? cnt - 1 : 0;
+  for (int i = __builtin_amdgcn_readfirstlane(tid >> 6); i < cnt + drafts; i += W) {
+    const bool second = i >= cnt;
+    const int64_t row = second ? a.batch * N + b * (N - 1) + (i - cnt) : b * N + i;
+    const RowSum r = row_sum(w.spans + row * cut.spans, cut.spans, second ? dq : dp, lane);
+    if (lane == 0) (second ? s.q[i - cnt] : s.p[i]) = r;
   }
   __syncthreads();
+  if (tid >= 64) return;
+  // a lane a draft: whether it is accepted
+  bool ok = false;
+  if (tid + 1 < cnt) {
+    const int64_t row = b * N + tid;
+    const int64_t x = a.tokens[row + 1];
+    const RowSum p = s.p[tid];
+    const double px = share_of(row_of<T>(a.target, b, tid), x, a.cols, a.suppress, dp, p);
+    double qx = 1.0;
+    bool has = true;
+    if (a.draft.x) {
+      const RowSum q = s.q[tid];
+      qx = share_of(row_of<T>(a.draft, b, tid), x, a.cols, a.suppress, dq, q);
+      has = q.m - q.m == 0.f;  // else a draft without a distribution
+    }
+    ok = has && p.m - p.m == 0.f && (double)clamp_uniform(a.uniforms[row]) * qx < px;
+  }
+  const int n = min((int)__popcll(__ballot(ok) & ~(__ballot(ok) + 1ull)), max(cnt - 1, 0));
   if (tid != 0) return;
-  int n = 0;
-  while (n + 1 < cnt && sOk[n]) ++n;
   Verdict v{n, NONE, -1, 0.f, 0.f, dp.c, dq.c, 0.0, 0.0};
-  if (cnt > 0 && sP[n].m - sP[n].m == 0.f) {
-    const RowSum p = sP[n], q = sQ[n];
+  if (cnt > 0 && s.p[n].m - s.p[n].m == 0.f) {
+    const RowSum p = s.p[n];
     v.mode = FROM_TARGET;
     v.m = p.m;
     v.ip = 1.0 / p.z;
@@ -514,15 +644,21 @@ __global__ __launch_bounds__(NT) void verify_decide_kernel(VerifyArgs a) {
       v.mode = CERTAIN;
       v.hot = p.col;
     } else if (n + 1 < cnt) {
-      if (a.draft.x && !dq.greedy) {
-        if (q.m - q.m == 0.f) v.mode = FROM_REST, v.mq = q.m, v.iq = 1.0 / q.z;
+      if (a.draft.x) {
+        const RowSum q = s.q[n];
+        if (q.m - q.m == 0.f) {
+          if (dq.greedy)
+            v.mode = FROM_OTHERS, v.hot = q.col;
+          else
+            v.mode = FROM_REST, v.mq = q.m, v.iq = 1.0 / q.z;
+        }
       } else {
-        const int64_t x = a.draft.x ? q.col : a.tokens[b * N + n + 1];
-        if (!a.draft.x || q.m - q.m == 0.f) v.mode = FROM_OTHERS, v.hot = x >= 0 && x < a.cols ? (int32_t)x : -1;
+        const int64_t x = a.tokens[b * N + n + 1];
+        v.mode = FROM_OTHERS, v.hot = x >= 0 && x < a.cols ? (int32_t)x : -1;
       }
     }
   }
-  w.verdict[b] = v;
+  s.verdict = v;
 }
 
 // What is left of the weight of the token at col: its value in the model's row, and in the draft's
@@ -534,92 +670,90 @@ struct Rest {
   int mode, hot;
   const uint32_t *suppress;
   __device__ __forceinline__ Rest(const VerifyArgs &a, const Verdict &v, int64_t b, const double *tp, const double *tq)
-      : x(row_of<T>(a.target, b * a.nodes + v.accepted)), y(x), p(v.c, v.m, tp), q(v.cq, v.mq, tq), ip(v.ip), iq(v.iq),
+      : x(row_of<T>(a.target, b, v.accepted)), y(x), p(v.c, v.m, tp), q(v.cq, v.mq, tq), ip(v.ip), iq(v.iq),
         mode(v.mode), hot(v.hot), suppress(a.suppress) {
-    if (mode == FROM_REST) y = row_of<T>(a.draft, b * (a.nodes - 1) + v.accepted);
+    if (mode == FROM_REST) y = row_of<T>(a.draft, b, v.accepted);
   }
   __device__ __forceinline__ double of(float xv, float yv, int col) const {
     const double w = share(p.of<T>(xv), ip);
     if (mode == FROM_REST) return left_of(w, share(q.of<T>(yv), iq));
     return mode == FROM_OTHERS && col == hot ? 0.0 : w;
   }
-  __device__ __forceinline__ double at(int col) const {
-    if (suppressed(suppress, col)) return 0.0;
-    return of(Logit<T>::one(x + col), mode == FROM_REST ? Logit<T>::one(y + col) : 0.f, col);
+  __device__ __forceinline__ void piece(int at, const Cut<T> &cut, double (&w)[Cut<T>::E]) const {
+    float xv[Cut<T>::E], yv[Cut<T>::E];
+    const uint32_t on = piece_of(x, at, cut, suppress, xv);
+    if (mode == FROM_REST) piece_of<T>(y, at, cut, nullptr, yv);
+#pragma unroll
+    for (int e = 0; e < Cut<T>::E; ++e) w[e] = (on >> e) & 1u ? of(xv[e], mode == FROM_REST ? yv[e] : 0.f, at * Cut<T>::E + e) : 0.0;
   }
 };
 
+constexpr int kDecideWaves = 16;
+template <typename T>
+__global__ __launch_bounds__(64 * kDecideWaves) void verify_decide_kernel(VerifyArgs a) {
+  __shared__ Nodes<kDecideWaves> sNodes;
+  const Cut<T> cut(a.cols);
+  const VerifyWork work = verify_work(a, cut);
+  decide<T, kDecideWaves>(a, work, cut, blockIdx.x, sNodes, threadIdx.x);
+  if (threadIdx.x == 0) work.verdict[blockIdx.x] = sNodes.verdict;
+}
+
+// The sums of what is left of a row over 64 pieces, a piece a lane
 template <typename T>
 __global__ __launch_bounds__(NT) void verify_rest_kernel(VerifyArgs a, int groups) {
-  using L = Logit<T>;
   constexpr bool I8 = std::is_same<T, int8_t>::value;
-  constexpr int E = L::E, P = kSpanPieces / 64;
   __shared__ double sP[I8 ? 256 : 1], sQ[I8 ? 256 : 1];
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x;
   const int64_t b = (uint32_t)blockIdx.x / (uint32_t)groups;
   const Cut<T> cut(a.cols);
-  const VerifyWork w = verify_work(a, cut);
-  const Verdict v = w.verdict[b];
+  const VerifyWork work = verify_work(a, cut);
+  const Verdict v = work.verdict[b];
   if (v.mode != FROM_REST && v.mode != FROM_OTHERS) return;
   if (I8) {
     fill_table(sP, v.c, tid);
-    fill_table(sQ, v.cq, tid);
+    if (v.mode == FROM_REST) fill_table(sQ, v.cq, tid);
     lds_barrier();
   }
-  const int s = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (s >= cut.spans) return;
-  const Rest<T> rest(a, v, b, sP, sQ);
-  double z = 0.0;
+  const int i = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (i >= cut.parts) return;
+  double w[Cut<T>::E], z = 0.0;
+  Rest<T>(a, v, b, sP, sQ).piece(64 * i + (tid & 63), cut, w);
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int at = s * kSpanPieces + 64 * p + lane;
-    if (at < cut.pieces) {
-      const uint4 xp = load_piece(rest.x + (int64_t)at * E), yp = load_piece(rest.y + (int64_t)at * E);
-      const uint32_t off = hidden_bits(a.suppress, at * E, E, a.cols);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const double one = rest.of(L::get(xp, e), L::get(yp, e), at * E + e);
-        z += (off >> e) & 1u ? 0.0 : one;
-      }
-    }
-  }
-  const int extra = cut.pieces * E + lane;
-  if (s == cut.spans - 1 && extra < a.cols) z += rest.at(extra);
+  for (int e = 0; e < Cut<T>::E; ++e) z += w[e];
   z = wave_sum_f64(z);
-  if (lane == 0) w.rest[b * cut.spans + s] = z;
+  if ((tid & 63) == 0) work.rest[b * cut.parts + i] = z;
 }
 
+// The token after the accepted drafts
 template <typename T>
 __global__ __launch_bounds__(NT) void verify_pick_kernel(VerifyArgs a) {
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   __shared__ double sP[I8 ? 256 : 1], sQ[I8 ? 256 : 1];
-  __shared__ Block s;
-  const int tid = threadIdx.x;
+  __shared__ Block<kWaves> s;
+  const int tid = threadIdx.x, N = a.nodes;
   const int64_t b = blockIdx.x;
   const Cut<T> cut(a.cols);
-  const VerifyWork w = verify_work(a, cut);
-  Verdict v = w.verdict[b];
-  const int N = a.nodes;
+  const VerifyWork work = verify_work(a, cut);
+  Verdict v = work.verdict[b];
   if (I8) {
     fill_table(sP, v.c, tid);
-    fill_table(sQ, v.cq, tid);
+    if (v.mode == FROM_REST) fill_table(sQ, v.cq, tid);
     __syncthreads();
   }
   int tok = v.mode == CERTAIN ? v.hot : -1;
   const double u = (double)clamp_uniform(a.uniforms[b * N + N - 1]);
-  double whole;
-  if (v.mode == FROM_REST || v.mode == FROM_OTHERS) {
+  const double *rests = work.rest + b * cut.parts;
+  const Span *spans = work.spans + (b * N + v.accepted) * cut.spans;
+  while (v.mode == FROM_TARGET || v.mode == FROM_REST || v.mode == FROM_OTHERS) {
+    const bool target = v.mode == FROM_TARGET;
     const Rest<T> rest(a, v, b, sP, sQ);
-    const double *sums = w.rest + b * cut.spans;
-    tok = draw(cut, u, [&](int i) { return sums[i]; }, [&](int col) { return rest.at(col); }, &whole, s, tid);
-    if (tok < 0) v.mode = FROM_TARGET;  // nothing is left: both are the same, or the draft is no token
+    double whole;
+    tok = draw<T>(target ? cut.spans : cut.parts, target ? kSpanPieces : 64, u,
+                  [&](int i) { return target ? rest.ip * span_sum(spans[i], rest.p) : rests[i]; },
+                  [&](int at, double (&w)[Cut<T>::E]) { rest.piece(at, cut, w); }, &whole, s, tid);
+    if (tok >= 0 || target) break;
+    v.mode = FROM_TARGET;  // nothing is left: both are the same, or the draft is no token
     __syncthreads();
-  }
-  if (v.mode == FROM_TARGET) {
-    const Rest<T> rest(a, v, b, sP, sQ);
-    const Span *spans = w.spans + (b * N + v.accepted) * cut.spans;
-    tok = draw(cut, u, [&](int i) { return rest.ip * span_sum(spans[i], rest.p); },
-               [&](int col) { return rest.at(col); }, &whole, s, tid);
   }
   if (tid < N) {
     int64_t c = -1;
@@ -667,12 +801,13 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
   sp.spans = reinterpret_cast<Span *>(static_cast<Verdict *>(a.workspace) + a.batch);
   int rc = launch_spans<T>(sp, a.batch * (a.draft.x ? 2 * a.nodes - 1 : a.nodes), s);
   if (rc) return rc;
-  hipLaunchKernelGGL((verify_decide_kernel<T>), dim3((unsigned)a.batch), dim3(NT), 0, s, a);
+  hipLaunchKernelGGL((verify_decide_kernel<T>), dim3((unsigned)a.batch), dim3(64 * kDecideWaves), 0, s, a);
   rc = check_launch("verify_decide_kernel");
   if (rc) return rc;
-  const int groups = (Cut<T>(a.cols).spans + kWaves - 1) / kWaves;
   if (a.nodes > 1) {  // a row of one node has nothing to reject
-    hipLaunchKernelGGL((verify_rest_kernel<T>), dim3((unsigned)(a.batch * groups)), dim3(NT), 0, s, a, groups);
+    const int64_t groups = (Cut<T>(a.cols).parts + kWaves - 1) / kWaves;
+    if (a.batch * groups >= (1LL << 32) / NT) return fail("too many logits for one call");
+    hipLaunchKernelGGL((verify_rest_kernel<T>), dim3((unsigned)(a.batch * groups)), dim3(NT), 0, s, a, (int)groups);
     rc = check_launch("verify_rest_kernel");
     if (rc) return rc;
   }
@@ -680,23 +815,32 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
   return check_launch("verify_pick_kernel");
 }
 
-int64_t spans_of(int type, int64_t cols) {
+struct Sizes {
+  int64_t spans, parts;
+};
+template <typename T>
+Sizes sizes(int64_t cols) {
+  const Cut<T> cut((int)cols);
+  return Sizes{cut.spans, cut.parts};
+}
+Sizes sizes_of(int type, int64_t cols) {
   switch (type) {
-    case LOGIT_I8: return Cut<int8_t>((int)cols).spans;
-    case LOGIT_F32: return Cut<float>((int)cols).spans;
-    default: return Cut<__half>((int)cols).spans;
+    case LOGIT_I8: return sizes<int8_t>(cols);
+    case LOGIT_F32: return sizes<float>(cols);
+    default: return sizes<__half>(cols);
   }
 }
 
 }  // namespace
 
 int64_t sample_workspace(int type, int64_t rows, int64_t cols) {
-  return rows * spans_of(type, cols) * (int64_t)sizeof(Span);
+  return rows * sizes_of(type, cols).spans * (int64_t)sizeof(Span);
 }
 
 int64_t verify_workspace(int type, int64_t batch, int64_t nodes, int64_t cols, bool draft) {
-  const int64_t rows = draft ? 2 * nodes - 1 : nodes, spans = spans_of(type, cols);
-  return batch * ((int64_t)sizeof(Verdict) + rows * spans * (int64_t)sizeof(Span) + spans * 8);
+  const int64_t rows = draft ? 2 * nodes - 1 : nodes;
+  const Sizes n = sizes_of(type, cols);
+  return batch * ((int64_t)sizeof(Verdict) + rows * n.spans * (int64_t)sizeof(Span) + n.parts * 8);
 }
 
 int launch_sample_tokens(const SampleArgs &a, hipStream_t s) {

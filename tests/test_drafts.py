@@ -301,11 +301,12 @@ def weights(x, scale, t, suppress=()):
 
 
 def drawn_by(tok, w, u, scale_of=1.0):
-    """tok is the token that u draws from w. A weight is off by its exponent's rounding (|t| 2^t 2^-52, t = log2 w) and
-    6e-15, a sum by one rounding a term: a border by less than (V + 100) 2^-52 of the whole."""
+    """tok is the token that u draws from w. A weight is off by 7.8e-13 of itself (the polynomial) and its exponent's
+    rounding (|t| 2^t 2^-52 < 2^-52 of the largest, t = log2 w), a sum by one rounding a term: a border and the whole that
+    it is a share of by less than 2 * 7.8e-13 + (V + 100) 2^-52 of the whole."""
     u = min(max(float(u), 0.0), 1 - 2.0 ** -24)
     c = np.cumsum(w)
-    room = (len(w) + 100) * 2.0 ** -52 * scale_of
+    room = (2 * 7.8e-13 + (len(w) + 100) * 2.0 ** -52) * scale_of
     assert 0 <= tok < len(w) and w[tok] > 0, tok
     assert c[tok] - w[tok] <= u * c[-1] + room and c[tok] > u * c[-1] - room, (tok, c[tok], u * c[-1])
 
