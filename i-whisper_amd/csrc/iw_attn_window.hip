@@ -38,6 +38,8 @@ __device__ __forceinline__ Seen seen_from(const WindowArgs &t, int len, int64_t 
 // the lowest n bits of 16, n clamped to [0, 16]
 __device__ __forceinline__ uint32_t low_bits(int n) { return (1u << clampi(n, 0, 16)) - 1u; }
 
+__device__ __forceinline__ uint32_t low4(int n) { return (1u << clampi(n, 0, 4)) - 1u; }
+
 // Minimum and maximum over the 16 lanes of a DPP row, in every lane of it
 __device__ __forceinline__ int row16_max(int v) {
   v = max(v, __builtin_amdgcn_update_dpp(INT32_MIN, v, 0xB1, 0xf, 0xf, false));
@@ -47,11 +49,116 @@ __device__ __forceinline__ int row16_max(int v) {
 }
 __device__ __forceinline__ int row16_min(int v) { return ~row16_max(~v); }
 
-// KS: 64-column parts of the head; QUADS: V in key quads; QT: 16-query tiles of the block; NW waves.
-template <int KS, bool QUADS, int QT, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_window_kernel(WindowArgs t, int qblocks, int blocks, int per_xcd,
-                                                              int per_word, int table_off) {
-  constexpr int QR = 16 * QT, OLD = 64 * KS + 4;
+// The score where bit i of `hidden` is 0, else INT32_MIN. The bit spread over the word is opaque to the compiler,
+// which makes a compare and a select of each otherwise (the score comes from a matrix instruction, so that the
+// instruction which reads it has to be the compiler's).
+__device__ __forceinline__ int32_t hide(int32_t score, uint32_t hidden, int i) {
+  int32_t no;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(no) : "v"(hidden), "n"(i));
+  return (no & INT32_MIN) | (~no & score);
+}
+
+// The bytes of w whose bit of the four is set, 0 in the others: a byte permute gives 0 for a selector of 12, 0xff
+// for 13
+__device__ __forceinline__ uint32_t keep_bytes(uint32_t w, uint32_t four) {
+  const uint32_t sel = (__umul24(four, 0x00204081u) & 0x01010101u) | 0x0c0c0c0cu;
+  return w & __builtin_amdgcn_perm(w, w, sel);
+}
+
+// Four bytes as a word
+__device__ __forceinline__ uint32_t pack4(uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0c0c0400u), __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u),
+                               0x05040100u);
+}
+
+// The last steps of a row: sums * inv, twice, and the output's scale, each rounded. Products of 24-bit numbers take
+// a quarter of a 32-bit one's time: the first shift leaves 24 bits where it is 8 or more, and the second 24 - 8.
+struct Finish {
+  bool brief;  // the shifts allow it
+  int32_t off, av_s, av_m, off_half, av_half;
+  __device__ __forceinline__ explicit Finish(const AttnArgs &a)
+      : brief(a.rsqrt_off >= 8 && a.av_s >= 1 && a.av_s <= 31), off((int32_t)a.rsqrt_off), av_s((int32_t)a.av_s),
+        av_m((int32_t)a.av_m), off_half(a.rsqrt_off ? 1 << (a.rsqrt_off - 1) : 0), av_half(a.av_s >= 1 && a.av_s <= 31 ? 1 << (a.av_s - 1) : 0) {}
+  static __device__ __forceinline__ int32_t shift(int32_t x, int32_t half, int32_t s) {
+    return (int32_t)((uint32_t)x + (uint32_t)half + (uint32_t)(x >> 31)) >> s;
+  }
+  __device__ __forceinline__ uint32_t word(const AttnArgs &a, const uint32_t *sums, int32_t inv, bool fast) const {
+    if (!fast) return output_word(a, sums, inv);
+    uint32_t b[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      int32_t y = shift((int32_t)(sums[c] * (uint32_t)inv), off_half, off);
+      y = shift(__mul24(y, inv), off_half, off);
+      y = shift(__mul24(y, av_m), av_half, av_s);
+      b[c] = (uint32_t)clampi(y, -127, 127);
+    }
+    return pack4(b[0], b[1], b[2], b[3]);
+  }
+};
+
+// Row q from element r of a lane's products, four columns of each
+template <int KS>
+__device__ __forceinline__ void finish_row(const WindowArgs &t, const Finish &fin, int8_t *obase, int q, int cnt,
+                                           const v4i (&o)[KS][4], int r, int32_t inv, bool fast, int n) {
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const uint32_t sums[4] = {(uint32_t)o[ks][0][r], (uint32_t)o[ks][1][r], (uint32_t)o[ks][2][r], (uint32_t)o[ks][3][r]};
+    const uint32_t w = fin.word(t.a, sums, inv, fast);
+    const int d = 64 * ks + 4 * n;
+    if (q < t.a.Tq && d < t.a.D) *reinterpret_cast<uint32_t *>(obase + (int64_t)q * t.a.o_st + d) = q < cnt ? w : 0u;
+  }
+}
+
+constexpr int rows_waves(int ks, int qt) { return ks * qt <= 2 ? 4 : 2; }
+
+// The chunks of 64 keys that any of the 16 queries of a tile sees: the first ns hold first keys, the others follow
+// one another from w0 on. And the keys that all of them see.
+struct Tile {
+  int ns, w0, nch, start, end, first, all_from, all_to;
+  __device__ __forceinline__ int at(int c) const { return c < ns ? c : w0 + c - ns; }
+  __device__ __forceinline__ bool whole(int kc) const { return 64 * kc >= all_from && 64 * kc + 64 <= all_to; }
+  // The first and last key of the chunk at kc that any of them sees: no others are read (2560 heads of 128: one query a
+  // tile, 128 keys and four first ones, 16.3 us with whole chunks, 15.6 so; 257 frames, 35.8 and 31.4).
+  __device__ __forceinline__ int low(int kc) const { return 64 * kc < first ? 0 : max(start - 64 * kc, 0); }
+  __device__ __forceinline__ int high(int kc) const { return min((kc < w0 ? first : end) - 64 * kc, 64) - 1; }
+};
+// the tile at q0 < cnt, lane n & 15 has query q0 + n (queries past the count repeat the last one)
+__device__ __forceinline__ Tile tile_of(const WindowArgs &t, int64_t b, int len, int cnt, int q, int sinks, Seen &seen) {
+  const int64_t p = t.positions ? (int64_t)t.positions[b * t.pos_sb + q] : (int64_t)len - cnt + q;
+  seen = seen_from(t, len, p);
+  const int start = __builtin_amdgcn_readfirstlane(row16_min(seen.start));
+  const int end = __builtin_amdgcn_readfirstlane(row16_max(seen.end));
+  Tile x;
+  x.start = start, x.end = end, x.first = min(sinks, end);
+  x.all_from = __builtin_amdgcn_readfirstlane(row16_max(seen.start));
+  x.all_to = __builtin_amdgcn_readfirstlane(row16_min(seen.end));
+  x.w0 = min(start, end) / 64;
+  x.ns = min((min(sinks, end) + 63) / 64, x.w0);
+  x.nch = x.ns + max(0, (end + 63) / 64 - x.w0);
+  return x;
+}
+
+// Where several blocks share the chunks of a tile: a part's words in the workspace are the sums of P.V of its rows,
+// those of P, the row maxima. Every part but the last has as many chunks, the last ones may have none.
+constexpr int part_words(int ks) { return 16 * (64 * ks + 2); }
+template <int KS>
+__device__ __forceinline__ uint32_t *part_of(const WindowArgs &t, int64_t block, int part, int parts) {
+  return t.workspace + (block * parts + part) * part_words(KS);
+}
+__device__ __forceinline__ int part_share(int nch, int parts) { return max(1, (nch + parts - 1) / parts); }
+
+// Of all keys, or of blockIdx.y's part of them: the row maxima, or with every part's maxima the sums
+enum { ALL, PART_MAX, PART_SUM };
+
+// Few queries, or positions in any order: a block has one tile, its waves take the chunks in turn. KS: 64-column parts
+// of the head; QUADS: V in key quads; NW waves; NC > 0: a wave has at most NC chunks, whose K and V are all requested at the
+// start and kept.
+constexpr int window_waves(int ks, int nc) { return ks * (nc > 0 ? nc : 1) == 1 ? 4 : ks * nc <= 2 ? 3 : 2; }
+template <int KS, bool QUADS, int NW, int NC, int MODE>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(window_waves(KS, NC)))) void attn_window_kernel(
+    WindowArgs t, int qblocks, int blocks, int per_xcd, int per_word, int table_off) {
+  constexpr int QR = 16, OLD = 64 * KS + 4, HC = NC > 0 ? NC : 1;
+  static_assert(MODE == ALL || NC == 0, "parts loop over their chunks");
   __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
   __shared__ int32_t sMax[NW][QR];
   __shared__ uint32_t sSum[NW][QR];
@@ -75,28 +182,451 @@ __global__ __launch_bounds__(64 * NW) void attn_window_kernel(WindowArgs t, int 
   const int8_t *const vbase = a.vt + b * a.v_sb + (int64_t)h * a.v_sh;
   int8_t *const obase = a.out + b * a.o_sb + (int64_t)h * D;
   const int words = D / 4, rows = min(N - q0, QR);
-  // i / words for the i < 2^11 of the output
+  // i / words for the i < 2^9 of the output
   const auto by_words = [&](int i) { return (int)__umul24(i, per_word) >> 16; };
 
   if (q0 >= cnt) {  // no query of these is in use
+    if (MODE != ALL) return;
     for (int i = tid; i < rows * words; i += 64 * NW) {
       const int q = by_words(i);
       *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + q) * a.o_st + 4 * (i - q * words)) = 0u;
     }
     return;
   }
+  const int q = min(q0 + n, cnt - 1);
+  Seen seen;
+  const Tile tile = tile_of(t, b, len, cnt, q, t.sinks, seen);
+  const int parts = MODE == ALL ? 1 : (int)gridDim.y, part = MODE == ALL ? 0 : (int)blockIdx.y;
+  const int share = MODE == ALL ? tile.nch : part_share(tile.nch, parts);
+  const int c_lo = part * share, c_hi = min(c_lo + share, tile.nch);  // this block's chunks
+  if (MODE != ALL && part > 0 && c_lo >= tile.nch) return;
 
-  // ---- queries, what each sees, and what any and all of the block see ----
+  // The K operands of the chunk at kc: keys that no query sees repeat the next one that any does, head dims past D the
+  // last ones (the query is zero there). A chunk's base is uniform, its lanes' offsets fit 32 bits and are the same
+  // for every chunk of which all keys are read.
+  const int kcol = 16 * g, key0 = 16 * (n >> 2) + (n & 3);
+  uint32_t koff[KS], voff[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    koff[ks] = (uint32_t)key0 * (uint32_t)a.k_st + (uint32_t)min(64 * ks + kcol, D - 16);
+    const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
+    voff[ks] = QUADS ? (uint32_t)(4 * g) * (uint32_t)a.v_sq + 4 * d0 : d0 * (uint32_t)a.v_sd + (uint32_t)(16 * g);
+  }
+  auto load_k = [&](int kc, v4i (&f)[4][KS]) {
+    const int8_t *base = kbase + (int64_t)(64 * kc) * a.k_st;
+    const int low = tile.low(kc), high = tile.high(kc);
+    if (low == 0 && high == 63) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          f[i][ks] = *reinterpret_cast<const v4i *>(base + (int64_t)(4 * i) * a.k_st + koff[ks]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          f[i][ks] = *reinterpret_cast<const v4i *>(base + ((uint32_t)clampi(key0 + 4 * i, low, high) * (uint32_t)a.k_st +
+                                                            (uint32_t)min(64 * ks + kcol, D - 16)));
+    }
+  };
+  // Quads and transposed rows hold words of four keys of one column. Columns past D
+  // repeat the last ones; their sums are not stored.
+  auto load_v = [&](int kc, v4i (&f)[KS][4]) {
+    const int8_t *base = vbase + (QUADS ? (int64_t)(16 * kc) * a.v_sq : (int64_t)(64 * kc));
+    const int low = tile.low(kc), high = tile.high(kc);
+    if (low == 0 && high == 63) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          f[ks][i] = *reinterpret_cast<const v4i *>(base + (int64_t)i * (QUADS ? a.v_sq : a.v_sd) + voff[ks]);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          f[ks][i] = *reinterpret_cast<const v4i *>(
+              base + (QUADS ? (uint32_t)clampi(4 * g + i, low >> 2, high >> 2) * (uint32_t)a.v_sq + 4 * d0
+                            : (d0 + i) * (uint32_t)a.v_sd + (uint32_t)clampi(16 * g, low & ~15, high & ~15)));
+      }
+    }
+  };
+
+  // ---- everything that the start can ask for ----
+  v4i kf[HC][4][KS], vf[HC][KS][4], qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int d0 = 64 * ks + 16 * g;
+    qf[ks] = v4i{0, 0, 0, 0};
+    if (d0 < D) qf[ks] = *reinterpret_cast<const v4i *>(a.q + b * a.q_sb + (int64_t)q * a.q_st + (int64_t)h * D + d0);
+  }
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i < tile.nch) load_k(tile.at(wave + NW * i), kf[i]);
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i < tile.nch) load_v(tile.at(wave + NW * i), vf[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const bool table = table_off >= 0;
+  const int zero = table ? shift_exp_zero(a.frac_bits) : IW_SEXP_LUT - 1;
+  if (MODE != PART_MAX && table)
+    for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
+      *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
+
+  auto scores = [&](const v4i (&f)[KS]) {
+    v4i s{0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[ks], qf[ks], s, 0, 0, 0);
+    return s;
+  };
+  // which of the lane group's 16 keys of the chunk at kc this lane's query sees
+  auto counted = [&](int kc) -> uint32_t {
+    const int k0 = 64 * kc + 16 * g;
+    return (low_bits(seen.end - k0) & ~low_bits(seen.start - k0)) | low_bits(seen.first - k0);
+  };
+
+  // ---- pass 1: row maximum of the raw scores ----
+  int32_t mx = INT32_MIN;
+  auto chunk_max = [&](int kc, const v4i (&f)[4][KS]) {
+    v4i s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = scores(f[i]);
+    if (!tile.whole(kc)) {
+      const uint32_t off = ~counted(kc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] = hide(s[i][r], off, 4 * i + r);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx = max(max(max(mx, s[i][0]), s[i][1]), max(s[i][2], s[i][3]));
+  };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i < tile.nch) chunk_max(tile.at(wave + NW * i), kf[i]);
+  } else if constexpr (MODE != PART_SUM) {
+    v4i kn[4][KS];
+#pragma unroll 1
+    for (int c = c_lo + wave; c < c_hi; c += 2 * NW) {
+      load_k(tile.at(c), kf[0]);
+      if (c + NW < c_hi) load_k(tile.at(c + NW), kn);
+      chunk_max(tile.at(c), kf[0]);
+      if (c + NW < c_hi) chunk_max(tile.at(c + NW), kn);
+    }
+  }
+  if (MODE == PART_SUM)  // the maxima of the parts that have chunks, shared out to the waves' lane groups
+    for (int p = NW * g + wave; p == 0 || p * share < tile.nch; p += 4 * NW)
+      mx = max(mx, (int32_t)part_of<KS>(t, block, p, parts)[QR * (64 * KS + 1) + n]);
+  mx = max(mx, __shfl_xor(mx, 16));
+  mx = max(mx, __shfl_xor(mx, 32));
+  if (lane < 16) sMax[wave][lane] = mx;
+  lds_barrier();  // the table too
+#pragma unroll
+  for (int w = 0; w < NW; ++w) mx = max(mx, sMax[w][n]);
+  if constexpr (MODE == PART_MAX) {
+    if (tid < 16) part_of<KS>(t, block, part, parts)[QR * (64 * KS + 1) + tid] = (uint32_t)mx;
+    return;
+  }
+  // requantization keeps the order, so the maximum's is the maximum; a query without keys may have any
+  const int32_t rowmax = mx == INT32_MIN ? 0 : qk_requant16(mx, a.qk_m, a.qk_s);
+  // The short index where no row maximum wraps and none is so low that saturated scores are near it: the keys that
+  // count lie at a distance of 1 at least, the others are taken for such.
+  const bool brief = table && !__any(rowmax >= 32767 || rowmax < zero - 32768);
+
+  // ---- pass 2: P and P.V over this wave's keys ----
+  v4i o[KS][4];
+  uint32_t psum = 0u;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[ks][i] = v4i{0, 0, 0, 0};
+  // operand i of the products with V: column 64 ks + 4 n + i of the lane group's 16 keys
+  auto add_pv = [&](const v4i (&f)[KS][4], const v4i &x) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v4i v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = QUADS ? f[ks][j][i] : f[ks][i][j];
+        o[ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, v, o[ks][i], 0, 0, 0);
+      }
+  };
+  ScoreIndex ix(a, rowmax, zero);
+  ix.flo = 1, ix.fhi = zero;
+  auto chunk_brief = [&](int kc, const v4i (&f)[4][KS], const v4i (&v)[KS][4]) {
+    v4i s[4], p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = scores(f[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      p[i] = (int)pack4(sTable[ix.full(s[i][0])], sTable[ix.full(s[i][1])], sTable[ix.full(s[i][2])], sTable[ix.full(s[i][3])]);
+    if (!tile.whole(kc)) {
+      const uint32_t ok = counted(kc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = (int)keep_bytes((uint32_t)p[i], (ok >> (4 * i)) & 15u);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) psum = __builtin_amdgcn_udot4((uint32_t)p[i], 0x01010101u, psum, false);
+    add_pv(v, p);
+  };
+  // Any row maximum, any precision. A P of 128 (a row maximum of 32767 wraps) is too much for the signed product: the
+  // rest of it goes in twice.
+  auto chunk_any = [&](int kc, const v4i (&f)[4][KS], const v4i (&v)[KS][4]) {
+    const uint32_t ok = counted(kc);
+    v4i p, rest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const v4i s = scores(f[i]);
+      uint32_t w = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t d = ix.any(s[r]);
+        const uint32_t e = table ? (uint32_t)sTable[d] : shift_exp((int32_t)d, a.frac_bits);
+        w |= ((ok >> (4 * i + r)) & 1u ? e & 0xffu : 0u) << (8 * r);
+      }
+      psum = __builtin_amdgcn_udot4(w, 0x01010101u, psum, false);
+      p[i] = (int)(w & 0x7f7f7f7fu), rest[i] = (int)((w >> 1) & 0x40404040u);
+    }
+    add_pv(v, p);
+    add_pv(v, rest);
+    add_pv(v, rest);
+  };
+  auto all_chunks = [&](auto chunk) {
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (wave + NW * i < tile.nch) chunk(tile.at(wave + NW * i), kf[i], vf[i]);
+    } else {
+#pragma unroll 1
+      for (int c = c_lo + wave; c < c_hi; c += NW) {
+        load_k(tile.at(c), kf[0]);
+        load_v(tile.at(c), vf[0]);
+        chunk(tile.at(c), kf[0], vf[0]);
+      }
+    }
+  };
+  if (brief)
+    all_chunks(chunk_brief);
+  else
+    all_chunks(chunk_any);
+
+  // ---- the waves' sums meet in LDS: a lane's four products are four columns of a row ----
+  psum += (uint32_t)__shfl_xor((int)psum, 16);
+  psum += (uint32_t)__shfl_xor((int)psum, 32);
+  if (lane < 16) sSum[wave][lane] = psum;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<v4i *>(&sO[wave][(4 * g + r) * OLD + 64 * ks + 4 * n]) =
+          v4i{o[ks][0][r], o[ks][1][r], o[ks][2][r], o[ks][3][r]};
+  lds_barrier();
+  auto sum_of = [&](int at) {
+    v4i v = *reinterpret_cast<const v4i *>(&sO[0][at]);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const v4i *>(&sO[w][at]);
+    return v;
+  };
+  uint32_t sum = 0;
+  if (tid < QR) {
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += sSum[w][tid];
+  }
+  if constexpr (MODE == PART_SUM) {
+    uint32_t *mine = part_of<KS>(t, block, part, parts);
+    for (int i = 4 * tid; i < QR * 64 * KS; i += 4 * 64 * NW)
+      *reinterpret_cast<v4i *>(mine + i) = sum_of(i / (64 * KS) * OLD + i % (64 * KS));
+    if (tid < QR) mine[QR * 64 * KS + tid] = sum;
+    return;
+  }
+  if (tid < QR) sInv[tid] = fisr((int32_t)sum, a.rsqrt_off);
+  lds_barrier();
+  for (int i = tid; i < rows * words; i += 64 * NW) {
+    const int r = by_words(i), d = 4 * (i - r * words);
+    uint32_t w = 0;
+    if (q0 + r < cnt) {
+      const v4i v = sum_of(r * OLD + d);
+      const uint32_t sums[4] = {(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
+      w = output_word(a, sums, sInv[r]);
+    }
+    *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + r) * a.o_st + d) = w;
+  }
+}
+
+// Adds the parts of a tile's row and finishes it, a wave a row: lane l has word l % W of parts l / W, l / W + 64 / W, ...,
+// four of them on the way at once.
+template <int KS>
+__global__ __launch_bounds__(256) void attn_window_join_kernel(WindowArgs t, int qblocks, int parts) {
+  constexpr int QR = 16, W = 16 * KS, AT_ONCE = 64 / W;
+  const AttnArgs &a = t.a;
+  const int lane = threadIdx.x & 63, w = lane % W;
+  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), block = blockIdx.y;
+  const int q0 = block % qblocks * QR, q = q0 + row, bh = block / qblocks, h = bh % a.H;
+  const int64_t b = bh / a.H;
+  if (q >= a.Tq) return;
+  const int len = t.lengths ? clampi(t.lengths[b], 0, a.Tk) : a.Tk;
+  const int cnt = t.counts ? clampi(t.counts[b], 0, a.Tq) : a.Tq;
+  uint32_t sums[4] = {0u, 0u, 0u, 0u}, psum = 0u;
+  if (q < cnt) {
+    Seen seen;
+    const Tile tile = tile_of(t, b, len, cnt, min(q0 + (lane & 15), cnt - 1), t.sinks, seen);
+    const int share = part_share(tile.nch, parts);
+    const int used = max(1, (tile.nch + share - 1) / share);  // parts that have chunks, or the first
+    for (int p0 = lane / W; p0 < used; p0 += 4 * AT_ONCE) {
+      v4i x[4];
+      uint32_t y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t *from = part_of<KS>(t, block, min(p0 + j * AT_ONCE, used - 1), parts);
+        x[j] = *reinterpret_cast<const v4i *>(from + row * 64 * KS + 4 * w);
+        y[j] = from[QR * 64 * KS + row];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (p0 + j * AT_ONCE < used) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sums[c] += (uint32_t)x[j][c];
+          psum += y[j];
+        }
+    }
+#pragma unroll
+    for (int m = W; m < 64; m *= 2) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sums[c] += (uint32_t)__shfl_xor((int)sums[c], m);
+      psum += (uint32_t)__shfl_xor((int)psum, m);
+    }
+  }
+  if (lane < a.D / 4)
+    *reinterpret_cast<uint32_t *>(a.out + b * a.o_sb + (int64_t)q * a.o_st + (int64_t)h * a.D + 4 * lane) =
+        q < cnt ? output_word(a, sums, fisr((int32_t)psum, a.rsqrt_off)) : 0u;
+}
+
+// Word j of lane group g (16 lanes) becomes word g of lane group j
+__device__ __forceinline__ void transpose_groups(v4i &p) {
+  const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)p[0], (uint32_t)p[2], false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)p[1], (uint32_t)p[3], false, false);
+  const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  p = v4i{(int)c[0], (int)c[1], (int)d[0], (int)d[1]};
+}
+
+// Many queries at the row's last positions: a block has 16 * QT queries of each of its NW waves, whose windows
+// follow one another, and every wave goes through the chunks that any of them sees. A chunk is copied to LDS once a
+// block, as the register images of the products' operands (1 KB each, a lane's 16 bytes at 16 * lane, so reads have no
+// conflicts), two chunks ahead and without registers. First every chunk's K passes for the maxima, then K and V.
+// Row 4g + r of score product i is key 16i + 4g + r: a product is 16 keys in a row, and at a window's borders those
+// that no query sees are left out and those that all see need no mask. Byte 4i + r of lane group g's P.V operand is
+// that key too, and V in quads has words of four keys. Transposed rows have 16 keys in a row, for which the lane groups
+// exchange their words of P.
+template <int KS, bool QUADS, int QT, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(KS, QT)))) void attn_window_rows_kernel(
+    WindowArgs t, int qblocks, int blocks, int per_xcd, int table_off) {
+  constexpr int QW = 16 * QT, QR = QW * NW, SLOTS = 3, IMAGES = 4 * KS, PLACE = 2 * IMAGES * 1024;
+  static_assert(NW == 4, "each wave copies KS images of K and of V");
+  __shared__ __attribute__((aligned(1024))) int8_t sChunk[SLOTS * PLACE];
+  __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
+
+  const int block = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (block >= blocks) return;
+  const AttnArgs &a = t.a;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int q0 = block % qblocks * QR, bh = block / qblocks;
+  const int h = bh % a.H;
+  const int64_t b = bh / a.H;
+  const int D = a.D, N = a.Tq;
+  const int len = t.lengths ? clampi(t.lengths[b], 0, a.Tk) : a.Tk;
+  const int cnt = t.counts ? clampi(t.counts[b], 0, N) : N;
+  const int8_t *const kbase = a.k + b * a.k_sb + (int64_t)h * a.k_sh;
+  const int8_t *const vbase = a.vt + b * a.v_sb + (int64_t)h * a.v_sh;
+  int8_t *const obase = a.out + b * a.o_sb + (int64_t)h * D;
+  // positions rise by one: what the first query sees begins and ends first
+  auto seen_by = [&](int q) { return seen_from(t, len, (int64_t)len - cnt + q); };
+  const int used = min(q0 + QR, cnt);  // queries of the block that are in use end here
+  int nch = 0, ns = 0, w0 = 0;
+  if (q0 < used) {
+    const Seen first = seen_by(q0), last = seen_by(used - 1);
+    w0 = min(first.start, last.end) / 64;
+    ns = min((min(t.sinks, last.end) + 63) / 64, w0);
+    nch = ns + max(0, (last.end + 63) / 64 - w0);
+  }
+  auto chunk_at = [&](int c) { return c < ns ? c : w0 + c - ns; };
+
+  // ---- copies to LDS: image j of a chunk's K (keys past the last repeat it, head dims past D the last ones), of its V ----
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(sChunk));
+  // A lane's offsets from a chunk's base are the same in every chunk that ends before the row does.
+  const auto k_at = [&](int w, int last) {
+    const int j = wave + NW * w, i = j / KS, ks = j % KS;
+    return (uint32_t)min(16 * i + n, last) * (uint32_t)a.k_st + (uint32_t)min(64 * ks + 16 * g, D - 16);
+  };
+  const auto v_at = [&](int w, int last) {  // the chunk's last key
+    const int j = wave + NW * w, ks = j / 4, i = j % 4;
+    const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
+    return QUADS ? (uint32_t)min(4 * i + g, last >> 2) * (uint32_t)a.v_sq + 4 * d0
+                 : (d0 + i) * (uint32_t)a.v_sd + (uint32_t)min(16 * g, last & ~15);
+  };
+  uint32_t koff[KS], voff[KS];
+#pragma unroll
+  for (int w = 0; w < KS; ++w) koff[w] = k_at(w, 63), voff[w] = v_at(w, 63);
+  auto copy_chunk = [&](int kc, uint32_t to, bool with_v) {
+    const int8_t *kb = kbase + (int64_t)(64 * kc) * a.k_st;
+    const int8_t *vb = vbase + (QUADS ? (int64_t)(16 * kc) * a.v_sq : (int64_t)(64 * kc));
+    const int last = len - 1 - 64 * kc;
+    if (last >= 63) {
+#pragma unroll
+      for (int w = 0; w < KS; ++w) dma16_lds(kb, koff[w], to + 1024 * (wave + NW * w));
+      if (with_v) {
+#pragma unroll
+        for (int w = 0; w < KS; ++w) dma16_lds(vb, voff[w], to + 1024 * (IMAGES + wave + NW * w));
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < KS; ++w) dma16_lds(kb, k_at(w, last), to + 1024 * (wave + NW * w));
+      if (with_v) {
+#pragma unroll
+        for (int w = 0; w < KS; ++w) dma16_lds(vb, v_at(w, last), to + 1024 * (IMAGES + wave + NW * w));
+      }
+    }
+  };
+  // Step s of 2 * nch is K of chunk s, or K and V of chunk s - nch; they are copied in turn, each to the next place.
+  int next = 0;
+  bool with_v = false;
+  uint32_t to = 0;
+  auto copy = [&]() {
+    copy_chunk(chunk_at(next), lds0 + to, with_v);
+    to = to == (SLOTS - 1) * PLACE ? 0 : to + PLACE;
+    if (++next == nch) next = 0, with_v = true;
+  };
+  // The copies of step s are there, those of step s + 1 may be on the way. The barrier also says that every wave is
+  // done with step s - 1, whose place step s + 2 takes.
+  uint32_t from = (SLOTS - 1) * PLACE;
+  auto arrive = [&](int s) {
+    if (s + 1 >= 2 * nch)
+      wait_vm<0>();
+    else if (s + 1 >= nch)
+      wait_vm<2 * KS>();
+    else
+      wait_vm<KS>();
+    lds_barrier();
+    from = from == (SLOTS - 1) * PLACE ? 0 : from + PLACE;
+    if (s + 2 < 2 * nch) copy();
+  };
+
+  // ---- queries, and what they see ----
+  const int qw = q0 + wave * QW;
   v4i qf[QT][KS];
   Seen seen[QT];
-  int start = INT32_MAX, end = 0, all_from = 0, all_to = INT32_MAX;
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
-    const int q = min(q0 + 16 * u + n, cnt - 1);  // queries past the count repeat the last one
-    const int64_t p = t.positions ? (int64_t)t.positions[b * t.pos_sb + q] : (int64_t)len - cnt + q;
-    seen[u] = seen_from(t, len, p);
-    start = min(start, seen[u].start), end = max(end, seen[u].end);
-    all_from = max(all_from, seen[u].start), all_to = min(all_to, seen[u].end);
+    const int q = max(0, min(qw + 16 * u + n, cnt - 1));  // queries past the count repeat the last one
+    seen[u] = seen_by(q);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d0 = 64 * ks + 16 * g;
@@ -104,128 +634,102 @@ __global__ __launch_bounds__(64 * NW) void attn_window_kernel(WindowArgs t, int 
       if (d0 < D) qf[u][ks] = *reinterpret_cast<const v4i *>(a.q + b * a.q_sb + (int64_t)q * a.q_st + (int64_t)h * D + d0);
     }
   }
-  start = __builtin_amdgcn_readfirstlane(row16_min(start));
-  end = __builtin_amdgcn_readfirstlane(row16_max(end));
-  all_from = __builtin_amdgcn_readfirstlane(row16_max(all_from));
-  all_to = __builtin_amdgcn_readfirstlane(row16_min(all_to));
-  // chunk c of the block's list is chunk c of the keys while it holds first keys, then w0 + c - ns
-  const int w0 = min(start, end) / 64, w1 = (end + 63) / 64;
-  const int ns = min((min(t.sinks, end) + 63) / 64, w0);
-  const int nch = ns + max(0, w1 - w0);
-  auto chunk_at = [&](int c) { return c < ns ? c : w0 + c - ns; };
-
-  // The K operands of chunk c: keys past the last repeat it, head dims past D the
-  // last ones (the query is zero there). A chunk's base is uniform, its lanes'
-  // offsets fit 32 bits.
-  const int kcol = 16 * g, key0 = 16 * (n >> 2) + (n & 3);
-  auto load_k = [&](int c, v4i (&f)[4][KS]) {
-    const int8_t *base = kbase + (int64_t)(64 * c) * a.k_st;
-    const int last = len - 64 * c - 1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        f[i][ks] = *reinterpret_cast<const v4i *>(base + ((uint32_t)min(key0 + 4 * i, last) * (uint32_t)a.k_st +
-                                                          (uint32_t)min(64 * ks + kcol, D - 16)));
-  };
-  // Quads and transposed rows hold words of four keys of one column. Columns past D
-  // repeat the last ones; their sums are not stored.
-  auto load_v = [&](int c, int ks, v4i (&f)[4]) {
-    const uint32_t d0 = (uint32_t)min(64 * ks + 4 * n, D - 4);
-    if (QUADS) {
-      const int8_t *base = vbase + (int64_t)(16 * c) * a.v_sq;
-      const int last = ((len - 1) >> 2) - 16 * c;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        f[j] = *reinterpret_cast<const v4i *>(base + ((uint32_t)min(4 * g + j, last) * (uint32_t)a.v_sq + 4 * d0));
-    } else {
-      const int8_t *base = vbase + 64 * c;
-      const uint32_t at = (uint32_t)min(16 * g, (len - 1 - 64 * c) & ~15);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        f[i] = *reinterpret_cast<const v4i *>(base + ((d0 + i) * (uint32_t)a.v_sd + at));
-    }
-  };
-  // the operand of product i: column 64 ks + 4 n + i of the lane group's 16 keys
-  auto v_operands = [&](const v4i (&f)[4], v4i (&o)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = QUADS ? f[j][i] : f[i][j];
-  };
-
   const bool table = table_off >= 0;
   const int zero = table ? shift_exp_zero(a.frac_bits) : IW_SEXP_LUT - 1;
   if (table)
     for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
       *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
-
-  auto scores = [&](const v4i (&f)[KS], int u) {
-    v4i s{0, 0, 0, 0};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[ks], qf[u][ks], s, 0, 0, 0);
-    return s;
+  wait_vm<0>();  // the copies are counted from here on
+  if (nch > 0) {
+    copy();
+    copy();  // there are two steps at least
+  }
+  // In products of 16 keys: those that any of this wave's queries sees a key of ([p_from, p_to) and below p_first), and
+  // those that all see all of ([p_all, p_end))
+  const int qe = min(qw + QW, cnt) - 1;
+  Seen wf{0, 0, 0}, wl{0, 0, 0};
+  if (qw <= qe) wf = seen_by(qw), wl = seen_by(qe);
+  const int p_from = wf.start / 16, p_to = (wl.end + 15) / 16, p_first = (wl.first + 15) / 16;
+  const int p_all = (wl.start + 15) / 16, p_end = wf.end / 16;
+  auto some = [&](int p0, int m) { return (p0 < p_to && p0 + m > p_from) || p0 < p_first; };
+  auto whole = [&](int p0, int m) { return p0 >= p_all && p0 + m <= p_end; };
+  // which of the four keys from k0 + 4 g on this lane's query of tile u sees; borders that lie elsewhere cost nothing
+  auto counted = [&](int p0, int u) -> uint32_t {
+    const int k = 16 * p0 + 4 * g;
+    uint32_t ok = 15u;
+    if (p0 >= p_end) ok = low4(seen[u].end - k);
+    if (p0 < p_all) ok &= ~low4(seen[u].start - k);
+    if (p0 < p_first) ok |= low4(seen[u].first - k);
+    return ok;
   };
-  // every query of the block sees every key of the chunk at kc
-  auto whole = [&](int kc) { return 64 * kc >= all_from && 64 * kc + 64 <= all_to; };
-  // which of the lane group's 16 keys of the chunk at kc this lane's query of tile u sees
-  auto counted = [&](int kc, int u) -> uint32_t {
-    const int k0 = 64 * kc + 16 * g;
-    return (low_bits(seen[u].end - k0) & ~low_bits(seen[u].start - k0)) | low_bits(seen[u].first - k0);
+  auto image = [&](int j) { return *reinterpret_cast<const v4i *>(&sChunk[from + 1024 * j + 16 * lane]); };
+  auto scores = [&](int i, v4i (&out)[QT]) {
+#pragma unroll
+    for (int u = 0; u < QT; ++u) out[u] = v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const v4i f = image(i * KS + ks);
+#pragma unroll
+      for (int u = 0; u < QT; ++u) out[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, qf[u][ks], out[u], 0, 0, 0);
+    }
   };
 
   // ---- pass 1: row maximum of the raw scores ----
   int32_t mx[QT];
 #pragma unroll
   for (int u = 0; u < QT; ++u) mx[u] = INT32_MIN;
-  v4i kf[4][KS];
-#pragma unroll 1
-  for (int c = wave; c < nch; c += NW) {
-    const int kc = chunk_at(c);
-    load_k(kc, kf);
+  auto more = [&](const v4i (&x)[QT]) {
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-      if (whole(kc)) {
+      mx[u] = max(max(mx[u], x[u][0]), x[u][1]);
+      mx[u] = max(max(mx[u], x[u][2]), x[u][3]);
+    }
+  };
+#pragma unroll 1
+  for (int s = 0; s < nch; ++s) {
+    arrive(s);
+    const int p0 = 4 * chunk_at(s);
+    if (!some(p0, 4)) continue;
+    if (whole(p0, 4)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4i s = scores(kf[i], u);
-          mx[u] = max(max(mx[u], s[0]), s[1]);
-          mx[u] = max(max(mx[u], s[2]), s[3]);
-        }
-      } else {
-        const uint32_t ok = counted(kc, u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4i s = scores(kf[i], u);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if ((ok >> (4 * i + r)) & 1u) mx[u] = max(mx[u], s[r]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        v4i x[QT];
+        scores(i, x);
+        more(x);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (some(p0 + i, 1)) {
+          v4i x[QT];
+          scores(i, x);
+          if (!whole(p0 + i, 1)) {
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+              const uint32_t off = ~counted(p0 + i, u);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) x[u][r] = hide(x[u][r], off, r);
+            }
+          }
+          more(x);
+        }
     }
   }
-#pragma unroll
-  for (int u = 0; u < QT; ++u) {
-    mx[u] = max(mx[u], __shfl_xor(mx[u], 16));
-    mx[u] = max(mx[u], __shfl_xor(mx[u], 32));
-    if (lane < 16) sMax[wave][16 * u + lane] = mx[u];
-  }
-  lds_barrier();
   int32_t rowmax[QT];
   bool sat = false;
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mx[u] = max(mx[u], sMax[w][16 * u + n]);
-    // requantization keeps the order, so the maximum's is the maximum
-    rowmax[u] = mx[u] == INT32_MIN ? -32768 : qk_requant16(mx[u], a.qk_m, a.qk_s);
-    sat = sat || rowmax[u] >= 32767;
+    mx[u] = max(mx[u], __shfl_xor(mx[u], 16));
+    mx[u] = max(mx[u], __shfl_xor(mx[u], 32));
+    // requantization keeps the order, so the maximum's is the maximum; a query without keys may have any
+    rowmax[u] = mx[u] == INT32_MIN ? 0 : qk_requant16(mx[u], a.qk_m, a.qk_s);
+    sat = sat || rowmax[u] >= 32767 || rowmax[u] < zero - 32768;
   }
-  // the short index where no row maximum wraps: the keys that count lie at a
-  // distance of 1 at least, the others are taken for such
+  // The short index where no row maximum wraps and none is so low that saturated scores are near it: the keys that
+  // count lie at a distance of 1 at least, the others are taken for such.
   const bool brief = table && !__any(sat);
 
-  // ---- pass 2: P and P.V over this wave's keys ----
+  // ---- pass 2: P and P.V ----
   v4i o[QT][KS][4];
   uint32_t psum[QT];
 #pragma unroll
@@ -236,135 +740,234 @@ __global__ __launch_bounds__(64 * NW) void attn_window_kernel(WindowArgs t, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[u][ks][i] = v4i{0, 0, 0, 0};
   }
-  // P of the chunk at kc as the operands of its products; hi where a P of 128 (a row maximum
-  // of 32767 wraps) is left out, as the product is signed: it goes in as twice 64
-  auto chunk_p = [&](int kc, const v4i (&f)[4][KS], v4i (&p)[QT], v4i (&hi)[QT]) {
-    bool any_hi = false;
+  // operand c of the products with V: columns 64 ks + 4 n + c
+  auto v_operands = [&](int ks, v4i (&v)[4]) {
+    v4i f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = image(IMAGES + 4 * ks + i);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[c][i] = QUADS ? f[i][c] : f[c][i];
+  };
+  auto add_pv = [&](v4i (&x)[QT]) {
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-      ScoreIndex ix(a, rowmax[u], zero);
-      ix.flo = max(ix.flo, 1);
-      if (brief) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4i s = scores(f[i], u);
-          p[u][i] = (int)((uint32_t)sTable[ix.full(s[0])] | (uint32_t)sTable[ix.full(s[1])] << 8 |
-                          (uint32_t)sTable[ix.full(s[2])] << 16 | (uint32_t)sTable[ix.full(s[3])] << 24);
-        }
-        if (!whole(kc)) {
-          const uint32_t ok = counted(kc, u);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[u][i] &= (int)byte_mask((ok >> (4 * i)) & 15u);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) psum[u] = __builtin_amdgcn_udot4((uint32_t)p[u][i], 0x01010101u, psum[u], false);
-      } else {
-        const uint32_t ok = counted(kc, u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4i s = scores(f[i], u);
-          uint32_t w = 0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t d = ix.any(s[r]);
-            const uint32_t e = table ? (uint32_t)sTable[d] : shift_exp((int32_t)d, a.frac_bits);
-            w |= ((ok >> (4 * i + r)) & 1u ? e & 0xffu : 0u) << (8 * r);
-          }
-          psum[u] = __builtin_amdgcn_udot4(w, 0x01010101u, psum[u], false);
-          p[u][i] = (int)(w & 0x7f7f7f7fu), hi[u][i] = (int)((w >> 1) & 0x40404040u);
-        }
-        any_hi = any_hi || (hi[u][0] | hi[u][1] | hi[u][2] | hi[u][3]) != 0;
-      }
+      for (int i = 0; i < 4; ++i) psum[u] = __builtin_amdgcn_udot4((uint32_t)x[u][i], 0x01010101u, psum[u], false);
+      if (!QUADS) transpose_groups(x[u]);
     }
-    return __any(any_hi) != 0;
-  };
-  v4i p[QT], hi[QT];
-#pragma unroll 1
-  for (int c = wave; c < nch; c += NW) {
-    const int kc = chunk_at(c);
-    v4i vr[KS][4];
-    load_k(kc, kf);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) load_v(kc, ks, vr[ks]);
-    const bool any_hi = chunk_p(kc, kf, p, hi);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       v4i v[4];
-      v_operands(vr[ks], v);
-      auto pv = [&](const v4i (&x)[QT]) {
+      v_operands(ks, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int u = 0; u < QT; ++u)
+          o[u][ks][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u], v[c], o[u][ks][c], 0, 0, 0);
+    }
+  };
+  ScoreIndex ix(a, 0, zero);
+  ix.flo = 1, ix.fhi = zero;
+  int32_t K[QT];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[u][ks][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u], v[i], o[u][ks][i], 0, 0, 0);
-      };
-      pv(p);
-      if (any_hi) {
-        pv(hi);
-        pv(hi);
+  for (int u = 0; u < QT; ++u) K[u] = ScoreIndex(a, rowmax[u], zero).fK;
+  auto values = [&](const v4i &x, int u) {
+    ix.fK = K[u];
+    return pack4(sTable[ix.full(x[0])], sTable[ix.full(x[1])], sTable[ix.full(x[2])], sTable[ix.full(x[3])]);
+  };
+#pragma unroll 1
+  for (int s = nch; s < 2 * nch; ++s) {
+    arrive(s);
+    const int p0 = 4 * chunk_at(s - nch);
+    if (!some(p0, 4)) continue;
+    v4i p[QT];
+    if (brief) {
+      if (whole(p0, 4)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v4i x[QT];
+          scores(i, x);
+#pragma unroll
+          for (int u = 0; u < QT; ++u) p[u][i] = (int)values(x[u], u);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < QT; ++u) p[u] = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (some(p0 + i, 1)) {
+            v4i x[QT];
+            scores(i, x);
+#pragma unroll
+            for (int u = 0; u < QT; ++u) p[u][i] = (int)values(x[u], u);
+            if (!whole(p0 + i, 1)) {
+#pragma unroll
+              for (int u = 0; u < QT; ++u) p[u][i] = (int)keep_bytes((uint32_t)p[u][i], counted(p0 + i, u));
+            }
+          }
+      }
+      add_pv(p);
+    } else {
+      // Any row maximum, any precision, a tile at a time. A P of 128 (a row maximum of 32767 wraps) is too much for
+      // the signed product: the rest of it goes in twice.
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        const ScoreIndex at(a, rowmax[u], zero);
+        v4i p1, rest;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v4i x{0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            x = __builtin_amdgcn_mfma_i32_16x16x64_i8(image(i * KS + ks), qf[u][ks], x, 0, 0, 0);
+          const uint32_t ok = counted(p0 + i, u);
+          uint32_t w = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t d = at.any(x[r]);
+            const uint32_t e = table ? (uint32_t)sTable[d] : shift_exp((int32_t)d, a.frac_bits);
+            w |= ((ok >> r) & 1u ? e & 0xffu : 0u) << (8 * r);
+          }
+          psum[u] = __builtin_amdgcn_udot4(w, 0x01010101u, psum[u], false);
+          p1[i] = (int)(w & 0x7f7f7f7fu), rest[i] = (int)((w >> 1) & 0x40404040u);
+        }
+        if (!QUADS) transpose_groups(p1), transpose_groups(rest);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          v4i v[4];
+          v_operands(ks, v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            v4i &to = o[u][ks][c];
+            to = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, v[c], to, 0, 0, 0);
+            to = __builtin_amdgcn_mfma_i32_16x16x64_i8(rest, v[c], to, 0, 0, 0);
+            to = __builtin_amdgcn_mfma_i32_16x16x64_i8(rest, v[c], to, 0, 0, 0);
+          }
+        }
       }
     }
   }
 
-  // ---- the waves' sums meet in LDS: a lane's four products are four columns of a row ----
+  // a lane group finds the roots of one tile's queries: group u those of tile u
+  const Finish fin(a);
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
     psum[u] += (uint32_t)__shfl_xor((int)psum[u], 16);
     psum[u] += (uint32_t)__shfl_xor((int)psum[u], 32);
-    if (lane < 16) sSum[wave][16 * u + lane] = psum[u];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<v4i *>(&sO[wave][(16 * u + 4 * g + r) * OLD + 64 * ks + 4 * n]) =
-            v4i{o[u][ks][0][r], o[u][ks][1][r], o[u][ks][2][r], o[u][ks][3][r]};
   }
-  lds_barrier();
-  if (tid < QR) {
-    uint32_t sum = 0;
+  uint32_t mine = psum[0];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) sum += sSum[w][tid];
-    sInv[tid] = fisr((int32_t)sum, a.rsqrt_off);
-  }
-  lds_barrier();
-  for (int i = tid; i < rows * words; i += 64 * NW) {
-    const int q = by_words(i), d = 4 * (i - q * words);
-    uint32_t w = 0;
-    if (q0 + q < cnt) {
-      v4i v = *reinterpret_cast<const v4i *>(&sO[0][q * OLD + d]);
+  for (int u = 1; u < QT; ++u) mine = g == u ? psum[u] : mine;
+  const int32_t inv = fisr((int32_t)mine, a.rsqrt_off);
+  const bool fast = fin.brief && !__any((inv << 8) >> 8 != inv);
 #pragma unroll
-      for (int j = 1; j < NW; ++j) v += *reinterpret_cast<const v4i *>(&sO[j][q * OLD + d]);
-      const uint32_t sums[4] = {(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
-      w = output_word(a, sums, sInv[q]);
-    }
-    *reinterpret_cast<uint32_t *>(obase + (int64_t)(q0 + q) * a.o_st + d) = w;
-  }
+  for (int u = 0; u < QT; ++u)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      finish_row<KS>(t, fin, obase, qw + 16 * u + 4 * g + r, cnt, o[u], r, __shfl(inv, 16 * u + 4 * g + r), fast, n);
 }
 
-template <int KS, bool QUADS, int QT, int NW>
-int launch_window(const WindowArgs &t, hipStream_t s) {
-  const int64_t qblocks = (t.a.Tq + 16 * QT - 1) / (16 * QT), blocks = qblocks * t.a.B * t.a.H;
+template <int KS, bool QUADS, int QT>
+int launch_window_rows(const WindowArgs &t, hipStream_t s) {
+  constexpr int NW = 4;
+  const int64_t qblocks = (t.a.Tq + 16 * QT * NW - 1) / (16 * QT * NW), blocks = qblocks * t.a.B * t.a.H;
+  const int64_t per_xcd = (blocks + 7) / 8;
+  const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
+  if (8 * per_xcd * 64 * NW >= 1LL << 32) return fail("too many heads and queries for one call");
+  hipLaunchKernelGGL((attn_window_rows_kernel<KS, QUADS, QT, NW>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t,
+                     (int)qblocks, (int)blocks, (int)per_xcd, table);
+  return check_launch("attn_window_rows_kernel");
+}
+
+template <int KS, bool QUADS, int NW, int NC, int MODE = ALL>
+int launch_window(const WindowArgs &t, hipStream_t s, int parts = 1) {
+  const int64_t qblocks = (t.a.Tq + 15) / 16, blocks = qblocks * t.a.B * t.a.H;
   const int64_t per_xcd = (blocks + 7) / 8;
   const int words = t.a.D / 4, per_word = (65536 + words - 1) / words;
   const int table = t.a.frac_bits <= kTableBits ? table_at(t.a.frac_bits) : -1;
   // a grid has fewer than 2^32 threads
   if (8 * per_xcd * 64 * NW >= 1LL << 32) return fail("too many heads and queries for one call");
-  hipLaunchKernelGGL((attn_window_kernel<KS, QUADS, QT, NW>), dim3((unsigned)(8 * per_xcd)), dim3(64 * NW), 0, s, t,
-                     (int)qblocks, (int)blocks, (int)per_xcd, per_word, table);
+  hipLaunchKernelGGL((attn_window_kernel<KS, QUADS, NW, NC, MODE>), dim3((unsigned)(8 * per_xcd), (unsigned)parts),
+                     dim3(64 * NW), 0, s, t, (int)qblocks, (int)blocks, (int)per_xcd, per_word, table);
   return check_launch("attn_window_kernel");
+}
+
+template <int KS, bool QUADS>
+int launch_window_parts(const WindowArgs &t, int parts, hipStream_t s) {
+  int rc = launch_window<KS, true, 8, 0, PART_MAX>(t, s, parts);  // reads K only
+  if (rc == 0) rc = launch_window<KS, QUADS, 8, 0, PART_SUM>(t, s, parts);
+  if (rc) return rc;
+  const int qblocks = (t.a.Tq + 15) / 16;
+  hipLaunchKernelGGL((attn_window_join_kernel<KS>), dim3(4, (unsigned)(qblocks * t.a.B * t.a.H)), dim3(256), 0, s, t,
+                     qblocks, parts);
+  return check_launch("attn_window_join_kernel");
+}
+
+// The most chunks that a tile of queries has, whatever the lengths: its windows (16 queries at positions that
+// follow one another, or one at any) from any key on, and the first keys.
+int64_t most_chunks(int64_t queries, int64_t cap, int64_t before, int64_t after, int64_t sinks) {
+  const int64_t keys = std::min(cap, before + after + std::min<int64_t>(queries, 16));
+  return std::min((cap + 63) / 64, (keys + 62) / 64 + 1 + (std::min(sinks, cap) + 63) / 64);
+}
+
+// Blocks that share the chunks of a tile. Three launches and the sums' way through memory are worth it where each
+// block is left with much less. One query of heads of 64 columns, us in one block of 8 waves and in parts:
+//   heads x parts    4096 keys      8192 keys      16384 keys
+//   8 x 8 to 32      14.4, 11.6     23.6, 12.3     45.1, 15.0
+//   64 x 4           17.7, 18.0     30.2, 25.7     60.1, 39.9
+//   120 x 2          19.6, 25.4     37.0, 40.2     84.7, 72.7
+// and of 128 columns 2048 keys: 26.2 and 14.9 for 8 heads, 27.2 and 20.3 for 64, 28.2 and 26.7 for 120 (1024 keys: 15.9
+// in one).
+constexpr int kCus = 256;
+int window_parts(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, int64_t before, int64_t after, int64_t sinks) {
+  if (cap < 1024) return 1;
+  const int64_t blocks = heads * ((queries + 15) / 16), chunks = most_chunks(queries, cap, before, after, sinks);
+  const int64_t parts = std::min(kCus / blocks, (chunks + 7) / 8);
+  return parts > 1 && parts * chunks > (head_dim <= 64 ? 256 : 64) ? (int)parts : 1;
+}
+
+// Which of the kernels, with the same results. Queries at the last positions share chunks in LDS where 64 of them a block
+// fill the device: heads of 128 columns from a block a CU on, of 64 columns from two (us of a block a 16-query tile and
+// so, windows of 512 keys: 20 heads of 1500 queries, 480 blocks, 54.5 and 30.0 with 128 columns, 23.0 and 22.2 with 64;
+// 64 of 300, 320 blocks, 37.1 and 29.7, 16.4 and 21.9; 64 of 128, 128 blocks, 18.1 and 23.0, 9.9 and 16.4), but not for 32
+// queries or fewer (1280 heads of 32: 78.8 and 87.2, 30.6 and 33.1; of 64: 137 and 90, 54 and 36).
+// Two tiles a wave pay where windows are long (16 rows of 20 heads of 1500 frames, all of them: 158 us with one, 142 with two;
+// 8192 positions with windows of 1024: 170 and 123; 1280 heads of 300, 512 keys: 359 and 315 with 128 columns, 141 and 152
+// with 64; 128 keys: 184 and 179, 79 and 91).
+// Else a wave holds its chunks where they are few: heads of 64, one query, 128 keys: 5.4 us in a loop and 5.2 so;
+// 384 keys, two chunks a wave, 6.2 and 5.8; 2560 heads of it 28.4 and 25.9. Eight waves take long windows faster if there
+// are few tiles: 1024 keys, 20 heads 8.9 and 7.6, 256 heads 12.0 and 11.1, 640 heads 22.4 and 25.3.
+template <int KS, bool QUADS>
+int launch_form(const WindowArgs &t, hipStream_t s) {
+  const int64_t heads = (int64_t)t.a.B * t.a.H, tiles = (t.a.Tq + 15) / 16;
+  if (!t.positions && t.a.Tq > 32) {
+    if (std::min<int64_t>(t.before + t.after, t.a.Tk) >= 7 * 64 && heads * ((tiles + 7) / 8) >= kCus)
+      return launch_window_rows<KS, QUADS, 2>(t, s);
+    if (heads * ((tiles + 3) / 4) >= (KS == 1 ? 2 : 1) * kCus) return launch_window_rows<KS, QUADS, 1>(t, s);
+  }
+  const int parts = window_parts(heads, t.a.Tq, t.a.D, t.a.Tk, t.before, t.after, t.sinks);
+  if (parts > 1) return launch_window_parts<KS, QUADS>(t, parts, s);
+  const int64_t any = (t.a.Tk + 63) / 64;  // queries at positions that need not follow one another
+  const int64_t most = t.positions && t.a.Tq > 1 ? any : most_chunks(t.a.Tq, t.a.Tk, t.before, t.after, t.sinks);
+  if (most <= 4) return launch_window<KS, QUADS, 4, 1>(t, s);
+  if (most <= 8) return launch_window<KS, QUADS, 4, 2>(t, s);
+  return heads * tiles <= kCus ? launch_window<KS, QUADS, 8, 0>(t, s) : launch_window<KS, QUADS, 4, 0>(t, s);
 }
 
 }  // namespace
 
 int64_t attn_window_workspace(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, int64_t before,
                               int64_t after, int64_t sinks) {
-  return 0;
+  const int64_t parts = window_parts(heads, queries, head_dim, cap, before, after, sinks);
+  return parts == 1 ? 0 : 4 * heads * ((queries + 15) / 16) * parts * part_words(head_dim <= 64 ? 1 : 2);
 }
 
 int launch_attn_window(const WindowArgs &t, hipStream_t s) {
   const bool quads = t.a.v_sq != 4;
-  if (t.a.D <= 64) return quads ? launch_window<1, true, 1, 4>(t, s) : launch_window<1, false, 1, 4>(t, s);
-  return quads ? launch_window<2, true, 1, 4>(t, s) : launch_window<2, false, 1, 4>(t, s);
+  if (t.a.D <= 64) return quads ? launch_form<1, true>(t, s) : launch_form<1, false>(t, s);
+  return quads ? launch_form<2, true>(t, s) : launch_form<2, false>(t, s);
 }
 
 }  // namespace iw

@@ -166,6 +166,11 @@ __device__ __forceinline__ void dma16_lds(const int8_t *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
                : "memory", "m0");
 }
+// The same from a wave-uniform base and a lane's 32-bit offset.
+__device__ __forceinline__ void dma16_lds(const int8_t *base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 template <int N>

@@ -167,6 +167,30 @@ def test_window_local_rows(iw, oracle, gpu, N, before, after, sinks):
     Window(N, 1, 3, 64, N, N, before, after, sinks, k_rows=True).check(iw, oracle)
 
 
+@pytest.mark.parametrize("layout", ["vt", "quads"])
+@pytest.mark.parametrize("D,B,N,before,after,sinks", [
+    (64, 260, 33, 100, 0, 3), (48, 260, 64, 17, 40, 70), (64, 129, 70, 63, 64, 0), (16, 256, 48, 250, 250, 1),
+    (128, 130, 40, 63, 0, 4), (80, 128, 64, 30, 31, 0), (112, 65, 65, 200, 3, 80),
+    (64, 130, 33, 448, 0, 20), (32, 65, 129, 300, 200, 0), (128, 130, 50, 449, 0, 0), (96, 64, 200, 200, 260, 100),
+    (128, 64, 257, None, 0, 0)])
+def test_window_many_rows(iw, oracle, gpu, D, B, N, before, after, sinks, layout):
+    """Batches whose queries share keys: ragged lengths and counts, rows without either, every path of the scalars."""
+    print("case: window many rows", D, B, N, before, after, sinks, layout, flush=True)
+    r = gen.rng(B + N + D)
+    cap = 600
+    lengths = r.integers(0, cap + 1, B)
+    counts = r.integers(0, N + 1, B)
+    lengths[:6], counts[:6] = [cap, cap - 1, 0, 1, 300, N], [N, N - 1, N, N, 0, N]
+    rows = [0, 1, 2, 3, 4, 5, B // 2, B - 2, B - 1]
+    for scalars in (None, (255, 0, 7, 130, 9), (200, 4, 10, 255, 12), (3, 9, 12, 90, 7)):
+        w = Window(D + N, B, 2, D, cap, N, before, after, sinks, lengths=lengths, counts=counts, layout=layout, scalars=scalars)
+        got, want = host(w.run(iw)), w.expected(oracle, rows)
+        bad = np.argwhere(got[rows] != want[rows])
+        assert not len(bad), (scalars, len(bad), bad[:4])
+        unused = np.arange(N) >= np.asarray(counts)[:, None]
+        assert not got[unused].any()
+
+
 @pytest.mark.parametrize("B,H,D,cap,N", [(1, 20, 64, 300, 300), (40, 20, 64, 100, 7), (129, 3, 64, 100, 40), (16, 20, 64, 130, 100),
                                          (24, 20, 96, 130, 100), (9, 16, 128, 260, 200), (2, 2, 64, 2000, 1500), (130, 20, 64, 448, 1),
                                          (700, 8, 64, 150, 33)])
