@@ -507,6 +507,288 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(WindowArgs t, int
         q < cnt ? output_word(a, sums, fisr((int32_t)psum, a.rsqrt_off)) : 0u;
 }
 
+// One value a lane that is the sum over the 4 * KS lanes of a group: lane c of it gets that of x[c]
+template <int CTRL>
+__device__ __forceinline__ int32_t swap_add(bool upper, int32_t lower_one, int32_t upper_one) {
+  return (upper ? upper_one : lower_one) +
+         __builtin_amdgcn_update_dpp(0, upper ? lower_one : upper_one, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ int32_t sums_of_4(const int32_t *x, int lane) {
+  const int32_t a = swap_add<0xB1>(lane & 1, x[0], x[1]), b = swap_add<0xB1>(lane & 1, x[2], x[3]);
+  return swap_add<0x4E>(lane & 2, a, b);
+}
+__device__ __forceinline__ int32_t sums_of_8(const int32_t *x, int lane) {
+  int32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = swap_add<0x141>(lane & 4, x[i], x[i + 4]);  // lane 7 - c has the other halves
+  return sums_of_4(y, lane);
+}
+__device__ __forceinline__ int32_t lanes_max(int32_t v) {
+  v = row16_max(v);
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+__device__ __forceinline__ int32_t dpp_sum(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
+  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
+         (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+__device__ __forceinline__ int32_t dot16(const v4i &x, const v4i &y, int32_t sum) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_sdot4(x[j], y[j], sum, false);
+  return sum;
+}
+
+// Where several blocks share the chunks of a head: the workspace has `chunks` times 64 scores a head, then each part's
+// sums of P.V, those of P and the row maximum, in words
+constexpr int token_words(int ks) { return 64 * ks + 4; }
+__device__ __forceinline__ uint32_t *token_part(const WindowArgs &t, int ks, int blocks, int block, int part, int parts) {
+  return t.workspace + t.scores + ((int64_t)block * parts + part) * token_words(ks);
+}
+
+// One query a row. Matrix products would have the same 16 rows: here 16 / KS keys are a load of 16 bytes a lane, the
+// lanes of a key add up their dot products so that every lane is left with the score of one key of 64, and P is a byte in
+// LDS that the lanes of its value find there. Keys are taken in units of 16, those of the first keys and then the
+// window's as one list, four units a chunk, the chunks by NW waves in turn. NC > 0: at most NC chunks a wave, whose K and V
+// are all requested at the start; else scores wait in LDS for the row maximum. Either way K and V are read once, and that
+// is what bounds it: 2560 heads of 64 columns and 2048 keys take 124 us in quads, 5.4 TB/s, and 1024 keys 65.
+template <int KS, bool QUADS, int NW, int NC, int MODE>
+__global__ __launch_bounds__(64 * NW) void attn_window_token_kernel(WindowArgs t, int blocks, int per_xcd, int chunks) {
+  static_assert(MODE == ALL || NC == 0, "parts loop over their chunks");
+  constexpr int LOADS = 4 * KS, LPQ = 16 * KS, ACCS = QUADS ? 4 : LOADS, HC = NC > 0 ? NC : 1;
+  extern __shared__ int32_t sScores[];
+  __shared__ __attribute__((aligned(16))) uint8_t sP[NW][HC][64];
+  __shared__ int32_t sMax[NW];
+  __shared__ uint32_t sSum[NW];
+  __shared__ __attribute__((aligned(16))) uint32_t sO[NW][64 * KS];
+
+  const int block = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (block >= blocks) return;
+  const AttnArgs &a = t.a;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = block % a.H, D = a.D;
+  const int64_t b = block / a.H;
+  const int len = t.lengths ? clampi(t.lengths[b], 0, a.Tk) : a.Tk;
+  const int cnt = t.counts ? clampi(t.counts[b], 0, 1) : 1;
+  const int8_t *const kbase = a.k + b * a.k_sb + (int64_t)h * a.k_sh;
+  const int8_t *const vbase = a.vt + b * a.v_sb + (int64_t)h * a.v_sh;
+  const Seen seen = seen_from(t, len, t.positions ? (int64_t)t.positions[b * t.pos_sb] : (int64_t)len - 1);
+  const int w0 = seen.start / 16, ns = min((seen.first + 15) / 16, w0);
+  const int nu = cnt ? ns + max(0, (seen.end + 15) / 16 - w0) : 0;
+  // this block's chunks
+  const int parts = MODE == ALL ? 1 : (int)gridDim.y, share = part_share((nu + 3) / 4, parts);
+  const int c_lo = MODE == ALL ? 0 : (int)blockIdx.y * share, nch = MODE == ALL ? (nu + 3) / 4 : min(c_lo + share, (nu + 3) / 4);
+  uint32_t *const record = MODE == ALL ? nullptr : token_part(t, KS, blocks, block, blockIdx.y, parts);
+  int32_t *const scores = MODE == ALL ? sScores : reinterpret_cast<int32_t *>(t.workspace) + (int64_t)block * chunks * 64;
+  // the first key of unit u (those past the last repeat it)
+  auto unit_at = [&](int u) { return 16 * (u < ns ? u : w0 + u - ns); };
+  // the first and last key of the unit from key k0 on that the query sees: no others are read
+  auto low = [&](int k0) { return k0 < seen.first ? 0 : max(seen.start - k0, 0); };
+  auto high = [&](int k0) { return min((k0 < 16 * w0 ? seen.first : seen.end) - k0, 16) - 1; };
+
+  const int c = lane % LOADS, kk = lane / LOADS, part = lane & 3, n = lane % LPQ, qd = lane / LPQ;
+  const uint32_t kcol = (uint32_t)min(16 * c, D - 16), k_st16 = (uint32_t)a.k_st >> 4, v_sq16 = (uint32_t)a.v_sq >> 4;
+  auto load_k = [&](int ch, v4i (&f)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int k0 = unit_at(min(4 * ch + i / KS, nu - 1));
+      const int key = clampi(i % KS * 8 + kk, low(k0), high(k0));
+      f[i] = *reinterpret_cast<const v4i *>(kbase + k0 * a.k_st + (__umul24(key, k_st16) * 16 + kcol));
+    }
+  };
+  // quads: load i has 4 / KS of them, whole; transposed rows: 16 columns, four units of each
+  auto load_v = [&](int ch, v4i (&f)[LOADS]) {
+    if constexpr (QUADS) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int k0 = unit_at(min(4 * ch + i / KS, nu - 1));
+        const int quad = clampi(i % KS * 2 + qd, low(k0) >> 2, high(k0) >> 2);
+        f[i] = *reinterpret_cast<const v4i *>(vbase + (k0 >> 2) * a.v_sq + (__umul24(quad, v_sq16) * 16 + 4 * min(4 * n, D - 4)));
+      }
+    } else {
+      const uint32_t at = (uint32_t)(lane >> 2) * (uint32_t)a.v_sd + (uint32_t)unit_at(min(4 * ch + part, nu - 1));
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        f[i] = *reinterpret_cast<const v4i *>(vbase + 16 * min(i, D / 16 - 1) * a.v_sd + at);
+    }
+  };
+
+  v4i kf[HC][LOADS], vf[HC][LOADS], qf{0, 0, 0, 0};
+  if (16 * c < D) qf = *reinterpret_cast<const v4i *>(a.q + b * a.q_sb + (int64_t)h * D + 16 * c);
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i < nch) load_k(wave + NW * i, kf[i]);
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i < nch) load_v(wave + NW * i, vf[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // this lane's key of a chunk: its score, INT32_MIN where the query does not see it
+  auto score = [&](int ch, const v4i (&f)[LOADS]) {
+    int32_t x[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) x[i] = dot16(f[i], qf, 0);
+    const int32_t s = KS == 1 ? sums_of_4(x, lane) : sums_of_8(x, lane);
+    const int u = 4 * ch + c / KS, key = unit_at(u) + c % KS * 8 + kk;
+    return u < nu && ((key >= seen.start && key < seen.end) || key < seen.first) ? s : INT32_MIN;
+  };
+  int32_t mx = INT32_MIN, held[HC];
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      held[i] = INT32_MIN;
+      if (wave + NW * i < nch) held[i] = score(wave + NW * i, kf[i]);
+      mx = max(mx, held[i]);
+    }
+  } else {
+    auto one = [&](int ch, const v4i (&f)[LOADS]) {
+      const int32_t s = score(ch, f);
+      scores[64 * ch + lane] = s;
+      mx = max(mx, s);
+    };
+    if (MODE != PART_SUM) {
+      v4i kn[LOADS];
+      if (c_lo + wave < nch) load_k(c_lo + wave, kf[0]);
+#pragma unroll 1
+      for (int ch = c_lo + wave; ch < nch; ch += 2 * NW) {
+        if (ch + NW < nch) load_k(ch + NW, kn);
+        one(ch, kf[0]);
+        if (ch + 2 * NW < nch) load_k(ch + 2 * NW, kf[0]);
+        if (ch + NW < nch) one(ch + NW, kn);
+      }
+    }
+    if (MODE != PART_MAX && c_lo + wave < nch) load_v(c_lo + wave, vf[0]);
+    if (MODE == PART_SUM)
+      for (int p = lane; p < parts; p += 64) mx = max(mx, (int32_t)token_part(t, KS, blocks, block, p, parts)[64 * KS + 1]);
+  }
+  mx = lanes_max(mx);
+  if constexpr (MODE != PART_SUM) {
+    if (lane == 0) sMax[wave] = mx;
+    lds_barrier();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mx = max(mx, sMax[w]);
+  }
+  if constexpr (MODE == PART_MAX) {
+    if (tid == 0) record[64 * KS + 1] = (uint32_t)mx;
+    return;
+  }
+  // requantization keeps the order, so the maximum's is the maximum; a query without keys may have any
+  const int32_t rowmax = mx == INT32_MIN ? 0 : qk_requant16(mx, a.qk_m, a.qk_s);
+  const bool wraps = rowmax >= 32767;  // a P of 128 is too much for the signed product: the rest of it goes in twice
+  const ScoreIndex ix(a, rowmax);
+
+  int32_t acc[ACCS];
+  uint32_t psum = 0u;
+#pragma unroll
+  for (int i = 0; i < ACCS; ++i) acc[i] = 0;
+  auto add = [&](int32_t s, const v4i (&f)[LOADS], uint8_t *at) {
+    const uint32_t p = s == INT32_MIN ? 0u : shift_exp((int32_t)ix.any(s), a.frac_bits) & 0xffu;
+    psum += p;
+    at[16 / KS * c + kk] = (uint8_t)p;
+    __builtin_amdgcn_wave_barrier();
+    auto products = [&](auto of) {
+      if constexpr (QUADS) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int32_t w = of(*reinterpret_cast<const int32_t *>(at + 16 / KS * i + 4 * qd));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_sdot4(f[i][j], w, acc[j], false);
+        }
+      } else {
+        v4i w = *reinterpret_cast<const v4i *>(at + 16 * part);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = of(w[j]);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) acc[i] = dot16(f[i], w, acc[i]);
+      }
+    };
+    products([](int32_t w) { return w & 0x7f7f7f7f; });
+    if (wraps) {
+      products([](int32_t w) { return (w >> 1) & 0x40404040; });
+      products([](int32_t w) { return (w >> 1) & 0x40404040; });
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (wave + NW * i < nch) add(held[i], vf[i], sP[wave][i]);
+  } else {
+    v4i vn[LOADS];
+    const int first = c_lo + wave;
+    int32_t s0 = first < nch ? scores[64 * first + lane] : 0, s1 = 0;
+#pragma unroll 1
+    for (int ch = first; ch < nch; ch += 2 * NW) {
+      if (ch + NW < nch) load_v(ch + NW, vn), s1 = scores[64 * (ch + NW) + lane];
+      add(s0, vf[0], sP[wave][0]);
+      if (ch + 2 * NW < nch) load_v(ch + 2 * NW, vf[0]), s0 = scores[64 * (ch + 2 * NW) + lane];
+      if (ch + NW < nch) add(s1, vn, sP[wave][0]);
+    }
+  }
+
+  // the lanes' and then the waves' sums
+  psum = (uint32_t)dpp_sum((int32_t)psum);
+  if (lane == 0) sSum[wave] = psum;
+  if constexpr (QUADS) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (KS == 1) acc[j] += __shfl_xor(acc[j], 16);
+      acc[j] += __shfl_xor(acc[j], 32);
+    }
+    if (lane < LPQ) *reinterpret_cast<v4i *>(&sO[wave][4 * n]) = v4i{acc[0], acc[1], acc[2], acc[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < KS; ++i) sO[wave][64 * i + 16 * part + (lane >> 2)] = (uint32_t)sums_of_4(acc + 4 * i, lane);
+  }
+  lds_barrier();
+  if (4 * tid < D) {
+    v4i v = *reinterpret_cast<const v4i *>(&sO[0][4 * tid]);
+    uint32_t sum = sSum[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += *reinterpret_cast<const v4i *>(&sO[w][4 * tid]), sum += sSum[w];
+    if constexpr (MODE == PART_SUM) {
+      *reinterpret_cast<v4i *>(record + 4 * tid) = v;
+      if (tid == 0) record[64 * KS] = sum;
+      return;
+    }
+    const uint32_t sums[4] = {(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
+    *reinterpret_cast<uint32_t *>(a.out + b * a.o_sb + (int64_t)h * D + 4 * tid) =
+        output_word(a, sums, fisr((int32_t)sum, a.rsqrt_off));
+  }
+}
+
+// Adds a head's parts and finishes them: a wave a head, lane l has word l % W of parts l / W, l / W + 64 / W, ...
+template <int KS>
+__global__ __launch_bounds__(64) void attn_window_token_join_kernel(WindowArgs t, int parts) {
+  constexpr int W = 16 * KS, AT_ONCE = 64 / W;
+  const AttnArgs &a = t.a;
+  const int lane = threadIdx.x, w = lane % W, block = blockIdx.x, blocks = gridDim.x;
+  v4i sum{0, 0, 0, 0};
+  uint32_t psum = 0u;
+#pragma unroll 4
+  for (int p = lane / W; p < parts; p += AT_ONCE) {
+    const uint32_t *from = token_part(t, KS, blocks, block, p, parts);
+    sum += *reinterpret_cast<const v4i *>(from + 4 * min(w, a.D / 4 - 1));
+    psum += from[64 * KS];
+  }
+#pragma unroll
+  for (int m = W; m < 64; m *= 2) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], m);
+    psum += (uint32_t)__shfl_xor((int)psum, m);
+  }
+  const uint32_t sums[4] = {(uint32_t)sum[0], (uint32_t)sum[1], (uint32_t)sum[2], (uint32_t)sum[3]};
+  if (lane < a.D / 4)
+    *reinterpret_cast<uint32_t *>(a.out + block / a.H * a.o_sb + (int64_t)(block % a.H) * a.D + 4 * lane) =
+        output_word(a, sums, fisr((int32_t)psum, a.rsqrt_off));
+}
+
 // Word j of lane group g (16 lanes) becomes word g of lane group j
 __device__ __forceinline__ void transpose_groups(v4i &p) {
   const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)p[0], (uint32_t)p[2], false, false);
@@ -894,6 +1176,26 @@ int launch_window(const WindowArgs &t, hipStream_t s, int parts = 1) {
   return check_launch("attn_window_kernel");
 }
 
+template <int KS, bool QUADS, int NW, int NC, int MODE = ALL>
+int launch_window_token(const WindowArgs &t, int64_t chunks, hipStream_t s, int parts = 1) {
+  const int64_t blocks = (int64_t)t.a.B * t.a.H, per_xcd = (blocks + 7) / 8;
+  if (8 * per_xcd * 64 * NW >= 1LL << 32) return fail("too many heads and queries for one call");
+  hipLaunchKernelGGL((attn_window_token_kernel<KS, QUADS, NW, NC, MODE>), dim3((unsigned)(8 * per_xcd), (unsigned)parts),
+                     dim3(64 * NW), NC > 0 || MODE != ALL ? 0 : (unsigned)(256 * chunks), s, t, (int)blocks, (int)per_xcd, (int)chunks);
+  return check_launch("attn_window_token_kernel");
+}
+
+template <int KS, bool QUADS>
+int launch_token_parts(WindowArgs t, int64_t chunks, int parts, hipStream_t s) {
+  const int64_t blocks = (int64_t)t.a.B * t.a.H;
+  t.scores = blocks * chunks * 64;
+  int rc = launch_window_token<KS, true, 8, 0, PART_MAX>(t, chunks, s, parts);  // reads K only
+  if (rc == 0) rc = launch_window_token<KS, QUADS, 8, 0, PART_SUM>(t, chunks, s, parts);
+  if (rc) return rc;
+  hipLaunchKernelGGL((attn_window_token_join_kernel<KS>), dim3((unsigned)blocks), dim3(64), 0, s, t, parts);
+  return check_launch("attn_window_token_join_kernel");
+}
+
 template <int KS, bool QUADS>
 int launch_window_parts(const WindowArgs &t, int parts, hipStream_t s) {
   int rc = launch_window<KS, true, 8, 0, PART_MAX>(t, s, parts);  // reads K only
@@ -913,12 +1215,12 @@ int64_t most_chunks(int64_t queries, int64_t cap, int64_t before, int64_t after,
 }
 
 // Blocks that share the chunks of a tile. Three launches and the sums' way through memory are worth it where each
-// block is left with much less. One query of heads of 64 columns, us in one block of 8 waves and in parts:
-//   heads x parts    4096 keys      8192 keys      16384 keys
-//   8 x 8 to 32      14.4, 11.6     23.6, 12.3     45.1, 15.0
-//   64 x 4           17.7, 18.0     30.2, 25.7     60.1, 39.9
-//   120 x 2          19.6, 25.4     37.0, 40.2     84.7, 72.7
-// and of 128 columns 2048 keys: 26.2 and 14.9 for 8 heads, 27.2 and 20.3 for 64, 28.2 and 26.7 for 120 (1024 keys: 15.9
+// block is left with much less. 20 queries of heads of 64 columns, us in a block of 8 waves a tile and in parts:
+//   tiles x parts    4096 keys      8192 keys      16384 keys
+//   16 x 8 to 16     14.6, 12.2     23.8, 12.8     45.0, 15.9
+//   64 x 4           16.7, 15.8     27.7, 19.6     49.6, 27.2
+//   128 x 2          17.8, 20.0     29.8, 27.6     59.1, 43.6
+// and of 128 columns 2048 keys: 26.5 and 15.6 for 16 tiles, 27.4 and 19.5 for 64, 27.8 and 25.0 for 128 (1024 keys: 16.4
 // in one).
 constexpr int kCus = 256;
 int window_parts(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, int64_t before, int64_t after, int64_t sinks) {
@@ -926,6 +1228,24 @@ int window_parts(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, 
   const int64_t blocks = heads * ((queries + 15) / 16), chunks = most_chunks(queries, cap, before, after, sinks);
   const int64_t parts = std::min(kCus / blocks, (chunks + 7) / 8);
   return parts > 1 && parts * chunks > (head_dim <= 64 ? 256 : 64) ? (int)parts : 1;
+}
+
+// Chunks of one query: of keys in units of 16
+int64_t token_chunks(int64_t cap, int64_t before, int64_t after, int64_t sinks) {
+  const int64_t units = (std::min(cap, before + after + 1) + 14) / 16 + 1 + (std::min(sinks, cap) + 15) / 16;
+  return (std::min((cap + 15) / 16, units) + 3) / 4;
+}
+constexpr int64_t kTokenScores = 224;  // chunks whose scores fit a block's LDS
+// Blocks that share the chunks of one query's head, us in one block of 8 waves and so, 64 columns a head:
+//   heads x parts    2048 keys      4096 keys      8192 keys
+//   8 x 5 to 17      7.9, 9.6       11.4, 10.0     18.4, 9.9
+//   32 x 8           7.9, 10.1      14.9, 11.7     26.0, 15.2
+//   64 x 4           9.5, 11.8      15.3, 15.2     25.7, 19.9
+//   120 x 2          10.8, 15.0     16.7, 20.7     37.6, 36.0
+// (128 columns, 32 heads: 12.4 and 12.9, 21.3 and 16.1, 37.6 and 20.5)
+int token_parts(int64_t heads, int64_t chunks) {
+  const int64_t parts = std::min(kCus / heads, (chunks + 7) / 8);
+  return parts > 1 && parts * chunks > 256 ? (int)parts : 1;
 }
 
 // Which of the kernels, with the same results. Queries at the last positions share chunks in LDS where 64 of them a block
@@ -936,9 +1256,12 @@ int window_parts(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, 
 // Two tiles a wave pay where windows are long (16 rows of 20 heads of 1500 frames, all of them: 158 us with one, 142 with two;
 // 8192 positions with windows of 1024: 170 and 123; 1280 heads of 300, 512 keys: 359 and 315 with 128 columns, 141 and 152
 // with 64; 128 keys: 184 and 179, 79 and 91).
-// Else a wave holds its chunks where they are few: heads of 64, one query, 128 keys: 5.4 us in a loop and 5.2 so;
-// 384 keys, two chunks a wave, 6.2 and 5.8; 2560 heads of it 28.4 and 25.9. Eight waves take long windows faster if there
-// are few tiles: 1024 keys, 20 heads 8.9 and 7.6, 256 heads 12.0 and 11.1, 640 heads 22.4 and 25.3.
+// One query has its own kernel, a wave a chunk where there are few (quads, 64 columns, us with this and with the next: 20
+// heads of 128 keys, 4.5 and 5.3, of 384 keys, 5.3 and 5.9; 2560 heads of them 12.0 and 15.9, 23.0 and 26.8), else eight
+// waves (1024 keys, 20 heads 7.0 and 7.8, 2560 heads 65 and 85; four waves 8.4 and 68, sixteen 7.5 and 74).
+// Else a wave holds its chunks where they are few: 8 queries of 20 heads of 64, 128 keys, 5.5 us in a loop and 5.5 so, 2560
+// heads of 16 keys 14.2 and 12.5; 256 keys, two chunks a wave, 6.4 and 6.1. Eight waves take long windows
+// faster if there are few tiles: 1024 keys, 20 heads 9.1 and 7.8, 256 heads 12.1 and 11.1, 640 heads 22.7 and 25.4.
 template <int KS, bool QUADS>
 int launch_form(const WindowArgs &t, hipStream_t s) {
   const int64_t heads = (int64_t)t.a.B * t.a.H, tiles = (t.a.Tq + 15) / 16;
@@ -946,6 +1269,15 @@ int launch_form(const WindowArgs &t, hipStream_t s) {
     if (std::min<int64_t>(t.before + t.after, t.a.Tk) >= 7 * 64 && heads * ((tiles + 7) / 8) >= kCus)
       return launch_window_rows<KS, QUADS, 2>(t, s);
     if (heads * ((tiles + 3) / 4) >= (KS == 1 ? 2 : 1) * kCus) return launch_window_rows<KS, QUADS, 1>(t, s);
+  }
+  if (t.a.Tq == 1) {
+    const int64_t chunks = token_chunks(t.a.Tk, t.before, t.after, t.sinks);
+    const int parts = token_parts(heads, chunks);
+    if (parts > 1) return launch_token_parts<KS, QUADS>(t, chunks, parts, s);
+    if (chunks <= 1) return launch_window_token<KS, QUADS, 1, 1>(t, chunks, s);
+    if (chunks <= 4) return launch_window_token<KS, QUADS, 4, 1>(t, chunks, s);
+    if (chunks <= 8) return launch_window_token<KS, QUADS, 8, 1>(t, chunks, s);
+    if (chunks <= kTokenScores) return launch_window_token<KS, QUADS, 8, 0>(t, chunks, s);
   }
   const int parts = window_parts(heads, t.a.Tq, t.a.D, t.a.Tk, t.before, t.after, t.sinks);
   if (parts > 1) return launch_window_parts<KS, QUADS>(t, parts, s);
@@ -960,6 +1292,12 @@ int launch_form(const WindowArgs &t, hipStream_t s) {
 
 int64_t attn_window_workspace(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, int64_t before,
                               int64_t after, int64_t sinks) {
+  if (queries == 1) {
+    const int64_t chunks = token_chunks(cap, before, after, sinks);
+    const int parts = token_parts(heads, chunks);
+    if (parts > 1) return 4 * heads * (64 * chunks + parts * token_words(head_dim <= 64 ? 1 : 2));
+    if (chunks <= kTokenScores) return 0;
+  }
   const int64_t parts = window_parts(heads, queries, head_dim, cap, before, after, sinks);
   return parts == 1 ? 0 : 4 * heads * ((queries + 15) / 16) * parts * part_words(head_dim <= 64 ? 1 : 2);
 }

@@ -19,6 +19,7 @@ struct WindowArgs {
   int64_t before = 0, after = 0;       // keys before and after a query's position that it sees
   int32_t sinks = 0;                   // first keys that stay visible
   uint32_t *workspace = nullptr;       // attn_window_workspace bytes
+  int64_t scores = 0;                  // words of scores in it
 };
 // heads of all rows
 int64_t attn_window_workspace(int64_t heads, int64_t queries, int64_t head_dim, int64_t cap, int64_t before,

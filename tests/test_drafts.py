@@ -216,6 +216,38 @@ def test_window_long(iw, oracle, gpu, D, cap, N, before, layout):
         Window(N + D, 2, 2, D, cap, N, before, 0, 70, lengths=lengths, counts=[N, max(1, N - 1)], layout=layout).check(iw, oracle)
 
 
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("D", [16, 48, 64, 80, 128])
+@pytest.mark.parametrize("cap,before,after,sinks", [
+    (64, 15, 0, 0), (200, 0, 0, 1), (333, 127, 0, 4), (900, 100, 100, 20), (900, 400, 3, 0), (1500, 1000, 200, 40),
+    (1000, None, None, 0), (6000, 4500, 0, 33)])
+def test_window_one_query(iw, oracle, gpu, cap, before, after, sinks, D, layout):
+    """A token a row: first keys inside the window and beside it, positions before the first key and behind the last."""
+    print("case: window one query", cap, before, after, sinks, D, layout, flush=True)
+    r = gen.rng(cap + D)
+    lengths = [cap, cap - 1, 0, 1, 17, cap // 2, cap // 2 + 1, cap]
+    counts = [1, 1, 1, 1, 1, 1, 1, 0]
+    positions = [[cap - 1], [-5], [3], [0], [40], [cap // 3], [2 ** 31 - 1], [5]]
+    for given in (None, positions):
+        for scalars in (None, (255, 0, 7, 130, 9), (1, 0, 13, 90, 3)):
+            Window(int(r.integers(1 << 20)), 8, 2, D, cap, 1, before, after, sinks, lengths=lengths, counts=counts,
+                   positions=given, layout=layout, scalars=scalars).check(iw, oracle)
+
+
+@pytest.mark.parametrize("layout", ["vt", "quads"])
+@pytest.mark.parametrize("D,B,cap", [(16, 66, 16000), (80, 33, 16000), (64, 260, 700)])
+def test_window_one_query_many_heads(iw, oracle, gpu, D, B, cap, layout):
+    """A token of many rows, over more keys than a block keeps scores of too."""
+    print("case: window one query many heads", D, B, cap, layout, flush=True)
+    r = gen.rng(cap + D)
+    lengths = r.integers(0, cap + 1, B)
+    lengths[0] = cap
+    w = Window(D + B, B, 4, D, cap, 1, cap - 1000 if cap > 1000 else None, 0, 10, lengths=lengths, layout=layout)
+    rows = [0, 1, B // 2, B - 1]
+    got, want = host(w.run(iw)), w.expected(oracle, rows)
+    assert (got[rows] == want[rows]).all()
+
+
 @pytest.mark.parametrize("f", range(1, 14))
 @pytest.mark.parametrize("qk", [(255, 0), (1, 0), (200, 4), (3, 9), (255, 31), (255, 40), (0, 3)])
 def test_window_scalars(iw, oracle, gpu, f, qk):
