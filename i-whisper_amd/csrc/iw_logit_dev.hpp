@@ -115,11 +115,17 @@ struct Logit<float> : FloatMax<Logit<float>, 4> {
 template <uint32_t INF>
 struct Half {
   static constexpr int E = 8;
+  // the bits spread over the halves are opaque to the compiler, which makes a compare and a select of each otherwise
   static __device__ __forceinline__ void mask(uint4 &w, uint32_t off) {
     uint32_t *v = &w.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if ((off >> i) & 1u) v[i >> 1] = (i & 1) ? (v[i >> 1] & 0xffffu) | INF << 16 : (v[i >> 1] & 0xffff0000u) | INF;
+    for (int i = 0; i < 4; ++i) {
+      uint32_t lo, hi;
+      asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(lo) : "v"(off), "n"(2 * i));
+      asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(hi) : "v"(off), "n"(2 * i + 1));
+      const uint32_t no = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+      v[i] = (v[i] & ~no) | (INF * 0x10001u & no);
+    }
   }
 };
 template <>

@@ -110,17 +110,15 @@ __device__ __forceinline__ float clamp_uniform(float u) { return fminf(fmaxf(u, 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef v4u v4u_any __attribute__((aligned(1)));
 template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T *p) {
-  const v4u x = *reinterpret_cast<const v4u_any *>(p);
+__device__ __forceinline__ uint4 load_piece(const T *row, int piece) {
+  const v4u x = *reinterpret_cast<const v4u_any *>(reinterpret_cast<const char *>(row) + 16u * (uint32_t)piece);
   return make_uint4(x.x, x.y, x.z, x.w);
 }
 
-// The bits of the suppressed ones among n <= 16 columns from col on
-__device__ __forceinline__ uint32_t hidden_bits(const uint32_t *words, int col, int n, int cols) {
-  if (!words) return 0u;
-  const int i = col >> 5;
-  const uint64_t two = (uint64_t)words[min(i + 1, (cols - 1) >> 5)] << 32 | words[i];
-  return (uint32_t)(two >> (col & 31)) & ((1u << n) - 1u);
+// The bits of the suppressed ones among a piece's N columns from col on: they lie in one word
+template <int N>
+__device__ __forceinline__ uint32_t hidden_bits(const uint32_t *words, uint32_t col) {
+  return words ? (words[col >> 5] >> (col & 31)) & ((1u << N) - 1u) : 0u;
 }
 
 // A row as a distribution, as every launch looks at it. A temperature of 0 (or none at all) gives the first
@@ -190,14 +188,14 @@ struct SumWeights {
     const double mc = (double)m * c, whole = rint(mc);
     magic = 0x1.8p52 - whole;
     rest = fma((double)m, c, -whole);
-    least = (double)m - 1200.0 / c;
+    least = (double)m - 1200.0 * __builtin_amdgcn_rcp(c);
     fits = fabs(mc) < 0x1p40 && c > 0x1p-60;
   }
   __device__ __forceinline__ double of(float x) const {
     const double v = fmax((double)x, least), u = fma(v, c, magic), n = u - magic;
     return ldexp(exp2_part(fma(v, c, -n)), (int)(uint32_t)__double_as_longlong(u));
   }
-  __device__ __forceinline__ double scaled(double sum) const { return sum * exp2_64(-rest); }
+  __device__ __forceinline__ double scaled(double sum) const { return sum * exp2_part(-rest); }
 };
 
 template <typename T>
@@ -223,7 +221,7 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
   uint4 w[P];
   if (cut.full > 0) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) w[p] = load_piece(x + (int64_t)min(p0 + 64 * p, cut.full - 1) * E);
+    for (int p = 0; p < P; ++p) w[p] = load_piece(x, min(p0 + 64 * p, cut.full - 1));
   }
   const int extra = cut.full * E + lane;
   const bool has_extra = s == cut.spans - 1 && extra < a.cols && !suppressed(a.suppress, extra);
@@ -231,7 +229,7 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
   uint32_t off[P];  // not counted: past the last piece, or suppressed
 #pragma unroll
   for (int p = 0; p < P; ++p)
-    off[p] = p0 + 64 * p >= cut.full ? ALL : hidden_bits(a.suppress, (p0 + 64 * p) * E, E, a.cols);
+    off[p] = p0 + 64 * p >= cut.full ? ALL : hidden_bits<E>(a.suppress, (p0 + 64 * p) * E);
   const Row dist = second ? Row(a.d[1], outer) : Row(a.d[0], outer);
   if (I8) {
     if (!dist.greedy) fill_table(sTable, dist.c, tid);
@@ -450,15 +448,15 @@ template <typename T>
 __device__ __forceinline__ uint32_t piece_of(const T *x, int piece, const Cut<T> &cut, const uint32_t *suppress, float (&v)[Cut<T>::E]) {
   constexpr int E = Cut<T>::E;
   if (piece < cut.full) {
-    const uint4 w = load_piece(x + (int64_t)piece * E);
+    const uint4 w = load_piece(x, piece);
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = Logit<T>::get(w, e);
-    return ~hidden_bits(suppress, piece * E, E, cut.cols);
+    return ~hidden_bits<E>(suppress, piece * E);
   }
   const int left = max(cut.cols - piece * E, 0);  // fewer than E
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = e < left ? Logit<T>::one(x + (int64_t)piece * E + e) : 0.f;
-  return left > 0 ? ~hidden_bits(suppress, piece * E, E, cut.cols) & ((1u << left) - 1u) : 0u;
+  return left > 0 ? ~hidden_bits<E>(suppress, piece * E) & ((1u << left) - 1u) : 0u;
 }
 
 // a row's largest logit; its first column for rows that take it
