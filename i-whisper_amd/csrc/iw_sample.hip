@@ -122,14 +122,14 @@ __device__ __forceinline__ uint32_t hidden_bits(const uint32_t *words, uint32_t 
 }
 
 // A row as a distribution, as every launch looks at it. A temperature of 0 (or none at all) gives the first
-// of the largest logits all of the weight.
+// of the largest logits all of the weight. Logits lie 2^-149 apart at least: above 2^300, c makes no difference.
 struct Row {
   double c;
   bool greedy;
   __device__ __forceinline__ Row(const DistRows &d, int64_t outer) {
     const double t = d.temperatures ? (double)d.temperatures[outer] : d.temperature;
     greedy = !(t > 0.0);
-    c = greedy ? 0.0 : kLog2E * (d.scale / t);
+    c = greedy ? 0.0 : fmin(kLog2E * (d.scale / t), 0x1p300);
   }
 };
 template <typename T>
@@ -197,6 +197,29 @@ struct SumWeights {
   }
   __device__ __forceinline__ double scaled(double sum) const { return sum * exp2_part(-rest); }
 };
+
+// The first logit of a piece that is m, the largest, E or more if none: those that `off` hides are less, or m is int8's lowest
+template <typename T>
+__device__ __forceinline__ uint32_t first_with(const uint4 &w, uint32_t off, float m) {
+  constexpr int E = Logit<T>::E;
+  if constexpr (std::is_same<T, int8_t>::value) {
+    if (m == -128.f) return (uint32_t)__ffs((int)(~off & 0xffffu)) - 1u;
+    const uint32_t bits = Logit<T>::reaching(w, (int)m);  // bit 8 i + q: byte i of word q
+    uint32_t first = ~0u;
+#pragma unroll
+    for (int q = 3; q >= 0; --q) {
+      const uint32_t word = (bits >> q) & 0x01010101u;
+      if (word) first = 4u * q + ((uint32_t)(__ffs((int)word) - 1) >> 3);
+    }
+    return first;
+  } else {
+    uint32_t first = ~0u;
+#pragma unroll
+    for (int e = E - 1; e >= 0; --e)
+      if (Logit<T>::get(w, e) == m) first = e;
+    return first;
+  }
+}
 
 template <typename T>
 __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
@@ -276,10 +299,10 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
   if (dist.greedy) {
     uint32_t col = has_extra && xe == m ? (uint32_t)extra : ~0u;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!((off[p] >> e) & 1u) && L::get(w[p], e) == m) col = min(col, (uint32_t)((p0 + 64 * p) * E + e));
+    for (int p = P - 1; p >= 0; --p) {
+      const uint32_t first = first_with<T>(w[p], off[p], m);
+      if (first < (uint32_t)E) col = (uint32_t)((p0 + 64 * p) * E) + first;
+    }
     out.col = (int32_t)~wave_max_u32_dpp(~col);
   } else if (m - m == 0.f) {
     double z = 0.0;
@@ -294,10 +317,10 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
                                top - (w[p].w ^ 0x80808080u)};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const double a0 = *reinterpret_cast<const double *>(table + ((v[q] << 3) & 0x7f8u));
-          const double a1 = *reinterpret_cast<const double *>(table + ((v[q] >> 5) & 0x7f8u));
-          const double a2 = *reinterpret_cast<const double *>(table + ((v[q] >> 13) & 0x7f8u));
-          const double a3 = *reinterpret_cast<const double *>(table + ((v[q] >> 21) & 0x7f8u));
+          const double a0 = *reinterpret_cast<const double *>(table + (v[q] & 0xffu) * 8);
+          const double a1 = *reinterpret_cast<const double *>(table + ((v[q] >> 8) & 0xffu) * 8);
+          const double a2 = *reinterpret_cast<const double *>(table + ((v[q] >> 16) & 0xffu) * 8);
+          const double a3 = *reinterpret_cast<const double *>(table + ((v[q] >> 24) & 0xffu) * 8);
           z += (a0 + a1) + (a2 + a3);
         }
       }
@@ -329,118 +352,80 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
 }
 
 // ---- a row's block: from the spans to a token ----
-template <int W>
-struct Block {
-  double wave[W];
-  uint32_t max[W];
-  int owner;
-  int found;
-  double base;
+// The place in n numbers where their running sum passes u times the whole, and the sum below it; -1 if none is above 0. Only
+// numbers above 0 are asked, as rounding may lift the running sum over another; if none passes, the last of them. A wave
+// finds it by itself.
+struct Place {
+  int at;
+  double whole, target, below;
 };
-
-// The largest of every thread's values, in every thread
-template <int W>
-__device__ __forceinline__ uint32_t block_max(uint32_t v, Block<W> &s, int tid) {
-  v = wave_max_u32_dpp(v);
-  if ((tid & 63) == 0) s.max[tid >> 6] = v;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; ++w) v = max(v, s.max[w]);
-  __syncthreads();
-  return v;
-}
-
-// Which thread holds the place where the running sum of the threads' sums passes a target (made from the whole),
-// and the sum below it. Only threads with a sum are asked, as rounding may lift the running sum over one without.
-// If none passes, the last thread with a sum; -1 if there is none.
-template <int W, typename F>
-__device__ __forceinline__ int find_owner(double sum, F target_of, double *target, double *base, Block<W> &s, int tid) {
-  const int lane = tid & 63, wave = tid >> 6;
-  const double up = wave_scan_f64(sum);
-  if (tid == 0) s.owner = -1;
-  if (lane == 63) s.wave[wave] = up;
-  __syncthreads();
-  double below = 0.0, total = 0.0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (w == wave) below = total;
-    total += s.wave[w];
-  }
-  *target = target_of(total);
-  const uint64_t some = __ballot(sum > 0.0), passed = __ballot(sum > 0.0 && below + up > *target);
-  if (lane == 0 && passed != 0) atomicMax(&s.owner, (1 << 20) + (64 * W - 1 - (64 * wave + __ffsll((long long)passed) - 1)));
-  if (lane == 0 && some != 0) atomicMax(&s.owner, 64 * wave + 63 - __clzll((long long)some));
-  __syncthreads();
-  const int o = s.owner;
-  const int owner = o >= 1 << 20 ? 64 * W - 1 - (o - (1 << 20)) : o;
-  if (tid == owner) s.base = below + (up - sum);
-  __syncthreads();
-  *base = s.base;
-  __syncthreads();
-  return owner;
-}
-
-// The first of n numbers whose running sum from `base` passes target, else the last above 0, else 0; and the sum below it
 template <typename F>
-__device__ __forceinline__ int find_at(int n, double *base, double target, F value) {
-  int got = 0;
-  double run = *base;
-  for (int i = 0; i < n; ++i) {
-    const double v = value(i);
-    if (!(v > 0.0)) continue;
-    got = i;
-    *base = run;
-    run += v;
-    if (run > target) break;
+__device__ __forceinline__ Place place_of(int n, double u, F value, int lane) {
+  const double first = lane < n ? value(lane) : 0.0;
+  double sum = first;
+  for (int i = lane + 64; i < n; i += 64) sum += value(i);
+  Place r{-1, wave_sum_f64(sum), 0.0, 0.0};
+  r.target = u * r.whole;
+  double run = 0.0;
+  for (int i = 0; i < n; i += 64) {
+    const double v = i == 0 ? first : i + lane < n ? value(i + lane) : 0.0, up = run + wave_scan_f64(v);
+    const uint64_t some = __ballot(v > 0.0), passed = __ballot(v > 0.0 && up > r.target);
+    if (some != 0) {
+      const int l = passed != 0 ? __ffsll((long long)passed) - 1 : 63 - __clzll((long long)some);
+      r.at = i + l;
+      r.below = lane_f64(up - v, l);
+    }
+    if (passed != 0) break;
+    run = lane_f64(up, 63);
   }
-  return got;
+  return r;
 }
 
-// The token of a row whose `spans` spans of `pieces` pieces have the sums span_sum(s): the place of u times their sum,
-// found again among the weights of that span's logits, a piece a thread (weigh(piece, w): the weights of its columns, 0
-// past the last).
-template <typename T, int W, typename F, typename G>
-__device__ __forceinline__ int draw(int spans, int pieces, double u, F span_sum, G weigh, double *whole, Block<W> &s, int tid) {
+// The token at `place` among the spans of `pieces` pieces, which are looked at again, a piece a thread (weigh(piece, w):
+// the weights of its columns, 0 past the last), for the one thread that has it; -1 for the others.
+template <typename T, typename G>
+__device__ __forceinline__ int draw(const Place &place, int pieces, G weigh, double (&sWave)[kWaves], int tid) {
   constexpr int E = Cut<T>::E;
-  const int each = (spans + 64 * W - 1) / (64 * W), s0 = tid * each, n = clampi(spans - s0, 0, each);
-  double sum = 0.0;
-  for (int i = 0; i < n; ++i) sum += span_sum(s0 + i);
-  double target, base;
-  int owner = find_owner(sum, [&](double total) { *whole = total; return u * total; }, &target, &base, s, tid);
-  if (owner < 0) return -1;  // no weight at all
-  if (tid == owner) {
-    s.found = s0 + find_at(n, &base, target, [&](int i) { return span_sum(s0 + i); });
-    s.base = base;
-  }
-  __syncthreads();
-  const int span = s.found;
-  const double below = s.base;
-  __syncthreads();
-  double w[E];
-  sum = 0.0;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  double w[E], sum = 0.0;
   if (tid < pieces) {
-    weigh(span * pieces + tid, w);
+    weigh(place.at * pieces + tid, w);
 #pragma unroll
     for (int e = 0; e < E; ++e) sum += w[e];
   }
-  owner = find_owner(sum, [&](double) { return target - below; }, &target, &base, s, tid);
-  if (owner < 0) return -1;
-  if (tid == owner) {
-    // the first whose running sum passes, else the last with a weight
-    int got = 0;
-    bool passed = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (!passed && w[e] > 0.0) {
-        got = e;
-        base += w[e];
-        passed = base > target;
-      }
-    }
-    s.found = (span * pieces + tid) * E + got;
-  }
+  const double up = wave_scan_f64(sum), target = place.target - place.below;
+  if (lane == 63) sWave[wave] = up;
   __syncthreads();
-  return s.found;
+  // the wave whose sums pass the target, or the last with one
+  double run = 0.0, below = 0.0;
+  int owner = -1;
+  bool passed = false;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const double t = sWave[i];
+    if (!passed && t > 0.0) {
+      owner = i;
+      below = run;
+      passed = run + t > target;
+    }
+    run += t;
+  }
+  if (wave != owner) return -1;
+  const uint64_t some = __ballot(sum > 0.0), over = __ballot(sum > 0.0 && below + up > target);
+  if (lane != (over != 0 ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)some))) return -1;
+  // the first whose running sum passes, else the last with a weight
+  double base = below + (up - sum);
+  int got = 0;
+  passed = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (!passed && w[e] > 0.0) {
+      got = e;
+      base += w[e];
+      passed = base > target;
+    }
+  }
+  return (place.at * pieces + tid) * E + got;
 }
 
 // The logits of a piece, and the bits of those that count
@@ -459,21 +444,6 @@ __device__ __forceinline__ uint32_t piece_of(const T *x, int piece, const Cut<T>
   return left > 0 ? ~hidden_bits<E>(suppress, piece * E) & ((1u << left) - 1u) : 0u;
 }
 
-// a row's largest logit; its first column for rows that take it
-template <typename T, int W>
-__device__ __forceinline__ float row_max(const Span *spans, const Cut<T> &cut, bool greedy, int *col, Block<W> &s, int tid) {
-  uint32_t top = 0;
-  for (int i = tid; i < cut.spans; i += 64 * W) top = max(top, ordered(spans[i].m));
-  top = block_max(top, s, tid);
-  if (greedy) {
-    uint32_t c = 0;
-    for (int i = tid; i < cut.spans; i += 64 * W)
-      if (ordered(spans[i].m) == top) c = max(c, ~(uint32_t)spans[i].col);
-    *col = (int)~block_max(c, s, tid);
-  }
-  return key_value((uint64_t)top << 32);
-}
-
 // A span's sum relative to the row's largest logit; 0 where its logits' weights are next to vanishing, so that
 // a span with a sum has a logit with a weight.
 __device__ __forceinline__ double span_sum(const Span &s, const Weigh &row) {
@@ -481,39 +451,71 @@ __device__ __forceinline__ double span_sum(const Span &s, const Weigh &row) {
   return z > 1e-290 ? z : 0.0;
 }
 
+// A wave's look at a row's spans: the largest logit, and its first column for rows that take it. Lane l has span l;
+// more than 64 are read again.
+struct RowSpans {
+  const Span *spans;
+  int n, lane;
+  Span mine;
+  float m;
+  __device__ __forceinline__ RowSpans(const Span *spans_, int n_, int lane_) : spans(spans_), n(n_), lane(lane_) {
+    mine = Span{-INFINITY, -1, 0.0};
+    if (lane < n) mine = spans[lane];
+  }
+  __device__ __forceinline__ Span at(int i) const { return i == lane ? mine : spans[i]; }
+  __device__ __forceinline__ void find_max() {
+    uint32_t top = ordered(mine.m);
+    for (int i = lane + 64; i < n; i += 64) top = max(top, ordered(spans[i].m));
+    m = key_value((uint64_t)wave_max_u32_dpp(top) << 32);
+  }
+  __device__ __forceinline__ int column() const {
+    const uint32_t top = ordered(m);
+    uint32_t c = 0u;
+    for (int i = lane; i < n; i += 64)
+      if (ordered(at(i).m) == top) c = max(c, ~(uint32_t)at(i).col);
+    return (int)~wave_max_u32_dpp(c);
+  }
+};
+
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
   using L = Logit<T>;
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   __shared__ double sTable[I8 ? 256 : 1];
-  __shared__ Block<kWaves> s;
-  const int tid = threadIdx.x;
+  __shared__ double sWave[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const Cut<T> cut(a.cols);
+  RowSpans spans(static_cast<const Span *>(a.workspace) + row * cut.spans, cut.spans, lane);
+  const double u = (double)clamp_uniform(a.uniforms[row]);
   const Row dist(a.d, row);
-  const Span *spans = static_cast<const Span *>(a.workspace) + row * cut.spans;
   const T *x = row_of<T>(a.d, row, 0);
-  if (I8) fill_table(sTable, dist.c, tid);
+  spans.find_max();
+  const float m = spans.m;
   int tok = -1;
-  const float m = row_max(spans, cut, dist.greedy, &tok, s, tid);
   float lp = 0.f;
+  bool mine = tid == 0;
   if (!(m - m == 0.f)) {  // no distribution: a NaN, an infinity, nothing to choose from
-    tok = -1;
     lp = __uint_as_float(0x7fc00000u);
-  } else if (!dist.greedy) {
+  } else if (dist.greedy) {
+    tok = spans.column();
+  } else {
+    if (I8) fill_table(sTable, dist.c, tid);  // seen behind the barrier below
     const Weigh wt(dist.c, m, sTable);
-    double z = 0.0;
-    tok = draw<T>(cut.spans, kSpanPieces, (double)clamp_uniform(a.uniforms[row]), [&](int i) { return span_sum(spans[i], wt); },
-               [&](int piece, double (&w)[L::E]) {
-                 float v[L::E];
-                 const uint32_t on = piece_of(x, piece, cut, a.suppress, v);
+    const Place place = place_of(cut.spans, u, [&](int i) { return span_sum(spans.at(i), wt); }, lane);
+    if (I8) __syncthreads();
+    tok = draw<T>(place, kSpanPieces,
+                  [&](int piece, double (&w)[L::E]) {
+                    float v[L::E];
+                    const uint32_t on = piece_of(x, piece, cut, a.suppress, v);
 #pragma unroll
-                 for (int e = 0; e < L::E; ++e) w[e] = (on >> e) & 1u ? wt.of<T>(v[e]) : 0.0;
-               },
-               &z, s, tid);
-    if (tid == 0) lp = (float)(wt.log2_of(L::one(x + tok)) * kLn2 - log(z));
+                    for (int e = 0; e < L::E; ++e) w[e] = (on >> e) & 1u ? wt.of<T>(v[e]) : 0.0;
+                  },
+                  sWave, tid);
+    mine = tok >= 0;
+    if (mine) lp = (float)(wt.log2_of(L::one(x + tok)) * kLn2 - log(place.whole));
   }
-  if (tid == 0) {
+  if (mine) {
     a.tokens[row] = tok;
     if (a.logprob) a.logprob[row] = lp;
   }
@@ -535,25 +537,16 @@ struct RowSum {
   int32_t col;
   double z;
 };
-__device__ __forceinline__ RowSum row_sum(const Span *spans, int n, const Row &dist, int lane) {
-  const Span none{-INFINITY, -1, 0.0};
-  Span mine = lane < n ? spans[lane] : none;  // all of a row of 64 spans, the others are read again
-  uint32_t top = ordered(mine.m);
-  for (int i = lane + 64; i < n; i += 64) top = max(top, ordered(spans[i].m));
-  top = wave_max_u32_dpp(top);
-  RowSum r;
-  r.m = key_value((uint64_t)top << 32);
-  r.col = -1;
-  r.z = 1.0;
+__device__ __forceinline__ RowSum row_sum(const Span *from, int n, const Row &dist, int lane) {
+  RowSpans spans(from, n, lane);
+  spans.find_max();
+  RowSum r{spans.m, -1, 1.0};
   if (dist.greedy) {
-    uint32_t c = lane < n && ordered(mine.m) == top ? ~(uint32_t)mine.col : 0u;
-    for (int i = lane + 64; i < n; i += 64)
-      if (ordered(spans[i].m) == top) c = max(c, ~(uint32_t)spans[i].col);
-    r.col = (int32_t)~wave_max_u32_dpp(c);
+    r.col = spans.column();
   } else {
     const Weigh wt(dist.c, r.m, nullptr);
-    double z = span_sum(mine, wt);
-    for (int i = lane + 64; i < n; i += 64) z += span_sum(spans[i], wt);
+    double z = 0.0;
+    for (int i = lane; i < n; i += 64) z += span_sum(spans.at(i), wt);
     r.z = wave_sum_f64(z);
   }
   return r;
@@ -727,39 +720,39 @@ template <typename T>
 __global__ __launch_bounds__(NT) void verify_pick_kernel(VerifyArgs a) {
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   __shared__ double sP[I8 ? 256 : 1], sQ[I8 ? 256 : 1];
-  __shared__ Block<kWaves> s;
-  const int tid = threadIdx.x, N = a.nodes;
+  __shared__ double sWave[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, N = a.nodes;
   const int64_t b = blockIdx.x;
   const Cut<T> cut(a.cols);
   const VerifyWork work = verify_work(a, cut);
   Verdict v = work.verdict[b];
-  if (I8) {
-    fill_table(sP, v.c, tid);
-    if (v.mode == FROM_REST) fill_table(sQ, v.cq, tid);
-    __syncthreads();
-  }
-  int tok = v.mode == CERTAIN ? v.hot : -1;
   const double u = (double)clamp_uniform(a.uniforms[b * N + N - 1]);
-  const double *rests = work.rest + b * cut.parts;
-  const Span *spans = work.spans + (b * N + v.accepted) * cut.spans;
-  while (v.mode == FROM_TARGET || v.mode == FROM_REST || v.mode == FROM_OTHERS) {
-    const bool target = v.mode == FROM_TARGET;
+  int tok = v.mode == CERTAIN ? v.hot : -1;
+  bool mine = tid == 0;
+  if (v.mode == FROM_TARGET || v.mode == FROM_REST || v.mode == FROM_OTHERS) {
+    if (I8) {  // seen behind the barrier below
+      fill_table(sP, v.c, tid);
+      if (v.mode == FROM_REST) fill_table(sQ, v.cq, tid);
+    }
+    Place place{-1, 0.0, 0.0, 0.0};
+    if (v.mode != FROM_TARGET) {
+      const double *rests = work.rest + b * cut.parts;
+      place = place_of(cut.parts, u, [&](int i) { return rests[i]; }, lane);
+      if (place.at < 0) v.mode = FROM_TARGET;  // nothing is left: both are the same, or the draft is no token
+    }
     const Rest<T> rest(a, v, b, sP, sQ);
-    double whole;
-    tok = draw<T>(target ? cut.spans : cut.parts, target ? kSpanPieces : 64, u,
-                  [&](int i) { return target ? rest.ip * span_sum(spans[i], rest.p) : rests[i]; },
-                  [&](int at, double (&w)[Cut<T>::E]) { rest.piece(at, cut, w); }, &whole, s, tid);
-    if (tok >= 0 || target) break;
-    v.mode = FROM_TARGET;  // nothing is left: both are the same, or the draft is no token
-    __syncthreads();
+    const bool target = v.mode == FROM_TARGET;
+    if (target) {
+      const RowSpans spans(work.spans + (b * N + v.accepted) * cut.spans, cut.spans, lane);
+      place = place_of(cut.spans, u, [&](int i) { return rest.ip * span_sum(spans.at(i), rest.p); }, lane);
+    }
+    if (I8) __syncthreads();
+    tok = draw<T>(place, target ? kSpanPieces : 64, [&](int at, double (&w)[Cut<T>::E]) { rest.piece(at, cut, w); }, sWave, tid);
+    mine = tok >= 0;
   }
-  if (tid < N) {
-    int64_t c = -1;
-    if (tid < v.accepted) c = a.tokens[b * N + tid + 1];
-    if (tid == v.accepted) c = tok;
-    a.choice[b * N + tid] = c;
-  }
-  if (tid == 0) {
+  if (tid < N && tid != v.accepted) a.choice[b * N + tid] = tid < v.accepted ? a.tokens[b * N + tid + 1] : -1;
+  if (mine) {
+    if (v.accepted < N) a.choice[b * N + v.accepted] = tok;
     a.accepted[b] = v.accepted;
     a.next[b] = tok;
   }

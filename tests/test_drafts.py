@@ -468,6 +468,22 @@ def test_sample_temperatures_of_rows(iw, gpu, dtype):
     assert int(got.tokens[0]) == int(x[0].double().argmax()) and int(got.tokens[10]) == 0
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("t,scale", [(5e-324, 1.0), (1e-310, 2.0 ** 100), (1e-300, 1e-30), (2.0 ** 100, 1e-300)])
+def test_sample_extreme_temperatures(iw, gpu, t, scale, dtype):
+    """Next to no temperature leaves the largest logits, in equal shares; one that is all too high, all logits."""
+    print("case: sample extreme temperatures", t, scale, dtype, flush=True)
+    V, ties = 1000, [3, 500, 998, 999]
+    x = torch.full((64, V), -7.0)
+    x[:, ties] = 5.0
+    u = ((torch.arange(64) + 0.5) / 64).cuda()
+    got = iw.drafts.sample_tokens(x.to(DTYPES[dtype]).cuda(), u, temperature=t, scale=scale)
+    low = t > 1
+    want = [int((i + 0.5) / 64 * V) if low else ties[i // 16] for i in range(64)]
+    assert host(got.tokens).tolist() == want
+    assert np.allclose(host(got.logprob), -math.log(V if low else 4), rtol=1e-6, atol=0)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("V", [20, 3000, 70001])
 def test_sample_special_values(iw, gpu, V, dtype):
