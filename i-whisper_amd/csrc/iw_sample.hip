@@ -150,8 +150,9 @@ struct Weigh {
     return exp2_64(log2_of(x));
   }
 };
+template <int THREADS = NT>
 __device__ __forceinline__ void fill_table(double *table, double c, int tid) {
-  for (int d = tid; d < 256; d += NT) table[d] = exp2_64(-((double)d * c));
+  for (int d = tid; d < 256; d += THREADS) table[d] = exp2_64(-((double)d * c));
 }
 
 // A row's pieces, the last of them perhaps in part, and spans
@@ -221,8 +222,11 @@ __device__ __forceinline__ uint32_t first_with(const uint4 &w, uint32_t off, flo
   }
 }
 
+// Two waves a block: a row's last block has at most one without a span (one, two or four waves: 128 times 8 drafts of int8
+// logits 57, 56 and 61 us, 2048 int8 rows 46, 43 and 47; rows of the other types differ by a few in a hundred).
+constexpr int kSpanWaves = 2;
 template <typename T>
-__global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
+__global__ __launch_bounds__(64 * kSpanWaves) void row_spans_kernel(SpanArgs a, int groups) {
   using L = Logit<T>;
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   constexpr int E = L::E, P = kSpanPieces / 64;
@@ -236,7 +240,7 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
   const uint32_t outer = (uint32_t)r / inner, at = (uint32_t)r % inner;
   if (a.counts && (int)at >= a.counts[outer] - (second ? 1 : 0)) return;
   const Cut<T> cut(a.cols);
-  const int s = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int s = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kSpanWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
   const T *x = reinterpret_cast<const T *>(second ? a.d[1].x : a.d[0].x) +
                (int64_t)outer * (second ? a.d[1].sb : a.d[0].sb) + (int64_t)at * (second ? a.d[1].st : a.d[0].st);
   // all that the wave reads is on the way before it waits for anything; pieces past the last read that again
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(NT) void row_spans_kernel(SpanArgs a, int groups) {
     off[p] = p0 + 64 * p >= cut.full ? ALL : hidden_bits<E>(a.suppress, (p0 + 64 * p) * E);
   const Row dist = second ? Row(a.d[1], outer) : Row(a.d[0], outer);
   if (I8) {
-    if (!dist.greedy) fill_table(sTable, dist.c, tid);
+    if (!dist.greedy) fill_table<64 * kSpanWaves>(sTable, dist.c, tid);
     lds_barrier();
   }
   if (s >= cut.spans) return;
@@ -670,10 +674,14 @@ struct Rest {
     if (mode == FROM_REST) return left_of(w, share(q.of<T>(yv), iq));
     return mode == FROM_OTHERS && col == hot ? 0.0 : w;
   }
-  __device__ __forceinline__ void piece(int at, const Cut<T> &cut, double (&w)[Cut<T>::E]) const {
-    float xv[Cut<T>::E], yv[Cut<T>::E];
-    const uint32_t on = piece_of(x, at, cut, suppress, xv);
+  // a piece's logits in both rows, and its weights
+  float xv[Cut<T>::E], yv[Cut<T>::E];
+  uint32_t on;
+  __device__ __forceinline__ void load(int at, const Cut<T> &cut) {
+    on = piece_of(x, at, cut, suppress, xv);
     if (mode == FROM_REST) piece_of<T>(y, at, cut, nullptr, yv);
+  }
+  __device__ __forceinline__ void weigh(int at, double (&w)[Cut<T>::E]) const {
 #pragma unroll
     for (int e = 0; e < Cut<T>::E; ++e) w[e] = (on >> e) & 1u ? of(xv[e], mode == FROM_REST ? yv[e] : 0.f, at * Cut<T>::E + e) : 0.0;
   }
@@ -700,15 +708,18 @@ __global__ __launch_bounds__(NT) void verify_rest_kernel(VerifyArgs a, int group
   const VerifyWork work = verify_work(a, cut);
   const Verdict v = work.verdict[b];
   if (v.mode != FROM_REST && v.mode != FROM_OTHERS) return;
+  const int i = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
+  Rest<T> rest(a, v, b, sP, sQ);
+  const int at = 64 * i + (tid & 63);
+  rest.load(at, cut);
   if (I8) {
     fill_table(sP, v.c, tid);
     if (v.mode == FROM_REST) fill_table(sQ, v.cq, tid);
     lds_barrier();
   }
-  const int i = (int)((uint32_t)blockIdx.x % (uint32_t)groups) * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
   if (i >= cut.parts) return;
   double w[Cut<T>::E], z = 0.0;
-  Rest<T>(a, v, b, sP, sQ).piece(64 * i + (tid & 63), cut, w);
+  rest.weigh(at, w);
 #pragma unroll
   for (int e = 0; e < Cut<T>::E; ++e) z += w[e];
   z = wave_sum_f64(z);
@@ -740,14 +751,14 @@ __global__ __launch_bounds__(NT) void verify_pick_kernel(VerifyArgs a) {
       place = place_of(cut.parts, u, [&](int i) { return rests[i]; }, lane);
       if (place.at < 0) v.mode = FROM_TARGET;  // nothing is left: both are the same, or the draft is no token
     }
-    const Rest<T> rest(a, v, b, sP, sQ);
+    Rest<T> rest(a, v, b, sP, sQ);
     const bool target = v.mode == FROM_TARGET;
     if (target) {
       const RowSpans spans(work.spans + (b * N + v.accepted) * cut.spans, cut.spans, lane);
       place = place_of(cut.spans, u, [&](int i) { return rest.ip * span_sum(spans.at(i), rest.p); }, lane);
     }
     if (I8) __syncthreads();
-    tok = draw<T>(place, target ? kSpanPieces : 64, [&](int at, double (&w)[Cut<T>::E]) { rest.piece(at, cut, w); }, sWave, tid);
+    tok = draw<T>(place, target ? kSpanPieces : 64, [&](int at, double (&w)[Cut<T>::E]) { rest.load(at, cut), rest.weigh(at, w); }, sWave, tid);
     mine = tok >= 0;
   }
   if (tid < N && tid != v.accepted) a.choice[b * N + tid] = tid < v.accepted ? a.tokens[b * N + tid + 1] : -1;
@@ -760,9 +771,9 @@ __global__ __launch_bounds__(NT) void verify_pick_kernel(VerifyArgs a) {
 
 template <typename T>
 int launch_spans(SpanArgs a, int64_t rows, hipStream_t s) {
-  const int groups = (Cut<T>(a.cols).spans + kWaves - 1) / kWaves;
-  if (rows * groups >= (1LL << 32) / NT) return fail("too many logits for one call");
-  hipLaunchKernelGGL((row_spans_kernel<T>), dim3((unsigned)(rows * groups)), dim3(NT), 0, s, a, groups);
+  const int groups = (Cut<T>(a.cols).spans + kSpanWaves - 1) / kSpanWaves;
+  if (rows * groups >= (1LL << 32) / (64 * kSpanWaves)) return fail("too many logits for one call");
+  hipLaunchKernelGGL((row_spans_kernel<T>), dim3((unsigned)(rows * groups)), dim3(64 * kSpanWaves), 0, s, a, groups);
   return check_launch("row_spans_kernel");
 }
 
