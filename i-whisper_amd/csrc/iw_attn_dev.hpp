@@ -60,6 +60,14 @@ struct ScoreIndex {
     const uint32_t y = (uint32_t)(__mul24(s, fnm) + fK) - (uint32_t)__builtin_amdgcn_sbfe(s, 31, fw);
     return (uint32_t)med3i((int32_t)y >> fsh, flo, fhi);
   }
+  // The same for shifts of 1 .. 29: a score's upper byte is its sign, which one instruction subtracts. A key that took part
+  // in the maximum is at a distance of 1 at least, and needs no lower bound.
+  __device__ __forceinline__ uint32_t seen(int32_t s) const {
+    return (uint32_t)min((__mul24(s, fnm) + fK - (s >> 24)) >> fsh, fhi);
+  }
+  __device__ __forceinline__ uint32_t bounded(int32_t s) const {
+    return (uint32_t)med3i((__mul24(s, fnm) + fK - (s >> 24)) >> fsh, flo, fhi);
+  }
   // requant (24-bit product: |score| < 2^21 and an 8-bit multiplier),
   // round-half-away shift, int16 saturation
   __device__ __forceinline__ uint32_t any(int32_t s) const {

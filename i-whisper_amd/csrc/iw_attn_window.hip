@@ -336,7 +336,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(window_
   const int32_t rowmax = mx == INT32_MIN ? 0 : qk_requant16(mx, a.qk_m, a.qk_s);
   // The short index where no row maximum wraps and none is so low that saturated scores are near it: the keys that
   // count lie at a distance of 1 at least, the others are taken for such.
-  const bool brief = table && !__any(rowmax >= 32767 || rowmax < zero - 32768);
+  const bool brief = table && a.qk_s >= 1 && a.qk_s < 30 && !__any(rowmax >= 32767 || rowmax < zero - 32768);
 
   // ---- pass 2: P and P.V over this wave's keys ----
   v4i o[KS][4];
@@ -363,13 +363,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(window_
     v4i s[4], p;
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = scores(f[i]);
+    if (tile.whole(kc)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      p[i] = (int)pack4(sTable[ix.full(s[i][0])], sTable[ix.full(s[i][1])], sTable[ix.full(s[i][2])], sTable[ix.full(s[i][3])]);
-    if (!tile.whole(kc)) {
+      for (int i = 0; i < 4; ++i)
+        p[i] = (int)pack4(sTable[ix.seen(s[i][0])], sTable[ix.seen(s[i][1])], sTable[ix.seen(s[i][2])], sTable[ix.seen(s[i][3])]);
+    } else {
       const uint32_t ok = counted(kc);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = (int)keep_bytes((uint32_t)p[i], (ok >> (4 * i)) & 15u);
+      for (int i = 0; i < 4; ++i)
+        p[i] = (int)keep_bytes(pack4(sTable[ix.bounded(s[i][0])], sTable[ix.bounded(s[i][1])], sTable[ix.bounded(s[i][2])],
+                                     sTable[ix.bounded(s[i][3])]), (ok >> (4 * i)) & 15u);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) psum = __builtin_amdgcn_udot4((uint32_t)p[i], 0x01010101u, psum, false);
@@ -801,17 +804,22 @@ __device__ __forceinline__ void transpose_groups(v4i &p) {
 // Many queries at the row's last positions: a block has 16 * QT queries of each of its NW waves, whose windows
 // follow one another, and every wave goes through the chunks that any of them sees. A chunk is copied to LDS once a
 // block, as the register images of the products' operands (1 KB each, a lane's 16 bytes at 16 * lane, so reads have no
-// conflicts), two chunks ahead and without registers. First every chunk's K passes for the maxima, then K and V.
+// conflicts), a step ahead and without registers. First every chunk's K passes for the maxima, four chunks a step, then K
+// and V, two chunks a step (steps of one chunk, three of them in LDS: 143 us in the place of 136 for the case below).
 // Row 4g + r of score product i is key 16i + 4g + r: a product is 16 keys in a row, and at a window's borders those
 // that no query sees are left out and those that all see need no mask. Byte 4i + r of lane group g's P.V operand is
 // that key too, and V in quads has words of four keys. Transposed rows have 16 keys in a row, for which the lane groups
 // exchange their words of P.
+// A score takes an instruction for the maximum, a multiplication, three simple ones and a byte from the table for its
+// value, and P.V next to nothing: the vector units and the ways between them and LDS bound it. 16 rows of 20 heads of 1500
+// frames that see 511 and 16 others take 133 us, two thirds of them the vector units' own; its matrix products would
+// take 29. It needs its four waves a SIMD: with three and no spilled registers it takes 167.
 template <int KS, bool QUADS, int QT, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(KS, QT)))) void attn_window_rows_kernel(
     WindowArgs t, int qblocks, int blocks, int per_xcd, int table_off) {
-  constexpr int QW = 16 * QT, QR = QW * NW, SLOTS = 3, IMAGES = 4 * KS, PLACE = 2 * IMAGES * 1024;
+  constexpr int QW = 16 * QT, QR = QW * NW, IMAGES = 4 * KS, IMAGE = 1024, CHUNK = IMAGES * IMAGE, PLACE = 4 * CHUNK;
   static_assert(NW == 4, "each wave copies KS images of K and of V");
-  __shared__ __attribute__((aligned(1024))) int8_t sChunk[SLOTS * PLACE];
+  __shared__ __attribute__((aligned(1024))) int8_t sChunk[2 * PLACE];
   __shared__ __attribute__((aligned(16))) uint8_t sTable[kTableBytes];
 
   const int block = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
@@ -857,48 +865,40 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
   uint32_t koff[KS], voff[KS];
 #pragma unroll
   for (int w = 0; w < KS; ++w) koff[w] = k_at(w, 63), voff[w] = v_at(w, 63);
-  auto copy_chunk = [&](int kc, uint32_t to, bool with_v) {
-    const int8_t *kb = kbase + (int64_t)(64 * kc) * a.k_st;
-    const int8_t *vb = vbase + (QUADS ? (int64_t)(16 * kc) * a.v_sq : (int64_t)(64 * kc));
+  auto copy_k = [&](int kc, uint32_t to) {
+    const int8_t *base = kbase + (int64_t)(64 * kc) * a.k_st;
     const int last = len - 1 - 64 * kc;
-    if (last >= 63) {
 #pragma unroll
-      for (int w = 0; w < KS; ++w) dma16_lds(kb, koff[w], to + 1024 * (wave + NW * w));
-      if (with_v) {
+    for (int w = 0; w < KS; ++w) dma16_lds(base, last >= 63 ? koff[w] : k_at(w, last), to + IMAGE * (wave + NW * w));
+  };
+  auto copy_v = [&](int kc, uint32_t to) {
+    const int8_t *base = vbase + (QUADS ? (int64_t)(16 * kc) * a.v_sq : (int64_t)(64 * kc));
+    const int last = len - 1 - 64 * kc;
 #pragma unroll
-        for (int w = 0; w < KS; ++w) dma16_lds(vb, voff[w], to + 1024 * (IMAGES + wave + NW * w));
-      }
+    for (int w = 0; w < KS; ++w) dma16_lds(base, last >= 63 ? voff[w] : v_at(w, last), to + IMAGE * (wave + NW * w));
+  };
+  // The first steps have K of four chunks each, the others K and V of two. A barrier says that the copies of its step are
+  // there and that every wave is done with the one before, whose place those of the next take.
+  const int steps = (nch + 3) / 4, all_steps = steps + (nch + 1) / 2;
+  auto copy = [&](int s) {
+    const uint32_t to = lds0 + (s & 1) * PLACE;
+    if (s < steps) {
+#pragma unroll 1
+      for (int c = 4 * s; c < min(4 * s + 4, nch); ++c) copy_k(chunk_at(c), to + CHUNK * (c & 3));
     } else {
-#pragma unroll
-      for (int w = 0; w < KS; ++w) dma16_lds(kb, k_at(w, last), to + 1024 * (wave + NW * w));
-      if (with_v) {
-#pragma unroll
-        for (int w = 0; w < KS; ++w) dma16_lds(vb, v_at(w, last), to + 1024 * (IMAGES + wave + NW * w));
+      const int c0 = 2 * (s - steps);
+#pragma unroll 1
+      for (int c = c0; c < min(c0 + 2, nch); ++c) {
+        copy_k(chunk_at(c), to + 2 * CHUNK * (c & 1));
+        copy_v(chunk_at(c), to + 2 * CHUNK * (c & 1) + CHUNK);
       }
     }
   };
-  // Step s of 2 * nch is K of chunk s, or K and V of chunk s - nch; they are copied in turn, each to the next place.
-  int next = 0;
-  bool with_v = false;
-  uint32_t to = 0;
-  auto copy = [&]() {
-    copy_chunk(chunk_at(next), lds0 + to, with_v);
-    to = to == (SLOTS - 1) * PLACE ? 0 : to + PLACE;
-    if (++next == nch) next = 0, with_v = true;
-  };
-  // The copies of step s are there, those of step s + 1 may be on the way. The barrier also says that every wave is
-  // done with step s - 1, whose place step s + 2 takes.
-  uint32_t from = (SLOTS - 1) * PLACE;
+  uint32_t from = 0;
   auto arrive = [&](int s) {
-    if (s + 1 >= 2 * nch)
-      wait_vm<0>();
-    else if (s + 1 >= nch)
-      wait_vm<2 * KS>();
-    else
-      wait_vm<KS>();
+    wait_vm<0>();
     lds_barrier();
-    from = from == (SLOTS - 1) * PLACE ? 0 : from + PLACE;
-    if (s + 2 < 2 * nch) copy();
+    if (s + 1 < all_steps) copy(s + 1);
   };
 
   // ---- queries, and what they see ----
@@ -921,11 +921,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
   if (table)
     for (int i = 16 * tid; i <= zero; i += 16 * 64 * NW)
       *reinterpret_cast<uint4 *>(sTable + i) = *reinterpret_cast<const uint4 *>(kTables.v + table_off + i);
-  wait_vm<0>();  // the copies are counted from here on
-  if (nch > 0) {
-    copy();
-    copy();  // there are two steps at least
-  }
+  if (nch > 0) copy(0);
   // In products of 16 keys: those that any of this wave's queries sees a key of ([p_from, p_to) and below p_first), and
   // those that all see all of ([p_all, p_end))
   const int qe = min(qw + QW, cnt) - 1;
@@ -944,7 +940,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
     if (p0 < p_first) ok |= low4(seen[u].first - k);
     return ok;
   };
-  auto image = [&](int j) { return *reinterpret_cast<const v4i *>(&sChunk[from + 1024 * j + 16 * lane]); };
+  auto image = [&](int j) { return *reinterpret_cast<const v4i *>(&sChunk[from + IMAGE * j + 16 * lane]); };
   auto scores = [&](int i, v4i (&out)[QT]) {
 #pragma unroll
     for (int u = 0; u < QT; ++u) out[u] = v4i{0, 0, 0, 0};
@@ -969,7 +965,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
   };
 #pragma unroll 1
   for (int s = 0; s < nch; ++s) {
-    arrive(s);
+    if ((s & 3) == 0) arrive(s / 4);
+    from = (s / 4 & 1) * PLACE + CHUNK * (s & 3);
     const int p0 = 4 * chunk_at(s);
     if (!some(p0, 4)) continue;
     if (whole(p0, 4)) {
@@ -1009,7 +1006,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
   }
   // The short index where no row maximum wraps and none is so low that saturated scores are near it: the keys that
   // count lie at a distance of 1 at least, the others are taken for such.
-  const bool brief = table && !__any(sat);
+  const bool brief = table && a.qk_s >= 1 && a.qk_s < 30 && !__any(sat);
 
   // ---- pass 2: P and P.V ----
   v4i o[QT][KS][4];
@@ -1057,22 +1054,28 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
   for (int u = 0; u < QT; ++u) K[u] = ScoreIndex(a, rowmax[u], zero).fK;
   auto values = [&](const v4i &x, int u) {
     ix.fK = K[u];
-    return pack4(sTable[ix.full(x[0])], sTable[ix.full(x[1])], sTable[ix.full(x[2])], sTable[ix.full(x[3])]);
+    return pack4(sTable[ix.seen(x[0])], sTable[ix.seen(x[1])], sTable[ix.seen(x[2])], sTable[ix.seen(x[3])]);
+  };
+  auto some_values = [&](const v4i &x, int u) {
+    ix.fK = K[u];
+    return pack4(sTable[ix.bounded(x[0])], sTable[ix.bounded(x[1])], sTable[ix.bounded(x[2])], sTable[ix.bounded(x[3])]);
   };
 #pragma unroll 1
-  for (int s = nch; s < 2 * nch; ++s) {
-    arrive(s);
-    const int p0 = 4 * chunk_at(s - nch);
+  for (int s = 0; s < nch; ++s) {
+    if ((s & 1) == 0) arrive(steps + s / 2);
+    from = (steps + s / 2 & 1) * PLACE + 2 * CHUNK * (s & 1);
+    const int p0 = 4 * chunk_at(s);
     if (!some(p0, 4)) continue;
     v4i p[QT];
     if (brief) {
       if (whole(p0, 4)) {
+        v4i x[2][QT];
+        scores(0, x[0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v4i x[QT];
-          scores(i, x);
+          if (i < 3) scores(i + 1, x[(i + 1) & 1]);
 #pragma unroll
-          for (int u = 0; u < QT; ++u) p[u][i] = (int)values(x[u], u);
+          for (int u = 0; u < QT; ++u) p[u][i] = (int)values(x[i & 1][u], u);
         }
       } else {
 #pragma unroll
@@ -1083,11 +1086,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_wa
             v4i x[QT];
             scores(i, x);
 #pragma unroll
-            for (int u = 0; u < QT; ++u) p[u][i] = (int)values(x[u], u);
-            if (!whole(p0 + i, 1)) {
-#pragma unroll
-              for (int u = 0; u < QT; ++u) p[u][i] = (int)keep_bytes((uint32_t)p[u][i], counted(p0 + i, u));
-            }
+            for (int u = 0; u < QT; ++u) p[u][i] = (int)keep_bytes(some_values(x[u], u), counted(p0 + i, u));
           }
       }
       add_pv(p);
@@ -1249,13 +1248,13 @@ int token_parts(int64_t heads, int64_t chunks) {
 }
 
 // Which of the kernels, with the same results. Queries at the last positions share chunks in LDS where 64 of them a block
-// fill the device: heads of 128 columns from a block a CU on, of 64 columns from two (us of a block a 16-query tile and
-// so, windows of 512 keys: 20 heads of 1500 queries, 480 blocks, 54.5 and 30.0 with 128 columns, 23.0 and 22.2 with 64;
-// 64 of 300, 320 blocks, 37.1 and 29.7, 16.4 and 21.9; 64 of 128, 128 blocks, 18.1 and 23.0, 9.9 and 16.4), but not for 32
-// queries or fewer (1280 heads of 32: 78.8 and 87.2, 30.6 and 33.1; of 64: 137 and 90, 54 and 36).
-// Two tiles a wave pay where windows are long (16 rows of 20 heads of 1500 frames, all of them: 158 us with one, 142 with two;
-// 8192 positions with windows of 1024: 170 and 123; 1280 heads of 300, 512 keys: 359 and 315 with 128 columns, 141 and 152
-// with 64; 128 keys: 184 and 179, 79 and 91).
+// fill the device: heads of 128 columns from a block a CU on, of 64 columns from one and a half (us of a block a 16-query
+// tile and so, windows of 512 keys, with 64 and 128 columns: 20 heads of 1500 queries, 480 blocks, 22.9 and 20.4, 54.5 and
+// 28.7; 64 of 300, 320 blocks, 15.6 and 16.9, 34.4 and 24.9; 64 of 128, 128 blocks, 9.0 and 14.2, 18.5 and 23.2), but not
+// for 32 queries or fewer (1280 heads of 32: 34.4 and 38.1, 56.0 and 54.2; of 64: 45.2 and 32.5, 126 and 76).
+// Two tiles a wave pay where windows are longer and their 128 queries a block fill the device too (320 heads of 1500
+// queries with 64 and 128 columns, one tile and two: 256 keys 111 and 101, 253 and 203; 512 keys 145 and 129, 343 and 265;
+// 1280 of 300 with 128 keys 78 and 85, 171 and 173; of 64 with 512 keys, half of a block, 32.5 and 38.8, 76 and 91).
 // One query has its own kernel, a wave a chunk where there are few (quads, 64 columns, us with this and with the next: 20
 // heads of 128 keys, 4.5 and 5.3, of 384 keys, 5.3 and 5.9; 2560 heads of them 12.0 and 15.9, 23.0 and 26.8), else eight
 // waves (1024 keys, 20 heads 7.0 and 7.8, 2560 heads 65 and 85; four waves 8.4 and 68, sixteen 7.5 and 74).
@@ -1266,9 +1265,9 @@ template <int KS, bool QUADS>
 int launch_form(const WindowArgs &t, hipStream_t s) {
   const int64_t heads = (int64_t)t.a.B * t.a.H, tiles = (t.a.Tq + 15) / 16;
   if (!t.positions && t.a.Tq > 32) {
-    if (std::min<int64_t>(t.before + t.after, t.a.Tk) >= 7 * 64 && heads * ((tiles + 7) / 8) >= kCus)
+    if (std::min<int64_t>(t.before + t.after, t.a.Tk) >= 3 * 64 && t.a.Tq > 96 && heads * ((tiles + 7) / 8) >= kCus)
       return launch_window_rows<KS, QUADS, 2>(t, s);
-    if (heads * ((tiles + 3) / 4) >= (KS == 1 ? 2 : 1) * kCus) return launch_window_rows<KS, QUADS, 1>(t, s);
+    if (2 * heads * ((tiles + 3) / 4) >= (KS == 1 ? 3 : 2) * kCus) return launch_window_rows<KS, QUADS, 1>(t, s);
   }
   if (t.a.Tq == 1) {
     const int64_t chunks = token_chunks(t.a.Tk, t.before, t.after, t.sinks);
