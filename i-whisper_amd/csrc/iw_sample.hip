@@ -448,9 +448,11 @@ __device__ __forceinline__ uint32_t piece_of(const T *x, int piece, const Cut<T>
   return left > 0 ? ~hidden_bits<E>(suppress, piece * E) & ((1u << left) - 1u) : 0u;
 }
 
-// A span's sum relative to the row's largest logit; 0 where its logits' weights are next to vanishing, so that
+// A span's sum relative to the row's largest logit (as it is where that is the span's: the polynomial's 1 is off by
+// 2.4e-13, and numbers like 1/2 are drawn at the borders of equal logits); 0 where its logits' weights are next to vanishing, so that
 // a span with a sum has a logit with a weight.
 __device__ __forceinline__ double span_sum(const Span &s, const Weigh &row) {
+  if (s.m == row.m) return s.z;
   const double z = s.z * exp2_64(row.log2_of(s.m));
   return z > 1e-290 ? z : 0.0;
 }
