@@ -1156,7 +1156,7 @@ int iw_attention_window(const iw_attention_window_args *args, iw_stream_t stream
   if (rc) return rc;
   IW_REQUIRE(p.queries >= 0 && p.queries <= (1 << 24), "at most 2^24 queries of a row");
   IW_REQUIRE(p.batch >= 0 && p.batch <= (1 << 22) && p.batch * p.heads <= (1 << 22) && p.positions_sb >= 0 &&
-                 p.batch * p.heads * ((p.queries + 15) / 16) < (1 << 25),
+                 p.batch * p.heads * ((p.queries + 15) / 16) <= (1 << 24) - 8,
              "invalid attention shape");
   IW_REQUIRE(p.before >= 0 && p.before <= INT32_MAX && p.after >= 0 && p.after <= INT32_MAX && p.sinks >= 0 &&
                  p.sinks <= INT32_MAX,

@@ -727,7 +727,7 @@ int64_t iw_token_logprobs_workspace(int32_t type, int64_t rows, int64_t cols, in
  * base + b*sb + i*st + h*head_dim + d; K and V as iw_attention_tree takes them
  * (K of projected rows has k_sh = head_dim), scalars as there. Rows of queries past the count, and
  * of queries that see no key, are zeros. queries <= 2^24, head_dim % 16 == 0, head_dim
- * <= 128, cache_positions < 2^24, batch * heads <= 2^22, fewer than 2^25 blocks of 16
+ * <= 128, cache_positions < 2^24, batch * heads <= 2^22, at most 2^24 - 8 tiles of 16
  * queries; before, after and sinks in [0, 2^31); operands and strides are multiples
  * of 16 bytes; k_st, v_sd, v_sq < 2^25. out is q itself or shares no memory with q,
  * K or V; it may lie in other columns of rows of K with its strides. workspace:
@@ -763,7 +763,8 @@ int64_t iw_attention_window_workspace(int64_t batch, int64_t heads, int64_t quer
  * scalar temperature; where it is not above 0 the token is the first of the
  * largest logits, with logprob 0. uniforms are clamped to [0, 1 - 2^-24], a NaN is 0. A
  * row with a NaN or +inf, or without any finite logit, gives token -1 and logprob NaN.
- * logits: type as iw_token_logprobs, row stride ld. Weights and sums are 64-bit. rows <=
+ * logits: type as iw_token_logprobs, row stride ld. Weights and sums are 64-bit, a
+ * weight off by at most 8e-13 of itself. rows <=
  * 2^22, cols < 2^23. workspace: iw_sample_tokens_workspace bytes, 16-byte aligned,
  * used during the call's work only. The struct is read during the call. */
 typedef struct iw_sample_tokens_args {
