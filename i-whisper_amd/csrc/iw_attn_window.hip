@@ -117,8 +117,8 @@ struct Tile {
   int ns, w0, nch, start, end, first, all_from, all_to;
   __device__ __forceinline__ int at(int c) const { return c < ns ? c : w0 + c - ns; }
   __device__ __forceinline__ bool whole(int kc) const { return 64 * kc >= all_from && 64 * kc + 64 <= all_to; }
-  // The first and last key of the chunk at kc that any of them sees: no others are read (2560 heads of 128: one query a
-  // tile, 128 keys and four first ones, 16.3 us with whole chunks, 15.6 so; 257 frames, 35.8 and 31.4).
+  // The first and last key of the chunk at kc that any of them sees: no others are read (2560 heads of 64, one query a
+  // tile: 128 keys and four first ones 16.3 us with whole chunks, 15.6 so; 257 frames 35.8 and 31.4).
   __device__ __forceinline__ int low(int kc) const { return 64 * kc < first ? 0 : max(start - 64 * kc, 0); }
   __device__ __forceinline__ int high(int kc) const { return min((kc < w0 ? first : end) - 64 * kc, 64) - 1; }
 };
@@ -813,7 +813,7 @@ __device__ __forceinline__ void transpose_groups(v4i &p) {
 // A score takes an instruction for the maximum, a multiplication, three simple ones and a byte from the table for its
 // value, and P.V next to nothing: the vector units and the ways between them and LDS bound it. 16 rows of 20 heads of 1500
 // frames that see 511 and 16 others take 133 us, two thirds of them the vector units' own; its matrix products would
-// take 29. It needs its four waves a SIMD: with three and no spilled registers it takes 167.
+// take 29. It needs its four waves a SIMD: with three and no spilled registers (8 now, between the passes) it takes 167.
 template <int KS, bool QUADS, int QT, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(KS, QT)))) void attn_window_rows_kernel(
     WindowArgs t, int qblocks, int blocks, int per_xcd, int table_off) {
