@@ -766,8 +766,9 @@ __global__ __launch_bounds__(64 * NW) void attn_window_token_kernel(WindowArgs t
   }
 }
 
-// Adds a head's parts and finishes them (a launch: added in memory by the parts and finished by the last of them, the
-// fences between dies that this takes made it 47 us in the place of 16 for 32 heads of 4096 keys): a wave a head, lane l has word l % W of parts l / W, l / W + 64 / W, ...
+// Adds a head's parts and finishes them (added in memory by the parts and finished by the last of them, the fences
+// between dies that this takes made it 47 us in the place of 16 for 32 heads of 4096 keys): a wave a head, lane l has
+// word l % W of parts l / W, l / W + 64 / W, ...
 template <int KS>
 __global__ __launch_bounds__(64) void attn_window_token_join_kernel(WindowArgs t, int parts) {
   constexpr int W = 16 * KS, AT_ONCE = 64 / W;
