@@ -1,11 +1,12 @@
 """The operators of sampled decoding at the ends of what they take: workspaces of any content, caches in
-other orders, keys beyond 32-bit offsets, the widest vocabularies and the most rows, graphs on two streams."""
+other orders, keys beyond 32-bit offsets, the widest vocabularies and the most rows, graphs on two streams,
+a decoder on its device and in a graph."""
 import numpy as np
 import pytest
 import torch
 
 from tests import gen
-from tests.test_drafts import DTYPES, T, Window, check_samples, check_verdict, host, make_drafts, make_logits
+from tests.test_drafts import DTYPES, T, Window, check_samples, check_verdict, host, make_drafts, make_logits, small_model
 from tests.test_speculative_sizes import reordered
 
 pytestmark = pytest.mark.gpu
@@ -180,3 +181,88 @@ def test_graphs_on_two_streams(iw, oracle, gpu):
         torch.cuda.synchronize()
         for _, outs, want, *_ in runs:
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_draft_decoder_launches_on_its_device(iw, gpu, monkeypatch):
+    """Every launch of a decoder's start and step is made with the tensors' device as the current
+    one, whichever is current outside."""
+    print("case: draft decoder's device", flush=True)
+    dims, model = small_model(iw)
+    mel = iw.synth.synthetic_mel(1, dims.n_mels, 2 * dims.n_audio_ctx, seed=24)
+    entered, outside, streams, own = [], [], [], []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            entered.pop()
+            return super().__exit__(*a)
+    with torch.no_grad():
+        runner = iw.DecoderRunner(model.decoder, 1, dims.n_audio_ctx)
+        runner.set_audio(model.embed_audio(T(mel)))
+        dec = iw.drafts.DraftDecoder(runner, 3, window=2, audio=8)
+        call, launch = iw._lib.call, iw.speculative._launch
+
+        def counted(name, *args):
+            streams.append(name)
+            if not own and entered[-1:] != [0]:  # _launch turns to the tensors' device itself
+                outside.append(name)
+            return call(name, *args)
+
+        def launching(*args):
+            own.append(1)
+            try:
+                return launch(*args)
+            finally:
+                own.pop()
+        monkeypatch.setattr(torch.cuda, "device", Device)
+        monkeypatch.setattr(iw._lib, "call", counted)
+        monkeypatch.setattr(iw.speculative, "_launch", launching)
+        monkeypatch.setattr(iw.drafts, "_launch", launching)
+        frames = torch.tensor([5], dtype=torch.int32, device="cuda")
+        last = dec.start(T(np.array([[1, 2, 3]], np.int64)), torch.rand(1, device="cuda"))
+        dec.step(last, torch.rand((1, 5), device="cuda"), frames=frames)
+        torch.cuda.synchronize()
+    assert {"iw_attention_window", "iw_sample_tokens", "iw_verify_drafts"} <= set(streams)
+    assert outside == []
+
+
+def test_draft_step_captured(iw, gpu):
+    """A decoder's whole step as a graph: replays give what eager steps of a second decoder give."""
+    print("case: captured step", flush=True)
+    dims, model = small_model(iw)
+    mel = T(iw.synth.synthetic_mel(2, dims.n_mels, 2 * dims.n_audio_ctx, seed=25))
+    prompt = T(np.array([[1, 2, 3], [4, 5, 6]], np.int64))
+    r = gen.rng(9)
+    first, u = T(r.random(2, np.float32)), [T(r.random((2, 5), np.float32)) for _ in range(6)]
+    with torch.no_grad():
+        def decoder():
+            runner = iw.DecoderRunner(model.decoder, 2, dims.n_audio_ctx)
+            runner.set_audio(model.embed_audio(mel))
+            dec = iw.drafts.DraftDecoder(runner, 3, window=4)
+            return dec, dec.start(prompt, first, 0.9)
+        dec, last = decoder()
+        want = []
+        for x in u:
+            res = dec.step(last, x, 0.9)
+            last = res.accept.next_token
+            want.append([a.clone() for a in (*res.verdict, last, dec.lengths)])
+        dec, last = decoder()
+        now, x = last.clone(), u[0].clone()
+        res = dec.step(now, x, 0.9)  # the first step, outside the graph
+        got = [[a.clone() for a in (*res.verdict, res.accept.next_token, dec.lengths)]]
+        now.copy_(res.accept.next_token)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = dec.step(now, x, 0.9)
+        for i in range(1, len(u)):
+            x.copy_(u[i])
+            g.replay()
+            torch.cuda.synchronize()
+            got.append([a.clone() for a in (*res.verdict, res.accept.next_token, dec.lengths)])
+            now.copy_(res.accept.next_token)
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
