@@ -157,6 +157,12 @@ class DraftVerdict(NamedTuple):
     accepted: Tensor    # int32 [B]: the number of drafts accepted (0 .. N - 1)
     next_token: Tensor  # int64 [B]: the token after them, -1 for none
 
+    def nodes(self, counts: Optional[Tensor] = None) -> Tensor:
+        """int32 [B]: each row's nodes up to its last accepted draft, the ``counts`` of ``TreeCaches.accept``;
+        ``counts`` are those that ``verify_drafts`` was given."""
+        taken = self.accepted + 1
+        return taken if counts is None else torch.minimum(taken, counts)
+
 
 def _node_logits(logits: Tensor, shape, name: str, dev: int) -> Tuple[int, int]:
     """(batch, node) strides of logits [B, N, vocab] with contiguous rows."""
@@ -186,9 +192,10 @@ def verify_drafts(logits: Tensor, tokens: Tensor, draft_logits: Optional[Tensor]
 
     ``temperature`` (one, or float32 [B]; 0: the first of the largest logits) and ``scale`` are those of
     ``sample_tokens``, for the drafts ``draft_temperature`` and ``draft_scale`` (None: the same);
-    ``suppress`` counts for both. ``choice`` is what ``TreeCaches.accept`` takes for the chain of the
-    nodes. A row whose next token has no distribution (NaN, +inf, no finite logit) gives -1, and so
-    does one without nodes."""
+    ``suppress`` counts for both. A row whose next token has no distribution (NaN, +inf, no finite logit)
+    gives -1, and so does one without nodes; a draft whose logits have none is refused, and the token drawn
+    from p may be that draft again. So ``TreeCaches.accept`` takes ``choice`` for the chain of the nodes
+    together with ``nodes(counts)`` of the verdict, which end where the accepted drafts do."""
     kind = _logit_type(logits, "logits", "[batch, nodes, vocab]")
     if logits.dim() != 3 or not 1 <= logits.shape[1] <= MAX_NODES or logits.shape[2] < 1:
         raise RuntimeError(f"logits must be [batch, nodes, vocab] with 1 to {MAX_NODES} nodes")
@@ -360,6 +367,6 @@ class DraftDecoder:
         verdict = verify_drafts(logits, tokens, self.draft_logits.transpose(0, 1) if n > 1 else None,
                                 uniforms[:, n - 1:].contiguous(), temperature=temperature, scale=self.runner.logit_scale,
                                 suppress=self.suppress)
-        got = self.tree.caches.accept(tokens, self.parents, verdict.choice, self.lengths, eot=eot)
+        got = self.tree.caches.accept(tokens, self.parents, verdict.choice, self.lengths, verdict.nodes(), eot=eot)
         self.lengths.add_(got.accepted)
         return DraftStep(tokens.clone(), verdict, got)

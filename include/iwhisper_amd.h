@@ -793,7 +793,9 @@ int64_t iw_sample_tokens_workspace(int32_t type, int64_t rows, int64_t cols);
  *   max(p_a - q_a, 0) where a draft was refused (from p_a where nothing is left of
  *   it), else from p_a.
  * So the tokens are distributed as p whatever q is. choice[b][i] = tokens[b][i + 1]
- * for i < a, next[b] for i = a, then -1: what iw_tree_accept takes for a chain. A row
+ * for i < a, next[b] for i = a, then -1: what iw_tree_accept takes for a chain, with
+ * min(a + 1, counts[b]) as its counts. (Without those it may pass node a: next[b] can be -1, as can a
+ * draft, or the draft that was refused.) A row
  * without nodes has a = 0 and next -1, and so has one whose p_a has a NaN or +inf or no finite
  * logit; a token outside the vocabulary has probability 0, a draft row without a
  * distribution is refused and leaves p. tokens, uniforms (float32), choice [batch][nodes], accepted,
