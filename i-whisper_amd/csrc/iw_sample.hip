@@ -42,21 +42,21 @@ struct Span {
   double z;
 };
 
-// 2^f for |f| <= 1/2: the polynomial of degree 8 with the smallest relative error, 7.8e-13 (found by exchange; a
-// degree more or less, 1.4e-14 or 4.0e-11). A vocabulary of 2^16 tokens has its borders right to 8e-13 of the whole then,
-// and 4e-8 of all numbers would draw another token than exact ones.
+// 2^f for |f| <= 1/2: of the polynomials of degree 8 that are 1 at 0 the one with the smallest relative error, 8.14e-13
+// (found by linear programming; 7.8e-13 without that condition, a degree more or less 1.4e-14 or 4.0e-11). The
+// largest logit's weight is 1 exactly, so equal ones have exact sums and meet at exact borders.
 __device__ __forceinline__ double exp2_part(double f) {
   // the two constants of the first step: an instruction reads one from scalar registers
-  double second = 0x1.00dad2504eb63p-16;
+  double second = 0x1.00d8533f3e35fp-16;
   asm("" : "+v"(second));
-  double p = fma(0x1.61afcebb0e8b4p-20, f, second);
-  p = fma(p, f, 0x1.430acca346a3ep-13);
-  p = fma(p, f, 0x1.5d874838559edp-10);
-  p = fma(p, f, 0x1.3b2ab5c52926cp-7);
-  p = fma(p, f, 0x1.c6b08dd46d391p-5);
-  p = fma(p, f, 0x1.ebfbdff9319e1p-3);
-  p = fma(p, f, 0x1.62e42fef8615ep-1);
-  return fma(p, f, 0x1.ffffffffff7a3p-1);
+  double p = fma(0x1.61c4f11ba3bb2p-20, f, second);
+  p = fma(p, f, 0x1.430aa882746bep-13);
+  p = fma(p, f, 0x1.5d874d0702cb5p-10);
+  p = fma(p, f, 0x1.3b2ab5ed6ffb2p-7);
+  p = fma(p, f, 0x1.c6b08dced351ap-5);
+  p = fma(p, f, 0x1.ebfbdff8ede81p-3);
+  p = fma(p, f, 0x1.62e42fef89d1ep-1);
+  return fma(p, f, 1.0);
 }
 // 2^t, 0 far below. A NaN (a masked logit of a row that has no other) gives 0.
 __device__ __forceinline__ double exp2_64(double t) {
@@ -180,23 +180,18 @@ struct SpanArgs {
 // The larger of two, NaN where either is
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Sum of 2^((x - m) c) as 2^(x c - M) * 2^(M - m c), M = m c as a whole number: a constant's low word counts the exponents, and
-// the part beyond the whole number is exact, so a logit takes 14 instructions. `least` stands for -inf: its weight is 0.
+// Adds the weight 2^((x - m) c) of a span's logit to its sum: a constant's low word counts the exponents, with which the
+// rest's power is multiplied in the addition. Weights below 2^-1000, -inf's too, are 2^-1000, which a sum with the largest's 1
+// does not hold. The distance comes first, so that the largest's weight is 1 exactly.
 struct SumWeights {
-  double c, magic, rest, least;
-  bool fits;
-  __device__ __forceinline__ SumWeights(double c_, float m) : c(c_) {
-    const double mc = (double)m * c, whole = rint(mc);
-    magic = 0x1.8p52 - whole;
-    rest = fma((double)m, c, -whole);
-    least = (double)m - 1200.0 * __builtin_amdgcn_rcp(c);
-    fits = fabs(mc) < 0x1p40 && c > 0x1p-60;
+  double c, m, least;
+  __device__ __forceinline__ SumWeights(double c_, float m_)
+      : c(fmax(c_, 0x1p-900)), m(m_), least(-1000.0 * __builtin_amdgcn_rcp(c)) {}
+  __device__ __forceinline__ double add(float x, double sum) const {
+    const double d = fmax((double)x - m, least), u = fma(d, c, 0x1.8p52 + 1023.0), n = u - (0x1.8p52 + 1023.0);
+    const double whole = __longlong_as_double((long long)((uint64_t)((uint32_t)__double_as_longlong(u) << 20) << 32));
+    return fma(exp2_part(fma(d, c, -n)), whole, sum);
   }
-  __device__ __forceinline__ double of(float x) const {
-    const double v = fmax((double)x, least), u = fma(v, c, magic), n = u - magic;
-    return ldexp(exp2_part(fma(v, c, -n)), (int)(uint32_t)__double_as_longlong(u));
-  }
-  __device__ __forceinline__ double scaled(double sum) const { return sum * exp2_part(-rest); }
 };
 
 // The first logit of a piece that is m, the largest, E or more if none: those that `off` hides are less, or m is int8's lowest
@@ -332,23 +327,13 @@ __global__ __launch_bounds__(64 * kSpanWaves) void row_spans_kernel(SpanArgs a, 
       z -= (double)hidden * sTable[(int)m + 128];
     } else {
       const SumWeights sum(dist.c, m);
-      if (sum.fits) {
-        if (has_extra) z = sum.of(xe);
+      if (has_extra) z = sum.add(xe, z);
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-          if (__any(off[p] != ALL)) {
+      for (int p = 0; p < P; ++p)
+        if (__any(off[p] != ALL)) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) z += sum.of(L::get(w[p], e));
-          }
-        z = sum.scaled(z);
-      } else {
-        const Weigh wt(dist.c, m, nullptr);
-        if (has_extra) z = wt.of<T>(xe);
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-          for (int e = 0; e < E; ++e) z += wt.of<T>(L::get(w[p], e));
-      }
+          for (int e = 0; e < E; ++e) z = sum.add(L::get(w[p], e), z);
+        }
     }
     out.z = wave_sum_f64(z);
   }
@@ -448,9 +433,8 @@ __device__ __forceinline__ uint32_t piece_of(const T *x, int piece, const Cut<T>
   return left > 0 ? ~hidden_bits<E>(suppress, piece * E) & ((1u << left) - 1u) : 0u;
 }
 
-// A span's sum relative to the row's largest logit (as it is where that is the span's: the polynomial's 1 is off by
-// 2.4e-13, and numbers like 1/2 are drawn at the borders of equal logits); 0 where its logits' weights are next to vanishing, so that
-// a span with a sum has a logit with a weight.
+// A span's sum relative to the row's largest logit, as it is where that is the span's; 0 where its logits' weights are next
+// to vanishing, so that a span with a sum has a logit with a weight.
 __device__ __forceinline__ double span_sum(const Span &s, const Weigh &row) {
   if (s.m == row.m) return s.z;
   const double z = s.z * exp2_64(row.log2_of(s.m));
@@ -756,8 +740,9 @@ __global__ __launch_bounds__(NT) void verify_pick_kernel(VerifyArgs a) {
     Rest<T> rest(a, v, b, sP, sQ);
     const bool target = v.mode == FROM_TARGET;
     if (target) {
+      rest.ip = 1.0;  // weights as a sampled row has them
       const RowSpans spans(work.spans + (b * N + v.accepted) * cut.spans, cut.spans, lane);
-      place = place_of(cut.spans, u, [&](int i) { return rest.ip * span_sum(spans.at(i), rest.p); }, lane);
+      place = place_of(cut.spans, u, [&](int i) { return span_sum(spans.at(i), rest.p); }, lane);
     }
     if (I8) __syncthreads();
     tok = draw<T>(place, target ? kSpanPieces : 64, [&](int at, double (&w)[Cut<T>::E]) { rest.load(at, cut), rest.weigh(at, w); }, sWave, tid);

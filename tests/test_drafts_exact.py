@@ -1,11 +1,12 @@
-"""Sampled decoding at its limits: verdicts that the caches' acceptance follows."""
+"""Sampled decoding at its limits: verdicts that the caches' acceptance follows, equal logits at
+numbers that are their borders."""
 import math
 
 import pytest
 import torch
 
 from tests import gen
-from tests.test_drafts import PROMPT, T, bit_words, host, small_model
+from tests.test_drafts import DTYPES, PROMPT, T, bit_words, host, small_model
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +75,45 @@ def test_step_without_any_token(iw, gpu):
             assert (res.verdict.accepted == 0).all() and (res.verdict.choice == -1).all()
             assert (res.accept.accepted == 1).all() and (res.accept.next_token == -1).all()
             assert (dec.lengths == PROMPT.shape[1] + 1 + i).all()
+
+
+# ---------------------------------------------------------------------------
+# borders
+# ---------------------------------------------------------------------------
+
+def drawn_either_way(iw, x, u, t):
+    """Tokens of rows by sample_tokens, and as the tokens after chains of no drafts."""
+    last = torch.zeros((len(u), 1), dtype=torch.int64, device="cuda")
+    return (iw.drafts.sample_tokens(x, u, temperature=t).tokens,
+            iw.drafts.verify_drafts(x[:, None], last, None, u[:, None], temperature=t).next_token)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("apart", [1, 37, 1100, 5000])
+def test_equal_logits_share_exactly(iw, gpu, apart, dtype):
+    """Two to sixteen equal logits in a row of less likely ones: a number that is the border of two of them draws the
+    second, the one before it the first."""
+    print("case: equal logits", apart, dtype, flush=True)
+    values = [0, -3, 1, 64, 127, -100] if dtype == "int8" else [0.0, -3.25, 1.0, 5.0, 7.5, 0.28125, -11.0]
+    for k in (2, 4, 8, 16):
+        V = apart * k + 3
+        x = torch.full((len(values), V), -127 if dtype == "int8" else -math.inf, dtype=DTYPES[dtype])
+        for i, v in enumerate(values):
+            x[i, 2:2 + apart * k:apart] = v
+        j = torch.arange(k, dtype=torch.float32)
+        u = torch.stack([j / k, torch.nextafter((j + 1) / k, torch.zeros(k))], 1).reshape(-1)
+        want = (2 + apart * j.long()).repeat_interleave(2)
+        for t in ((0.001,) if dtype == "int8" else (1.0, 0.7, 3.0)):  # int8: the others' weights are 0
+            for row in x:
+                for got in drawn_either_way(iw, row.cuda().expand(2 * k, V), u.cuda(), t):
+                    assert torch.equal(got.cpu(), want), (k, t, float(row.max()), got.tolist())
+
+
+@pytest.mark.parametrize("k", [3, 5, 6, 7, 10, 12, 24, 100])
+def test_equal_int8_logits_of_any_number_share_exactly(iw, gpu, k):
+    print("case: equal int8 logits", k, flush=True)
+    x = torch.full((1, 900), -127, dtype=torch.int8)
+    x[0, 5:5 + 7 * k:7] = 3
+    j = torch.arange(64)
+    for got in drawn_either_way(iw, x.cuda().expand(64, 900), (j / 64).cuda(), 0.001):
+        assert torch.equal(got.cpu(), 5 + 7 * (j * k // 64))
