@@ -137,6 +137,13 @@ __device__ __forceinline__ const T *row_of(const DistRows &d, int64_t outer, int
   return reinterpret_cast<const T *>(d.x) + outer * d.sb + inner * d.st;
 }
 
+// Weight of an int8 logit at a distance from the largest, to 44 bits (off by another 2.8e-14): sums of some 64 equal ones are exact,
+// so those of suppressed logits leave nothing where they are taken off a span's sum again.
+__device__ __forceinline__ double weight_at(double distance, double c) {
+  const uint64_t b = __double_as_longlong(exp2_64(-(distance * c)));
+  return __longlong_as_double((long long)((b + 0x100u) & ~0x1ffull));
+}
+
 // Weight of a logit relative to the largest, m; int8 rows have those of all distances in a table. The
 // distance comes first: as a difference of two products it would be lost where c is large.
 struct Weigh {
@@ -152,7 +159,7 @@ struct Weigh {
 };
 template <int THREADS = NT>
 __device__ __forceinline__ void fill_table(double *table, double c, int tid) {
-  for (int d = tid; d < 256; d += THREADS) table[d] = exp2_64(-((double)d * c));
+  for (int d = tid; d < 256; d += THREADS) table[d] = weight_at((double)d, c);
 }
 
 // A row's pieces, the last of them perhaps in part, and spans
@@ -323,7 +330,7 @@ __global__ __launch_bounds__(64 * kSpanWaves) void row_spans_kernel(SpanArgs a, 
           z += (a0 + a1) + (a2 + a3);
         }
       }
-      // the rest of a sum that cancels is whole multiples of one weight, or far above its rounding
+      // exact for lanes with nothing else
       z -= (double)hidden * sTable[(int)m + 128];
     } else {
       const SumWeights sum(dist.c, m);
@@ -560,7 +567,9 @@ __device__ __forceinline__ double share_of(const T *x, int64_t col, int cols, co
   if (col < 0 || col >= cols || suppressed(suppress, (int)col)) return 0.0;
   if (dist.greedy) return col == r.col ? 1.0 : 0.0;
   const Weigh wt(dist.c, r.m, nullptr);
-  return share(exp2_64(wt.log2_of(Logit<T>::one(x + col))), 1.0 / r.z);
+  const float v = Logit<T>::one(x + col);
+  const double w = std::is_same<T, int8_t>::value ? weight_at((double)r.m - v, dist.c) : exp2_64(wt.log2_of(v));
+  return share(w, 1.0 / r.z);
 }
 
 struct VerifyWork {

@@ -1,7 +1,8 @@
-"""Sampled decoding at its limits: verdicts that the caches' acceptance follows, equal logits at
-numbers that are their borders."""
+"""Sampled decoding at its limits: verdicts that the caches' acceptance follows, log-probabilities of
+certain tokens, equal logits at numbers that are their borders."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -75,6 +76,30 @@ def test_step_without_any_token(iw, gpu):
             assert (res.verdict.accepted == 0).all() and (res.verdict.choice == -1).all()
             assert (res.accept.accepted == 1).all() and (res.accept.next_token == -1).all()
             assert (dec.lengths == PROMPT.shape[1] + 1 + i).all()
+
+
+# ---------------------------------------------------------------------------
+# log-probabilities
+# ---------------------------------------------------------------------------
+
+# A lane's suppressed int8 logits are summed with its others and taken off again. A weight has 44 bits, so 64 equal ones have an
+# exact sum, and one of 1 among them too where they are 2^-7 or more; less of them leave the sum below 2: 65
+# roundings by 2^-53
+SUPPRESSED = 66 * 2.0 ** -53
+
+
+@pytest.mark.parametrize("V", [5, 33, 200, 4096, 4100, 9000])
+def test_suppressed_int8_logits_leave_nothing(iw, gpu, V):
+    """A row's only token that is not suppressed, at every value and many temperatures, has next to all of the weight."""
+    print("case: suppressed int8 logits", V, flush=True)
+    at = V // 3
+    off = T(bit_words([j for j in range(V) if j != at], V))
+    x = torch.full((256, V), -128, dtype=torch.int8, device="cuda")
+    x[:, at] = torch.arange(-128, 128).to(torch.int8)
+    u = torch.full((256,), 0.5, device="cuda")
+    for t in np.linspace(0.05, 40, 60).tolist():
+        got = iw.drafts.sample_tokens(x, u, temperature=t, scale=0.5, suppress=off)
+        assert (got.tokens == at).all() and float(got.logprob.abs().max()) <= SUPPRESSED, t
 
 
 # ---------------------------------------------------------------------------
