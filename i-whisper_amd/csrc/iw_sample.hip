@@ -510,7 +510,8 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs a) {
                   },
                   sWave, tid);
     mine = tok >= 0;
-    if (mine) lp = (float)(wt.log2_of(L::one(x + tok)) * kLn2 - log(place.whole));
+    // the sum has the token's weight in it but may be a rounding below it
+    if (mine) lp = (float)fmin(wt.log2_of(L::one(x + tok)) * kLn2 - log(place.whole), 0.0);
   }
   if (mine) {
     a.tokens[row] = tok;

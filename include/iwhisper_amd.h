@@ -759,7 +759,7 @@ int64_t iw_attention_window_workspace(int64_t batch, int64_t heads, int64_t quer
 /* A token of each row of logits, drawn by a given number. Row r's weights are
  * w_j = exp((x_j - max x) * scale / T), 0 for a token of the bitmask suppress (or NULL)
  * and for -inf; tokens[r] is the least j with w_0 + .. + w_j > uniforms[r] * (sum of w),
- * logprob[r] (or NULL) log(w_j / sum). T is temperatures[r] (float32), or for NULL the
+ * logprob[r] (or NULL) log(w_j / sum), at most 0. T is temperatures[r] (float32), or for NULL the
  * scalar temperature; where it is not above 0 the token is the first of the
  * largest logits, with logprob 0. uniforms are clamped to [0, 1 - 2^-24], a NaN is 0. A
  * row with a NaN or +inf, or without any finite logit, gives token -1 and logprob NaN.

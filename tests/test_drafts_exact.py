@@ -102,6 +102,44 @@ def test_suppressed_int8_logits_leave_nothing(iw, gpu, V):
         assert (got.tokens == at).all() and float(got.logprob.abs().max()) <= SUPPRESSED, t
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_logprob_is_never_above_0(iw, gpu, dtype):
+    """A row's only token has log-probability 0, one that has nearly all of the weight no more than that."""
+    print("case: certain tokens", dtype, flush=True)
+    values = [0.0, 1.0, -3.25, 5.0, 7.5, -0.4375, 17.0, -30.0, 3.0, 11.0]
+    if dtype == "int8":
+        values = [0, 1, -3, 5, 127, -128, 17, -30, 64, 99]
+    n, low = len(values), -128 if dtype == "int8" else -math.inf
+    u = T(gen.rng(2).random(n, np.float32))
+    for V in (1, 3, 40, 5000):
+        only = torch.full((n, V), low, dtype=DTYPES[dtype])
+        at = [(7 * i) % V for i in range(n)]
+        for i, v in enumerate(values):
+            only[i, at[i]] = v
+        for t in (1.0, 0.7, 0.01, 0.0):
+            # the token alone; int8 rows, whose lowest value is a logit like others, with all others suppressed
+            for i in range(n):
+                off = None if dtype != "int8" or V == 1 else T(bit_words([j for j in range(V) if j != at[i]], V))
+                got = iw.drafts.sample_tokens(only[i:i + 1].cuda(), u[i:i + 1], temperature=t, scale=0.5, suppress=off)
+                lp = float(got.logprob[0])
+                assert int(got.tokens[0]) == at[i]
+                assert lp == 0.0 if off is None else -SUPPRESSED <= lp <= 0.0, (V, t, values[i], lp)
+    if dtype == "int8":
+        x = torch.full((256, 200), -128, dtype=torch.int8, device="cuda")
+        x[:, 66] = torch.arange(-128, 128).to(torch.int8)
+        off = T(bit_words([j for j in range(200) if j != 66], 200))
+        for t in np.linspace(0.05, 40, 60).tolist():
+            got = iw.drafts.sample_tokens(x, torch.full((256,), 0.5, device="cuda"), temperature=t, scale=0.5, suppress=off)
+            assert (got.logprob <= 0).all(), t
+    V = 3001
+    x = torch.from_numpy(gen.rng(3).normal(0, 1, (64, V)))
+    x[:, 11] = torch.linspace(10, 60, 64)
+    scale = 0.5 if dtype == "int8" else 1.0
+    x = (x / scale).round().clamp(-127, 127).to(torch.int8) if dtype == "int8" else x.to(DTYPES[dtype])
+    got = iw.drafts.sample_tokens(x.cuda(), torch.full((64,), 0.3, device="cuda"), scale=scale)
+    assert (got.tokens == 11).all() and (got.logprob <= 0).all()
+
+
 # ---------------------------------------------------------------------------
 # borders
 # ---------------------------------------------------------------------------
