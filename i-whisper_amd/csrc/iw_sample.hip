@@ -44,7 +44,8 @@ struct Span {
 
 // 2^f for |f| <= 1/2: of the polynomials of degree 8 that are 1 at 0 the one with the smallest relative error, 8.14e-13
 // (found by linear programming; 7.8e-13 without that condition, a degree more or less 1.4e-14 or 4.0e-11). The
-// largest logit's weight is 1 exactly, so equal ones have exact sums and meet at exact borders.
+// largest logit's weight is 1 exactly, so equal ones have exact sums and meet at exact borders. A border's share s of the whole is right
+// to 2 s (1 - s) 8.2e-13 then, at most 4.1e-13, and up to 2e-8 of all numbers draw another token of 2^16 than exact ones.
 __device__ __forceinline__ double exp2_part(double f) {
   // the two constants of the first step: an instruction reads one from scalar registers
   double second = 0x1.00d8533f3e35fp-16;
@@ -441,10 +442,11 @@ __device__ __forceinline__ uint32_t piece_of(const T *x, int piece, const Cut<T>
 }
 
 // A span's sum relative to the row's largest logit, as it is where that is the span's; 0 where its logits' weights are next
-// to vanishing, so that a span with a sum has a logit with a weight.
+// to vanishing, so that a span with a sum has a logit with a weight. The factor is the library's power, right to a rounding: the
+// polynomial's errors would add up, and a weight is to be off by one of them.
 __device__ __forceinline__ double span_sum(const Span &s, const Weigh &row) {
   if (s.m == row.m) return s.z;
-  const double z = s.z * exp2_64(row.log2_of(s.m));
+  const double z = s.z * exp2(row.log2_of(s.m));
   return z > 1e-290 ? z : 0.0;
 }
 

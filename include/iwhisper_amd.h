@@ -764,7 +764,7 @@ int64_t iw_attention_window_workspace(int64_t batch, int64_t heads, int64_t quer
  * largest logits, with logprob 0. uniforms are clamped to [0, 1 - 2^-24], a NaN is 0. A
  * row with a NaN or +inf, or without any finite logit, gives token -1 and logprob NaN.
  * logits: type as iw_token_logprobs, row stride ld. Weights and sums are 64-bit, a
- * weight off by at most 8e-13 of itself. rows <=
+ * weight off by at most 8.5e-13 of itself. rows <=
  * 2^22, cols < 2^23. workspace: iw_sample_tokens_workspace bytes, 16-byte aligned,
  * used during the call's work only. The struct is read during the call. */
 typedef struct iw_sample_tokens_args {

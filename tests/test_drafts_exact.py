@@ -1,5 +1,6 @@
 """Sampled decoding at its limits: verdicts that the caches' acceptance follows, log-probabilities of
-certain tokens, equal logits at numbers that are their borders."""
+certain tokens, equal logits at numbers that are their borders, borders as close as a weight is exact."""
+import decimal
 import math
 
 import numpy as np
@@ -180,3 +181,70 @@ def test_equal_int8_logits_of_any_number_share_exactly(iw, gpu, k):
     j = torch.arange(64)
     for got in drawn_either_way(iw, x.cuda().expand(64, 900), (j / 64).cuda(), 0.001):
         assert torch.equal(got.cpu(), 5 + 7 * (j * k // 64))
+
+
+# Logits (a, m, x, r) and numbers: of rows with a in column 0, m in column 1024, x in the 1023 after that, no r
+NEAR = """
+0x1.b8f478p-4 -0x1.eb4d6ep+0 -0x1.a4759ap+2 -inf 0x1.a72acap-2
+0x1.bb9382p-4 -0x1.eb4d6ep+0 -0x1.a4759ap+2 -inf 0x1.a75378p-2
+0x1.06070ep+1 -0x1.4809dp-2 -0x1.57d8dp+2 -inf 0x1.2bf87p-1
+-0x1.ac36cp+0 -0x1.c142cap+1 -0x1.08ee9ap+3 -inf 0x1.92d3eep-2
+-0x1.6d8c96p-5 -0x1.1c7f48p+1 -0x1.bfdce8p+2 -inf 0x1.e9c4cep-2
+-0x1.264ffap+1 -0x1.1f82f2p+2 -0x1.2c321ep+3 -inf 0x1.03bee2p-1
+-0x1.367bf8p-2 -0x1.2b7c3ep+1 -0x1.c5c85cp+2 -inf 0x1.c03746p-2
+0x1.5c416p+2 0x1.065edp+2 -0x1.503bep+0 -inf 0x1.a16646p-2
+0x1.c3f1e8p+2 0x1.33af4p+2 0x1.bb4ap-6 -inf 0x1.fe705ep-2
+-0x1.21a412p-1 -0x1.4be7eep+1 -0x1.e54818p+2 -inf 0x1.f3c27cp-2
+0x1.71d4d2p+1 0x1.637c64p-3 -0x1.060294p+2 -inf 0x1.fc3d0ap-2
+0x1.48b566p+0 -0x1.887744p-1 -0x1.7e3a0ap+2 -inf 0x1.14aaaep-1
+0x1.d45662p+2 0x1.60d566p+2 0x1.80dfep-2 -inf 0x1.db94a6p-2
+-0x1.520436p-3 -0x1.38375p+1 -0x1.d7deep+2 -inf 0x1.132dcp-1
+0x1.cc6642p-1 -0x1.045f58p+0 -0x1.73f99ep+2 -inf 0x1.ac0f4ap-2
+-0x1.ef2044p+0 -0x1.c19496p+1 -0x1.14a516p+3 -inf 0x1.a1ab6ap-2
+-0x1.419a6cp+0 -0x1.a5c9f4p+1 -0x1.17ed1p+3 -inf 0x1.2d070cp-1
+-0x1.7aa9eap+0 -0x1.fdfb6cp+1 -0x1.0fb0ep+3 -inf 0x1.fef0cp-2
+0x1.48756ep+1 0x1.a8f366p-4 -0x1.2c2c18p+2 -inf 0x1.1b4fbp-1
+0x1.2be034p+0 -0x1.2b7e72p-1 -0x1.84e1b2p+2 -inf 0x1.0d593cp-1
+-0x1.51d1ccp+1 -0x1.58679ep+2 -0x1.3cca9cp+3 -inf 0x1.1f19fap-1
+-0x1.a0f4ccp+0 -0x1.1e4512p+2 -0x1.12db8ap+3 -inf 0x1.f8cacep-2
+"""
+
+
+# and of rows with a in the first 1024 columns and r in column 2048
+FARTHER = """
+0x1.63e88cp+2 0x1.b6776cp+2 0x1.5813a4p+2 0x1.d73444p+2 0x1.164802p-1
+0x1.22817ep+0 0x1.0458dp+1 0x1.2a1052p+0 0x1.cae124p+1 0x1.f54d96p-2
+0x1.033658p+2 0x1.53347ap+2 0x1.dcae92p+1 0x1.08efeep+3 0x1.1dcc6ap-1
+0x1.703cccp+1 0x1.1baacp+2 0x1.805c48p+1 0x1.dd36a2p+2 0x1.ca9632p-2
+0x1.502036p+0 0x1.1b4198p+2 0x1.1d47ccp+0 0x1.595226p+2 0x1.0d9fe8p-1
+0x1.54d118p+1 0x1.d557ap+1 0x1.73d36p+1 0x1.922bbp+2 0x1.bae584p-2
+-0x1.c6c0cap-1 0x1.5ac112p+0 -0x1.f680ccp-1 0x1.8232bcp+1 0x1.04318p-1
+0x1.2e0104p+2 0x1.67102p+2 0x1.25e01cp+2 0x1.cbc346p+2 0x1.0e5d78p-1
+0x1.f2fedep+0 0x1.d29ec8p+1 0x1.f8c4f8p+0 0x1.652edep+2 0x1.f01dcap-2
+0x1.70ef16p+2 0x1.e123dcp+2 0x1.77ca94p+2 0x1.1e959p+3 0x1.de3162p-2
+0x1.10700cp-1 0x1.9a8d7p+1 0x1.67959p-2 0x1.e0553ap+1 0x1.117618p-1
+0x1.c4992ap+0 0x1.4d1b8ep+1 0x1.873a8ep+0 0x1.ab976ep+1 0x1.1d8cc6p-1
+-0x1.93098p+0 0x1.a7f2ep-1 -0x1.7033ccp+0 0x1.ac4514p+1 0x1.bf4e6cp-2
+0x1.dea006p+1 0x1.310eccp+2 0x1.f1b3c8p+1 0x1.d11262p+2 0x1.d2659ap-2
+"""
+
+
+@pytest.mark.parametrize("copies,rows", [(1, NEAR), (1024, FARTHER)], ids=["two spans", "three spans"])
+def test_borders_as_near_as_a_weight_is_exact(iw, gpu, copies, rows):
+    """A weight is off by at most 8.2e-13 of itself (the polynomial's 8.14e-13 and the roundings of an exponent and a product), so
+    a share s of the whole by less than s (1 - s) 2 * 8.2e-13, at most 4.1e-13, and by the sums' roundings, some 2e-15: numbers
+    at 4.3e-13 to 6.1e-13 from a border draw the right one of its tokens."""
+    print("case: near borders", copies, flush=True)
+    rows = [[float.fromhex(v) for v in line.split()] for line in rows.split("\n") if line]
+    x = torch.full((len(rows), 2050), -math.inf)
+    want = []
+    with decimal.localcontext() as ctx:
+        ctx.prec = 40
+        for i, (a, m, low, r, u) in enumerate(rows):
+            x[i, :copies], x[i, 1024], x[i, 1025:2048], x[i, 2048] = a, m, low, r
+            ea, em, el, er = (decimal.Decimal(v).exp() if v > -math.inf else decimal.Decimal(0) for v in (a, m, low, r))
+            off = copies * ea / (copies * ea + em + 1023 * el + er) - decimal.Decimal(u)
+            assert decimal.Decimal("4.2e-13") < abs(off) < decimal.Decimal("6.5e-13")
+            want.append(off > 0)
+    got = iw.drafts.sample_tokens(x.cuda(), torch.tensor([r[4] for r in rows], device="cuda"))
+    assert [int(v) < 1024 for v in got.tokens] == want
