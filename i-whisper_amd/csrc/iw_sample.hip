@@ -183,6 +183,7 @@ struct SpanArgs {
   const uint32_t *suppress = nullptr;
   int cols = 0;
   Span *spans = nullptr;
+  int64_t row0 = 0;         // the first of this launch
 };
 
 // The larger of two, NaN where either is
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(64 * kSpanWaves) void row_spans_kernel(SpanArgs a, 
   constexpr uint32_t ALL = (1u << E) - 1u;
   __shared__ double sTable[I8 ? 256 : 1];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t row = (uint32_t)blockIdx.x / (uint32_t)groups;
+  const int64_t row = a.row0 + (uint32_t)blockIdx.x / (uint32_t)groups;
   const bool second = row >= a.first;
   const int64_t r = second ? row - a.first : row;
   const uint32_t inner = (uint32_t)(second ? a.d[1].inner : a.d[0].inner);
@@ -697,11 +698,11 @@ __global__ __launch_bounds__(64 * kDecideWaves) void verify_decide_kernel(Verify
 
 // The sums of what is left of a row over 64 pieces, a piece a lane
 template <typename T>
-__global__ __launch_bounds__(NT) void verify_rest_kernel(VerifyArgs a, int groups) {
+__global__ __launch_bounds__(NT) void verify_rest_kernel(VerifyArgs a, int groups, int64_t b0) {
   constexpr bool I8 = std::is_same<T, int8_t>::value;
   __shared__ double sP[I8 ? 256 : 1], sQ[I8 ? 256 : 1];
   const int tid = threadIdx.x;
-  const int64_t b = (uint32_t)blockIdx.x / (uint32_t)groups;
+  const int64_t b = b0 + (uint32_t)blockIdx.x / (uint32_t)groups;
   const Cut<T> cut(a.cols);
   const VerifyWork work = verify_work(a, cut);
   const Verdict v = work.verdict[b];
@@ -768,12 +769,26 @@ __global__ __launch_bounds__(NT) void verify_pick_kernel(VerifyArgs a) {
   }
 }
 
+// Launches of a row's `groups` blocks: launch(first, rows) for as many rows at a time as a grid takes, which has fewer than
+// 2^32 threads.
+template <typename F>
+int launch_rows(int64_t rows, int64_t groups, int threads, F launch) {
+  const int64_t most = ((1LL << 32) - 1) / threads / groups;
+  for (int64_t first = 0; first < rows; first += most) {
+    const int rc = launch(first, std::min(most, rows - first));
+    if (rc) return rc;
+  }
+  return 0;
+}
+
 template <typename T>
 int launch_spans(SpanArgs a, int64_t rows, hipStream_t s) {
   const int groups = (Cut<T>(a.cols).spans + kSpanWaves - 1) / kSpanWaves;
-  if (rows * groups >= (1LL << 32) / (64 * kSpanWaves)) return fail("too many logits for one call");
-  hipLaunchKernelGGL((row_spans_kernel<T>), dim3((unsigned)(rows * groups)), dim3(64 * kSpanWaves), 0, s, a, groups);
-  return check_launch("row_spans_kernel");
+  return launch_rows(rows, groups, 64 * kSpanWaves, [&](int64_t first, int64_t n) {
+    a.row0 = first;
+    hipLaunchKernelGGL((row_spans_kernel<T>), dim3((unsigned)(n * groups)), dim3(64 * kSpanWaves), 0, s, a, groups);
+    return check_launch("row_spans_kernel");
+  });
 }
 
 template <typename T>
@@ -807,9 +822,10 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
   if (rc) return rc;
   if (a.nodes > 1) {  // a row of one node has nothing to reject
     const int64_t groups = (Cut<T>(a.cols).parts + kWaves - 1) / kWaves;
-    if (a.batch * groups >= (1LL << 32) / NT) return fail("too many logits for one call");
-    hipLaunchKernelGGL((verify_rest_kernel<T>), dim3((unsigned)(a.batch * groups)), dim3(NT), 0, s, a, (int)groups);
-    rc = check_launch("verify_rest_kernel");
+    rc = launch_rows(a.batch, groups, NT, [&](int64_t first, int64_t n) {
+      hipLaunchKernelGGL((verify_rest_kernel<T>), dim3((unsigned)(n * groups)), dim3(NT), 0, s, a, (int)groups, first);
+      return check_launch("verify_rest_kernel");
+    });
     if (rc) return rc;
   }
   hipLaunchKernelGGL((verify_pick_kernel<T>), dim3((unsigned)a.batch), dim3(NT), 0, s, a);

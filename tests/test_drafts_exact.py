@@ -1,5 +1,5 @@
 """Sampled decoding at its limits: verdicts that the caches' acceptance follows, log-probabilities of
-certain tokens, equal logits at numbers that are their borders, borders as close as a weight is exact."""
+certain tokens, equal logits at numbers that are their borders, borders as close as a weight is exact, the largest batches."""
 import decimal
 import math
 
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tests import gen
-from tests.test_drafts import DTYPES, PROMPT, T, bit_words, host, small_model
+from tests.test_drafts import DTYPES, PROMPT, T, bit_words, drawn_by, host, small_model
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +248,46 @@ def test_borders_as_near_as_a_weight_is_exact(iw, gpu, copies, rows):
             want.append(off > 0)
     got = iw.drafts.sample_tokens(x.cuda(), torch.tensor([r[4] for r in rows], device="cuda"))
     assert [int(v) < 1024 for v in got.tokens] == want
+
+
+# ---------------------------------------------------------------------------
+# sizes
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("N,V,some", [(32, 5, 1 << 20), (64, 3, 1 << 20), (2, 70001, 300)])
+def test_verify_as_many_rows_as_a_call_takes(iw, gpu, N, V, some):
+    """2^20 rows of one text's logits, of many nodes and of a wide vocabulary."""
+    print("case: most rows of drafts", N, V, flush=True)
+    B = 1 << 20
+    r = gen.rng(N)
+    x = torch.from_numpy(r.integers(-12, 13, V).astype(np.int8))
+    g = torch.Generator(device="cuda").manual_seed(N)
+    u = torch.rand((B, N), generator=g, device="cuda")
+    tokens = torch.randint(0, V, (B, N), generator=g, device="cuda")
+    if V > 100:
+        tokens[:, 1] = int(x.argmax())
+    got = iw.drafts.verify_drafts(x.cuda().expand(B, N, V), tokens, None, u, scale=0.25)
+    w = np.exp(x.double().numpy() * 0.25)
+    p = torch.from_numpy(w / w.sum()).cuda()
+    ok = u[:, :-1].double() < p[tokens[:, 1:]]
+    taken = ok.long().cumprod(1).sum(1)
+    assert torch.equal(got.accepted.long(), taken)
+    i = torch.arange(N, device="cuda")
+    kept = torch.where(i[:-1] < taken[:, None], tokens[:, 1:], -1)
+    assert torch.equal(torch.where(i[:-1] == taken[:, None], -1, got.choice[:, :-1]), kept)
+    assert torch.equal(got.choice.gather(1, taken[:, None])[:, 0], got.next_token)
+    if some < B:
+        for b in np.linspace(0, B - 1, some).astype(int).tolist():
+            left = w.copy()
+            if int(taken[b]) < N - 1:
+                left[int(tokens[b, int(taken[b]) + 1])] = 0
+            drawn_by(int(got.next_token[b]), left, float(u[b, N - 1]), left.sum())
+        return
+    left = p.expand(B, V).clone()
+    more = torch.nonzero(taken < N - 1)[:, 0]
+    left[more, tokens[more, taken[more] + 1]] = 0
+    c = left.cumsum(1)
+    at = u[:, -1:].double() * c[:, -1:]
+    want = (c <= at).sum(1)
+    clear = ((c - at).abs() > 1e-12).all(1)  # numbers that no rounding moves
+    assert clear.float().mean() > 0.999 and torch.equal(got.next_token[clear], want[clear])
