@@ -109,7 +109,8 @@ __device__ __forceinline__ void finish_row(const WindowArgs &t, const Finish &fi
   }
 }
 
-constexpr int rows_waves(int ks, int qt) { return ks * qt <= 2 ? 4 : 2; }
+// waves a SIMD: registers allow four with 64 columns a head; two blocks of 128 columns fill a CU's LDS (70 528 bytes each)
+constexpr int rows_waves(int ks) { return ks == 1 ? 4 : 2; }
 
 // The chunks of 64 keys that any of the 16 queries of a tile sees: the first ns hold first keys, the others follow
 // one another from w0 on. And the keys that all of them see.
@@ -815,9 +816,10 @@ __device__ __forceinline__ void transpose_groups(v4i &p) {
 // A score takes an instruction for the maximum, a multiplication, three simple ones and a byte from the table for its
 // value, and P.V next to nothing: the vector units and the ways between them and LDS bound it. 16 rows of 20 heads of 1500
 // frames that see 511 and 16 others take 133 us, two thirds of them the vector units' own; its matrix products would
-// take 29. It needs its four waves a SIMD: with three and no spilled registers (8 now, between the passes) it takes 167.
+// take 29. It needs its four waves a SIMD: with three and no spilled registers (8 now, 10 with
+// quads, between the passes) it takes 167. 128 columns a head have two, as two blocks fill a CU's LDS.
 template <int KS, bool QUADS, int QT, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(KS, QT)))) void attn_window_rows_kernel(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(KS)))) void attn_window_rows_kernel(
     WindowArgs t, int qblocks, int blocks, int per_xcd, int table_off) {
   constexpr int QW = 16 * QT, QR = QW * NW, IMAGES = 4 * KS, IMAGE = 1024, CHUNK = IMAGES * IMAGE, PLACE = 4 * CHUNK;
   static_assert(NW == 4, "each wave copies KS images of K and of V");
@@ -1251,12 +1253,13 @@ int token_parts(int64_t heads, int64_t chunks) {
 
 // Which of the kernels, with the same results. Queries at the last positions share chunks in LDS where 64 of them a block
 // fill the device: heads of 128 columns from a block a CU on, of 64 columns from one and a half (us of a block a 16-query
-// tile and so, windows of 512 keys, with 64 and 128 columns: 20 heads of 1500 queries, 480 blocks, 22.9 and 20.4, 54.5 and
-// 28.7; 64 of 300, 320 blocks, 15.6 and 16.9, 34.4 and 24.9; 64 of 128, 128 blocks, 9.0 and 14.2, 18.5 and 23.2), but not
-// for 32 queries or fewer (1280 heads of 32: 34.4 and 38.1, 56.0 and 54.2; of 64: 45.2 and 32.5, 126 and 76).
+// tile and so, windows of 512 keys, with 64 and 128 columns: 20 heads of 1500 queries, 480 blocks, 29 and 19, 54 and
+// 26; 64 of 300, 320 blocks, 11.5 and 12.9, 22 and 16; 64 of 128, 128 blocks, 9.5 and 15.7, 18 and 23), but not
+// for 32 queries or fewer (1280 heads of 32: 40 and 41, 81 and 79; of 64: 63 and 43, 139 and 81).
 // Two tiles a wave pay where windows are longer and their 128 queries a block fill the device too (320 heads of 1500
-// queries with 64 and 128 columns, one tile and two: 256 keys 111 and 101, 253 and 203; 512 keys 145 and 129, 343 and 265;
-// 1280 of 300 with 128 keys 78 and 85, 171 and 173; of 64 with 512 keys, half of a block, 32.5 and 38.8, 76 and 91).
+// queries with 64 and 128 columns, one tile and two: 256 keys 107 and 92, 223 and 179; 512 keys 150 and 122, 324 and 245;
+// 1280 of 300 with 128 keys 66 and 68, 131 and 124; of 64 with 512 keys, half of a block, 43 and 51, 81 and 102). Blocks of
+// 128 columns are two to a CU with either, whose LDS they fill.
 // One query has its own kernel, a wave a chunk where there are few (quads, 64 columns, us with this and with the next: 20
 // heads of 128 keys, 4.5 and 5.3, of 384 keys, 5.3 and 5.9; 2560 heads of them 12.0 and 15.9, 23.0 and 26.8), else eight
 // waves (1024 keys, 20 heads 7.0 and 7.8, 2560 heads 65 and 85; four waves 8.4 and 68, sixteen 7.5 and 74).
