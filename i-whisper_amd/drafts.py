@@ -6,8 +6,9 @@ transcribe.py). Here the random numbers are given, so a run can be repeated,
 and several tokens of a row can be drafted and verified in one decoder pass
 without changing their distribution: a draft x drawn from q is accepted with
 probability min(1, p(x) / q(x)), else replaced by a token of max(p - q, 0).
-Drafts may come from any model, or from this one at a fraction of a step's cost
-over a window of the keys: a step's time is the reading of K and V.
+Drafts may come from any model, or from this one over a window of the keys: where
+the reading of K and V bounds a step such a draft costs less (128 rows of the large
+shape with 257 of 1500 audio positions 3.3 ms, a step 5.4), for a row alone as much.
 
 * ``window_attention``  integer attention over the keys around each query's position and a
                         few first ones (also an encoder's local attention)
